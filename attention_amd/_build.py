@@ -59,7 +59,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(out, flush=True)
 
 
-HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla"]
+HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla", "tree_decode", "qk_norm_rope", "kv_compact"]
+TORCH_SOURCES = ["torch_ops", "serving_ops"]
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 
 # Per-source flags.  mla: MFMA accumulators in VGPRs where the register
@@ -99,15 +100,24 @@ def _torch_flags() -> tuple[list[str], str]:
             library_paths()[0])
 
 
-def torch_object_cmd() -> list[str]:
+def torch_object_cmd(name: str) -> list[str]:
     flags, _ = _torch_flags()
-    return ["g++", "-O2", "-std=c++17", "-fPIC", *flags, "-c", os.path.join(CSRC, "torch_ops.cpp"),
-            "-o", os.path.join(OBJ_DIR, "torch_ops.o")]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", *flags, "-c", os.path.join(CSRC, f"{name}.cpp"),
+            "-o", os.path.join(OBJ_DIR, f"{name}.o")]
+
+
+def _torch_stale(name: str) -> bool:
+    obj = os.path.join(OBJ_DIR, f"{name}.o")
+    if not os.path.exists(obj):
+        return True
+    deps = [os.path.join(CSRC, f"{name}.cpp"), os.path.join(CSRC, "torch_desc.h"),
+            os.path.join(INCLUDE, "qd_attention.h")]
+    return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 
 
 def torch_link_cmd() -> list[str]:
     _, torch_lib = _torch_flags()
-    return ["g++", "-shared", os.path.join(OBJ_DIR, "torch_ops.o"), "-o", TORCH_LIB + ".tmp",
+    return ["g++", "-shared", *[os.path.join(OBJ_DIR, f"{n}.o") for n in TORCH_SOURCES], "-o", TORCH_LIB + ".tmp",
             f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-lamdhip64",
             f"-L{LIB_DIR}", "-l:libqd_attention.so",
             "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
@@ -120,11 +130,7 @@ def build(verbose: bool = False, incremental: bool = False) -> None:
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
     cmds = [hip_object_cmd(n) for n in HIP_SOURCES if not incremental or _stale(n)]
-    torch_obj = os.path.join(OBJ_DIR, "torch_ops.o")
-    if (not incremental or not os.path.exists(torch_obj)
-            or os.path.getmtime(os.path.join(CSRC, "torch_ops.cpp")) > os.path.getmtime(torch_obj)
-            or os.path.getmtime(os.path.join(INCLUDE, "qd_attention.h")) > os.path.getmtime(torch_obj)):
-        cmds.append(torch_object_cmd())
+    cmds += [torch_object_cmd(n) for n in TORCH_SOURCES if not incremental or _torch_stale(n)]
     with ThreadPoolExecutor(max_workers=max(1, len(cmds))) as ex:
         for f in [ex.submit(_run, c, verbose) for c in cmds]:
             f.result()

@@ -132,6 +132,22 @@ def lib():
         L.qd_mla_decode.restype = I
         L.qd_mla_decode.argtypes = ([V] * 11 + [ctypes.c_size_t] + [I] * 9 + [I64] + [I] * 3 + [F]
                                     + [I, I, V])
+        L.qd_gqa_decode_tree_validate.restype = I
+        L.qd_gqa_decode_tree_validate.argtypes = [P] * 6 + [ctypes.c_double, I64, I64] + MSG
+        L.qd_gqa_decode_tree_workspace_bytes.restype = ctypes.c_size_t
+        L.qd_gqa_decode_tree_workspace_bytes.argtypes = [I] * 12
+        L.qd_gqa_decode_tree_info.restype = I
+        L.qd_gqa_decode_tree_info.argtypes = [I] * 12 + [ctypes.POINTER(I)] * 2
+        L.qd_gqa_decode_tree.restype = I
+        L.qd_gqa_decode_tree.argtypes = [V] * 8 + [ctypes.c_size_t] + [I] * 7 + [I64, I, F, I, I, I, V]
+        L.qd_qk_norm_rope_write_validate.restype = I
+        L.qd_qk_norm_rope_write_validate.argtypes = [P] * 10 + [ctypes.c_double] + MSG
+        L.qd_qk_norm_rope_write.restype = I
+        L.qd_qk_norm_rope_write.argtypes = [V] * 11 + [I64] + [I] * 4 + [I64] * 5 + [I, I, F, I, V]
+        L.qd_kv_compact_validate.restype = I
+        L.qd_kv_compact_validate.argtypes = [P] * 4 + MSG
+        L.qd_kv_compact.restype = I
+        L.qd_kv_compact.argtypes = [ctypes.POINTER(V), I, V, V, V, I, I, I, I, I64, I64, V]
         _lib = L
     return _lib
 
@@ -361,3 +377,57 @@ def mla_decode(q, qr, cache, table, lens, pos, wk, wv, out, *, scale, indices=No
                                None if indices is None else indices.data_ptr(), out.data_ptr(), ws.data_ptr(),
                                ws.numel(), B, T, H, Dn, Dc, Dr, Dv, cache.shape[1], table.shape[1], cache.shape[0],
                                nk, int(causal), DTYPE[q.dtype], float(scale), splits, flags, _stream(q, stream))
+
+
+# ---- Drafted tokens and sliding windows ------------------------------------
+
+QD_TREE_VALU, QD_TREE_MFMA, QD_TREE_MFMA_SPLIT = 0, 1, 2
+
+
+def validate_gqa_decode_tree(q, k, v, table, lens, mask=None, scale=0.125, window=0, sinks=0):
+    return _msg_call(lib().qd_gqa_decode_tree_validate, *(ctypes.byref(d) for d in (q, k, v, table, lens)), _ref(mask),
+                     scale, window, sinks)
+
+
+def gqa_decode_tree_info(B, T, Hq, Hkv, D, P, maxP, has_mask=1, window=0, sinks=0, dtype=2, flags=0):
+    """(kind, workgroups, rows per workgroup) from qd_gqa_decode_tree_info."""
+    w, r = ctypes.c_int(), ctypes.c_int()
+    kind = lib().qd_gqa_decode_tree_info(B, T, Hq, Hkv, D, P, maxP, has_mask, window, sinks, dtype, flags,
+                                         ctypes.byref(w), ctypes.byref(r))
+    return kind, w.value, r.value
+
+
+def gqa_decode_tree(q, k, v, table, lens, mask, out, *, scale, window=0, sinks=0, flags=0, workspace=None, stream=None):
+    """Calls qd_gqa_decode_tree on torch device tensors (no validation); mask
+    None: q [B, Hq, D]."""
+    B, T = q.shape[0], q.shape[1] if mask is not None else 1
+    Hq, D = q.shape[-2:]
+    _, P, Hkv, _ = k.shape
+    shape = (B, T, Hq, Hkv, D, P, table.shape[1])
+    n = lib().qd_gqa_decode_tree_workspace_bytes(*shape, int(mask is not None), window, sinks, DTYPE[q.dtype], flags)
+    if workspace is None and n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+    return lib().qd_gqa_decode_tree(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        None if mask is None else mask.data_ptr(), out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() if workspace is not None else 0, *shape, k.shape[0], DTYPE[q.dtype], float(scale), window,
+        sinks, flags, _stream(q, stream))
+
+
+def validate_qk_norm_rope_write(q, key, value, cos_sin, positions, kc, vc, slots, qw=None, kw=None, eps=1e-6):
+    return _msg_call(lib().qd_qk_norm_rope_write_validate,
+                     *(ctypes.byref(d) for d in (q, key, value, cos_sin, positions, kc, vc, slots)), _ref(qw), _ref(kw),
+                     eps)
+
+
+def validate_kv_compact(cache, table, lens, accepted):
+    return _msg_call(lib().qd_kv_compact_validate, *(ctypes.byref(d) for d in (cache, table, lens, accepted)))
+
+
+def kv_compact(caches, table, lens, accepted, stream=None):
+    """Calls qd_kv_compact on torch device tensors (no validation)."""
+    pointers = (ctypes.c_void_p * len(caches))(*(c.data_ptr() for c in caches))
+    c = caches[0]
+    return lib().qd_kv_compact(pointers, len(caches), table.data_ptr(), lens.data_ptr(), accepted.data_ptr(),
+                               accepted.shape[0], accepted.shape[1], c.shape[1], table.shape[1], c.shape[0],
+                               c[0, 0].numel() * c.element_size(), _stream(c, stream))

@@ -432,6 +432,117 @@ int qd_mla_decode(const void* q_nope, const void* q_rope, const void* cache, con
                   int max_pages, int64_t num_blocks, int num_indices, int causal, int dtype, float scale,
                   int splits, int flags, void* stream);
 
+/* ---- Decoding with drafted tokens and sliding windows ----------------
+ * No counterpart in the reference: the operators around gqa_decode that a
+ * serving engine needs when it drafts several tokens per step or when a
+ * layer keeps only the last tokens in sight.  One step is
+ *   qd_qk_norm_rope_write   per-head norms, rotation, cache write
+ *   qd_gqa_decode_tree      attention of the drafted tokens over the cache
+ *                           (window and first tokens optional; q_len 1 and
+ *                           no mask: one query per sequence)
+ *   qd_kv_compact           the accepted drafted tokens' rows move next to
+ *                           the context.
+ * Caches, block_table and context_lens are those of gqa_decode.  Nothing
+ * here allocates, synchronizes or reads metadata on the host. */
+
+/* Largest number of drafted tokens per sequence (bits of a mask). */
+enum { QD_TREE_MAX_DRAFTS = 64 };
+
+/* Checks of qd_gqa_decode_tree in order.  tree_mask undefined or NULL: one
+ * query per sequence, q [batch, q_heads, head_dim]; else q [batch, q_len,
+ * q_heads, head_dim] and tree_mask [batch, q_len] int64, q_len in [1, 64].
+ * window 0 means none; sinks needs a window. */
+int qd_gqa_decode_tree_validate(const qd_tensor_desc* q, const qd_tensor_desc* k_cache,
+                                const qd_tensor_desc* v_cache, const qd_tensor_desc* block_table,
+                                const qd_tensor_desc* context_lens, const qd_tensor_desc* tree_mask, double scale,
+                                int64_t window, int64_t sinks, char* msg, size_t msg_cap);
+
+/* Workspace bytes of qd_gqa_decode_tree (fp32 partials of contexts split
+ * over workgroups); 0 when none is needed.  16-byte aligned, no zeroing
+ * needed: every call writes what it reads.  Calls that can overlap need
+ * different workspaces.  Depends on the current device, like the launch. */
+size_t qd_gqa_decode_tree_workspace_bytes(int batch, int q_len, int q_heads, int kv_heads, int head_dim,
+                                          int block_size, int max_pages, int has_mask, int window, int sinks,
+                                          int dtype, int flags);
+
+/* What qd_gqa_decode_tree runs for these shapes on aligned tensors:
+ * QD_TREE_* or -1 for invalid shapes, with *workgroups of the attention
+ * kernel and *rows of one workgroup (queries x q-heads of a kv-head).
+ * Output pointers may be NULL. */
+enum { QD_TREE_VALU = 0, QD_TREE_MFMA = 1, QD_TREE_MFMA_SPLIT = 2 };
+int qd_gqa_decode_tree_info(int batch, int q_len, int q_heads, int kv_heads, int head_dim, int block_size,
+                            int max_pages, int has_mask, int window, int sinks, int dtype, int flags,
+                            int* workgroups, int* rows);
+
+/* out = softmax(q . k * scale) . v over the tokens that a query sees.
+ * With a mask, len = context_lens[b] tokens precede the drafted ones and
+ * drafted token j lies at token len + j of the cache.  Query t's mask m_t
+ * (bits at and above q_len are ignored) holds the drafted tokens it sees,
+ * itself among them, and puts it at position p_t = len + popcount(m_t) - 1.
+ * m_t = 0 marks padding: a zero row.  Query t sees
+ *   context token i < len    iff window == 0 or i > p_t - window or i < sinks
+ *   drafted token j          iff bit j of m_t is set, and window == 0 or
+ *                            p_j > p_t - window or p_j < sinks.
+ * Without a mask, the query is the last of len = context_lens[b] tokens
+ * (p = len - 1).  Lengths are clamped to [0, max_pages * block_size], tokens
+ * past the table are not seen, page ids are clamped to the pool; table
+ * entries of tokens that no query of the sequence can see by its length,
+ * window and sinks are never read.  A query that sees nothing gets a zero
+ * row.  Whatever a token holds that a query does not see (NaN included)
+ * does not reach that query's row.
+ * flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
+int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                       const int32_t* context_lens, const int64_t* tree_mask, void* out, void* workspace,
+                       size_t workspace_bytes, int batch, int q_len, int q_heads, int kv_heads, int head_dim,
+                       int block_size, int max_pages, int64_t num_blocks, int dtype, float scale, int window,
+                       int sinks, int flags, void* stream);
+
+/* Checks of qd_qk_norm_rope_write in order.  `contiguous` of q, key and value
+ * means that the rows of one token are ([heads, head_dim] row-major; tokens
+ * may lie any stride apart).  q_weight and k_weight may be NULL or undefined
+ * (no norm); weight dtype is q's or float32, the same for both. */
+int qd_qk_norm_rope_write_validate(const qd_tensor_desc* q, const qd_tensor_desc* key, const qd_tensor_desc* value,
+                                   const qd_tensor_desc* cos_sin, const qd_tensor_desc* positions,
+                                   const qd_tensor_desc* k_cache, const qd_tensor_desc* v_cache,
+                                   const qd_tensor_desc* slots, const qd_tensor_desc* q_weight,
+                                   const qd_tensor_desc* k_weight, double eps, char* msg, size_t msg_cap);
+
+/* For every token n: y = x * rsqrt(mean(x^2) + eps) * weight over each head of
+ * q and key (weights NULL: y = x), then the first rotary_dim elements turned
+ * by cos_sin[positions[n]] = {cos[rotary_dim / 2], sin[rotary_dim / 2]}
+ * (float32 [max_positions, rotary_dim]): pairs (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) when `interleaved`, (a, b) -> (a cos - b sin, b cos + a sin).
+ * fp32 arithmetic, one rounding.  q goes to q_out [tokens, q_heads, head_dim]
+ * (contiguous), key and value to flat row slots[n] of the caches [cache_rows,
+ * kv_heads, head_dim].  q_stride, k_stride and v_stride are the elements from
+ * one token to the next.  Slots must be distinct; one outside [0, cache_rows)
+ * is skipped.  A position outside the table gives a zero q row and writes
+ * nothing to the caches. */
+int qd_qk_norm_rope_write(const void* q, const void* key, const void* value, const float* cos_sin,
+                          const int32_t* positions, void* k_cache, void* v_cache, const int64_t* slots,
+                          const void* q_weight, const void* k_weight, void* q_out, int64_t tokens, int q_heads,
+                          int kv_heads, int head_dim, int rotary_dim, int64_t q_stride, int64_t k_stride,
+                          int64_t v_stride, int64_t max_positions, int64_t cache_rows, int dtype, int weight_dtype,
+                          float eps, int interleaved, void* stream);
+
+/* Checks of qd_kv_compact in order, on the first of the caches (all have one
+ * shape) and the metadata. */
+int qd_kv_compact_validate(const qd_tensor_desc* cache, const qd_tensor_desc* block_table,
+                           const qd_tensor_desc* context_lens, const qd_tensor_desc* accepted, char* msg,
+                           size_t msg_cap);
+
+/* Moves, in every one of num_caches caches [num_blocks, block_size, row]
+ * (row_bytes each row; K and V of any layers, or latent caches), token
+ * context_lens[b] + accepted[b][i] to token context_lens[b] + i, for every i
+ * in [0, count) with accepted[b][i] >= 0, as if all rows were read before any
+ * is written.  count <= 64.  Tokens past the table, page ids outside the pool
+ * and negative lengths are skipped (nothing is read or written).  `caches` is
+ * a host array of device pointers, read during the call; the caches must not
+ * overlap (checked). */
+int qd_kv_compact(void* const* caches, int num_caches, const int32_t* block_table, const int32_t* context_lens,
+                  const int32_t* accepted, int batch, int count, int block_size, int max_pages, int64_t num_blocks,
+                  int64_t row_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
