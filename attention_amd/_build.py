@@ -59,7 +59,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(out, flush=True)
 
 
-HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla", "tree_decode", "qk_norm_rope", "kv_compact"]
+HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla", "tree_decode", "tree_mfma_bf16", "tree_mfma_f16",
+               "tree_mfma_f32", "qk_norm_rope", "kv_compact"]
 TORCH_SOURCES = ["torch_ops", "serving_ops"]
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 
@@ -87,6 +88,8 @@ def _stale(name: str) -> bool:
         return True
     deps = [os.path.join(CSRC, f"{name}.hip"), os.path.join(CSRC, "qd_device.h"),
             os.path.join(INCLUDE, "qd_attention.h")]
+    if name.startswith("tree_"):
+        deps.append(os.path.join(CSRC, "tree_kernels.h"))
     return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 
 

@@ -16,88 +16,14 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
-#include "qd_attention.h"
-#include "qd_device.h"
+#include "tree_kernels.h"
 
 void qd_set_last_error(int status, const std::string& msg);
 
 namespace {
-
-struct TreeParams {
-  const void* q;
-  const void* k;
-  const void* v;
-  const int32_t* table;
-  const int32_t* lens;
-  const int64_t* mask;  // null: one query per sequence, the last of its tokens
-  void* out;
-  float* part;          // partials of split contexts
-  int B, T, Hq, Hkv, D, P, maxP;
-  int64_t num_blocks;
-  int window, sinks;
-  float sl2;  // scale * log2(e)
-  int splits;
-};
-
-// Tokens of sequence b in its table.
-__device__ __forceinline__ int context_len(const TreeParams& p, int b) {
-  const int64_t cap = static_cast<int64_t>(p.maxP) * p.P;
-  const int64_t len = max(p.lens[b], 0);
-  return static_cast<int>(len < cap ? len : cap);
-}
-
-__device__ __forceinline__ uint64_t draft_bits(const TreeParams& p, int b, int t) {
-  const uint64_t m = static_cast<uint64_t>(p.mask[static_cast<int64_t>(b) * p.T + t]);
-  return p.T >= 64 ? m : m & ((uint64_t{1} << p.T) - 1);
-}
-
-// What query t of sequence b sees: context tokens [0, sinks) and [lo, len),
-// sinks <= lo <= len, and drafted token j (token len + j) where bit j of `seen`
-// is set.
-struct Row {
-  int len, lo, sinks;
-  uint64_t seen;
-};
-
-__device__ __forceinline__ Row row_view(const TreeParams& p, int b, int t) {
-  Row r;
-  r.len = context_len(p, b);
-  r.seen = 0;
-  int depth = -1;
-  if (p.mask) {
-    const uint64_t m = draft_bits(p, b, t);
-    if (m == 0) {  // padding
-      r.len = r.lo = r.sinks = 0;
-      return r;
-    }
-    depth = __builtin_popcountll(m) - 1;
-    // Drafted tokens past the table are not seen.
-    const int64_t room = static_cast<int64_t>(p.maxP) * p.P - r.len;
-    r.seen = room >= 64 ? m : room > 0 ? m & ((uint64_t{1} << room) - 1) : 0;
-    // The window hides drafted tokens only where it is shorter than a path.
-    if (p.window > 0 && p.window <= depth + 1)
-      for (uint64_t left = r.seen; left; left &= left - 1) {
-        const int j = __builtin_ctzll(left);
-        const int dj = __builtin_popcountll(draft_bits(p, b, j)) - 1;
-        if (dj <= depth - p.window && r.len + static_cast<int64_t>(dj) >= p.sinks) r.seen &= ~(uint64_t{1} << j);
-      }
-  }
-  int64_t lo = p.window > 0 ? static_cast<int64_t>(r.len) + depth - p.window + 1 : 0;
-  lo = lo < 0 ? 0 : lo;
-  r.lo = static_cast<int>(lo < r.len ? lo : r.len);
-  r.sinks = min(p.sinks, r.lo);
-  return r;
-}
-
-// Pool row of token `tok`; page ids are clamped to the pool.
-__device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok) {
-  const int page = tok / p.P;
-  int64_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page];
-  phys = phys < 0 ? 0 : phys >= p.num_blocks ? p.num_blocks - 1 : phys;
-  return phys * p.P + (tok - page * p.P);
-}
 
 // Any head_dim, alignment and type, on the VALU: a workgroup per (query head,
 // split); its four waves take 64-token blocks in turn, a lane per token for
@@ -251,6 +177,69 @@ int generic_splits(int batch, int q_len, int q_heads, int64_t capacity) {
   return static_cast<int>(std::max<int64_t>(1, std::min({want, (capacity + 511) / 512, int64_t{64}})));
 }
 
+int tree_cu_count() {
+  static std::atomic<int> cached[16];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) {
+    (void)hipGetLastError();
+    dev = 0;
+  }
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) {
+    (void)hipGetLastError();
+    return 256;  // no device: MI355X
+  }
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// How a call runs.  All from static shapes and the device.
+struct TreePlan {
+  bool mfma;
+  int splits;                                  // VALU kernel
+  int dp, nb, wr, chunks, chunk_rows, W, grid;  // matrix-core kernel
+  size_t meta_bytes, bytes;
+};
+
+// Contexts of at most this many tiles are not split over workgroups.
+constexpr int kTreeDirectTiles = 4;
+
+TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim, int block_size, int max_pages,
+                   int has_mask, int window, int sinks, int dtype, int flags) {
+  TreePlan pl{};
+  const int64_t cap = visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks);
+  pl.mfma = head_dim % 8 == 0 && !(flags & QD_FLAG_FORCE_GENERIC);
+  if (!pl.mfma) {
+    pl.splits = generic_splits(batch, q_len, q_heads, cap);
+    if (pl.splits > 1)
+      pl.bytes = sizeof(float) * static_cast<size_t>(batch) * q_len * q_heads * pl.splits * (head_dim + 2);
+    return pl;
+  }
+  const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
+  pl.dp = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 && es == 2 ? 192 : 256;
+  // Up to 128 rows per workgroup; fp32 above head_dim 128: 16, whose state is
+  // what the registers hold.
+  const int most = es == 4 && pl.dp == 256 ? 16 : 128;
+  const int R = q_len * (q_heads / kv_heads);
+  pl.chunks = (R + most - 1) / most;
+  pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
+  pl.nb = pl.chunk_rows <= 16 ? 1 : 2;
+  pl.wr = pl.chunk_rows <= 32 ? 1 : pl.chunk_rows <= 64 ? 2 : 4;
+  const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
+  const int64_t tiles = (cap + kTreeTile - 1) / kTreeTile;
+  if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced) {
+    pl.grid = static_cast<int>(items);
+    return pl;
+  }
+  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(es, pl.dp, pl.nb, pl.wr);
+  pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / kTreeMinCost)));
+  pl.grid = pl.W;
+  pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;
+  pl.bytes = pl.meta_bytes + sizeof(float) * 2 * static_cast<size_t>(pl.W) * (16 * pl.nb * pl.wr) * (head_dim + 2);
+  return pl;
+}
+
 template <int DT>
 void launch_generic(const TreeParams& p, hipStream_t st) {
   const uint32_t rows = static_cast<uint32_t>(p.B * p.T * p.Hq);
@@ -328,27 +317,29 @@ int qd_gqa_decode_tree_validate(const qd_tensor_desc* q, const qd_tensor_desc* k
 size_t qd_gqa_decode_tree_workspace_bytes(int batch, int q_len, int q_heads, int kv_heads, int head_dim,
                                           int block_size, int max_pages, int has_mask, int window, int sinks,
                                           int dtype, int flags) {
-  (void)flags;
   if (!tree_shape_ok(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window, sinks, dtype))
     return 0;
-  const int splits =
-      generic_splits(batch, q_len, q_heads, visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks));
-  if (splits == 1) return 0;
-  return sizeof(float) * static_cast<size_t>(batch) * q_len * q_heads * splits * (head_dim + 2);
+  if (batch == 0) return 0;
+  const size_t bytes = tree_plan(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window,
+                                 sinks, dtype, flags)
+                           .bytes;
+  if (flags & QD_FLAG_FORCE_GENERIC) return bytes;
+  // Unaligned tensors take the VALU kernel.
+  return std::max(bytes, tree_plan(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window,
+                                   sinks, dtype, flags | QD_FLAG_FORCE_GENERIC)
+                             .bytes);
 }
 
 int qd_gqa_decode_tree_info(int batch, int q_len, int q_heads, int kv_heads, int head_dim, int block_size,
                             int max_pages, int has_mask, int window, int sinks, int dtype, int flags,
                             int* workgroups, int* rows) {
-  (void)flags;
   if (!tree_shape_ok(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window, sinks, dtype))
     return -1;
-  if (workgroups)
-    *workgroups = batch * q_len * q_heads *
-                  generic_splits(batch, q_len, q_heads,
-                                 visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks));
-  if (rows) *rows = 1;
-  return QD_TREE_VALU;
+  const TreePlan pl = tree_plan(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window,
+                                sinks, dtype, flags);
+  if (workgroups) *workgroups = pl.mfma ? pl.grid : batch * q_len * q_heads * pl.splits;
+  if (rows) *rows = pl.mfma ? pl.chunk_rows : 1;
+  return !pl.mfma ? QD_TREE_VALU : pl.W > 0 ? QD_TREE_MFMA_SPLIT : QD_TREE_MFMA;
 }
 
 int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -365,9 +356,13 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   if (batch == 0) return QD_OK;
   if (!q || !k_cache || !v_cache || !block_table || !context_lens || !out)
     return tree_fail(nullptr, 0, "null tensor pointer");
-  const size_t need = qd_gqa_decode_tree_workspace_bytes(batch, q_len, q_heads, kv_heads, head_dim, block_size,
-                                                         max_pages, has_mask, window, sinks, dtype, flags);
-  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+        reinterpret_cast<uintptr_t>(out)) &
+       15u) != 0)
+    flags |= QD_FLAG_FORCE_GENERIC;
+  const TreePlan pl = tree_plan(batch, q_len, q_heads, kv_heads, head_dim, block_size, max_pages, has_mask, window,
+                                sinks, dtype, flags);
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return tree_fail(nullptr, 0, "workspace too small or not 16-byte aligned");
   TreeParams p;
   p.q = q;
@@ -377,7 +372,8 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   p.lens = context_lens;
   p.mask = tree_mask;
   p.out = out;
-  p.part = static_cast<float*>(workspace);
+  p.meta = static_cast<int32_t*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.meta_bytes);
   p.B = batch;
   p.T = q_len;
   p.Hq = q_heads;
@@ -389,16 +385,29 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   p.window = window;
   p.sinks = sinks;
   p.sl2 = scale * kLog2e;
-  p.splits =
-      generic_splits(batch, q_len, q_heads, visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks));
+  p.splits = pl.splits;
+  p.G = q_heads / kv_heads;
+  p.R = q_len * p.G;
+  p.chunks = pl.chunks;
+  p.chunk_rows = pl.chunk_rows;
+  p.W = pl.W;
+  p.pshift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
-  switch (dtype) {
-    case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;
-    case QD_DTYPE_F16: launch_generic<QD_DTYPE_F16>(p, st); break;
-    default: launch_generic<QD_DTYPE_BF16>(p, st); break;
+  hipError_t e = hipSuccess;
+  if (pl.mfma) {
+    const auto run = dtype == QD_DTYPE_F32   ? qd_tree_mfma_launch_f32
+                     : dtype == QD_DTYPE_F16 ? qd_tree_mfma_launch_f16
+                                             : qd_tree_mfma_launch_bf16;
+    e = static_cast<hipError_t>(run(p, pl.dp, pl.nb, pl.wr, pl.grid, stream));
+  } else {
+    switch (dtype) {
+      case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;
+      case QD_DTYPE_F16: launch_generic<QD_DTYPE_F16>(p, st); break;
+      default: launch_generic<QD_DTYPE_BF16>(p, st); break;
+    }
+    e = hipGetLastError();
   }
-  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     qd_set_last_error(static_cast<int>(e),
                       std::string("gqa_decode_tree kernel launch failed: ") + hipGetErrorString(e));

@@ -1,0 +1,802 @@
+// Device code of windowed and tree decode shared by the VALU kernel
+// (tree_decode.hip) and the matrix-core kernels (tree_mfma_*.hip): what a query
+// sees, and the matrix-core kernel itself.  Everything lives in an anonymous
+// namespace, so each translation unit keeps its own copy.
+#ifndef QD_TREE_KERNELS_H
+#define QD_TREE_KERNELS_H
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "qd_attention.h"
+#include "qd_device.h"
+
+// Arguments of the matrix-core kernels, passed between translation units.
+struct TreeParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* table;
+  const int32_t* lens;
+  const int64_t* mask;  // null: one query per sequence, the last of its tokens
+  void* out;
+  float* part;          // partials of split contexts
+  int32_t* meta;        // matrix-core kernel: {first workgroup, workgroups} per item
+  int B, T, Hq, Hkv, D, P, maxP;
+  int64_t num_blocks;
+  int window, sinks;
+  float sl2;  // scale * log2(e)
+  int splits;    // VALU kernel: context splits
+  int G, R;      // q-heads per kv-head, rows (queries x G) per (sequence, kv-head)
+  int chunks;    // workgroups that share a (sequence, kv-head)'s rows
+  int chunk_rows;
+  int W;         // workgroups of a balanced launch; 0: one per item
+  int pshift;    // log2(P), or -1
+};
+
+// Runs the matrix-core kernel for padded head_dim dp and 16 nb wr rows per
+// workgroup (tree_mfma_*.hip); grid workgroups.  Returns a hipError_t.
+int qd_tree_mfma_launch_f32(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
+int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
+int qd_tree_mfma_launch_bf16(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
+
+namespace {
+
+// Tokens of a table row; the last 256 below 2^31 are left out, so that token
+// numbers and their tiles fit 32 bits.
+__device__ __forceinline__ int64_t capacity(const TreeParams& p) {
+  return min(static_cast<int64_t>(p.maxP) * p.P, static_cast<int64_t>(INT32_MAX - 255));
+}
+
+// Tokens of sequence b in its table.
+__device__ __forceinline__ int context_len(const TreeParams& p, int b) {
+  const int64_t cap = capacity(p);
+  const int64_t len = max(p.lens[b], 0);
+  return static_cast<int>(len < cap ? len : cap);
+}
+
+__device__ __forceinline__ uint64_t draft_bits(const TreeParams& p, int b, int t) {
+  const uint64_t m = static_cast<uint64_t>(p.mask[static_cast<int64_t>(b) * p.T + t]);
+  return p.T >= 64 ? m : m & ((uint64_t{1} << p.T) - 1);
+}
+
+// What query t of sequence b sees: context tokens [0, sinks) and [lo, len),
+// sinks <= lo <= len, and drafted token j (token len + j) where bit j of `seen`
+// is set.
+struct Row {
+  int len, lo, sinks;
+  uint64_t seen;
+};
+
+__device__ __forceinline__ Row row_view(const TreeParams& p, int b, int t) {
+  Row r;
+  r.len = context_len(p, b);
+  r.seen = 0;
+  int depth = -1;
+  if (p.mask) {
+    const uint64_t m = draft_bits(p, b, t);
+    if (m == 0) {  // padding
+      r.len = r.lo = r.sinks = 0;
+      return r;
+    }
+    depth = __builtin_popcountll(m) - 1;
+    // Drafted tokens past the table are not seen.
+    const int64_t room = capacity(p) - r.len;
+    r.seen = room >= 64 ? m : room > 0 ? m & ((uint64_t{1} << room) - 1) : 0;
+    // The window hides drafted tokens only where it is shorter than a path.
+    if (p.window > 0 && p.window <= depth + 1)
+      for (uint64_t left = r.seen; left; left &= left - 1) {
+        const int j = __builtin_ctzll(left);
+        const int dj = __builtin_popcountll(draft_bits(p, b, j)) - 1;
+        if (dj <= depth - p.window && r.len + static_cast<int64_t>(dj) >= p.sinks) r.seen &= ~(uint64_t{1} << j);
+      }
+  }
+  int64_t lo = p.window > 0 ? static_cast<int64_t>(r.len) + depth - p.window + 1 : 0;
+  lo = lo < 0 ? 0 : lo;
+  r.lo = static_cast<int>(lo < r.len ? lo : r.len);
+  r.sinks = min(p.sinks, r.lo);
+  return r;
+}
+
+// Pool row of token `tok`; page ids are clamped to the pool.
+__device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok) {
+  const int page = p.pshift >= 0 ? tok >> p.pshift : tok / p.P;
+  int64_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page];
+  phys = phys < 0 ? 0 : phys >= p.num_blocks ? p.num_blocks - 1 : phys;
+  return phys * p.P + (tok - page * p.P);
+}
+
+
+// ----------------------------------------------------------------------------
+// The matrix-core kernel
+// ----------------------------------------------------------------------------
+//
+// An item is a (sequence, kv-head, chunk of its rows); a row is a (query,
+// q-head of the kv-head's group).  A workgroup of four waves goes through an
+// item's virtual tokens in tiles of 64: all waves load the tile's K and V rows
+// (registers, one tile ahead, then LDS), and wave (wr, wt) multiplies row
+// blocks [16 NB wr, 16 NB (wr + 1)) with tokens [64 / WT wt, ...):
+//   scores   S^T = K Q^T, 16x16 blocks (A = K rows from LDS, B = Q from
+//            registers): a lane holds one row and 4 tokens per block
+//   softmax  per lane; the reference maximum of a row moves only when a score
+//            exceeds it by 2^8, so most tiles exchange nothing between lanes
+//   output   O^T += V^T P^T: the score layout is already the B operand, V^T
+//            comes from transposing LDS reads.  16-bit weights go in as two
+//            parts (split2): one rounding would add an error as large as the
+//            output's own.
+// Waves that share rows (WT > 1) merge at the end of an item through LDS.
+
+constexpr int kTreeTile = 64;
+// Balanced launches: an item costs its tiles and one more (its queries, first
+// round trips and stores take about as long).
+constexpr int kTreeItemCost = 1;
+// Least cost of a workgroup's range: shorter ones gain less than their
+// partials cost.
+constexpr int kTreeMinCost = 4;
+// Sequences whose prefix of costs fits the kernel's LDS.
+constexpr int kTreeMaxBalanced = 1024;
+
+// Bytes of LDS and resident workgroups per CU of an instance; es: element size.
+__host__ __device__ constexpr int tree_lds_bytes(int es, int dp, int bufs) {
+  return bufs * kTreeTile * (2 * dp * es + 16 + (es == 2 ? 32 : 16)) + 32;
+}
+__host__ __device__ constexpr int tree_bufs(int es, int dp) { return tree_lds_bytes(es, dp, 2) <= 150 * 1024 ? 2 : 1; }
+__host__ __device__ constexpr int tree_occupancy(int es, int dp, int nb, int wr) {
+  // Registers: O, Q, the staged tile, scores and weights.
+  const int steps = dp * es / 64, pass = dp * es / 64, blocks = wr;  // token blocks: 4 / (4 / wr)
+  const int regs = 4 * nb * (dp / 16) + 4 * nb * steps + 8 * pass + 8 * blocks * nb;
+  const int by_regs = regs > 190 ? 1 : regs > 90 ? 2 : regs > 64 ? 3 : 4;
+  const int by_lds = 160 * 1024 / (tree_lds_bytes(es, dp, tree_bufs(es, dp)) + 8 * kTreeMaxBalanced);
+  return by_lds < by_regs ? (by_lds < 1 ? 1 : by_lds) : by_regs;
+}
+
+template <int DT, int DP, int NB, int WR>
+struct TreeShape {
+  static constexpr int kWT = 4 / WR;
+  static constexpr int kES = DT == QD_DTYPE_F32 ? 4 : 2;
+  static constexpr int kRow = DP * kES;                      // bytes of a head's row, padded
+  // Row strides in LDS: rows 16 bytes (K) and 32 bytes (V, two lanes' worth of
+  // a transposing read) further round the 64 banks each.
+  static constexpr int kKS = kRow + 16;
+  static constexpr int kVS = kRow + (kES == 2 ? 32 : 16);
+  static constexpr int kBuf = kTreeTile * (kKS + kVS);
+  static constexpr int kBufs = tree_bufs(kES, DP);
+  static constexpr int kChunks = kRow / 16;                  // 16-byte chunks of a row
+  static constexpr int kPass = kChunks / 4;                  // a wave loads 16 rows
+  static constexpr int kSteps = kRow / 64;
+  static constexpr int kTW = kTreeTile / kWT;                // tokens of a wave in a tile
+  static constexpr int kTB = kTW / 16;
+  static constexpr int kCols = DP / 16;
+  static constexpr int kRows = 16 * NB * WR;                 // rows of a workgroup
+  static constexpr int kCtl = 32;                            // three words of tokens with non-finite values
+  static constexpr int kLds = tree_lds_bytes(kES, DP, kBufs);
+  static constexpr int kOcc = tree_occupancy(kES, DP, NB, WR);
+};
+
+__device__ __forceinline__ float tree_max_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float tree_sum_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Workgroup barrier that waits for LDS traffic only: the tile being loaded
+// into registers stays in flight.
+__device__ __forceinline__ void tree_barrier() {
+  constexpr int imm = 0x3F | (0x3 << 14) | (0x7 << 4) | (0x0 << 8);  // vmcnt max, lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(imm);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Four transposed 16-bit elements: lane (g4, r16) of the wave gets column r16
+// of the 4 x 16 block whose row r16 / 4, columns 4 (r16 % 4).. this lane
+// addresses.
+__device__ __forceinline__ u32x2 tree_tr_read(const char* p) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+}
+
+template <int DT>
+__device__ __forceinline__ bool chunk_not_finite(u32x4 x) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == QD_DTYPE_F32) {
+      bad |= (x[i] & 0x7F800000u) == 0x7F800000u;
+    } else {
+      constexpr uint32_t e = DT == QD_DTYPE_F16 ? 0x7C00u : 0x7F80u;
+      bad |= (x[i] & e) == e || ((x[i] >> 16) & e) == e;
+    }
+  }
+  return bad;
+}
+
+// Tokens [0, sinks) and [lo, len) and nd drafted ones of an item: what its
+// rows see at most.
+struct Span {
+  int len, lo, sinks, nd, n;
+};
+
+__device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
+  Span s;
+  s.len = context_len(p, b);
+  s.nd = p.mask ? static_cast<int>(min(static_cast<int64_t>(p.T), capacity(p) - s.len)) : 0;
+  // The first query's window is the earliest: position len, or len - 1
+  // without a mask.
+  const int64_t lo = p.window > 0 ? static_cast<int64_t>(s.len) + (p.mask ? 1 : 0) - p.window : 0;
+  s.lo = static_cast<int>(lo < 0 ? 0 : lo < s.len ? lo : s.len);
+  s.sinks = min(p.sinks, s.lo);
+  s.n = s.sinks + s.len - s.lo + s.nd;
+  return s;
+}
+
+__device__ __forceinline__ int span_tiles(const Span& s) { return (s.n + kTreeTile - 1) / kTreeTile; }
+
+template <int DT, int DP, int NB, int WR>
+__global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_mfma_kernel(TreeParams p) {
+  using Sh = TreeShape<DT, DP, NB, WR>;
+  using E = Elem<DT>;
+  using S = typename E::S;
+  constexpr bool k16 = DT != QD_DTYPE_F32;
+  constexpr int WT = Sh::kWT, TB = Sh::kTB, ES = Sh::kES;
+  // fp16 weights up to 2^8 above the reference maximum's stay below 2^15, and
+  // their low parts above the smallest subnormal.
+  constexpr float kShift = DT == QD_DTYPE_F16 ? 7.f : 0.f;
+  constexpr float kLazy = 8.f;
+  extern __shared__ __align__(16) char smem[];
+  uint64_t* bad_words = reinterpret_cast<uint64_t*>(smem + Sh::kBufs * Sh::kBuf);
+  int64_t* incl = reinterpret_cast<int64_t*>(smem + Sh::kLds);
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  const int wr = wv / WT, wt = wv % WT;
+  const int per_seq = p.Hkv * p.chunks;
+  const int row_bytes = p.D * ES;
+
+  auto process = [&](int b, int hc, const Span& sp, int t0, int t1, bool whole, int64_t slot) {
+    const int h = hc / p.chunks;
+    const int row0 = (hc % p.chunks) * p.chunk_rows;
+    const int rows = min(p.chunk_rows, p.R - row0);
+    const int q0 = row0 / p.G, q1 = (row0 + rows - 1) / p.G;  // the chunk's queries
+    // Lane t: what query q0 + t sees (at most 64 queries).
+    Row mine;
+    mine.len = mine.lo = mine.sinks = 0;
+    mine.seen = 0;
+    bool sees = false;
+    if (q0 + lane <= q1) {
+      sees = !p.mask || draft_bits(p, b, q0 + lane) != 0;
+      if (sees) mine = row_view(p, b, q0 + lane);
+    }
+    uint64_t any_seen = mine.seen;
+    int lo_max = sees ? mine.lo : 0;
+    for (int off = 32; off >= 1; off >>= 1) {
+      any_seen |= static_cast<uint64_t>(__shfl_xor(static_cast<long long>(any_seen), off));
+      lo_max = max(lo_max, __shfl_xor(lo_max, off));
+    }
+    // This lane's rows.
+    bool active[NB];
+    int lo[NB], sinks[NB];
+    uint64_t seen[NB];
+    int64_t q_at[NB];  // element offset of the row in q and out, -1: no such row
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int rr = 16 * (NB * wr + nb) + r16;
+      const int row = row0 + (rr < rows ? rr : 0);
+      const int t = row / p.G;
+      const int src = t - q0;
+      active[nb] = rr < rows && __shfl(static_cast<int>(sees), src) != 0;
+      lo[nb] = __shfl(mine.lo, src);
+      sinks[nb] = __shfl(mine.sinks, src);
+      seen[nb] = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), src));
+      q_at[nb] = rr < rows
+                     ? ((static_cast<int64_t>(b) * p.T + t) * p.Hq + static_cast<int64_t>(h) * p.G + (row - t * p.G)) * p.D
+                     : -1;
+    }
+    u32x4 qf[NB][Sh::kSteps];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int s = 0; s < Sh::kSteps; ++s) {
+        const int at = 64 * s + 16 * g4;
+        qf[nb][s] = q_at[nb] >= 0 && at < row_bytes
+                        ? *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.q) + q_at[nb] * ES + at)
+                        : u32x4{0u, 0u, 0u, 0u};
+      }
+    f32x4 acc[Sh::kCols][NB];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = -INFINITY;
+      l[nb] = 0.f;
+#pragma unroll
+      for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int context = sp.sinks + sp.len - sp.lo;
+    auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
+    // Lane's staged row of a tile: row 16 wv + r16.  Its page, looked up a
+    // tile ahead of the loads.
+    auto staged = [&](int tile) { return kTreeTile * tile + 16 * wv + r16; };
+    auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
+    auto row_seen = [&](int v) { return v < context || (v < sp.n && ((any_seen >> (v - context)) & 1)); };
+    auto look_up = [&](int tile) -> int32_t {
+      const int v = staged(tile);
+      if (!row_seen(v)) return -1;
+      const int32_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page_of(token(v))];
+      return phys < 0 ? 0 : phys;
+    };
+    auto offset_of = [&](int tile, int32_t phys) -> int64_t {  // bytes, -1: not read
+      if (phys < 0) return -1;
+      const int tok = token(staged(tile));
+      const int64_t page = phys < p.num_blocks ? phys : p.num_blocks - 1;
+      return ((page * p.P + (tok - page_of(tok) * p.P)) * p.Hkv + h) * row_bytes;
+    };
+    u32x4 kreg[Sh::kPass], vreg[Sh::kPass];
+    auto load = [&](int64_t off) {
+#pragma unroll
+      for (int i = 0; i < Sh::kPass; ++i) {
+        const int c = 64 * i + lane;
+        const int row = c / Sh::kChunks, chunk = c % Sh::kChunks;
+        const int64_t at = __shfl(static_cast<long long>(off), row);
+        kreg[i] = vreg[i] = u32x4{0u, 0u, 0u, 0u};
+        if (at >= 0 && 16 * chunk < row_bytes) {
+          kreg[i] = stream_load16(static_cast<const char*>(p.k) + at + 16 * chunk);
+          vreg[i] = stream_load16(static_cast<const char*>(p.v) + at + 16 * chunk);
+        }
+      }
+    };
+    // Every row of the chunk sees all (existing) tokens of the tile.
+    auto uniform = [&](int tile) {
+      const int a = kTreeTile * tile, e = a + kTreeTile;
+      return e <= sp.sinks || (a >= sp.sinks + max(lo_max - sp.lo, 0) && e <= context) || (q0 == q1 && e <= sp.n);
+    };
+
+    tree_barrier();  // the previous item's merge and the prefix are done with LDS
+    if (tid < 3) bad_words[tid] = 0;
+    int32_t page = -1;
+    if (t0 < t1) {
+      page = look_up(t0);
+      load(offset_of(t0, page));
+    }
+    if (t0 + 1 < t1) page = look_up(t0 + 1);
+    tree_barrier();
+    for (int tile = t0; tile < t1; ++tile) {
+      const int turn = tile - t0;
+      char* buf = smem + (Sh::kBufs == 2 ? (turn & 1) * Sh::kBuf : 0);
+      const bool whole_tile = uniform(tile);
+      const bool mixed = !whole_tile && q0 != q1;
+      if (Sh::kBufs == 1 && turn > 0) tree_barrier();
+#pragma unroll
+      for (int i = 0; i < Sh::kPass; ++i) {
+        const int c = 64 * i + lane;
+        const int row = 16 * wv + c / Sh::kChunks, chunk = c % Sh::kChunks;
+        if (mixed && chunk_not_finite<DT>(vreg[i])) {
+          // A weight of 0 would not hide this value from the rows that do not
+          // see the token: it is added for the others below.
+          atomicOr(reinterpret_cast<unsigned long long*>(&bad_words[turn % 3]), 1ull << row);
+          vreg[i] = u32x4{0u, 0u, 0u, 0u};
+        }
+        *reinterpret_cast<u32x4*>(buf + row * Sh::kKS + 16 * chunk) = kreg[i];
+        *reinterpret_cast<u32x4*>(buf + kTreeTile * Sh::kKS + row * Sh::kVS + 16 * chunk) = vreg[i];
+      }
+      if (tid == 0) bad_words[(turn + 1) % 3] = 0;
+      if (tile + 1 < t1) {
+        load(offset_of(tile + 1, page));
+        if (tile + 2 < t1) page = look_up(tile + 2);
+      }
+      tree_barrier();
+
+      const char* kb = buf + (Sh::kTW * wt + r16) * Sh::kKS + 16 * g4;
+      f32x4 s[TB][NB];
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < Sh::kSteps; ++st)
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(kb + 16 * tb * Sh::kKS + 64 * st);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if constexpr (k16) {
+              s[tb][nb] = MfmaOps<DT>::mma32(a, qf[nb][st], s[tb][nb]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                s[tb][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(qf[nb][st][j]),
+                                                                 s[tb][nb], 0, 0, 0);
+            }
+          }
+        }
+      const int v0 = kTreeTile * tile + Sh::kTW * wt + 4 * g4;
+      auto visible = [&](int v, int nb) {
+        if (v >= context) return v < sp.n && ((seen[nb] >> (v - context)) & 1) != 0;
+        const int tok = token(v);
+        return tok < sinks[nb] || tok >= lo[nb];
+      };
+      if (!whole_tile) {
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              if (!visible(v0 + 16 * tb + i, nb)) s[tb][nb][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[tb][nb][i]);
+        if (__ballot(mx * p.sl2 > m[nb] + kLazy)) {
+          const float mn = fmaxf(m[nb], tree_max_groups(mx) * p.sl2);
+          const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
+          m[nb] = mn;
+          l[nb] *= alpha;
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= alpha;
+        }
+        const float ref = m[nb] == -INFINITY ? -kShift : m[nb] - kShift;
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = fast_exp2(fmaf(s[tb][nb][i], p.sl2, -ref));
+            s[tb][nb][i] = w;
+            l[nb] += w;
+          }
+      }
+      const char* vb = buf + kTreeTile * Sh::kKS + Sh::kTW * wt * Sh::kVS;
+      if constexpr (k16) {
+        u32x2 hi[TB][NB], lw[TB][NB];
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a, c;
+              MfmaOps<DT>::split2(s[tb][nb][2 * i], s[tb][nb][2 * i + 1], a, c);
+              hi[tb][nb][i] = a;
+              lw[tb][nb][i] = c;
+            }
+        // Masked weights are 0; split2's low part never is, which adds at
+        // most 2^-133 (bf16) or 2^-24 of 2^7 (fp16) of a masked value: none of
+        // the values in LDS is other than finite then, and where the tile is
+        // masked the low part is cleared.
+        if (!whole_tile) {
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+        const char* va = vb + (4 * g4 + (r16 >> 2)) * Sh::kVS + 8 * (r16 & 3);
+#pragma unroll
+        for (int c = 0; c < Sh::kCols; ++c) {
+          if constexpr (TB == 1) {
+            const u32x2 a = tree_tr_read(va + 32 * c);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              acc[c][nb] = MfmaOps<DT>::pv(a, hi[0][nb], acc[c][nb]);
+              acc[c][nb] = MfmaOps<DT>::pv(a, lw[0][nb], acc[c][nb]);
+            }
+          } else {
+#pragma unroll
+            for (int tb = 0; tb < TB; tb += 2) {
+              const u32x2 a0 = tree_tr_read(va + 16 * tb * Sh::kVS + 32 * c);
+              const u32x2 a1 = tree_tr_read(va + 16 * (tb + 1) * Sh::kVS + 32 * c);
+              const u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                acc[c][nb] = MfmaOps<DT>::mma32(a, u32x4{hi[tb][nb][0], hi[tb][nb][1], hi[tb + 1][nb][0], hi[tb + 1][nb][1]},
+                                                acc[c][nb]);
+                acc[c][nb] = MfmaOps<DT>::mma32(a, u32x4{lw[tb][nb][0], lw[tb][nb][1], lw[tb + 1][nb][0], lw[tb + 1][nb][1]},
+                                                acc[c][nb]);
+              }
+            }
+          }
+        }
+      } else {
+        const char* va = vb + 4 * g4 * Sh::kVS + 4 * r16;
+#pragma unroll
+        for (int c = 0; c < Sh::kCols; ++c)
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float a = *reinterpret_cast<const float*>(va + (16 * tb + i) * Sh::kVS + 64 * c);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                acc[c][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[tb][nb][i], acc[c][nb], 0, 0, 0);
+            }
+      }
+      if (mixed) {
+        // Non-finite values that some rows see: their products, one token
+        // after the other, for the rows that do.
+        uint64_t bad = bad_words[turn % 3] >> (Sh::kTW * wt);
+        if (Sh::kTW < 64) bad &= (uint64_t{1} << (Sh::kTW & 63)) - 1;
+        bad = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad), 0));
+        while (bad) {
+          const int x = __builtin_ctzll(bad);
+          bad &= bad - 1;
+          const int v = kTreeTile * tile + Sh::kTW * wt + x;
+          const int64_t at = (pool_row(p, b, token(v)) * p.Hkv + h) * row_bytes;
+          float w[NB];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float mine_w = 0.f;
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (x / 16 == tb && x % 4 == i) mine_w = s[tb][nb][i];
+            w[nb] = __shfl(mine_w, 16 * ((x % 16) / 4) + r16);
+          }
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c) {
+            const int byte = (16 * c + 4 * g4) * ES;
+            if (byte >= row_bytes) continue;
+            const char* src = static_cast<const char*>(p.v) + at;
+            if (!chunk_not_finite<DT>(*reinterpret_cast<const u32x4*>(src + (byte & ~15)))) continue;
+            const S* val = reinterpret_cast<const S*>(src + byte);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              if (visible(v, nb))
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[c][nb][i] += w[nb] * E::to_f(val[i]);
+          }
+        }
+      }
+    }
+
+    // The waves' parts of the same rows.
+    if constexpr (WT > 1) {
+      tree_barrier();
+      constexpr int kPart = NB * Sh::kCols * 1024 + NB * 512;  // acc, m, l of a wave
+      char* base = smem + (wr * (WT - 1) + wt - 1) * kPart;
+      if (wt > 0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c)
+            *reinterpret_cast<f32x4*>(base + (nb * Sh::kCols + c) * 1024 + 16 * lane) = acc[c][nb];
+          *reinterpret_cast<f32x2*>(base + NB * Sh::kCols * 1024 + nb * 512 + 8 * lane) = f32x2{m[nb], l[nb]};
+        }
+      }
+      tree_barrier();
+      if (wt == 0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float mx = m[nb];
+          f32x2 ml[WT];
+#pragma unroll
+          for (int w = 1; w < WT; ++w) {
+            const char* part = smem + (wr * (WT - 1) + w - 1) * kPart;
+            ml[w] = *reinterpret_cast<const f32x2*>(part + NB * Sh::kCols * 1024 + nb * 512 + 8 * lane);
+            mx = fmaxf(mx, ml[w][0]);
+          }
+          const float ref = mx == -INFINITY ? 0.f : mx;
+          float f = mx == m[nb] && mx != -INFINITY ? 1.f : fast_exp2(m[nb] - ref);
+          l[nb] *= f;
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= f;
+#pragma unroll
+          for (int w = 1; w < WT; ++w) {
+            const char* part = smem + (wr * (WT - 1) + w - 1) * kPart;
+            f = fast_exp2(ml[w][0] - ref);
+            l[nb] += f * ml[w][1];
+#pragma unroll
+            for (int c = 0; c < Sh::kCols; ++c)
+              acc[c][nb] += f * *reinterpret_cast<const f32x4*>(part + (nb * Sh::kCols + c) * 1024 + 16 * lane);
+          }
+          m[nb] = mx;
+        }
+      }
+    }
+    if (wt == 0) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float sum = tree_sum_groups(l[nb]);
+        const bool has = active[nb] && (sum > 0.f || sum != sum);
+        if (q_at[nb] < 0) continue;
+        const int rr = 16 * (NB * wr + nb) + r16;
+        if (whole) {
+          const float inv = has ? 1.f / sum : 0.f;
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c) {
+            const int d = 16 * c + 4 * g4;
+            if (d >= p.D) continue;
+            const f32x4 y = has ? acc[c][nb] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+            char* dst = static_cast<char*>(p.out) + (q_at[nb] + d) * ES;
+            if constexpr (k16)
+              *reinterpret_cast<u32x2*>(dst) = u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
+            else
+              *reinterpret_cast<f32x4*>(dst) = y;
+          }
+        } else {
+          float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (p.D + 2));
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c) {
+            const int d = 16 * c + 4 * g4;
+            if (d < p.D)
+              *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(rr) * p.D + d) =
+                  has ? acc[c][nb] : f32x4{0.f, 0.f, 0.f, 0.f};
+          }
+          if (g4 == 0)
+            *reinterpret_cast<f32x2*>(part + static_cast<int64_t>(Sh::kRows) * p.D + 2 * rr) =
+                has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
+        }
+      }
+    }
+  };
+
+  // Balanced: the costs of all items in a row, cut into equal ranges.
+  int64_t total = 0, used = 1, pos = 0, end = 1;
+  const int64_t w = blockIdx.x;
+  int b = 0;
+  if (p.W > 0) {
+    for (int i = tid; i < p.B; i += 256) {
+      const int tiles = span_tiles(item_span(p, i));
+      incl[i] = tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
+    }
+    __syncthreads();
+    if (wv == 0) {
+      int64_t carry = 0;
+      for (int base = 0; base < p.B; base += 64) {
+        const int i = base + lane;
+        const int64_t v = carry + wave_incl_scan_i64(i < p.B ? incl[i] : 0, lane);
+        if (i < p.B) incl[i] = v;
+        carry = __shfl(v, 63);
+      }
+    }
+    __syncthreads();
+    total = readlane_i64(incl[p.B - 1], 0);
+    used = min(static_cast<int64_t>(p.W), max<int64_t>(1, total / kTreeMinCost));
+    if (w >= used) return;
+    pos = w * total / used;
+    end = (w + 1) * total / used;
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+  } else {
+    b = static_cast<int>(blockIdx.x) / per_seq;
+  }
+  while (pos < end) {
+    int hc, t0 = 0, t1, tiles, step = 1;
+    Span sp;
+    if (p.W > 0) {
+      while (readlane_i64(incl[b], 0) <= pos) ++b;
+      const int64_t before = b > 0 ? readlane_i64(incl[b - 1], 0) : 0;
+      const int cost = static_cast<int>((readlane_i64(incl[b], 0) - before) / per_seq);
+      hc = static_cast<int>((pos - before) / cost);
+      const int off = static_cast<int>((pos - before) - static_cast<int64_t>(hc) * cost);
+      const int stop = static_cast<int>(min(static_cast<int64_t>(cost), off + (end - pos)));
+      t0 = max(0, off - kTreeItemCost);
+      t1 = max(0, stop - kTreeItemCost);
+      tiles = cost - kTreeItemCost;
+      step = stop - off;
+      if (t1 > t0 && t0 == 0 && tid == 0) {
+        const int64_t first = before + static_cast<int64_t>(hc) * cost + kTreeItemCost;  // the item's first tile
+        const int64_t last = ((first + tiles) * used - 1) / total;                       // holder of its last tile
+        int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * per_seq + hc);
+        meta[0] = static_cast<int32_t>(w);
+        meta[1] = static_cast<int32_t>(last - w + 1);
+      }
+      sp = item_span(p, b);
+    } else {
+      hc = static_cast<int>(blockIdx.x) % per_seq;
+      sp = item_span(p, b);
+      t1 = tiles = span_tiles(sp);
+    }
+    if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * w + (t0 == 0 ? 1 : 0));
+    pos += step;
+  }
+}
+
+// Log-sum-exp merge of the items that a balanced launch split, and the rows of
+// sequences without any token.  A workgroup of 4 waves serves 16 rows of an
+// item: 16 lanes per row, the lanes stride its columns.
+// grid (items, row blocks), block 256.
+template <int DT, int KROWS>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
+  using E = Elem<DT>;
+  const int per_seq = p.Hkv * p.chunks;
+  const int item = blockIdx.x;
+  const int b = item / per_seq, hc = item % per_seq;
+  const bool empty = span_tiles(item_span(p, b)) == 0;
+  const int first = empty ? 0 : p.meta[2 * static_cast<int64_t>(item)];
+  const int count = empty ? 0 : p.meta[2 * static_cast<int64_t>(item) + 1];
+  if (count == 1) return;
+  const int h = hc / p.chunks, row0 = (hc % p.chunks) * p.chunk_rows;
+  const int rows = min(p.chunk_rows, p.R - row0);
+  const int rr = 16 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x >> 4);
+  if (rr >= rows) return;
+  const int t = (row0 + rr) / p.G, g = (row0 + rr) % p.G;
+  typename E::S* out = static_cast<typename E::S*>(p.out) +
+                       ((static_cast<int64_t>(b) * p.T + t) * p.Hq + static_cast<int64_t>(h) * p.G + g) * p.D;
+  const int64_t slot_floats = static_cast<int64_t>(KROWS) * (p.D + 2);
+  auto part = [&](int s) { return p.part + (2 * static_cast<int64_t>(first + s) + (s == 0 ? 1 : 0)) * slot_floats; };
+  auto stat = [&](int s) { return *reinterpret_cast<const f32x2*>(part(s) + static_cast<int64_t>(KROWS) * p.D + 2 * rr); };
+  const int l16 = threadIdx.x & 15;
+  float mx = -INFINITY;
+  for (int s = l16; s < count; s += 16) mx = fmaxf(mx, stat(s)[0]);
+  for (int off = 8; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  for (int d = 4 * l16; d < p.D; d += 64) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < count; ++s) {
+      const f32x2 ml = stat(s);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part(s) + static_cast<int64_t>(rr) * p.D + d);
+      const float f = fast_exp2(ml[0] - ref);
+      sum += f * ml[1];
+      a += f * x;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[d + i] = E::from_f(sum > 0.f || sum != sum ? a[i] * inv : 0.f);
+  }
+}
+
+// One launch (and the merge of a balanced one).
+template <int DT, int DP, int NB, int WR>
+hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
+  using Sh = TreeShape<DT, DP, NB, WR>;
+  const size_t lds = Sh::kLds + (p.W > 0 ? sizeof(int64_t) * static_cast<size_t>(p.B) : 0);
+  void (*fn)(TreeParams) = tree_mfma_kernel<DT, DP, NB, WR>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which more than 64 KB of LDS were asked for
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             Sh::kLds + 8 * kTreeMaxBalanced);
+    if (e != hipSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(256), lds, st, p);
+  if (p.W > 0) {
+    void (*merge)(TreeParams) = tree_merge_kernel<DT, Sh::kRows>;
+    hipLaunchKernelGGL(merge, dim3(static_cast<uint32_t>(p.B * p.Hkv * p.chunks), static_cast<uint32_t>((p.chunk_rows + 15) / 16)),
+                       dim3(256), 0, st, p);
+  }
+  return hipGetLastError();
+}
+
+template <int DT, int DP>
+hipError_t tree_launch_rows(const TreeParams& p, int nb, int wr, int grid, hipStream_t st) {
+  if (nb == 1 && wr == 1) return tree_launch<DT, DP, 1, 1>(p, grid, st);
+  if constexpr (DT != QD_DTYPE_F32 || DP <= 128) {
+    if (nb == 2 && wr == 1) return tree_launch<DT, DP, 2, 1>(p, grid, st);
+    if (nb == 2 && wr == 2) return tree_launch<DT, DP, 2, 2>(p, grid, st);
+    if (nb == 2 && wr == 4) return tree_launch<DT, DP, 2, 4>(p, grid, st);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+#endif  // QD_TREE_KERNELS_H
