@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "qd_attention.h"
 #include "qd_device.h"
@@ -94,6 +95,172 @@ __global__ __launch_bounds__(256) void rope_generic_kernel(RopeParams p) {
   }
 }
 
+// Lanes of one head: four pairs (eight elements) per lane.
+__host__ __device__ constexpr int rope_lanes(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32; }
+
+// Four elements as loaded.
+template <int DT>
+struct RopeRaw {
+  using V = u32x2;
+};
+template <>
+struct RopeRaw<QD_DTYPE_F32> {
+  using V = u32x4;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4 rope_floats(typename RopeRaw<DT>::V v) {
+  if constexpr (DT == QD_DTYPE_F32) {
+    return __builtin_bit_cast(f32x4, v);
+  } else {
+    const f32x2 a = MfmaOps<DT>::unpack2(v[0]), b = MfmaOps<DT>::unpack2(v[1]);
+    return f32x4{a[0], a[1], b[0], b[1]};
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ typename RopeRaw<DT>::V rope_raw(f32x4 y) {
+  if constexpr (DT == QD_DTYPE_F32)
+    return __builtin_bit_cast(u32x4, y);
+  else
+    return u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
+}
+
+// Sum over the LANES lanes of a head.
+template <int LANES>
+__device__ __forceinline__ float head_sum(float x) {
+  x += dpp_f<0xB1>(x);   // quad_perm [1,0,3,2]
+  x += dpp_f<0x4E>(x);   // quad_perm [2,3,0,1]
+  x += dpp_f<0x141>(x);  // row_half_mirror
+  if (LANES >= 16) x += dpp_f<0x140>(x);  // row_mirror
+  if (LANES >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
+// head_dim a multiple of 8, tensors aligned to four elements: a workgroup per
+// token, LANES lanes per head, each with two groups of four elements.  In the
+// half-split rotation lane i < R / 8 holds pairs 4i.. as the groups at 4i and
+// R / 2 + 4i, the other lanes neighbouring groups past R; interleaved, and
+// for values, a lane's groups are neighbours.  So no element has its partner
+// in another lane, and a token's angles are loaded once for all its heads.
+// grid tokens, block a multiple of LANES.
+template <int DT, int WDT, int LANES, bool INTER>
+__global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
+  using E = Elem<DT>;
+  using S = typename E::S;
+  using V = typename RopeRaw<DT>::V;
+  constexpr int kAhead = 4;  // heads whose loads a lane has in flight
+  const int64_t n = blockIdx.x;
+  const int lane = static_cast<int>(threadIdx.x) % LANES;
+  const int team = static_cast<int>(threadIdx.x) / LANES, teams = static_cast<int>(blockDim.x) / LANES;
+  const int heads = p.Hq + 2 * p.Hkv;
+  const bool live = 8 * lane < p.D;
+  const int half = p.rot / 2;
+  // Element offsets of the lane's two groups.
+  const bool split = !INTER && 8 * lane < p.rot;
+  const int a_at = split ? 4 * lane : 8 * lane, b_at = split ? half + 4 * lane : 8 * lane + 4;
+  const int64_t at = p.pos[n], slot = p.slots[n];
+  auto source = [&](int h) -> const S* {
+    return h < p.Hq           ? static_cast<const S*>(p.q) + n * p.q_stride + static_cast<int64_t>(h) * p.D
+           : h < p.Hq + p.Hkv ? static_cast<const S*>(p.key) + n * p.k_stride + static_cast<int64_t>(h - p.Hq) * p.D
+                              : static_cast<const S*>(p.value) + n * p.v_stride +
+                                    static_cast<int64_t>(h - p.Hq - p.Hkv) * p.D;
+  };
+  V xa[kAhead], xb[kAhead];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = first + i * teams;
+      if (h >= heads || !live) continue;
+      const S* x = source(h);
+      xa[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(x + a_at));
+      xb[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(x + b_at));
+    }
+  };
+  load(team);
+  const bool turned = at >= 0 && at < p.max_positions;
+  const bool kept = turned && slot >= 0 && slot < p.cache_rows;
+  // The lane's angles: of pairs 4 lane.. (half-split), 4 lane.. as well
+  // (interleaved: group a holds pairs 4 lane and 4 lane + 1, b the next two).
+  f32x4 c = {1.f, 1.f, 1.f, 1.f}, s = {0.f, 0.f, 0.f, 0.f};
+  if (turned) {
+    const float* cs = p.cos_sin + at * p.rot;
+    if constexpr (INTER) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (8 * lane + 4 * g < p.rot) {
+          const f32x2 cg = *reinterpret_cast<const f32x2*>(cs + 4 * lane + 2 * g);
+          const f32x2 sg = *reinterpret_cast<const f32x2*>(cs + half + 4 * lane + 2 * g);
+          c[2 * g] = cg[0];
+          c[2 * g + 1] = cg[1];
+          s[2 * g] = sg[0];
+          s[2 * g + 1] = sg[1];
+        }
+    } else if (split) {
+      c = *reinterpret_cast<const f32x4*>(cs + 4 * lane);
+      s = *reinterpret_cast<const f32x4*>(cs + half + 4 * lane);
+    }
+  }
+  auto weights = [&](const void* w, f32x4& wa, f32x4& wb) {
+    wa = wb = f32x4{1.f, 1.f, 1.f, 1.f};
+    if (w && live) {
+      using W = typename Elem<WDT>::S;
+      using WV = typename RopeRaw<WDT>::V;
+      wa = rope_floats<WDT>(*reinterpret_cast<const WV*>(static_cast<const W*>(w) + a_at));
+      wb = rope_floats<WDT>(*reinterpret_cast<const WV*>(static_cast<const W*>(w) + b_at));
+    }
+  };
+  f32x4 qa, qb, ka, kb;
+  weights(p.qw, qa, qb);
+  weights(p.kw, ka, kb);
+  const float inv_d = 1.f / static_cast<float>(p.D);
+  for (int first = team; first < heads; first += kAhead * teams) {
+    if (first != team) load(first);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = first + i * teams;
+      if (h >= heads) break;  // the whole head's lanes
+      const bool is_q = h < p.Hq, is_k = !is_q && h < p.Hq + p.Hkv;
+      V ya = xa[i], yb = xb[i];
+      if (is_q || is_k) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        if (live) {
+          a = rope_floats<DT>(xa[i]);
+          b = rope_floats<DT>(xb[i]);
+        }
+        if (is_q ? p.qw != nullptr : p.kw != nullptr) {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum = fmaf(a[j], a[j], fmaf(b[j], b[j], sum));
+          const float r = 1.f / sqrtf(fmaf(head_sum<LANES>(sum), inv_d, p.eps));
+          a = a * r * (is_q ? qa : ka);
+          b = b * r * (is_q ? qb : kb);
+        }
+        if constexpr (INTER) {
+          const f32x4 u = a, w = b;
+          a = f32x4{u[0] * c[0] - u[1] * s[0], u[1] * c[0] + u[0] * s[0], u[2] * c[1] - u[3] * s[1],
+                    u[3] * c[1] + u[2] * s[1]};
+          b = f32x4{w[0] * c[2] - w[1] * s[2], w[1] * c[2] + w[0] * s[2], w[2] * c[3] - w[3] * s[3],
+                    w[3] * c[3] + w[2] * s[3]};
+        } else if (split) {
+          const f32x4 u = a;
+          a = u * c - b * s;
+          b = b * c + u * s;
+        }
+        if (is_q && !turned) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        ya = rope_raw<DT>(a);
+        yb = rope_raw<DT>(b);
+      }
+      if (!live || (!is_q && !kept)) continue;
+      S* y = is_q   ? static_cast<S*>(p.out) + (n * p.Hq + h) * p.D
+             : is_k ? static_cast<S*>(p.kc) + (slot * p.Hkv + (h - p.Hq)) * p.D
+                    : static_cast<S*>(p.vc) + (slot * p.Hkv + (h - p.Hq - p.Hkv)) * p.D;
+      *reinterpret_cast<V*>(y + a_at) = ya;
+      *reinterpret_cast<V*>(y + b_at) = yb;
+    }
+  }
+}
+
 int rope_fail(char* msg, size_t cap, const char* text) {
   qd_set_last_error(QD_ERR_INVALID_VALUE, text);
   if (msg && cap) {
@@ -109,6 +276,38 @@ bool float_dtype(int dt) { return dt == QD_DTYPE_F32 || dt == QD_DTYPE_F16 || dt
 
 template <int DT>
 void launch_rope(const RopeParams& p, int64_t tokens, int wdt, hipStream_t st) {
+  // The vector kernel's groups of four elements must not cross the end of the
+  // rotated part, and every row starts at a group.
+  constexpr uintptr_t kGroup = DT == QD_DTYPE_F32 ? 16 : 8;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.key) |
+                         reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.kc) |
+                         reinterpret_cast<uintptr_t>(p.vc) | reinterpret_cast<uintptr_t>(p.out);
+  const uintptr_t weights = reinterpret_cast<uintptr_t>(p.qw) | reinterpret_cast<uintptr_t>(p.kw);
+  if (p.D % 8 == 0 && p.rot % (p.interleaved ? 4 : 8) == 0 && bits % kGroup == 0 &&
+      (p.q_stride | p.k_stride | p.v_stride) % 4 == 0 && weights % (wdt == QD_DTYPE_F32 ? 16 : 8) == 0 &&
+      reinterpret_cast<uintptr_t>(p.cos_sin) % 16 == 0) {
+    const int lanes = rope_lanes(p.D);
+    const int teams = std::min(p.Hq + 2 * p.Hkv, 256 / lanes);
+    const dim3 block(static_cast<uint32_t>((teams * lanes + 63) / 64 * 64));
+    const dim3 grid(static_cast<uint32_t>(tokens));
+    auto run = [&](auto wtype, auto inter) {
+      constexpr int W = decltype(wtype)::value;
+      constexpr bool I = decltype(inter)::value;
+      if (lanes == 8)
+        hipLaunchKernelGGL((rope_vec_kernel<DT, W, 8, I>), grid, block, 0, st, p);
+      else if (lanes == 16)
+        hipLaunchKernelGGL((rope_vec_kernel<DT, W, 16, I>), grid, block, 0, st, p);
+      else
+        hipLaunchKernelGGL((rope_vec_kernel<DT, W, 32, I>), grid, block, 0, st, p);
+    };
+    using F = std::integral_constant<int, QD_DTYPE_F32>;
+    using T = std::integral_constant<int, DT>;
+    if (wdt == QD_DTYPE_F32)
+      p.interleaved ? run(F{}, std::true_type{}) : run(F{}, std::false_type{});
+    else
+      p.interleaved ? run(T{}, std::true_type{}) : run(T{}, std::false_type{});
+    return;
+  }
   const dim3 grid(static_cast<uint32_t>(tokens), static_cast<uint32_t>((p.Hq + 2 * p.Hkv + 3) / 4));
   if (wdt == QD_DTYPE_F32)
     hipLaunchKernelGGL((rope_generic_kernel<DT, QD_DTYPE_F32>), grid, dim3(256), 0, st, p);
