@@ -67,8 +67,9 @@ OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 # Per-source flags.  mla: MFMA accumulators in VGPRs where the register
 # budget allows (one wave per SIMD gives 512); with the default AGPR form the
 # attention kernels moved hundreds of registers between the two files per
-# cache tile.
-SOURCE_FLAGS = {"mla": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# cache tile.  The matrix-core tree kernels likewise.
+_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+SOURCE_FLAGS = {n: _VGPR_FORM for n in ("mla", "tree_mfma_bf16", "tree_mfma_f16", "tree_mfma_f32")}
 
 
 def hip_object_cmd(name: str) -> list[str]:

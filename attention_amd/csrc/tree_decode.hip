@@ -198,7 +198,7 @@ int tree_cu_count() {
 struct TreePlan {
   bool mfma;
   int splits;                                  // VALU kernel
-  int dp, nb, wr, chunks, chunk_rows, W, grid;  // matrix-core kernel
+  int dp, chunks, chunk_rows, W, grid;         // matrix-core kernel
   size_t meta_bytes, bytes;
 };
 
@@ -218,25 +218,22 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   }
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   pl.dp = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 && es == 2 ? 192 : 256;
-  // Up to 128 rows per workgroup; fp32 above head_dim 128: 16, whose state is
-  // what the registers hold.
-  const int most = es == 4 && pl.dp == 256 ? 16 : 128;
+  const int most = tree_most_rows(es, pl.dp);
   const int R = q_len * (q_heads / kv_heads);
   pl.chunks = (R + most - 1) / most;
   pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
-  pl.nb = pl.chunk_rows <= 16 ? 1 : 2;
-  pl.wr = pl.chunk_rows <= 32 ? 1 : pl.chunk_rows <= 64 ? 2 : 4;
+  const TreeWaves wv = tree_waves(pl.dp, pl.chunk_rows);
   const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
   const int64_t tiles = (cap + kTreeTile - 1) / kTreeTile;
   if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced) {
     pl.grid = static_cast<int>(items);
     return pl;
   }
-  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(es, pl.dp, pl.nb, pl.wr);
+  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(es, pl.dp, wv.nb, wv.nw);
   pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / kTreeMinCost)));
   pl.grid = pl.W;
   pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;
-  pl.bytes = pl.meta_bytes + sizeof(float) * 2 * static_cast<size_t>(pl.W) * (16 * pl.nb * pl.wr) * (head_dim + 2);
+  pl.bytes = pl.meta_bytes + sizeof(float) * 2 * static_cast<size_t>(pl.W) * (16 * wv.nb * wv.wr) * (head_dim + 2);
   return pl;
 }
 
@@ -399,7 +396,7 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
     const auto run = dtype == QD_DTYPE_F32   ? qd_tree_mfma_launch_f32
                      : dtype == QD_DTYPE_F16 ? qd_tree_mfma_launch_f16
                                              : qd_tree_mfma_launch_bf16;
-    e = static_cast<hipError_t>(run(p, pl.dp, pl.nb, pl.wr, pl.grid, stream));
+    e = static_cast<hipError_t>(run(p, pl.dp, pl.grid, stream));
   } else {
     switch (dtype) {
       case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;

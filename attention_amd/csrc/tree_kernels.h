@@ -37,11 +37,11 @@ struct TreeParams {
   int pshift;    // log2(P), or -1
 };
 
-// Runs the matrix-core kernel for padded head_dim dp and 16 nb wr rows per
-// workgroup (tree_mfma_*.hip); grid workgroups.  Returns a hipError_t.
-int qd_tree_mfma_launch_f32(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
-int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
-int qd_tree_mfma_launch_bf16(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream);
+// Runs the matrix-core kernel for padded head_dim dp (tree_mfma_*.hip); grid
+// workgroups.  Returns a hipError_t.
+int qd_tree_mfma_launch_f32(const TreeParams& p, int dp, int grid, void* stream);
+int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int grid, void* stream);
+int qd_tree_mfma_launch_bf16(const TreeParams& p, int dp, int grid, void* stream);
 
 namespace {
 
@@ -115,10 +115,11 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 // ----------------------------------------------------------------------------
 //
 // An item is a (sequence, kv-head, chunk of its rows); a row is a (query,
-// q-head of the kv-head's group).  A workgroup of four waves goes through an
+// q-head of the kv-head's group).  A workgroup of NW waves goes through an
 // item's virtual tokens in tiles of 64: all waves load the tile's K and V rows
 // (registers, one tile ahead, then LDS), and wave (wr, wt) multiplies row
-// blocks [16 NB wr, 16 NB (wr + 1)) with tokens [64 / WT wt, ...):
+// blocks [16 NB wr, 16 NB (wr + 1)) with tokens [64 / WT wt, ...), at most 32
+// of them at a time:
 //   scores   S^T = K Q^T, 16x16 blocks (A = K rows from LDS, B = Q from
 //            registers): a lane holds one row and 4 tokens per block
 //   softmax  per lane; the reference maximum of a row moves only when a score
@@ -144,18 +145,18 @@ __host__ __device__ constexpr int tree_lds_bytes(int es, int dp, int bufs) {
   return bufs * kTreeTile * (2 * dp * es + 16 + (es == 2 ? 32 : 16)) + 32;
 }
 __host__ __device__ constexpr int tree_bufs(int es, int dp) { return tree_lds_bytes(es, dp, 2) <= 150 * 1024 ? 2 : 1; }
-__host__ __device__ constexpr int tree_occupancy(int es, int dp, int nb, int wr) {
+__host__ __device__ constexpr int tree_occupancy(int es, int dp, int nb, int nw) {
   // Registers: O, Q, the staged tile, scores and weights.
-  const int steps = dp * es / 64, pass = dp * es / 64, blocks = wr;  // token blocks: 4 / (4 / wr)
-  const int regs = 4 * nb * (dp / 16) + 4 * nb * steps + 8 * pass + 8 * blocks * nb;
-  const int by_regs = regs > 190 ? 1 : regs > 90 ? 2 : regs > 64 ? 3 : 4;
+  const int regs = 4 * nb * (dp / 16) + 4 * nb * (dp * es / 64) + 32 * dp * es / 64 / nw + 24 * nb;
+  const int by_regs = (regs > 210 ? 1 : regs > 90 ? 2 : regs > 64 ? 3 : 4) * 4 / nw;
   const int by_lds = 160 * 1024 / (tree_lds_bytes(es, dp, tree_bufs(es, dp)) + 8 * kTreeMaxBalanced);
-  return by_lds < by_regs ? (by_lds < 1 ? 1 : by_lds) : by_regs;
+  const int n = by_lds < by_regs ? by_lds : by_regs;
+  return n < 1 ? 1 : n;
 }
 
-template <int DT, int DP, int NB, int WR>
+template <int DT, int DP, int NB, int WR, int NW>
 struct TreeShape {
-  static constexpr int kWT = 4 / WR;
+  static constexpr int kWT = NW / WR;
   static constexpr int kES = DT == QD_DTYPE_F32 ? 4 : 2;
   static constexpr int kRow = DP * kES;                      // bytes of a head's row, padded
   // Row strides in LDS: rows 16 bytes (K) and 32 bytes (V, two lanes' worth of
@@ -165,15 +166,17 @@ struct TreeShape {
   static constexpr int kBuf = kTreeTile * (kKS + kVS);
   static constexpr int kBufs = tree_bufs(kES, DP);
   static constexpr int kChunks = kRow / 16;                  // 16-byte chunks of a row
-  static constexpr int kPass = kChunks / 4;                  // a wave loads 16 rows
+  static constexpr int kLoadRows = kTreeTile / NW;           // rows that a wave loads
+  static constexpr int kPass = (kLoadRows * kChunks + 63) / 64;
+  static constexpr bool kEven = kLoadRows * kChunks % 64 == 0;
   static constexpr int kSteps = kRow / 64;
   static constexpr int kTW = kTreeTile / kWT;                // tokens of a wave in a tile
-  static constexpr int kTB = kTW / 16;
+  static constexpr int kTB = kTW >= 32 ? 2 : 1;              // 16-token blocks at a time
+  static constexpr int kSub = kTW / (16 * kTB);
   static constexpr int kCols = DP / 16;
   static constexpr int kRows = 16 * NB * WR;                 // rows of a workgroup
-  static constexpr int kCtl = 32;                            // three words of tokens with non-finite values
   static constexpr int kLds = tree_lds_bytes(kES, DP, kBufs);
-  static constexpr int kOcc = tree_occupancy(kES, DP, NB, WR);
+  static constexpr int kOcc = tree_occupancy(kES, DP, NB, NW);
 };
 
 __device__ __forceinline__ float tree_max_groups(float x) {
@@ -208,16 +211,27 @@ __device__ __forceinline__ u32x2 tree_tr_read(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
 }
 
+// Zeroes the elements of x that are Inf or NaN; returns whether there were any.
 template <int DT>
-__device__ __forceinline__ bool chunk_not_finite(u32x4 x) {
+__device__ __forceinline__ bool drop_not_finite(u32x4& x) {
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (DT == QD_DTYPE_F32) {
-      bad |= (x[i] & 0x7F800000u) == 0x7F800000u;
+      if ((x[i] & 0x7F800000u) == 0x7F800000u) {
+        x[i] = 0;
+        bad = true;
+      }
     } else {
       constexpr uint32_t e = DT == QD_DTYPE_F16 ? 0x7C00u : 0x7F80u;
-      bad |= (x[i] & e) == e || ((x[i] >> 16) & e) == e;
+      if ((x[i] & e) == e) {
+        x[i] &= 0xFFFF0000u;
+        bad = true;
+      }
+      if ((x[i] & (e << 16)) == e << 16) {
+        x[i] &= 0x0000FFFFu;
+        bad = true;
+      }
     }
   }
   return bad;
@@ -244,9 +258,9 @@ __device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
 
 __device__ __forceinline__ int span_tiles(const Span& s) { return (s.n + kTreeTile - 1) / kTreeTile; }
 
-template <int DT, int DP, int NB, int WR>
-__global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_mfma_kernel(TreeParams p) {
-  using Sh = TreeShape<DT, DP, NB, WR>;
+template <int DT, int DP, int NB, int WR, int NW>
+__global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW / 4)) void tree_mfma_kernel(TreeParams p) {
+  using Sh = TreeShape<DT, DP, NB, WR, NW>;
   using E = Elem<DT>;
   using S = typename E::S;
   constexpr bool k16 = DT != QD_DTYPE_F32;
@@ -256,7 +270,9 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
   constexpr float kShift = DT == QD_DTYPE_F16 ? 7.f : 0.f;
   constexpr float kLazy = 8.f;
   extern __shared__ __align__(16) char smem[];
-  uint64_t* bad_words = reinterpret_cast<uint64_t*>(smem + Sh::kBufs * Sh::kBuf);
+  // Tokens with non-finite values that not all rows see: drafted ones, and
+  // those at the window's edge (bit i: token lo + i).
+  unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * Sh::kBuf);
   int64_t* incl = reinterpret_cast<int64_t*>(smem + Sh::kLds);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
@@ -286,35 +302,28 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
       any_seen |= static_cast<uint64_t>(__shfl_xor(static_cast<long long>(any_seen), off));
       lo_max = max(lo_max, __shfl_xor(lo_max, off));
     }
-    // This lane's rows.
-    bool active[NB];
-    int lo[NB], sinks[NB];
-    uint64_t seen[NB];
-    int64_t q_at[NB];  // element offset of the row in q and out, -1: no such row
+    any_seen = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(any_seen), 0));
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    // This lane's rows: what they see is taken from lane (query - q0).
+    int query[NB];
+    bool real[NB];
+    u32x4 qf[NB][Sh::kSteps];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int rr = 16 * (NB * wr + nb) + r16;
-      const int row = row0 + (rr < rows ? rr : 0);
-      const int t = row / p.G;
-      const int src = t - q0;
-      active[nb] = rr < rows && __shfl(static_cast<int>(sees), src) != 0;
-      lo[nb] = __shfl(mine.lo, src);
-      sinks[nb] = __shfl(mine.sinks, src);
-      seen[nb] = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), src));
-      q_at[nb] = rr < rows
-                     ? ((static_cast<int64_t>(b) * p.T + t) * p.Hq + static_cast<int64_t>(h) * p.G + (row - t * p.G)) * p.D
-                     : -1;
-    }
-    u32x4 qf[NB][Sh::kSteps];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+      real[nb] = rr < rows;
+      const int row = row0 + (real[nb] ? rr : 0);
+      query[nb] = row / p.G;
+      const char* src =
+          static_cast<const char*>(p.q) +
+          ((static_cast<int64_t>(b) * p.T + query[nb]) * p.Hq + static_cast<int64_t>(h) * p.G + (row - query[nb] * p.G)) *
+              row_bytes;
 #pragma unroll
       for (int s = 0; s < Sh::kSteps; ++s) {
         const int at = 64 * s + 16 * g4;
-        qf[nb][s] = q_at[nb] >= 0 && at < row_bytes
-                        ? *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.q) + q_at[nb] * ES + at)
-                        : u32x4{0u, 0u, 0u, 0u};
+        qf[nb][s] = real[nb] && at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
       }
+    }
     f32x4 acc[Sh::kCols][NB];
     float m[NB], l[NB];
 #pragma unroll
@@ -326,15 +335,15 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
     }
 
     const int context = sp.sinks + sp.len - sp.lo;
+    const int edge = sp.sinks + max(lo_max - sp.lo, 0);  // virtual tokens [sinks, edge): only in some rows' windows
     auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
-    // Lane's staged row of a tile: row 16 wv + r16.  Its page, looked up a
-    // tile ahead of the loads.
-    auto staged = [&](int tile) { return kTreeTile * tile + 16 * wv + r16; };
+    // Lane's staged row of a tile: row kLoadRows wv + lane % kLoadRows.  Its
+    // page is looked up a tile ahead of the loads.
+    auto staged = [&](int tile) { return kTreeTile * tile + Sh::kLoadRows * wv + (lane & (Sh::kLoadRows - 1)); };
     auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
-    auto row_seen = [&](int v) { return v < context || (v < sp.n && ((any_seen >> (v - context)) & 1)); };
     auto look_up = [&](int tile) -> int32_t {
       const int v = staged(tile);
-      if (!row_seen(v)) return -1;
+      if (!(v < context || (v < sp.n && ((any_seen >> (v - context)) & 1)))) return -1;
       const int32_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page_of(token(v))];
       return phys < 0 ? 0 : phys;
     };
@@ -352,20 +361,15 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
         const int row = c / Sh::kChunks, chunk = c % Sh::kChunks;
         const int64_t at = __shfl(static_cast<long long>(off), row);
         kreg[i] = vreg[i] = u32x4{0u, 0u, 0u, 0u};
-        if (at >= 0 && 16 * chunk < row_bytes) {
+        if (at >= 0 && 16 * chunk < row_bytes && (Sh::kEven || row < Sh::kLoadRows)) {
           kreg[i] = stream_load16(static_cast<const char*>(p.k) + at + 16 * chunk);
           vreg[i] = stream_load16(static_cast<const char*>(p.v) + at + 16 * chunk);
         }
       }
     };
-    // Every row of the chunk sees all (existing) tokens of the tile.
-    auto uniform = [&](int tile) {
-      const int a = kTreeTile * tile, e = a + kTreeTile;
-      return e <= sp.sinks || (a >= sp.sinks + max(lo_max - sp.lo, 0) && e <= context) || (q0 == q1 && e <= sp.n);
-    };
 
     tree_barrier();  // the previous item's merge and the prefix are done with LDS
-    if (tid < 3) bad_words[tid] = 0;
+    if (tid < 2) bad_words[tid] = 0;
     int32_t page = -1;
     if (t0 < t1) {
       page = look_up(t0);
@@ -374,204 +378,175 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
     if (t0 + 1 < t1) page = look_up(t0 + 1);
     tree_barrier();
     for (int tile = t0; tile < t1; ++tile) {
-      const int turn = tile - t0;
-      char* buf = smem + (Sh::kBufs == 2 ? (turn & 1) * Sh::kBuf : 0);
-      const bool whole_tile = uniform(tile);
-      const bool mixed = !whole_tile && q0 != q1;
-      if (Sh::kBufs == 1 && turn > 0) tree_barrier();
+      char* buf = smem + (Sh::kBufs == 2 ? ((tile - t0) & 1) * Sh::kBuf : 0);
+      // Every row of the chunk sees all (existing) tokens of the tile.
+      const int first = kTreeTile * tile, stop = first + kTreeTile;
+      const bool whole_tile =
+          stop <= sp.sinks || ((first >= edge || edge == sp.sinks) && stop <= context) || (q0 == q1 && stop <= sp.n);
+      if (Sh::kBufs == 1 && tile > t0) tree_barrier();
+      if (!whole_tile && q0 != q1) {
+        // A weight of 0 would not hide Inf and NaN from the rows that do not
+        // see their token: they are left out here and join the rows that do at
+        // the item's end.
+#pragma unroll
+        for (int i = 0; i < Sh::kPass; ++i) {
+          const int v = first + Sh::kLoadRows * wv + (64 * i + lane) / Sh::kChunks;
+          if ((v >= context || (v >= sp.sinks && v < edge)) && drop_not_finite<DT>(vreg[i]))
+            atomicOr(&bad_words[v >= context ? 0 : 1], 1ull << (v >= context ? v - context : v - sp.sinks));
+        }
+      }
 #pragma unroll
       for (int i = 0; i < Sh::kPass; ++i) {
         const int c = 64 * i + lane;
-        const int row = 16 * wv + c / Sh::kChunks, chunk = c % Sh::kChunks;
-        if (mixed && chunk_not_finite<DT>(vreg[i])) {
-          // A weight of 0 would not hide this value from the rows that do not
-          // see the token: it is added for the others below.
-          atomicOr(reinterpret_cast<unsigned long long*>(&bad_words[turn % 3]), 1ull << row);
-          vreg[i] = u32x4{0u, 0u, 0u, 0u};
+        const int row = Sh::kLoadRows * wv + c / Sh::kChunks, chunk = c % Sh::kChunks;
+        if (Sh::kEven || c < Sh::kLoadRows * Sh::kChunks) {
+          *reinterpret_cast<u32x4*>(buf + row * Sh::kKS + 16 * chunk) = kreg[i];
+          *reinterpret_cast<u32x4*>(buf + kTreeTile * Sh::kKS + row * Sh::kVS + 16 * chunk) = vreg[i];
         }
-        *reinterpret_cast<u32x4*>(buf + row * Sh::kKS + 16 * chunk) = kreg[i];
-        *reinterpret_cast<u32x4*>(buf + kTreeTile * Sh::kKS + row * Sh::kVS + 16 * chunk) = vreg[i];
       }
-      if (tid == 0) bad_words[(turn + 1) % 3] = 0;
       if (tile + 1 < t1) {
         load(offset_of(tile + 1, page));
         if (tile + 2 < t1) page = look_up(tile + 2);
       }
       tree_barrier();
 
-      const char* kb = buf + (Sh::kTW * wt + r16) * Sh::kKS + 16 * g4;
-      f32x4 s[TB][NB];
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < Sh::kSteps; ++st)
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(kb + 16 * tb * Sh::kKS + 64 * st);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if constexpr (k16) {
-              s[tb][nb] = MfmaOps<DT>::mma32(a, qf[nb][st], s[tb][nb]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                s[tb][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(qf[nb][st][j]),
-                                                                 s[tb][nb], 0, 0, 0);
-            }
-          }
-        }
-      const int v0 = kTreeTile * tile + Sh::kTW * wt + 4 * g4;
-      auto visible = [&](int v, int nb) {
-        if (v >= context) return v < sp.n && ((seen[nb] >> (v - context)) & 1) != 0;
-        const int tok = token(v);
-        return tok < sinks[nb] || tok >= lo[nb];
-      };
-      if (!whole_tile) {
+#pragma unroll 1
+      for (int sub = 0; sub < Sh::kSub; ++sub) {
+        const int wave_tok = Sh::kTW * wt + 16 * TB * sub;
+        const char* kb = buf + (wave_tok + r16) * Sh::kKS + 16 * g4;
+        f32x4 s[TB][NB];
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-              if (!visible(v0 + 16 * tb + i, nb)) s[tb][nb][i] = -INFINITY;
-      }
+        for (int st = 0; st < Sh::kSteps; ++st)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[tb][nb][i]);
-        if (__ballot(mx * p.sl2 > m[nb] + kLazy)) {
-          const float mn = fmaxf(m[nb], tree_max_groups(mx) * p.sl2);
-          const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
-          m[nb] = mn;
-          l[nb] *= alpha;
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= alpha;
-        }
-        const float ref = m[nb] == -INFINITY ? -kShift : m[nb] - kShift;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float w = fast_exp2(fmaf(s[tb][nb][i], p.sl2, -ref));
-            s[tb][nb][i] = w;
-            l[nb] += w;
-          }
-      }
-      const char* vb = buf + kTreeTile * Sh::kKS + Sh::kTW * wt * Sh::kVS;
-      if constexpr (k16) {
-        u32x2 hi[TB][NB], lw[TB][NB];
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t a, c;
-              MfmaOps<DT>::split2(s[tb][nb][2 * i], s[tb][nb][2 * i + 1], a, c);
-              hi[tb][nb][i] = a;
-              lw[tb][nb][i] = c;
-            }
-        // Masked weights are 0; split2's low part never is, which adds at
-        // most 2^-133 (bf16) or 2^-24 of 2^7 (fp16) of a masked value: none of
-        // the values in LDS is other than finite then, and where the tile is
-        // masked the low part is cleared.
-        if (!whole_tile) {
-#pragma unroll
-          for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-        }
-        const char* va = vb + (4 * g4 + (r16 >> 2)) * Sh::kVS + 8 * (r16 & 3);
-#pragma unroll
-        for (int c = 0; c < Sh::kCols; ++c) {
-          if constexpr (TB == 1) {
-            const u32x2 a = tree_tr_read(va + 32 * c);
+          for (int tb = 0; tb < TB; ++tb) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(kb + 16 * tb * Sh::kKS + 64 * st);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              acc[c][nb] = MfmaOps<DT>::pv(a, hi[0][nb], acc[c][nb]);
-              acc[c][nb] = MfmaOps<DT>::pv(a, lw[0][nb], acc[c][nb]);
-            }
-          } else {
+              if constexpr (k16) {
+                s[tb][nb] = MfmaOps<DT>::mma32(a, qf[nb][st], s[tb][nb]);
+              } else {
 #pragma unroll
-            for (int tb = 0; tb < TB; tb += 2) {
-              const u32x2 a0 = tree_tr_read(va + 16 * tb * Sh::kVS + 32 * c);
-              const u32x2 a1 = tree_tr_read(va + 16 * (tb + 1) * Sh::kVS + 32 * c);
-              const u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                acc[c][nb] = MfmaOps<DT>::mma32(a, u32x4{hi[tb][nb][0], hi[tb][nb][1], hi[tb + 1][nb][0], hi[tb + 1][nb][1]},
-                                                acc[c][nb]);
-                acc[c][nb] = MfmaOps<DT>::mma32(a, u32x4{lw[tb][nb][0], lw[tb][nb][1], lw[tb + 1][nb][0], lw[tb + 1][nb][1]},
-                                                acc[c][nb]);
+                for (int j = 0; j < 4; ++j)
+                  s[tb][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(qf[nb][st][j]),
+                                                                   s[tb][nb], 0, 0, 0);
               }
             }
           }
-        }
-      } else {
-        const char* va = vb + 4 * g4 * Sh::kVS + 4 * r16;
+        if (!whole_tile) {
 #pragma unroll
-        for (int c = 0; c < Sh::kCols; ++c)
+          for (int nb = 0; nb < NB; ++nb) {
+            const int src = query[nb] - q0;
+            const int lo = __shfl(mine.lo, src), sinks = __shfl(mine.sinks, src);
+            const uint64_t seen = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), src));
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int v = first + wave_tok + 16 * tb + 4 * g4 + i;
+                const int tok = token(v);
+                const bool vis = v >= context ? v < sp.n && ((seen >> (v - context)) & 1) != 0 : tok < sinks || tok >= lo;
+                if (!vis) s[tb][nb][i] = -INFINITY;
+              }
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[tb][nb][i]);
+          if (__ballot(mx * p.sl2 > m[nb] + kLazy)) {
+            const float mn = fmaxf(m[nb], tree_max_groups(mx) * p.sl2);
+            const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
+            m[nb] = mn;
+            l[nb] *= alpha;
+#pragma unroll
+            for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= alpha;
+          }
+          const float ref = m[nb] == -INFINITY ? kShift : kShift - m[nb];
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float a = *reinterpret_cast<const float*>(va + (16 * tb + i) * Sh::kVS + 64 * c);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-                acc[c][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[tb][nb][i], acc[c][nb], 0, 0, 0);
+              const float w = fast_exp2(fmaf(s[tb][nb][i], p.sl2, ref));
+              s[tb][nb][i] = w;
+              l[nb] += w;
             }
-      }
-      if (mixed) {
-        // Non-finite values that some rows see: their products, one token
-        // after the other, for the rows that do.
-        uint64_t bad = bad_words[turn % 3] >> (Sh::kTW * wt);
-        if (Sh::kTW < 64) bad &= (uint64_t{1} << (Sh::kTW & 63)) - 1;
-        bad = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad), 0));
-        while (bad) {
-          const int x = __builtin_ctzll(bad);
-          bad &= bad - 1;
-          const int v = kTreeTile * tile + Sh::kTW * wt + x;
-          const int64_t at = (pool_row(p, b, token(v)) * p.Hkv + h) * row_bytes;
-          float w[NB];
+        }
+        const char* vb = buf + kTreeTile * Sh::kKS + wave_tok * Sh::kVS;
+        if constexpr (k16) {
+          u32x2 hi[TB][NB], lw[TB][NB];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float mine_w = 0.f;
+          for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint32_t a, c;
+                MfmaOps<DT>::split2(s[tb][nb][2 * i], s[tb][nb][2 * i + 1], a, c);
+                hi[tb][nb][i] = a;
+                lw[tb][nb][i] = c;
+              }
+          // split2's low part is never 0: cleared where the weight is a hidden
+          // token's.
+          if (!whole_tile) {
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (x / 16 == tb && x % 4 == i) mine_w = s[tb][nb][i];
-            w[nb] = __shfl(mine_w, 16 * ((x % 16) / 4) + r16);
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           }
+          const char* va = vb + (4 * g4 + (r16 >> 2)) * Sh::kVS + 8 * (r16 & 3);
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
-            const int byte = (16 * c + 4 * g4) * ES;
-            if (byte >= row_bytes) continue;
-            const char* src = static_cast<const char*>(p.v) + at;
-            if (!chunk_not_finite<DT>(*reinterpret_cast<const u32x4*>(src + (byte & ~15)))) continue;
-            const S* val = reinterpret_cast<const S*>(src + byte);
+            const u32x2 a0 = tree_tr_read(va + 32 * c);
+            if constexpr (TB == 1) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-              if (visible(v, nb))
+              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, hi[0][nb], acc[c][nb]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[c][nb][i] += w[nb] * E::to_f(val[i]);
+              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, lw[0][nb], acc[c][nb]);
+            } else {
+              const u32x2 a1 = tree_tr_read(va + 16 * Sh::kVS + 32 * c);
+              const u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                acc[c][nb] =
+                    MfmaOps<DT>::mma32(a, u32x4{hi[0][nb][0], hi[0][nb][1], hi[1][nb][0], hi[1][nb][1]}, acc[c][nb]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                acc[c][nb] =
+                    MfmaOps<DT>::mma32(a, u32x4{lw[0][nb][0], lw[0][nb][1], lw[1][nb][0], lw[1][nb][1]}, acc[c][nb]);
+            }
           }
+        } else {
+          const char* va = vb + 4 * g4 * Sh::kVS + 4 * r16;
+#pragma unroll
+          for (int c = 0; c < Sh::kCols; ++c)
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float a = *reinterpret_cast<const float*>(va + (16 * tb + i) * Sh::kVS + 64 * c);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                  acc[c][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[tb][nb][i], acc[c][nb], 0, 0, 0);
+              }
         }
       }
     }
 
     // The waves' parts of the same rows.
+    tree_barrier();
     if constexpr (WT > 1) {
-      tree_barrier();
       constexpr int kPart = NB * Sh::kCols * 1024 + NB * 512;  // acc, m, l of a wave
+      static_assert(WR * (WT - 1) * kPart <= Sh::kBufs * Sh::kBuf, "the waves' parts fit the tile buffers");
       char* base = smem + (wr * (WT - 1) + wt - 1) * kPart;
       if (wt > 0) {
 #pragma unroll
@@ -595,7 +570,7 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
             mx = fmaxf(mx, ml[w][0]);
           }
           const float ref = mx == -INFINITY ? 0.f : mx;
-          float f = mx == m[nb] && mx != -INFINITY ? 1.f : fast_exp2(m[nb] - ref);
+          float f = fast_exp2(m[nb] - ref);
           l[nb] *= f;
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= f;
@@ -613,24 +588,56 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
       }
     }
     if (wt == 0) {
+      // Inf and NaN that only some rows see: whatever their weight, the sum is
+      // no longer finite.
+#pragma unroll 1
+      for (int kind = 0; kind < 2; ++kind) {
+        uint64_t bad = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad_words[kind]), 0));
+        while (bad) {
+          const int x = __builtin_ctzll(bad);
+          bad &= bad - 1;
+          const int tok = kind == 0 ? sp.len + x : sp.lo + x;
+          const char* src = static_cast<const char*>(p.v) + (pool_row(p, b, tok) * p.Hkv + h) * row_bytes;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int from = query[nb] - q0;
+            const int lo = __shfl(mine.lo, from), sinks = __shfl(mine.sinks, from);
+            const uint64_t seen = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), from));
+            if (!(kind == 0 ? ((seen >> x) & 1) != 0 : tok < sinks || tok >= lo)) continue;
+#pragma unroll
+            for (int c = 0; c < Sh::kCols; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int d = 16 * c + 4 * g4 + i;
+                if (d >= p.D) continue;
+                const float val = E::to_f(reinterpret_cast<const S*>(src)[d]);
+                if (!(fabsf(val) < INFINITY)) acc[c][nb][i] += val;
+              }
+          }
+        }
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const float sum = tree_sum_groups(l[nb]);
-        const bool has = active[nb] && (sum > 0.f || sum != sum);
-        if (q_at[nb] < 0) continue;
+        const bool has = __shfl(static_cast<int>(sees), query[nb] - q0) != 0 && (sum > 0.f || sum != sum);
+        if (!real[nb]) continue;
         const int rr = 16 * (NB * wr + nb) + r16;
         if (whole) {
           const float inv = has ? 1.f / sum : 0.f;
+          char* out = static_cast<char*>(p.out) +
+                      ((static_cast<int64_t>(b) * p.T + query[nb]) * p.Hq + static_cast<int64_t>(h) * p.G +
+                       (row0 + rr - query[nb] * p.G)) *
+                          row_bytes;
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
             const int d = 16 * c + 4 * g4;
             if (d >= p.D) continue;
             const f32x4 y = has ? acc[c][nb] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
-            char* dst = static_cast<char*>(p.out) + (q_at[nb] + d) * ES;
             if constexpr (k16)
-              *reinterpret_cast<u32x2*>(dst) = u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
+              *reinterpret_cast<u32x2*>(out + d * ES) =
+                  u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
             else
-              *reinterpret_cast<f32x4*>(dst) = y;
+              *reinterpret_cast<f32x4*>(out + d * ES) = y;
           }
         } else {
           float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (p.D + 2));
@@ -654,7 +661,7 @@ __global__ __launch_bounds__(256, (TreeShape<DT, DP, NB, WR>::kOcc)) void tree_m
   const int64_t w = blockIdx.x;
   int b = 0;
   if (p.W > 0) {
-    for (int i = tid; i < p.B; i += 256) {
+    for (int i = tid; i < p.B; i += 64 * NW) {
       const int tiles = span_tiles(item_span(p, i));
       incl[i] = tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
     }
@@ -762,11 +769,11 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
 }
 
 // One launch (and the merge of a balanced one).
-template <int DT, int DP, int NB, int WR>
+template <int DT, int DP, int NB, int WR, int NW>
 hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
-  using Sh = TreeShape<DT, DP, NB, WR>;
+  using Sh = TreeShape<DT, DP, NB, WR, NW>;
   const size_t lds = Sh::kLds + (p.W > 0 ? sizeof(int64_t) * static_cast<size_t>(p.B) : 0);
-  void (*fn)(TreeParams) = tree_mfma_kernel<DT, DP, NB, WR>;
+  void (*fn)(TreeParams) = tree_mfma_kernel<DT, DP, NB, WR, NW>;
   static std::atomic<uint64_t> allowed{0};  // devices on which more than 64 KB of LDS were asked for
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
@@ -777,7 +784,7 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
     if (e != hipSuccess) return e;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(64 * NW), lds, st, p);
   if (p.W > 0) {
     void (*merge)(TreeParams) = tree_merge_kernel<DT, Sh::kRows>;
     hipLaunchKernelGGL(merge, dim3(static_cast<uint32_t>(p.B * p.Hkv * p.chunks), static_cast<uint32_t>((p.chunk_rows + 15) / 16)),
@@ -786,13 +793,41 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Row blocks per wave, waves along the rows and waves of a workgroup for a
+// chunk of rows.  Above 64 rows eight waves share a tile, two per SIMD: one
+// wave's products run under the other's softmax.  Heads above 128 elements
+// leave no registers for that.
+struct TreeWaves {
+  int nb, wr, nw;
+};
+__host__ __device__ constexpr TreeWaves tree_waves(int dp, int rows) {
+  return rows <= 16   ? TreeWaves{1, 1, 4}
+         : rows <= 32 ? TreeWaves{2, 1, 4}
+         : rows <= 64 ? TreeWaves{2, 2, 4}
+         : dp > 128   ? TreeWaves{2, 4, 4}
+         : rows <= 128 ? TreeWaves{2, 4, 8}
+                       : TreeWaves{2, 8, 8};
+}
+// The most rows of a chunk.  fp32 above head_dim 128: 16, whose state is what
+// the registers hold.
+__host__ __device__ constexpr int tree_most_rows(int es, int dp) {
+  return es == 4 ? (dp > 128 ? 16 : 128) : dp > 128 ? 128 : 256;
+}
+
 template <int DT, int DP>
-hipError_t tree_launch_rows(const TreeParams& p, int nb, int wr, int grid, hipStream_t st) {
-  if (nb == 1 && wr == 1) return tree_launch<DT, DP, 1, 1>(p, grid, st);
-  if constexpr (DT != QD_DTYPE_F32 || DP <= 128) {
-    if (nb == 2 && wr == 1) return tree_launch<DT, DP, 2, 1>(p, grid, st);
-    if (nb == 2 && wr == 2) return tree_launch<DT, DP, 2, 2>(p, grid, st);
-    if (nb == 2 && wr == 4) return tree_launch<DT, DP, 2, 4>(p, grid, st);
+hipError_t tree_launch_rows(const TreeParams& p, int grid, hipStream_t st) {
+  constexpr int kMost = tree_most_rows(DT == QD_DTYPE_F32 ? 4 : 2, DP);
+  if (p.chunk_rows <= 16) return tree_launch<DT, DP, 1, 1, 4>(p, grid, st);
+  if constexpr (kMost > 16) {
+    if (p.chunk_rows <= 32) return tree_launch<DT, DP, 2, 1, 4>(p, grid, st);
+    if (p.chunk_rows <= 64) return tree_launch<DT, DP, 2, 2, 4>(p, grid, st);
+    if constexpr (DP > 128) {
+      if (p.chunk_rows <= 128) return tree_launch<DT, DP, 2, 4, 4>(p, grid, st);
+    } else {
+      if (p.chunk_rows <= 128) return tree_launch<DT, DP, 2, 4, 8>(p, grid, st);
+      if constexpr (kMost > 128)
+        if (p.chunk_rows <= 256) return tree_launch<DT, DP, 2, 8, 8>(p, grid, st);
+    }
   }
   return hipErrorInvalidValue;
 }

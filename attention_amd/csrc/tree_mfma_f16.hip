@@ -3,14 +3,14 @@
 
 #include "tree_kernels.h"
 
-int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream) {
+int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int grid, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dp) {
-    case 64: return tree_launch_rows<QD_DTYPE_F16, 64>(p, nb, wr, grid, st);
-    case 96: return tree_launch_rows<QD_DTYPE_F16, 96>(p, nb, wr, grid, st);
-    case 128: return tree_launch_rows<QD_DTYPE_F16, 128>(p, nb, wr, grid, st);
-    case 192: return tree_launch_rows<QD_DTYPE_F16, 192>(p, nb, wr, grid, st);
-    case 256: return tree_launch_rows<QD_DTYPE_F16, 256>(p, nb, wr, grid, st);
+    case 64: return tree_launch_rows<QD_DTYPE_F16, 64>(p, grid, st);
+    case 96: return tree_launch_rows<QD_DTYPE_F16, 96>(p, grid, st);
+    case 128: return tree_launch_rows<QD_DTYPE_F16, 128>(p, grid, st);
+    case 192: return tree_launch_rows<QD_DTYPE_F16, 192>(p, grid, st);
+    case 256: return tree_launch_rows<QD_DTYPE_F16, 256>(p, grid, st);
     default: return hipErrorInvalidValue;
   }
 }

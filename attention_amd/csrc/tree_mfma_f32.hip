@@ -3,13 +3,13 @@
 
 #include "tree_kernels.h"
 
-int qd_tree_mfma_launch_f32(const TreeParams& p, int dp, int nb, int wr, int grid, void* stream) {
+int qd_tree_mfma_launch_f32(const TreeParams& p, int dp, int grid, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dp) {
-    case 64: return tree_launch_rows<QD_DTYPE_F32, 64>(p, nb, wr, grid, st);
-    case 96: return tree_launch_rows<QD_DTYPE_F32, 96>(p, nb, wr, grid, st);
-    case 128: return tree_launch_rows<QD_DTYPE_F32, 128>(p, nb, wr, grid, st);
-    case 256: return tree_launch_rows<QD_DTYPE_F32, 256>(p, nb, wr, grid, st);
+    case 64: return tree_launch_rows<QD_DTYPE_F32, 64>(p, grid, st);
+    case 96: return tree_launch_rows<QD_DTYPE_F32, 96>(p, grid, st);
+    case 128: return tree_launch_rows<QD_DTYPE_F32, 128>(p, grid, st);
+    case 256: return tree_launch_rows<QD_DTYPE_F32, 256>(p, grid, st);
     default: return hipErrorInvalidValue;
   }
 }
