@@ -209,7 +209,9 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
                    int has_mask, int window, int sinks, int dtype, int flags) {
   TreePlan pl{};
   const int64_t cap = visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks);
-  pl.mfma = head_dim % 8 == 0 && !(flags & QD_FLAG_FORCE_GENERIC);
+  // The matrix-core kernel's page and row offsets are 32 bits wide.
+  pl.mfma = head_dim % 8 == 0 && !(flags & QD_FLAG_FORCE_GENERIC) &&
+            static_cast<int64_t>(kv_heads) * head_dim * 4 * std::max(block_size, 16) < (int64_t{1} << 31);
   if (!pl.mfma) {
     pl.splits = generic_splits(batch, q_len, q_heads, cap);
     if (pl.splits > 1)
@@ -217,19 +219,20 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
     return pl;
   }
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
-  pl.dp = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 && es == 2 ? 192 : 256;
-  const int most = tree_most_rows(es, pl.dp);
+  pl.dp = tree_padded(es, head_dim);
+  const int slots = tree_slots(es, pl.dp), most = tree_most_rows(slots);
   const int R = q_len * (q_heads / kv_heads);
   pl.chunks = (R + most - 1) / most;
   pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
-  const TreeWaves wv = tree_waves(pl.dp, pl.chunk_rows);
+  const TreeWaves wv = tree_waves(slots, pl.chunk_rows);
   const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
-  const int64_t tiles = (cap + kTreeTile - 1) / kTreeTile;
+  const int tt = tree_tile(slots, wv.nw);
+  const int64_t tiles = (cap + tt - 1) / tt;
   if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced) {
     pl.grid = static_cast<int>(items);
     return pl;
   }
-  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(es, pl.dp, wv.nb, wv.nw);
+  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
   pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / kTreeMinCost)));
   pl.grid = pl.W;
   pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;
@@ -388,6 +391,7 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   p.chunks = pl.chunks;
   p.chunk_rows = pl.chunk_rows;
   p.W = pl.W;
+  p.last_block = static_cast<int32_t>(std::min<int64_t>(num_blocks - 1, INT32_MAX));
   p.pshift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();

@@ -35,6 +35,7 @@ struct TreeParams {
   int chunk_rows;
   int W;         // workgroups of a balanced launch; 0: one per item
   int pshift;    // log2(P), or -1
+  int32_t last_block;  // largest page id that a table entry can hold
 };
 
 // Runs the matrix-core kernel for padded head_dim dp (tree_mfma_*.hip); grid
@@ -116,10 +117,10 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 //
 // An item is a (sequence, kv-head, chunk of its rows); a row is a (query,
 // q-head of the kv-head's group).  A workgroup of NW waves goes through an
-// item's virtual tokens in tiles of 64: all waves load the tile's K and V rows
-// (registers, one tile ahead, then LDS), and wave (wr, wt) multiplies row
-// blocks [16 NB wr, 16 NB (wr + 1)) with tokens [64 / WT wt, ...), at most 32
-// of them at a time:
+// item's virtual tokens in tiles of TT: K and V rows come straight into a ring
+// of LDS buffers (global_load_lds), up to kBufs - 1 tiles ahead, and wave (wr,
+// wt) multiplies row blocks [16 NB wr, 16 NB (wr + 1)) with tokens [TT / WT
+// wt, ...), at most 32 of them at a time:
 //   scores   S^T = K Q^T, 16x16 blocks (A = K rows from LDS, B = Q from
 //            registers): a lane holds one row and 4 tokens per block
 //   softmax  per lane; the reference maximum of a row moves only when a score
@@ -129,8 +130,11 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 //            parts (split2): one rounding would add an error as large as the
 //            output's own.
 // Waves that share rows (WT > 1) merge at the end of an item through LDS.
+//
+// LDS rows are a power of two of 16-byte slots; chunk c of row r lies in slot
+// c ^ tree_swizzle(r), which spreads both the 16 rows of a K operand read and
+// the 32-byte pieces of a transposing V read over the 64 banks.
 
-constexpr int kTreeTile = 64;
 // Balanced launches: an item costs its tiles and one more (its queries, first
 // round trips and stores take about as long).
 constexpr int kTreeItemCost = 1;
@@ -140,43 +144,72 @@ constexpr int kTreeMinCost = 4;
 // Sequences whose prefix of costs fits the kernel's LDS.
 constexpr int kTreeMaxBalanced = 1024;
 
-// Bytes of LDS and resident workgroups per CU of an instance; es: element size.
-__host__ __device__ constexpr int tree_lds_bytes(int es, int dp, int bufs) {
-  return bufs * kTreeTile * (2 * dp * es + 16 + (es == 2 ? 32 : 16)) + 32;
+// Padded head_dim of an instance; es: element size.
+__host__ __device__ constexpr int tree_padded(int es, int d) {
+  return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 && es == 2 ? 192 : 256;
 }
-__host__ __device__ constexpr int tree_bufs(int es, int dp) { return tree_lds_bytes(es, dp, 2) <= 150 * 1024 ? 2 : 1; }
-__host__ __device__ constexpr int tree_occupancy(int es, int dp, int nb, int nw) {
-  // Registers: O, Q, the staged tile, scores and weights.
-  const int regs = 4 * nb * (dp / 16) + 4 * nb * (dp * es / 64) + 32 * dp * es / 64 / nw + 24 * nb;
-  const int by_regs = (regs > 210 ? 1 : regs > 90 ? 2 : regs > 64 ? 3 : 4) * 4 / nw;
-  const int by_lds = 160 * 1024 / (tree_lds_bytes(es, dp, tree_bufs(es, dp)) + 8 * kTreeMaxBalanced);
-  const int n = by_lds < by_regs ? by_lds : by_regs;
-  return n < 1 ? 1 : n;
+// 16-byte slots of an LDS row.
+__host__ __device__ constexpr int tree_slots(int es, int dp) {
+  return dp * es <= 128 ? 8 : dp * es <= 256 ? 16 : dp * es <= 512 ? 32 : 64;
+}
+// Tokens of a tile: a wave works on 16, 32 or 64 of them, so that what it does
+// once per tile stays small beside its products.
+__host__ __device__ constexpr int tree_tile(int slots, int nw) {
+  return slots == 64 ? 32 : slots <= 16 && nw == 8 ? 128 : 64;
+}
+// The most rows of a chunk: what the registers hold.
+__host__ __device__ constexpr int tree_most_rows(int slots) { return slots <= 16 ? 256 : slots == 32 ? 128 : 32; }
+
+// Row blocks per wave, waves along the rows and waves of a workgroup for a
+// chunk of rows.  Either two workgroups of four waves are resident on a CU or
+// one of eight: one wave's products run under another's softmax.
+struct TreeWaves {
+  int nb, wr, nw;
+};
+__host__ __device__ constexpr TreeWaves tree_waves(int slots, int rows) {
+  return slots == 64    ? TreeWaves{1, 2, 4}
+         : rows <= 16   ? TreeWaves{1, 1, 4}
+         : rows <= 32   ? TreeWaves{2, 1, 4}
+         : slots == 32  ? (rows <= 64 ? TreeWaves{1, 4, 8} : TreeWaves{1, 8, 8})
+         : rows <= 64   ? TreeWaves{2, 2, 4}
+         : rows <= 128  ? TreeWaves{2, 4, 8}
+                        : TreeWaves{2, 8, 8};
+}
+__host__ __device__ constexpr int tree_bufs(int slots, int nw) { return nw == 8 && slots == 8 ? 4 : 2; }
+__host__ __device__ constexpr int tree_lds_bytes(int slots, int nw) {
+  return tree_bufs(slots, nw) * 2 * tree_tile(slots, nw) * slots * 16 + 32;
+}
+// Resident workgroups per CU, which the launch bounds ask for.
+__host__ __device__ constexpr int tree_occupancy(int slots, int nb, int nw) {
+  const int by_lds = 160 * 1024 / (tree_lds_bytes(slots, nw) + 8 * kTreeMaxBalanced);
+  const int by_regs = nw == 8 ? 1 : slots >= 32 ? 1 : slots == 8 && nb == 1 ? 3 : 2;
+  return by_lds < by_regs ? by_lds : by_regs;
+}
+
+__device__ __forceinline__ int tree_swizzle(int slots, int row) {
+  return slots == 8 ? 2 * ((row >> 1) & 3) + ((row >> 3) & 1) : 2 * (row & 7) + ((row >> 3) & 1);
 }
 
 template <int DT, int DP, int NB, int WR, int NW>
 struct TreeShape {
-  static constexpr int kWT = NW / WR;
   static constexpr int kES = DT == QD_DTYPE_F32 ? 4 : 2;
-  static constexpr int kRow = DP * kES;                      // bytes of a head's row, padded
-  // Row strides in LDS: rows 16 bytes (K) and 32 bytes (V, two lanes' worth of
-  // a transposing read) further round the 64 banks each.
-  static constexpr int kKS = kRow + 16;
-  static constexpr int kVS = kRow + (kES == 2 ? 32 : 16);
-  static constexpr int kBuf = kTreeTile * (kKS + kVS);
-  static constexpr int kBufs = tree_bufs(kES, DP);
-  static constexpr int kChunks = kRow / 16;                  // 16-byte chunks of a row
-  static constexpr int kLoadRows = kTreeTile / NW;           // rows that a wave loads
-  static constexpr int kPass = (kLoadRows * kChunks + 63) / 64;
-  static constexpr bool kEven = kLoadRows * kChunks % 64 == 0;
-  static constexpr int kSteps = kRow / 64;
-  static constexpr int kTW = kTreeTile / kWT;                // tokens of a wave in a tile
+  static constexpr int kSlots = tree_slots(kES, DP);
+  static constexpr int TT = tree_tile(kSlots, NW);
+  static constexpr int kWT = NW / WR;
+  static constexpr int kRow = kSlots * 16;                   // bytes of an LDS row
+  static constexpr int kTile = TT * kRow;                    // bytes of K or V
+  static constexpr int kBufs = tree_bufs(kSlots, NW);
+  static constexpr int kLoadRows = TT / NW;                  // rows that a wave loads
+  static constexpr int kLoads = kLoadRows * kSlots / 64;     // its instructions, for K and for V
+  static constexpr int kSteps = DP * kES / 64;
+  static constexpr int kTW = TT / kWT;                       // tokens of a wave in a tile
   static constexpr int kTB = kTW >= 32 ? 2 : 1;              // 16-token blocks at a time
   static constexpr int kSub = kTW / (16 * kTB);
   static constexpr int kCols = DP / 16;
   static constexpr int kRows = 16 * NB * WR;                 // rows of a workgroup
-  static constexpr int kLds = tree_lds_bytes(kES, DP, kBufs);
-  static constexpr int kOcc = tree_occupancy(kES, DP, NB, NW);
+  static constexpr int kLds = tree_lds_bytes(kSlots, NW);
+  static constexpr int kOcc = tree_occupancy(kSlots, NB, NW);
+  static_assert(kTW >= 16 && kLoadRows * kSlots % 64 == 0 && kOcc >= 1, "waves do not fit the tile");
 };
 
 __device__ __forceinline__ float tree_max_groups(float x) {
@@ -193,14 +226,50 @@ __device__ __forceinline__ float tree_sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Workgroup barrier that waits for LDS traffic only: the tile being loaded
-// into registers stays in flight.
-__device__ __forceinline__ void tree_barrier() {
-  constexpr int imm = 0x3F | (0x3 << 14) | (0x7 << 4) | (0x0 << 8);  // vmcnt max, lgkmcnt(0)
+// Workgroup barrier for LDS traffic: waits for this wave's LDS operations and
+// for all but the last kLeft of its loads into LDS.
+template <int kLeft>
+__device__ __forceinline__ void tree_barrier_loads() {
+  static_assert(kLeft >= 0 && kLeft < 64, "vmcnt is 6 bits");
+  constexpr int imm = (kLeft & 0xF) | ((kLeft >> 4) << 14) | (0x7 << 4) | (0x0 << 8);  // lgkmcnt(0)
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(imm);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void tree_barrier() { tree_barrier_loads<63>(); }
+
+// 16 bytes per lane from `src` to LDS bytes lds + 16 lane.  Written in assembly
+// so that the compiler does not wait for it before LDS reads of other buffers:
+// tree_barrier_loads does.  At least one lane is active (the loads of a tile
+// are counted).  STREAM: not kept in the caches.
+template <bool STREAM>
+__device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+
+// The same from base + off (base wave-uniform).
+template <bool STREAM>
+__device__ __forceinline__ void tree_load_lds(const char* base, uint32_t off, uint32_t lds) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+
+__device__ __forceinline__ uint32_t tree_lds_address(const char* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
+}
+
+// A table entry at a wave-uniform place, through the scalar cache: a vector
+// load would complete only after the tiles in flight.
+__device__ __forceinline__ int32_t tree_scalar_load(const int32_t* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
 // Four transposed 16-bit elements: lane (g4, r16) of the wave gets column r16
@@ -238,9 +307,12 @@ __device__ __forceinline__ bool drop_not_finite(u32x4& x) {
 }
 
 // Tokens [0, sinks) and [lo, len) and nd drafted ones of an item: what its
-// rows see at most.
+// rows see at most (first tokens below `seen_sinks`, the others from `seen_lo`
+// on), widened to whole groups of 16 tokens where pages hold whole groups: a
+// wave then loads its rows from one page.
 struct Span {
   int len, lo, sinks, nd, n;
+  int seen_lo, seen_sinks;
 };
 
 __device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
@@ -250,13 +322,22 @@ __device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
   // The first query's window is the earliest: position len, or len - 1
   // without a mask.
   const int64_t lo = p.window > 0 ? static_cast<int64_t>(s.len) + (p.mask ? 1 : 0) - p.window : 0;
-  s.lo = static_cast<int>(lo < 0 ? 0 : lo < s.len ? lo : s.len);
-  s.sinks = min(p.sinks, s.lo);
+  s.seen_lo = static_cast<int>(lo < 0 ? 0 : lo < s.len ? lo : s.len);
+  s.seen_sinks = min(p.sinks, s.seen_lo);
+  s.lo = s.seen_lo;
+  s.sinks = s.seen_sinks;
+  if (p.P % 16 == 0) {
+    s.lo &= ~15;
+    s.sinks = min((s.sinks + 15) & ~15, s.lo);
+  }
   s.n = s.sinks + s.len - s.lo + s.nd;
   return s;
 }
 
-__device__ __forceinline__ int span_tiles(const Span& s) { return (s.n + kTreeTile - 1) / kTreeTile; }
+template <int TT>
+__device__ __forceinline__ int span_tiles(const Span& s) {
+  return (s.n + TT - 1) / TT;
+}
 
 template <int DT, int DP, int NB, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW / 4)) void tree_mfma_kernel(TreeParams p) {
@@ -271,8 +352,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   constexpr float kLazy = 8.f;
   extern __shared__ __align__(16) char smem[];
   // Tokens with non-finite values that not all rows see: drafted ones, and
-  // those at the window's edge (bit i: token lo + i).
-  unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * Sh::kBuf);
+  // those at the window's edge (bit i: token seen_lo + i).
+  unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * 2 * Sh::kTile);
   int64_t* incl = reinterpret_cast<int64_t*>(smem + Sh::kLds);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
@@ -334,86 +415,140 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    auto flip = [](const char* at, int bits) {  // swizzled slots: the chunk's bits are exchanged
+      return smem + (static_cast<uint32_t>(at - smem) ^ bits);
+    };
     const int context = sp.sinks + sp.len - sp.lo;
-    const int edge = sp.sinks + max(lo_max - sp.lo, 0);  // virtual tokens [sinks, edge): only in some rows' windows
+    const int edge = sp.sinks + max(lo_max - sp.lo, 0);  // virtual tokens below: not in every row's window
     auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
-    // Lane's staged row of a tile: row kLoadRows wv + lane % kLoadRows.  Its
-    // page is looked up a tile ahead of the loads.
-    auto staged = [&](int tile) { return kTreeTile * tile + Sh::kLoadRows * wv + (lane & (Sh::kLoadRows - 1)); };
     auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
-    auto look_up = [&](int tile) -> int32_t {
-      const int v = staged(tile);
-      if (!(v < context || (v < sp.n && ((any_seen >> (v - context)) & 1)))) return -1;
-      const int32_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page_of(token(v))];
-      return phys < 0 ? 0 : phys;
-    };
-    auto offset_of = [&](int tile, int32_t phys) -> int64_t {  // bytes, -1: not read
-      if (phys < 0) return -1;
-      const int tok = token(staged(tile));
-      const int64_t page = phys < p.num_blocks ? phys : p.num_blocks - 1;
-      return ((page * p.P + (tok - page_of(tok) * p.P)) * p.Hkv + h) * row_bytes;
-    };
-    u32x4 kreg[Sh::kPass], vreg[Sh::kPass];
-    auto load = [&](int64_t off) {
+    const int last_page = sp.n > 0 ? page_of(token(sp.n - 1)) : 0;
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.maxP;
+    auto clamped = [&](int32_t phys) { return static_cast<uint32_t>(min(max(phys, 0), p.last_block)); };
+    const uint32_t tok_bytes = static_cast<uint32_t>(p.Hkv) * row_bytes, page_bytes = tok_bytes * p.P;
+    // Place of this lane's 16 bytes of load i in a group of rows of one page.
+    // Slots past the head (head_dims below the row's power of two) are left
+    // out; K's are cleared once, below, since its products run over them.
+    const bool padded = row_bytes < Sh::kRow;
+    uint32_t lane_off[Sh::kLoads];
 #pragma unroll
-      for (int i = 0; i < Sh::kPass; ++i) {
-        const int c = 64 * i + lane;
-        const int row = c / Sh::kChunks, chunk = c % Sh::kChunks;
-        const int64_t at = __shfl(static_cast<long long>(off), row);
-        kreg[i] = vreg[i] = u32x4{0u, 0u, 0u, 0u};
-        if (at >= 0 && 16 * chunk < row_bytes && (Sh::kEven || row < Sh::kLoadRows)) {
-          kreg[i] = stream_load16(static_cast<const char*>(p.k) + at + 16 * chunk);
-          vreg[i] = stream_load16(static_cast<const char*>(p.v) + at + 16 * chunk);
+    for (int i = 0; i < Sh::kLoads; ++i) {
+      const int r = (64 * i + lane) / Sh::kSlots;
+      lane_off[i] = r * tok_bytes + h * row_bytes +
+                    16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r));
+    }
+    auto inside = [&](int i) {
+      const int r = (64 * i + lane) / Sh::kSlots;
+      return 16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
+    };
+    const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
+    // Starts the loads of this wave's rows of a tile.  Rows past the last token
+    // and drafted tokens that no row sees are loaded from some page of the
+    // sequence; they are cleared before they are used.
+    auto load_tile = [&](int tile, int slot) {
+      const int v0 = Sh::TT * tile + Sh::kLoadRows * wv;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
+      if (p.P % 16 == 0) {
+        const int tok0 = token(v0), page = page_of(tok0);
+        const uint32_t phys = clamped(tree_scalar_load(table + min(page, last_page)));
+        const uint64_t at = static_cast<uint64_t>(phys) * page_bytes + static_cast<uint32_t>(tok0 - page * p.P) * tok_bytes;
+        const char* k = static_cast<const char*>(p.k) + at;
+        const char* v = static_cast<const char*>(p.v) + at;
+        if (padded) {
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i)
+            if (inside(i)) {
+              tree_load_lds<true>(k, lane_off[i], to + 1024 * i);
+              tree_load_lds<true>(v, lane_off[i], to + Sh::kTile + 1024 * i);
+            }
+        } else if (p.chunks == 1) {
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<true>(k, lane_off[i], to + 1024 * i);
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<true>(v, lane_off[i], to + Sh::kTile + 1024 * i);
+        } else {  // the other chunks read the same rows
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<false>(k, lane_off[i], to + 1024 * i);
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<false>(v, lane_off[i], to + Sh::kTile + 1024 * i);
+        }
+        return;
+      }
+      // Any page size: lane r looks row r up.
+      const int tok = token(min(v0 + (lane & (Sh::kLoadRows - 1)), sp.n - 1));
+      int32_t phys = 0;
+#pragma unroll 1
+      for (int i = 0; i < Sh::kLoadRows; ++i) {
+        const int32_t x = tree_scalar_load(table + page_of(token(min(v0 + i, sp.n - 1))));
+        phys = lane == i ? x : phys;
+      }
+      const uint64_t row = static_cast<uint64_t>(clamped(phys)) * page_bytes +
+                           static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes;
+#pragma unroll
+      for (int i = 0; i < Sh::kLoads; ++i) {
+        const int r = (64 * i + lane) / Sh::kSlots;
+        const uint64_t at =
+            static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(row), r)) + (lane_off[i] - r * tok_bytes);
+        if (inside(i)) {
+          tree_load_lds<true>(static_cast<const char*>(p.k) + at, to + 1024 * i);
+          tree_load_lds<true>(static_cast<const char*>(p.v) + at, to + Sh::kTile + 1024 * i);
         }
       }
     };
 
     tree_barrier();  // the previous item's merge and the prefix are done with LDS
     if (tid < 2) bad_words[tid] = 0;
-    int32_t page = -1;
-    if (t0 < t1) {
-      page = look_up(t0);
-      load(offset_of(t0, page));
-    }
-    if (t0 + 1 < t1) page = look_up(t0 + 1);
-    tree_barrier();
-    for (int tile = t0; tile < t1; ++tile) {
-      char* buf = smem + (Sh::kBufs == 2 ? ((tile - t0) & 1) * Sh::kBuf : 0);
-      // Every row of the chunk sees all (existing) tokens of the tile.
-      const int first = kTreeTile * tile, stop = first + kTreeTile;
-      const bool whole_tile =
-          stop <= sp.sinks || ((first >= edge || edge == sp.sinks) && stop <= context) || (q0 == q1 && stop <= sp.n);
-      if (Sh::kBufs == 1 && tile > t0) tree_barrier();
-      if (!whole_tile && q0 != q1) {
-        // A weight of 0 would not hide Inf and NaN from the rows that do not
-        // see their token: they are left out here and join the rows that do at
-        // the item's end.
-#pragma unroll
-        for (int i = 0; i < Sh::kPass; ++i) {
-          const int v = first + Sh::kLoadRows * wv + (64 * i + lane) / Sh::kChunks;
-          if ((v >= context || (v >= sp.sinks && v < edge)) && drop_not_finite<DT>(vreg[i]))
-            atomicOr(&bad_words[v >= context ? 0 : 1], 1ull << (v >= context ? v - context : v - sp.sinks));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < Sh::kPass; ++i) {
-        const int c = 64 * i + lane;
-        const int row = Sh::kLoadRows * wv + c / Sh::kChunks, chunk = c % Sh::kChunks;
-        if (Sh::kEven || c < Sh::kLoadRows * Sh::kChunks) {
-          *reinterpret_cast<u32x4*>(buf + row * Sh::kKS + 16 * chunk) = kreg[i];
-          *reinterpret_cast<u32x4*>(buf + kTreeTile * Sh::kKS + row * Sh::kVS + 16 * chunk) = vreg[i];
-        }
-      }
-      if (tile + 1 < t1) {
-        load(offset_of(tile + 1, page));
-        if (tile + 2 < t1) page = look_up(tile + 2);
-      }
+    if (padded) {
+      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
+        *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
       tree_barrier();
+    }
+    for (int i = 0; i < Sh::kBufs - 1; ++i)
+      if (t0 + i < t1) load_tile(t0 + i, i);
+    // No register load is pending when the loop starts: the compiler would
+    // wait for it, and so for the tiles in flight, in every turn.
+    __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0)
+    int slot_now = 0;
+    for (int tile = t0; tile < t1; ++tile) {
+      // The tile has arrived, and every wave is done with the one before it.
+      const int left = min(t1 - 1 - tile, Sh::kBufs - 2);
+      if (Sh::kBufs == 2 || left == 0)
+        tree_barrier_loads<0>();
+      else if (left == 1)
+        tree_barrier_loads<2 * Sh::kLoads>();
+      else
+        tree_barrier_loads<4 * Sh::kLoads>();
+      if (tile + Sh::kBufs - 1 < t1) load_tile(tile + Sh::kBufs - 1, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1);
+      char* buf = smem + slot_now * 2 * Sh::kTile;
+      slot_now = slot_now == Sh::kBufs - 1 ? 0 : slot_now + 1;
+      // Every row of the chunk sees all (existing) tokens of the tile.
+      const int first = Sh::TT * tile, stop = first + Sh::TT;
+      const bool whole_tile = stop <= sp.seen_sinks || (first >= edge && (stop <= context || (p.T == 1 && stop <= sp.n)));
+      if (!whole_tile) {
+        // Values of tokens that no row sees are cleared.  Where only some rows
+        // see a token, a weight of 0 would not hide Inf and NaN from the
+        // others: they are left out here and join the rows that do at the
+        // item's end.
+        for (int i = tid; i < Sh::TT * Sh::kSlots; i += 64 * NW) {
+          const int v = first + i / Sh::kSlots, tok = token(v);
+          u32x4* at = reinterpret_cast<u32x4*>(buf + Sh::kTile) + i;
+          if (v < context ? tok >= sp.seen_sinks && tok < sp.seen_lo : v >= sp.n || !((any_seen >> (v - context)) & 1)) {
+            *at = u32x4{0u, 0u, 0u, 0u};
+          } else if (q0 != q1 && (v >= context || (tok >= sp.seen_lo && tok < lo_max))) {
+            u32x4 x = *at;
+            if (drop_not_finite<DT>(x)) {
+              *at = x;
+              atomicOr(&bad_words[v >= context ? 0 : 1], 1ull << (v >= context ? v - context : tok - sp.seen_lo));
+            }
+          }
+        }
+        tree_barrier();
+      }
 
 #pragma unroll 1
       for (int sub = 0; sub < Sh::kSub; ++sub) {
         const int wave_tok = Sh::kTW * wt + 16 * TB * sub;
-        const char* kb = buf + (wave_tok + r16) * Sh::kKS + 16 * g4;
+        const char* kb = buf + (wave_tok + r16) * Sh::kRow + 16 * (g4 ^ tree_swizzle(Sh::kSlots, r16));
         f32x4 s[TB][NB];
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb)
@@ -423,7 +558,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         for (int st = 0; st < Sh::kSteps; ++st)
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(kb + 16 * tb * Sh::kKS + 64 * st);
+            const u32x4 a = *reinterpret_cast<const u32x4*>(flip(kb, 64 * st) + 16 * tb * Sh::kRow);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
               if constexpr (k16) {
@@ -478,7 +613,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
               l[nb] += w;
             }
         }
-        const char* vb = buf + kTreeTile * Sh::kKS + wave_tok * Sh::kVS;
+        const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
         if constexpr (k16) {
           u32x2 hi[TB][NB], lw[TB][NB];
 #pragma unroll
@@ -503,17 +638,18 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
                 for (int i = 0; i < 4; ++i)
                   if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           }
-          const char* va = vb + (4 * g4 + (r16 >> 2)) * Sh::kVS + 8 * (r16 & 3);
+          const int vr = 4 * g4 + (r16 >> 2);
+          const char* va = vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tree_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1);
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
-            const u32x2 a0 = tree_tr_read(va + 32 * c);
+            const u32x2 a0 = tree_tr_read(flip(va, 32 * c));
             if constexpr (TB == 1) {
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, hi[0][nb], acc[c][nb]);
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, lw[0][nb], acc[c][nb]);
             } else {
-              const u32x2 a1 = tree_tr_read(va + 16 * Sh::kVS + 32 * c);
+              const u32x2 a1 = tree_tr_read(flip(va, 32 * c) + 16 * Sh::kRow);
               const u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
@@ -526,14 +662,15 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
             }
           }
         } else {
-          const char* va = vb + 4 * g4 * Sh::kVS + 4 * r16;
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c)
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float a = *reinterpret_cast<const float*>(va + (16 * tb + i) * Sh::kVS + 64 * c);
+                const int vr = 4 * g4 + i;
+                const char* va = vb + vr * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, vr)) + 4 * (r16 & 3);
+                const float a = *reinterpret_cast<const float*>(flip(va, 64 * c) + 16 * tb * Sh::kRow);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
                   acc[c][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[tb][nb][i], acc[c][nb], 0, 0, 0);
@@ -546,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     tree_barrier();
     if constexpr (WT > 1) {
       constexpr int kPart = NB * Sh::kCols * 1024 + NB * 512;  // acc, m, l of a wave
-      static_assert(WR * (WT - 1) * kPart <= Sh::kBufs * Sh::kBuf, "the waves' parts fit the tile buffers");
+      static_assert(WR * (WT - 1) * kPart <= Sh::kBufs * 2 * Sh::kTile, "the waves' parts fit the tile buffers");
       char* base = smem + (wr * (WT - 1) + wt - 1) * kPart;
       if (wt > 0) {
 #pragma unroll
@@ -596,7 +733,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         while (bad) {
           const int x = __builtin_ctzll(bad);
           bad &= bad - 1;
-          const int tok = kind == 0 ? sp.len + x : sp.lo + x;
+          const int tok = kind == 0 ? sp.len + x : sp.seen_lo + x;
           const char* src = static_cast<const char*>(p.v) + (pool_row(p, b, tok) * p.Hkv + h) * row_bytes;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
@@ -662,7 +799,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   int b = 0;
   if (p.W > 0) {
     for (int i = tid; i < p.B; i += 64 * NW) {
-      const int tiles = span_tiles(item_span(p, i));
+      const int tiles = span_tiles<Sh::TT>(item_span(p, i));
       incl[i] = tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
     }
     __syncthreads();
@@ -715,7 +852,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     } else {
       hc = static_cast<int>(blockIdx.x) % per_seq;
       sp = item_span(p, b);
-      t1 = tiles = span_tiles(sp);
+      t1 = tiles = span_tiles<Sh::TT>(sp);
     }
     if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * w + (t0 == 0 ? 1 : 0));
     pos += step;
@@ -732,7 +869,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
   const int per_seq = p.Hkv * p.chunks;
   const int item = blockIdx.x;
   const int b = item / per_seq, hc = item % per_seq;
-  const bool empty = span_tiles(item_span(p, b)) == 0;
+  const bool empty = item_span(p, b).n == 0;
   const int first = empty ? 0 : p.meta[2 * static_cast<int64_t>(item)];
   const int count = empty ? 0 : p.meta[2 * static_cast<int64_t>(item) + 1];
   if (count == 1) return;
@@ -793,41 +930,15 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Row blocks per wave, waves along the rows and waves of a workgroup for a
-// chunk of rows.  Above 64 rows eight waves share a tile, two per SIMD: one
-// wave's products run under the other's softmax.  Heads above 128 elements
-// leave no registers for that.
-struct TreeWaves {
-  int nb, wr, nw;
-};
-__host__ __device__ constexpr TreeWaves tree_waves(int dp, int rows) {
-  return rows <= 16   ? TreeWaves{1, 1, 4}
-         : rows <= 32 ? TreeWaves{2, 1, 4}
-         : rows <= 64 ? TreeWaves{2, 2, 4}
-         : dp > 128   ? TreeWaves{2, 4, 4}
-         : rows <= 128 ? TreeWaves{2, 4, 8}
-                       : TreeWaves{2, 8, 8};
-}
-// The most rows of a chunk.  fp32 above head_dim 128: 16, whose state is what
-// the registers hold.
-__host__ __device__ constexpr int tree_most_rows(int es, int dp) {
-  return es == 4 ? (dp > 128 ? 16 : 128) : dp > 128 ? 128 : 256;
-}
-
-template <int DT, int DP>
+template <int DT, int DP, int ROWS>
 hipError_t tree_launch_rows(const TreeParams& p, int grid, hipStream_t st) {
-  constexpr int kMost = tree_most_rows(DT == QD_DTYPE_F32 ? 4 : 2, DP);
-  if (p.chunk_rows <= 16) return tree_launch<DT, DP, 1, 1, 4>(p, grid, st);
-  if constexpr (kMost > 16) {
-    if (p.chunk_rows <= 32) return tree_launch<DT, DP, 2, 1, 4>(p, grid, st);
-    if (p.chunk_rows <= 64) return tree_launch<DT, DP, 2, 2, 4>(p, grid, st);
-    if constexpr (DP > 128) {
-      if (p.chunk_rows <= 128) return tree_launch<DT, DP, 2, 4, 4>(p, grid, st);
-    } else {
-      if (p.chunk_rows <= 128) return tree_launch<DT, DP, 2, 4, 8>(p, grid, st);
-      if constexpr (kMost > 128)
-        if (p.chunk_rows <= 256) return tree_launch<DT, DP, 2, 8, 8>(p, grid, st);
+  constexpr int kSlots = tree_slots(DT == QD_DTYPE_F32 ? 4 : 2, DP);
+  if constexpr (ROWS <= tree_most_rows(kSlots)) {
+    if (p.chunk_rows <= ROWS) {
+      constexpr TreeWaves w = tree_waves(kSlots, ROWS);
+      return tree_launch<DT, DP, w.nb, w.wr, w.nw>(p, grid, st);
     }
+    return tree_launch_rows<DT, DP, 2 * ROWS>(p, grid, st);
   }
   return hipErrorInvalidValue;
 }

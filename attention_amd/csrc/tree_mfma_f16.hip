@@ -6,11 +6,11 @@
 int qd_tree_mfma_launch_f16(const TreeParams& p, int dp, int grid, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dp) {
-    case 64: return tree_launch_rows<QD_DTYPE_F16, 64>(p, grid, st);
-    case 96: return tree_launch_rows<QD_DTYPE_F16, 96>(p, grid, st);
-    case 128: return tree_launch_rows<QD_DTYPE_F16, 128>(p, grid, st);
-    case 192: return tree_launch_rows<QD_DTYPE_F16, 192>(p, grid, st);
-    case 256: return tree_launch_rows<QD_DTYPE_F16, 256>(p, grid, st);
+    case 64: return tree_launch_rows<QD_DTYPE_F16, 64, 16>(p, grid, st);
+    case 96: return tree_launch_rows<QD_DTYPE_F16, 96, 16>(p, grid, st);
+    case 128: return tree_launch_rows<QD_DTYPE_F16, 128, 16>(p, grid, st);
+    case 192: return tree_launch_rows<QD_DTYPE_F16, 192, 16>(p, grid, st);
+    case 256: return tree_launch_rows<QD_DTYPE_F16, 256, 16>(p, grid, st);
     default: return hipErrorInvalidValue;
   }
 }

@@ -144,6 +144,7 @@ TREE_SHAPES = [
     (HF, 1, 12, 2, 1, 160, 16, [66], 3, 0, 0),
     (BF, 2, 3, 40, 1, 128, 16, [80, 81], 2, 0, 0),
     (BF, 1, 2, 71, 1, 64, 16, [333], 2, 0, 0),
+    (BF, 2, 3, 256, 1, 64, 16, [50, 200], 2, 0, 0),     # workgroups within one query
     (FP, 2, 8, 8, 2, 128, 16, [64, 300], 3, 0, 0),
     (FP, 2, 5, 4, 2, 64, 16, [0, 77], 2, 0, 0),
     (FP, 1, 20, 4, 1, 96, 8, [150], 3, 0, 0),
