@@ -52,12 +52,11 @@ __device__ __forceinline__ int64_t capacity(const TreeParams& p) {
   return min(static_cast<int64_t>(p.maxP) * p.P, static_cast<int64_t>(INT32_MAX - 255));
 }
 
-// Tokens of sequence b in its table.
-__device__ __forceinline__ int context_len(const TreeParams& p, int b) {
-  const int64_t cap = capacity(p);
-  const int64_t len = max(p.lens[b], 0);
-  return static_cast<int>(len < cap ? len : cap);
+// Tokens of a sequence in its table.
+__device__ __forceinline__ int clamp_len(const TreeParams& p, int32_t len) {
+  return static_cast<int>(min(static_cast<int64_t>(max(len, 0)), capacity(p)));
 }
+__device__ __forceinline__ int context_len(const TreeParams& p, int b) { return clamp_len(p, p.lens[b]); }
 
 __device__ __forceinline__ uint64_t draft_bits(const TreeParams& p, int b, int t) {
   const uint64_t m = static_cast<uint64_t>(p.mask[static_cast<int64_t>(b) * p.T + t]);
@@ -251,15 +250,17 @@ __device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
-// The same from base + off (base wave-uniform).
-template <bool STREAM>
-__device__ __forceinline__ void tree_load_lds(const char* base, uint32_t off, uint32_t lds) {
+// Load i of a run from base + off (base wave-uniform) to LDS bytes lds + 1024 i
+// + 16 lane.  The instruction's offset moves both sides, so `off` comes 1024 i
+// short; M0 (the LDS side) is set by tree_set_lds, once for a run.
+__device__ __forceinline__ void tree_set_lds(uint32_t lds) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"(lds) : "m0"); }
+template <bool STREAM, int I>
+__device__ __forceinline__ void tree_load_lds_run(const char* base, uint32_t off) {
+  static_assert(I >= 0 && I < 4, "the offset is 12 bits");
   if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory", "m0");
+    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2 nt" ::"v"(off), "s"(base), "n"(1024 * I) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory", "m0");
+    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" ::"v"(off), "s"(base), "n"(1024 * I) : "memory");
 }
 
 __device__ __forceinline__ uint32_t tree_lds_address(const char* p) {
@@ -306,6 +307,24 @@ __device__ __forceinline__ bool drop_not_finite(u32x4& x) {
   return bad;
 }
 
+// All loads of a wave for K or V of a tile: runs of four.
+template <bool STREAM, int LOADS>
+__device__ __forceinline__ void load_run_of(const char* base, const uint32_t (&off)[LOADS], uint32_t lds) {
+  if constexpr (LOADS <= 4) {
+    tree_set_lds(lds);
+    tree_load_lds_run<STREAM, 0>(base, off[0]);
+    if constexpr (LOADS > 1) tree_load_lds_run<STREAM, 1>(base, off[1] - 1024);
+    if constexpr (LOADS > 2) tree_load_lds_run<STREAM, 2>(base, off[2] - 2048);
+    if constexpr (LOADS > 3) tree_load_lds_run<STREAM, 3>(base, off[3] - 3072);
+  } else {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      tree_set_lds(__builtin_amdgcn_readfirstlane(lds + 1024 * i));
+      tree_load_lds_run<STREAM, 0>(base, off[i]);
+    }
+  }
+}
+
 // Tokens [0, sinks) and [lo, len) and nd drafted ones of an item: what its
 // rows see at most (first tokens below `seen_sinks`, the others from `seen_lo`
 // on), widened to whole groups of 16 tokens where pages hold whole groups: a
@@ -315,9 +334,9 @@ struct Span {
   int seen_lo, seen_sinks;
 };
 
-__device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
+__device__ __forceinline__ Span span_of(const TreeParams& p, int len) {
   Span s;
-  s.len = context_len(p, b);
+  s.len = len;
   s.nd = p.mask ? static_cast<int>(min(static_cast<int64_t>(p.T), capacity(p) - s.len)) : 0;
   // The first query's window is the earliest: position len, or len - 1
   // without a mask.
@@ -333,6 +352,8 @@ __device__ __forceinline__ Span item_span(const TreeParams& p, int b) {
   s.n = s.sinks + s.len - s.lo + s.nd;
   return s;
 }
+
+__device__ __forceinline__ Span item_span(const TreeParams& p, int b) { return span_of(p, context_len(p, b)); }
 
 template <int TT>
 __device__ __forceinline__ int span_tiles(const Span& s) {
@@ -368,6 +389,91 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     const int row0 = (hc % p.chunks) * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.R - row0);
     const int q0 = row0 / p.G, q1 = (row0 + rows - 1) / p.G;  // the chunk's queries
+    auto flip = [](const char* at, int bits) {  // swizzled slots: the chunk's bits are exchanged
+      return smem + (static_cast<uint32_t>(at - smem) ^ bits);
+    };
+    const int context = sp.sinks + sp.len - sp.lo;
+    auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
+    auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
+    const int last_page = sp.n > 0 ? page_of(token(sp.n - 1)) : 0;
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.maxP;
+    auto clamped = [&](int32_t phys) { return static_cast<uint32_t>(min(max(phys, 0), p.last_block)); };
+    const uint32_t tok_bytes = static_cast<uint32_t>(p.Hkv) * row_bytes, page_bytes = tok_bytes * p.P;
+    // Place of this lane's 16 bytes of load i in a group of rows of one page.
+    // Slots past the head (head_dims below the row's power of two) are left
+    // out; K's are cleared once, below, since its products run over them.
+    const bool padded = row_bytes < Sh::kRow;
+    uint32_t lane_off[Sh::kLoads];
+#pragma unroll
+    for (int i = 0; i < Sh::kLoads; ++i) {
+      const int r = (64 * i + lane) / Sh::kSlots;
+      lane_off[i] = r * tok_bytes + h * row_bytes +
+                    16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r));
+    }
+    auto inside = [&](int i) {
+      const int r = (64 * i + lane) / Sh::kSlots;
+      return 16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
+    };
+    const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
+    // Starts the loads of this wave's rows of a tile.  Rows past the last token
+    // and drafted tokens that no row sees are loaded from some page of the
+    // sequence; they are cleared before they are used.
+    auto load_tile = [&](int tile, int slot) {
+      const int v0 = Sh::TT * tile + Sh::kLoadRows * wv;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
+      if (p.P % 16 == 0) {
+        const int tok0 = token(v0), page = page_of(tok0);
+        const uint32_t phys = clamped(tree_scalar_load(table + min(page, last_page)));
+        const uint64_t at = static_cast<uint64_t>(phys) * page_bytes + static_cast<uint32_t>(tok0 - page * p.P) * tok_bytes;
+        const char* k = static_cast<const char*>(p.k) + at;
+        const char* v = static_cast<const char*>(p.v) + at;
+        if (padded) {
+#pragma unroll
+          for (int i = 0; i < Sh::kLoads; ++i)
+            if (inside(i)) {
+              tree_load_lds<true>(k + lane_off[i], to + 1024 * i);
+              tree_load_lds<true>(v + lane_off[i], to + Sh::kTile + 1024 * i);
+            }
+        } else if (p.chunks == 1) {
+          load_run_of<true>(k, lane_off, to);
+          load_run_of<true>(v, lane_off, to + Sh::kTile);
+        } else {  // the other chunks read the same rows
+          load_run_of<false>(k, lane_off, to);
+          load_run_of<false>(v, lane_off, to + Sh::kTile);
+        }
+        return;
+      }
+      // Any page size: lane r looks row r up.
+      const int tok = token(min(v0 + (lane & (Sh::kLoadRows - 1)), sp.n - 1));
+      int32_t phys = 0;
+#pragma unroll 1
+      for (int i = 0; i < Sh::kLoadRows; ++i) {
+        const int32_t x = tree_scalar_load(table + page_of(token(min(v0 + i, sp.n - 1))));
+        phys = lane == i ? x : phys;
+      }
+      const uint64_t row = static_cast<uint64_t>(clamped(phys)) * page_bytes +
+                           static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes;
+#pragma unroll
+      for (int i = 0; i < Sh::kLoads; ++i) {
+        const int r = (64 * i + lane) / Sh::kSlots;
+        const uint64_t at =
+            static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(row), r)) + (lane_off[i] - r * tok_bytes);
+        if (inside(i)) {
+          tree_load_lds<true>(static_cast<const char*>(p.k) + at, to + 1024 * i);
+          tree_load_lds<true>(static_cast<const char*>(p.v) + at, to + Sh::kTile + 1024 * i);
+        }
+      }
+    };
+
+    tree_barrier();  // the previous item's merge and the prefix are done with LDS
+    if (tid < 2) bad_words[tid] = 0;
+    if (padded) {
+      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
+        *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
+      tree_barrier();
+    }
+    for (int i = 0; i < Sh::kBufs - 1; ++i)
+      if (t0 + i < t1) load_tile(t0 + i, i);
     // Lane t: what query q0 + t sees (at most 64 queries).
     Row mine;
     mine.len = mine.lo = mine.sinks = 0;
@@ -415,96 +521,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto flip = [](const char* at, int bits) {  // swizzled slots: the chunk's bits are exchanged
-      return smem + (static_cast<uint32_t>(at - smem) ^ bits);
-    };
-    const int context = sp.sinks + sp.len - sp.lo;
     const int edge = sp.sinks + max(lo_max - sp.lo, 0);  // virtual tokens below: not in every row's window
-    auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
-    auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
-    const int last_page = sp.n > 0 ? page_of(token(sp.n - 1)) : 0;
-    const int32_t* table = p.table + static_cast<int64_t>(b) * p.maxP;
-    auto clamped = [&](int32_t phys) { return static_cast<uint32_t>(min(max(phys, 0), p.last_block)); };
-    const uint32_t tok_bytes = static_cast<uint32_t>(p.Hkv) * row_bytes, page_bytes = tok_bytes * p.P;
-    // Place of this lane's 16 bytes of load i in a group of rows of one page.
-    // Slots past the head (head_dims below the row's power of two) are left
-    // out; K's are cleared once, below, since its products run over them.
-    const bool padded = row_bytes < Sh::kRow;
-    uint32_t lane_off[Sh::kLoads];
-#pragma unroll
-    for (int i = 0; i < Sh::kLoads; ++i) {
-      const int r = (64 * i + lane) / Sh::kSlots;
-      lane_off[i] = r * tok_bytes + h * row_bytes +
-                    16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r));
-    }
-    auto inside = [&](int i) {
-      const int r = (64 * i + lane) / Sh::kSlots;
-      return 16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
-    };
-    const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
-    // Starts the loads of this wave's rows of a tile.  Rows past the last token
-    // and drafted tokens that no row sees are loaded from some page of the
-    // sequence; they are cleared before they are used.
-    auto load_tile = [&](int tile, int slot) {
-      const int v0 = Sh::TT * tile + Sh::kLoadRows * wv;
-      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
-      if (p.P % 16 == 0) {
-        const int tok0 = token(v0), page = page_of(tok0);
-        const uint32_t phys = clamped(tree_scalar_load(table + min(page, last_page)));
-        const uint64_t at = static_cast<uint64_t>(phys) * page_bytes + static_cast<uint32_t>(tok0 - page * p.P) * tok_bytes;
-        const char* k = static_cast<const char*>(p.k) + at;
-        const char* v = static_cast<const char*>(p.v) + at;
-        if (padded) {
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i)
-            if (inside(i)) {
-              tree_load_lds<true>(k, lane_off[i], to + 1024 * i);
-              tree_load_lds<true>(v, lane_off[i], to + Sh::kTile + 1024 * i);
-            }
-        } else if (p.chunks == 1) {
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<true>(k, lane_off[i], to + 1024 * i);
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<true>(v, lane_off[i], to + Sh::kTile + 1024 * i);
-        } else {  // the other chunks read the same rows
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<false>(k, lane_off[i], to + 1024 * i);
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i) tree_load_lds<false>(v, lane_off[i], to + Sh::kTile + 1024 * i);
-        }
-        return;
-      }
-      // Any page size: lane r looks row r up.
-      const int tok = token(min(v0 + (lane & (Sh::kLoadRows - 1)), sp.n - 1));
-      int32_t phys = 0;
-#pragma unroll 1
-      for (int i = 0; i < Sh::kLoadRows; ++i) {
-        const int32_t x = tree_scalar_load(table + page_of(token(min(v0 + i, sp.n - 1))));
-        phys = lane == i ? x : phys;
-      }
-      const uint64_t row = static_cast<uint64_t>(clamped(phys)) * page_bytes +
-                           static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes;
-#pragma unroll
-      for (int i = 0; i < Sh::kLoads; ++i) {
-        const int r = (64 * i + lane) / Sh::kSlots;
-        const uint64_t at =
-            static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(row), r)) + (lane_off[i] - r * tok_bytes);
-        if (inside(i)) {
-          tree_load_lds<true>(static_cast<const char*>(p.k) + at, to + 1024 * i);
-          tree_load_lds<true>(static_cast<const char*>(p.v) + at, to + Sh::kTile + 1024 * i);
-        }
-      }
-    };
-
-    tree_barrier();  // the previous item's merge and the prefix are done with LDS
-    if (tid < 2) bad_words[tid] = 0;
-    if (padded) {
-      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
-        *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
-      tree_barrier();
-    }
-    for (int i = 0; i < Sh::kBufs - 1; ++i)
-      if (t0 + i < t1) load_tile(t0 + i, i);
     // No register load is pending when the loop starts: the compiler would
     // wait for it, and so for the tiles in flight, in every turn.
     __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0)
@@ -607,12 +624,13 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float w = fast_exp2(fmaf(s[tb][nb][i], p.sl2, ref));
-              s[tb][nb][i] = w;
-              l[nb] += w;
-            }
+            for (int i = 0; i < 4; ++i) s[tb][nb][i] = fast_exp2(fmaf(s[tb][nb][i], p.sl2, ref));
         }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb)
+            l[nb] += (s[tb][nb][0] + s[tb][nb][1]) + (s[tb][nb][2] + s[tb][nb][3]);
         const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
         if constexpr (k16) {
           u32x2 hi[TB][NB], lw[TB][NB];
@@ -848,10 +866,10 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         meta[0] = static_cast<int32_t>(w);
         meta[1] = static_cast<int32_t>(last - w + 1);
       }
-      sp = item_span(p, b);
+      sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
     } else {
       hc = static_cast<int>(blockIdx.x) % per_seq;
-      sp = item_span(p, b);
+      sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
       t1 = tiles = span_tiles<Sh::TT>(sp);
     }
     if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * w + (t0 == 0 ? 1 : 0));
