@@ -142,6 +142,9 @@ constexpr int kTreeItemCost = 1;
 constexpr int kTreeMinCost = 4;
 // Sequences whose prefix of costs fits the kernel's LDS.
 constexpr int kTreeMaxBalanced = 1024;
+// Page ids that the kernel keeps in LDS at a time, one for each group of 16
+// tokens (one for each token where pages do not hold whole groups).
+constexpr int kTreePages = 1024;
 
 // Padded head_dim of an instance; es: element size.
 __host__ __device__ constexpr int tree_padded(int es, int d) {
@@ -176,7 +179,7 @@ __host__ __device__ constexpr TreeWaves tree_waves(int slots, int rows) {
 }
 __host__ __device__ constexpr int tree_bufs(int slots, int nw) { return nw == 8 && slots == 8 ? 4 : 2; }
 __host__ __device__ constexpr int tree_lds_bytes(int slots, int nw) {
-  return tree_bufs(slots, nw) * 2 * tree_tile(slots, nw) * slots * 16 + 32;
+  return tree_bufs(slots, nw) * 2 * tree_tile(slots, nw) * slots * 16 + 4 * kTreePages + 32;
 }
 // Resident workgroups per CU, which the launch bounds ask for.
 __host__ __device__ constexpr int tree_occupancy(int slots, int nb, int nw) {
@@ -205,6 +208,10 @@ struct TreeShape {
   static constexpr int kTB = kTW >= 32 ? 2 : 1;              // 16-token blocks at a time
   static constexpr int kSub = kTW / (16 * kTB);
   static constexpr int kCols = DP / 16;
+  // LDS reads ahead of their products, in steps of the scores and columns of
+  // the output.
+  static constexpr int kQkAhead = kSteps < 4 ? kSteps : 4;
+  static constexpr int kPvAhead = kES == 2 ? 4 : 2;
   static constexpr int kRows = 16 * NB * WR;                 // rows of a workgroup
   static constexpr int kLds = tree_lds_bytes(kSlots, NW);
   static constexpr int kOcc = tree_occupancy(kSlots, NB, NW);
@@ -225,6 +232,24 @@ __device__ __forceinline__ float tree_sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Or and maximum over the wave, in every lane: within rows of 16 lanes by DPP,
+// across them by lane swaps (no LDS round trips).
+template <int CTRL>
+__device__ __forceinline__ uint32_t tree_dpp(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(x), CTRL, 0xF, 0xF, false));
+}
+template <typename F>
+__device__ __forceinline__ uint32_t tree_wave_reduce(uint32_t x, F&& f) {
+  x = f(x, tree_dpp<0xB1>(x));   // quad_perm [1,0,3,2]
+  x = f(x, tree_dpp<0x4E>(x));   // quad_perm [2,3,0,1]
+  x = f(x, tree_dpp<0x141>(x));  // row_half_mirror
+  x = f(x, tree_dpp<0x140>(x));  // row_mirror
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return f(b[0], b[1]);
+}
+
 // Workgroup barrier for LDS traffic: waits for this wave's LDS operations and
 // for all but the last kLeft of its loads into LDS.
 template <int kLeft>
@@ -240,27 +265,53 @@ __device__ __forceinline__ void tree_barrier() { tree_barrier_loads<63>(); }
 
 // 16 bytes per lane from `src` to LDS bytes lds + 16 lane.  Written in assembly
 // so that the compiler does not wait for it before LDS reads of other buffers:
-// tree_barrier_loads does.  At least one lane is active (the loads of a tile
-// are counted).  STREAM: not kept in the caches.
+// tree_barrier_loads does.  M0 (the LDS side) is written and used within one
+// statement.  At least one lane is active (the loads of a tile are counted).
+// STREAM: not kept in the caches.
 template <bool STREAM>
 __device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
   if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
-// Load i of a run from base + off (base wave-uniform) to LDS bytes lds + 1024 i
-// + 16 lane.  The instruction's offset moves both sides, so `off` comes 1024 i
-// short; M0 (the LDS side) is set by tree_set_lds, once for a run.
-__device__ __forceinline__ void tree_set_lds(uint32_t lds) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"(lds) : "m0"); }
-template <bool STREAM, int I>
-__device__ __forceinline__ void tree_load_lds_run(const char* base, uint32_t off) {
-  static_assert(I >= 0 && I < 4, "the offset is 12 bits");
-  if constexpr (STREAM)
-    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2 nt" ::"v"(off), "s"(base), "n"(1024 * I) : "memory");
-  else
-    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" ::"v"(off), "s"(base), "n"(1024 * I) : "memory");
+// Up to four such loads from base + off[i] (base wave-uniform) to LDS bytes lds
+// + 1024 i + 16 lane.  The instruction's offset moves both sides, so off[i]
+// comes 1024 i short.
+template <bool STREAM, int N>
+__device__ __forceinline__ void tree_load_lds_run(const char* base, const uint32_t* off, uint32_t lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "runs of a wave");
+#define QD_LDS_LOAD(reg, at, policy) "\n\tglobal_load_lds_dwordx4 " reg ", %1 offset:" at policy
+#define QD_LDS_RUN(policy)                                                                                             \
+  if constexpr (N == 1)                                                                                                \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy)::"s"(lds), "s"(base), "v"(off[0])        \
+                 : "memory");                                                                                          \
+  else if constexpr (N == 2)                                                                                           \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy) QD_LDS_LOAD("%3", "1024", policy)::"s"(  \
+                     lds),                                                                                             \
+                 "s"(base), "v"(off[0]), "v"(off[1] - 1024)                                                            \
+                 : "memory");                                                                                          \
+  else                                                                                                                 \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy) QD_LDS_LOAD("%3", "1024", policy)        \
+                     QD_LDS_LOAD("%4", "2048", policy) QD_LDS_LOAD("%5", "3072", policy)::"s"(lds),                    \
+                 "s"(base), "v"(off[0]), "v"(off[1] - 1024), "v"(off[2] - 2048), "v"(off[3] - 3072)                    \
+                 : "memory")
+  if constexpr (STREAM) {
+    QD_LDS_RUN(" nt");
+  } else {
+    QD_LDS_RUN("");
+  }
+#undef QD_LDS_RUN
+#undef QD_LDS_LOAD
+}
+
+// All loads of a wave for K or V of a tile.
+template <bool STREAM, int LOADS>
+__device__ __forceinline__ void tree_load_lds_rows(const char* base, const uint32_t (&off)[LOADS], uint32_t lds) {
+#pragma unroll
+  for (int i = 0; i < LOADS; i += LOADS < 4 ? LOADS : 4)
+    tree_load_lds_run<STREAM, (LOADS < 4 ? LOADS : 4)>(base, off + i, lds + 1024 * i);
 }
 
 __device__ __forceinline__ uint32_t tree_lds_address(const char* p) {
@@ -305,24 +356,6 @@ __device__ __forceinline__ bool drop_not_finite(u32x4& x) {
     }
   }
   return bad;
-}
-
-// All loads of a wave for K or V of a tile: runs of four.
-template <bool STREAM, int LOADS>
-__device__ __forceinline__ void load_run_of(const char* base, const uint32_t (&off)[LOADS], uint32_t lds) {
-  if constexpr (LOADS <= 4) {
-    tree_set_lds(lds);
-    tree_load_lds_run<STREAM, 0>(base, off[0]);
-    if constexpr (LOADS > 1) tree_load_lds_run<STREAM, 1>(base, off[1] - 1024);
-    if constexpr (LOADS > 2) tree_load_lds_run<STREAM, 2>(base, off[2] - 2048);
-    if constexpr (LOADS > 3) tree_load_lds_run<STREAM, 3>(base, off[3] - 3072);
-  } else {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      tree_set_lds(__builtin_amdgcn_readfirstlane(lds + 1024 * i));
-      tree_load_lds_run<STREAM, 0>(base, off[i]);
-    }
-  }
 }
 
 // Tokens [0, sinks) and [lo, len) and nd drafted ones of an item: what its
@@ -375,6 +408,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   // Tokens with non-finite values that not all rows see: drafted ones, and
   // those at the window's edge (bit i: token seen_lo + i).
   unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * 2 * Sh::kTile);
+  int32_t* pages = reinterpret_cast<int32_t*>(bad_words + 4);
   int64_t* incl = reinterpret_cast<int64_t*>(smem + Sh::kLds);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
@@ -415,18 +449,39 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       return 16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
     };
     const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
-    // Starts the loads of this wave's rows of a tile.  Rows past the last token
-    // and drafted tokens that no row sees are loaded from some page of the
-    // sequence; they are cleared before they are used.
-    auto load_tile = [&](int tile, int slot) {
+    const bool grouped = p.P % 16 == 0;
+    // Fills the page list from a tile on; returns the first tile that it does
+    // not cover.
+    auto list_pages = [&](int tile) {
+      const int each = grouped ? 16 : 1;
+      const int until = min(sp.n, Sh::TT * t1);
+      for (int i = tid; i < kTreePages; i += 64 * NW) {
+        const int v = Sh::TT * tile + each * i;
+        if (v < until) pages[i] = min(max(table[page_of(token(v))], 0), p.last_block);
+      }
+      return tile + kTreePages * each / Sh::TT;
+    };
+    // Place of this wave's rows of a tile in the list that starts at tile
+    // `base`.  Groups past the last token take its page.
+    auto list_at = [&](int tile, int base) {
+      const int at = Sh::TT * (tile - base) + Sh::kLoadRows * wv;
+      return grouped ? min(at, sp.n - 1 - Sh::TT * base) / 16 : at;
+    };
+    // Starts the loads of this wave's rows of a tile, from page `phys` (grouped)
+    // or from the listed ones (`at`: this wave's first).  Rows past the last
+    // token and drafted tokens that no row sees are loaded from some page of
+    // the pool; they are cleared before they are used.
+    auto load_tile = [&](int tile, int slot, int32_t phys, int at) {
       const int v0 = Sh::TT * tile + Sh::kLoadRows * wv;
       const uint32_t to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
-      if (p.P % 16 == 0) {
-        const int tok0 = token(v0), page = page_of(tok0);
-        const uint32_t phys = clamped(tree_scalar_load(table + min(page, last_page)));
-        const uint64_t at = static_cast<uint64_t>(phys) * page_bytes + static_cast<uint32_t>(tok0 - page * p.P) * tok_bytes;
-        const char* k = static_cast<const char*>(p.k) + at;
-        const char* v = static_cast<const char*>(p.v) + at;
+      if (grouped) {
+        const int tok0 = token(v0);
+        const int64_t off = readlane_i64(  // the same in all lanes: scalar registers
+            static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(phys)) * page_bytes +
+                                 static_cast<uint32_t>(p.pshift >= 0 ? tok0 & (p.P - 1) : tok0 % p.P) * tok_bytes),
+            0);
+        const char* k = static_cast<const char*>(p.k) + off;
+        const char* v = static_cast<const char*>(p.v) + off;
         if (padded) {
 #pragma unroll
           for (int i = 0; i < Sh::kLoads; ++i)
@@ -435,62 +490,27 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
               tree_load_lds<true>(v + lane_off[i], to + Sh::kTile + 1024 * i);
             }
         } else if (p.chunks == 1) {
-          load_run_of<true>(k, lane_off, to);
-          load_run_of<true>(v, lane_off, to + Sh::kTile);
+          tree_load_lds_rows<true>(k, lane_off, to);
+          tree_load_lds_rows<true>(v, lane_off, to + Sh::kTile);
         } else {  // the other chunks read the same rows
-          load_run_of<false>(k, lane_off, to);
-          load_run_of<false>(v, lane_off, to + Sh::kTile);
+          tree_load_lds_rows<false>(k, lane_off, to);
+          tree_load_lds_rows<false>(v, lane_off, to + Sh::kTile);
         }
         return;
       }
-      // Any page size: lane r looks row r up.
-      const int tok = token(min(v0 + (lane & (Sh::kLoadRows - 1)), sp.n - 1));
-      int32_t phys = 0;
-#pragma unroll 1
-      for (int i = 0; i < Sh::kLoadRows; ++i) {
-        const int32_t x = tree_scalar_load(table + page_of(token(min(v0 + i, sp.n - 1))));
-        phys = lane == i ? x : phys;
-      }
-      const uint64_t row = static_cast<uint64_t>(clamped(phys)) * page_bytes +
-                           static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes;
 #pragma unroll
       for (int i = 0; i < Sh::kLoads; ++i) {
         const int r = (64 * i + lane) / Sh::kSlots;
-        const uint64_t at =
-            static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(row), r)) + (lane_off[i] - r * tok_bytes);
+        const int v = min(v0 + r, sp.n - 1), tok = token(v);
+        const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(pages[at + v - v0])) * page_bytes +
+                             static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes + (lane_off[i] - r * tok_bytes);
         if (inside(i)) {
-          tree_load_lds<true>(static_cast<const char*>(p.k) + at, to + 1024 * i);
-          tree_load_lds<true>(static_cast<const char*>(p.v) + at, to + Sh::kTile + 1024 * i);
+          tree_load_lds<true>(static_cast<const char*>(p.k) + off, to + 1024 * i);
+          tree_load_lds<true>(static_cast<const char*>(p.v) + off, to + Sh::kTile + 1024 * i);
         }
       }
     };
 
-    tree_barrier();  // the previous item's merge and the prefix are done with LDS
-    if (tid < 2) bad_words[tid] = 0;
-    if (padded) {
-      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
-        *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
-      tree_barrier();
-    }
-    for (int i = 0; i < Sh::kBufs - 1; ++i)
-      if (t0 + i < t1) load_tile(t0 + i, i);
-    // Lane t: what query q0 + t sees (at most 64 queries).
-    Row mine;
-    mine.len = mine.lo = mine.sinks = 0;
-    mine.seen = 0;
-    bool sees = false;
-    if (q0 + lane <= q1) {
-      sees = !p.mask || draft_bits(p, b, q0 + lane) != 0;
-      if (sees) mine = row_view(p, b, q0 + lane);
-    }
-    uint64_t any_seen = mine.seen;
-    int lo_max = sees ? mine.lo : 0;
-    for (int off = 32; off >= 1; off >>= 1) {
-      any_seen |= static_cast<uint64_t>(__shfl_xor(static_cast<long long>(any_seen), off));
-      lo_max = max(lo_max, __shfl_xor(lo_max, off));
-    }
-    any_seen = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(any_seen), 0));
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
     // This lane's rows: what they see is taken from lane (query - q0).
     int query[NB];
     bool real[NB];
@@ -511,6 +531,44 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         qf[nb][s] = real[nb] && at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
       }
     }
+    // The first tiles.  Their pages come through the scalar cache where one
+    // page serves a wave's rows; the list takes a barrier.
+    tree_barrier();  // the previous item's merge and the prefix are done with LDS
+    if (tid < 2) bad_words[tid] = 0;
+    if (padded) {
+      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
+        *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    int listed = 0, list_base = t0;  // the list covers tiles [list_base, listed)
+    if (!grouped && t0 < t1) listed = list_pages(t0);
+    if (padded || !grouped) tree_barrier();
+    for (int i = 0; i < Sh::kBufs - 1; ++i)
+      if (t0 + i < t1) {
+        int32_t phys = 0;
+        if (grouped)
+          phys = min(max(tree_scalar_load(table + min(page_of(token(Sh::TT * (t0 + i) + Sh::kLoadRows * wv)), last_page)), 0),
+                     p.last_block);
+        load_tile(t0 + i, i, phys, list_at(t0 + i, t0));
+      }
+    if (grouped && t0 + Sh::kBufs - 1 < t1) {
+      list_base = t0 + Sh::kBufs - 1;
+      listed = list_pages(list_base);
+    }
+    // Lane t: what query q0 + t sees (at most 64 queries).
+    Row mine;
+    mine.len = mine.lo = mine.sinks = 0;
+    mine.seen = 0;
+    bool sees = false;
+    if (q0 + lane <= q1) {
+      sees = !p.mask || draft_bits(p, b, q0 + lane) != 0;
+      if (sees) mine = row_view(p, b, q0 + lane);
+    }
+    auto bits_or = [](uint32_t x, uint32_t y) { return x | y; };
+    const uint32_t seen_low = __builtin_amdgcn_readfirstlane(tree_wave_reduce(static_cast<uint32_t>(mine.seen), bits_or));
+    const uint32_t seen_high = __builtin_amdgcn_readfirstlane(tree_wave_reduce(static_cast<uint32_t>(mine.seen >> 32), bits_or));
+    const uint64_t any_seen = static_cast<uint64_t>(seen_high) << 32 | seen_low;
+    const int lo_max = __builtin_amdgcn_readfirstlane(
+        tree_wave_reduce(sees ? mine.lo : 0, [](uint32_t x, uint32_t y) { return x > y ? x : y; }));
     f32x4 acc[Sh::kCols][NB];
     float m[NB], l[NB];
 #pragma unroll
@@ -535,7 +593,17 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         tree_barrier_loads<2 * Sh::kLoads>();
       else
         tree_barrier_loads<4 * Sh::kLoads>();
-      if (tile + Sh::kBufs - 1 < t1) load_tile(tile + Sh::kBufs - 1, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1);
+      const int next = tile + Sh::kBufs - 1;
+      if (next < t1) {
+        if (next >= listed) {
+          list_base = next;
+          listed = list_pages(next);
+          tree_barrier();
+        }
+        const int at = list_at(next, list_base);
+        load_tile(next, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1,
+                  grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
+      }
       char* buf = smem + slot_now * 2 * Sh::kTile;
       slot_now = slot_now == Sh::kBufs - 1 ? 0 : slot_now + 1;
       // Every row of the chunk sees all (existing) tokens of the tile.
@@ -571,11 +639,23 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // Operands are read ahead of their products: a product takes 16 cycles,
+        // an LDS read here well over 100.  The scheduling barriers keep the
+        // distance.
+        u32x4 ka[Sh::kQkAhead][TB];
+        auto read_k = [&](int st) {
 #pragma unroll
-        for (int st = 0; st < Sh::kSteps; ++st)
+          for (int tb = 0; tb < TB; ++tb)
+            ka[st % Sh::kQkAhead][tb] = *reinterpret_cast<const u32x4*>(flip(kb, 64 * st) + 16 * tb * Sh::kRow);
+        };
+#pragma unroll
+        for (int st = 0; st < Sh::kQkAhead; ++st) read_k(st);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < Sh::kSteps; ++st) {
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(flip(kb, 64 * st) + 16 * tb * Sh::kRow);
+            const u32x4 a = ka[st % Sh::kQkAhead][tb];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
               if constexpr (k16) {
@@ -588,6 +668,34 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
               }
             }
           }
+          if (st + Sh::kQkAhead < Sh::kSteps) read_k(st + Sh::kQkAhead);
+          if (Sh::kQkAhead < Sh::kSteps) __builtin_amdgcn_sched_barrier(0);
+        }
+        // V^T of the first columns, in flight during the softmax.
+        const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
+        const int vr = 4 * g4 + (k16 ? r16 >> 2 : 0);
+        const char* va =
+            k16 ? vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tree_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1) : vb;
+        u32x2 vf[Sh::kPvAhead][2 * TB];  // fp32: 4 TB values
+        auto read_v = [&](int c) {
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb) {
+            if constexpr (k16) {
+              vf[c % Sh::kPvAhead][tb] = tree_tr_read(flip(va, 32 * c) + 16 * tb * Sh::kRow);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = 4 * g4 + i;
+                const char* at = vb + row * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, row)) + 4 * (r16 & 3);
+                vf[c % Sh::kPvAhead][2 * tb + i / 2][i % 2] =
+                    *reinterpret_cast<const uint32_t*>(flip(at, 64 * c) + 16 * tb * Sh::kRow);
+              }
+            }
+          }
+        };
+#pragma unroll
+        for (int c = 0; c < Sh::kPvAhead; ++c) read_v(c);
+        __builtin_amdgcn_sched_barrier(0);
         if (!whole_tile) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
@@ -631,7 +739,6 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb)
             l[nb] += (s[tb][nb][0] + s[tb][nb][1]) + (s[tb][nb][2] + s[tb][nb][3]);
-        const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
         if constexpr (k16) {
           u32x2 hi[TB][NB], lw[TB][NB];
 #pragma unroll
@@ -656,19 +763,17 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
                 for (int i = 0; i < 4; ++i)
                   if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           }
-          const int vr = 4 * g4 + (r16 >> 2);
-          const char* va = vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tree_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
-            const u32x2 a0 = tree_tr_read(flip(va, 32 * c));
+            const u32x2* f = vf[c % Sh::kPvAhead];
             if constexpr (TB == 1) {
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, hi[0][nb], acc[c][nb]);
+              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(f[0], hi[0][nb], acc[c][nb]);
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(a0, lw[0][nb], acc[c][nb]);
+              for (int nb = 0; nb < NB; ++nb) acc[c][nb] = MfmaOps<DT>::pv(f[0], lw[0][nb], acc[c][nb]);
             } else {
-              const u32x2 a1 = tree_tr_read(flip(va, 32 * c) + 16 * Sh::kRow);
-              const u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
+              const u32x4 a = {f[0][0], f[0][1], f[1][0], f[1][1]};
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
                 acc[c][nb] =
@@ -678,21 +783,28 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
                 acc[c][nb] =
                     MfmaOps<DT>::mma32(a, u32x4{lw[0][nb][0], lw[0][nb][1], lw[1][nb][0], lw[1][nb][1]}, acc[c][nb]);
             }
+            if (c + Sh::kPvAhead < Sh::kCols) {
+              read_v(c + Sh::kPvAhead);
+              __builtin_amdgcn_sched_barrier(0);
+            }
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c)
+          for (int c = 0; c < Sh::kCols; ++c) {
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int vr = 4 * g4 + i;
-                const char* va = vb + vr * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, vr)) + 4 * (r16 & 3);
-                const float a = *reinterpret_cast<const float*>(flip(va, 64 * c) + 16 * tb * Sh::kRow);
+                const float a = __uint_as_float(vf[c % Sh::kPvAhead][2 * tb + i / 2][i % 2]);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
                   acc[c][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[tb][nb][i], acc[c][nb], 0, 0, 0);
               }
+            if (c + Sh::kPvAhead < Sh::kCols) {
+              read_v(c + Sh::kPvAhead);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         }
       }
     }
@@ -811,37 +923,49 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     }
   };
 
-  // Balanced: the costs of all items in a row, cut into equal ranges.
-  int64_t total = 0, used = 1, pos = 0, end = 1;
+  // Balanced: the costs of all items in a row, cut into equal ranges.  Up to 64
+  // sequences, every wave keeps the prefix of the costs in its lanes.
+  int64_t total = 0, used = 1, pos = 0, end = 1, mine_incl = 0;
   const int64_t w = blockIdx.x;
   int b = 0;
+  const bool in_lanes = p.B <= 64;
+  auto prefix = [&](int i) { return readlane_i64(in_lanes ? mine_incl : incl[i], in_lanes ? i : 0); };
   if (p.W > 0) {
-    for (int i = tid; i < p.B; i += 64 * NW) {
+    auto cost_of = [&](int i) -> int64_t {
       const int tiles = span_tiles<Sh::TT>(item_span(p, i));
-      incl[i] = tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
-    }
-    __syncthreads();
-    if (wv == 0) {
-      int64_t carry = 0;
-      for (int base = 0; base < p.B; base += 64) {
-        const int i = base + lane;
-        const int64_t v = carry + wave_incl_scan_i64(i < p.B ? incl[i] : 0, lane);
-        if (i < p.B) incl[i] = v;
-        carry = __shfl(v, 63);
+      return tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
+    };
+    if (in_lanes) {
+      mine_incl = wave_incl_scan_small(lane < p.B ? cost_of(lane) : 0, lane);
+    } else {
+      for (int i = tid; i < p.B; i += 64 * NW) incl[i] = cost_of(i);
+      __syncthreads();
+      if (wv == 0) {
+        int64_t carry = 0;
+        for (int base = 0; base < p.B; base += 64) {
+          const int i = base + lane;
+          const int64_t v = carry + wave_incl_scan_small(i < p.B ? incl[i] : 0, lane);
+          if (i < p.B) incl[i] = v;
+          carry = readlane_i64(v, 63);
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
-    total = readlane_i64(incl[p.B - 1], 0);
+    total = prefix(p.B - 1);
     used = min(static_cast<int64_t>(p.W), max<int64_t>(1, total / kTreeMinCost));
     if (w >= used) return;
-    pos = w * total / used;
-    end = (w + 1) * total / used;
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+    pos = div_nonneg(w * total, used);
+    end = div_nonneg((w + 1) * total, used);
+    if (in_lanes) {
+      b = __builtin_popcountll(__ballot(lane < p.B && mine_incl <= pos));
+    } else {
+      int lo = 0, hi = p.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
     }
-    b = __builtin_amdgcn_readfirstlane(lo);
   } else {
     b = static_cast<int>(blockIdx.x) / per_seq;
   }
@@ -849,10 +973,10 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     int hc, t0 = 0, t1, tiles, step = 1;
     Span sp;
     if (p.W > 0) {
-      while (readlane_i64(incl[b], 0) <= pos) ++b;
-      const int64_t before = b > 0 ? readlane_i64(incl[b - 1], 0) : 0;
-      const int cost = static_cast<int>((readlane_i64(incl[b], 0) - before) / per_seq);
-      hc = static_cast<int>((pos - before) / cost);
+      while (prefix(b) <= pos) ++b;
+      const int64_t before = b > 0 ? prefix(b - 1) : 0;
+      const int cost = static_cast<int>(div_nonneg(prefix(b) - before, per_seq));
+      hc = static_cast<int>(div_nonneg(pos - before, cost));
       const int off = static_cast<int>((pos - before) - static_cast<int64_t>(hc) * cost);
       const int stop = static_cast<int>(min(static_cast<int64_t>(cost), off + (end - pos)));
       t0 = max(0, off - kTreeItemCost);
@@ -861,7 +985,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       step = stop - off;
       if (t1 > t0 && t0 == 0 && tid == 0) {
         const int64_t first = before + static_cast<int64_t>(hc) * cost + kTreeItemCost;  // the item's first tile
-        const int64_t last = ((first + tiles) * used - 1) / total;                       // holder of its last tile
+        const int64_t last = div_nonneg((first + tiles) * used - 1, total);              // holder of its last tile
         int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * per_seq + hc);
         meta[0] = static_cast<int32_t>(w);
         meta[1] = static_cast<int32_t>(last - w + 1);
