@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void tree_generic_kernel(TreeParams p) {
   const int h = hq / (p.Hq / p.Hkv);
   const S* q = static_cast<const S*>(p.q) + row * p.D;
   for (int d = tid; d < p.D; d += 256) qs[d] = E::to_f(q[d]);
-  const Row r = row_view(p, b, t);
+  const Row r = row_view(p, b, context_len(p, b), p.mask ? draft_bits(p, b, t) : 0);
   __syncthreads();
   const int drafts = r.seen ? 64 - __builtin_clzll(r.seen) : 0;
   const int context = r.sinks + r.len - r.lo;
@@ -166,7 +166,8 @@ bool tree_shape_ok(int batch, int q_len, int q_heads, int kv_heads, int head_dim
 int64_t visible_capacity(int q_len, int block_size, int max_pages, int has_mask, int window, int sinks) {
   const int64_t cap = static_cast<int64_t>(block_size) * max_pages;
   if (window <= 0) return cap;
-  return std::min(cap, static_cast<int64_t>(window) + sinks + (has_mask ? q_len : 0));
+  // Widened to whole groups of 16 tokens at three ends (item_span).
+  return std::min(cap, static_cast<int64_t>(window) + sinks + (has_mask ? q_len : 0) + 48);
 }
 
 // Context splits of the VALU kernel: enough workgroups to fill the card, at
@@ -228,7 +229,7 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
   const int tt = tree_tile(slots, wv.nw);
   const int64_t tiles = (cap + tt - 1) / tt;
-  if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced) {
+  if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced || items * (tiles + kTreeItemCost) > INT32_MAX) {
     pl.grid = static_cast<int>(items);
     return pl;
   }
@@ -391,6 +392,7 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   p.chunks = pl.chunks;
   p.chunk_rows = pl.chunk_rows;
   p.W = pl.W;
+  p.capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(block_size) * max_pages, INT32_MAX - 255));
   p.last_block = static_cast<int32_t>(std::min<int64_t>(num_blocks - 1, INT32_MAX));
   p.pshift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -36,6 +36,9 @@ struct TreeParams {
   int W;         // workgroups of a balanced launch; 0: one per item
   int pshift;    // log2(P), or -1
   int32_t last_block;  // largest page id that a table entry can hold
+  // Tokens of a table row; the last 256 below 2^31 are left out, so that token
+  // numbers, their tiles and sums with a window or 64 drafts fit 32 bits.
+  int32_t capacity;
 };
 
 // Runs the matrix-core kernel for padded head_dim dp (tree_mfma_*.hip); grid
@@ -46,16 +49,8 @@ int qd_tree_mfma_launch_bf16(const TreeParams& p, int dp, int grid, void* stream
 
 namespace {
 
-// Tokens of a table row; the last 256 below 2^31 are left out, so that token
-// numbers and their tiles fit 32 bits.
-__device__ __forceinline__ int64_t capacity(const TreeParams& p) {
-  return min(static_cast<int64_t>(p.maxP) * p.P, static_cast<int64_t>(INT32_MAX - 255));
-}
-
 // Tokens of a sequence in its table.
-__device__ __forceinline__ int clamp_len(const TreeParams& p, int32_t len) {
-  return static_cast<int>(min(static_cast<int64_t>(max(len, 0)), capacity(p)));
-}
+__device__ __forceinline__ int clamp_len(const TreeParams& p, int32_t len) { return min(max(len, 0), p.capacity); }
 __device__ __forceinline__ int context_len(const TreeParams& p, int b) { return clamp_len(p, p.lens[b]); }
 
 __device__ __forceinline__ uint64_t draft_bits(const TreeParams& p, int b, int t) {
@@ -71,32 +66,32 @@ struct Row {
   uint64_t seen;
 };
 
-__device__ __forceinline__ Row row_view(const TreeParams& p, int b, int t) {
+// mask: draft_bits of the query (not read without masks); len: context_len.
+__device__ __forceinline__ Row row_view(const TreeParams& p, int b, int len, uint64_t mask) {
   Row r;
-  r.len = context_len(p, b);
+  r.len = len;
   r.seen = 0;
   int depth = -1;
   if (p.mask) {
-    const uint64_t m = draft_bits(p, b, t);
+    const uint64_t m = mask;
     if (m == 0) {  // padding
       r.len = r.lo = r.sinks = 0;
       return r;
     }
     depth = __builtin_popcountll(m) - 1;
     // Drafted tokens past the table are not seen.
-    const int64_t room = capacity(p) - r.len;
+    const int room = p.capacity - r.len;
     r.seen = room >= 64 ? m : room > 0 ? m & ((uint64_t{1} << room) - 1) : 0;
     // The window hides drafted tokens only where it is shorter than a path.
     if (p.window > 0 && p.window <= depth + 1)
       for (uint64_t left = r.seen; left; left &= left - 1) {
         const int j = __builtin_ctzll(left);
         const int dj = __builtin_popcountll(draft_bits(p, b, j)) - 1;
-        if (dj <= depth - p.window && r.len + static_cast<int64_t>(dj) >= p.sinks) r.seen &= ~(uint64_t{1} << j);
+        if (dj <= depth - p.window && r.len + dj >= p.sinks) r.seen &= ~(uint64_t{1} << j);
       }
   }
-  int64_t lo = p.window > 0 ? static_cast<int64_t>(r.len) + depth - p.window + 1 : 0;
-  lo = lo < 0 ? 0 : lo;
-  r.lo = static_cast<int>(lo < r.len ? lo : r.len);
+  const int lo = p.window > 0 ? r.len + depth - p.window + 1 : 0;
+  r.lo = min(max(lo, 0), r.len);
   r.sinks = min(p.sinks, r.lo);
   return r;
 }
@@ -136,7 +131,7 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 
 // Balanced launches: an item costs its tiles and one more (its queries, first
 // round trips and stores take about as long).
-constexpr int kTreeItemCost = 1;
+constexpr int kTreeItemCost = 4;
 // Least cost of a workgroup's range: shorter ones gain less than their
 // partials cost.
 constexpr int kTreeMinCost = 4;
@@ -183,7 +178,7 @@ __host__ __device__ constexpr int tree_lds_bytes(int slots, int nw) {
 }
 // Resident workgroups per CU, which the launch bounds ask for.
 __host__ __device__ constexpr int tree_occupancy(int slots, int nb, int nw) {
-  const int by_lds = 160 * 1024 / (tree_lds_bytes(slots, nw) + 8 * kTreeMaxBalanced);
+  const int by_lds = 160 * 1024 / (tree_lds_bytes(slots, nw) + 4 * kTreeMaxBalanced);
   const int by_regs = nw == 8 ? 1 : slots >= 32 ? 1 : slots == 8 && nb == 1 ? 3 : 2;
   return by_lds < by_regs ? by_lds : by_regs;
 }
@@ -232,6 +227,17 @@ __device__ __forceinline__ float tree_sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Inclusive prefix sum over the wave's 64 lanes (the DPP scan of
+// wave_incl_scan_small).
+__device__ __forceinline__ int tree_wave_scan(int x) {
+  x = dpp_add_i32<0x111, 0xF>(x);  // row_shr:1
+  x = dpp_add_i32<0x112, 0xF>(x);  // row_shr:2
+  x = dpp_add_i32<0x114, 0xF>(x);  // row_shr:4
+  x = dpp_add_i32<0x118, 0xF>(x);  // row_shr:8
+  x = dpp_add_i32<0x142, 0xA>(x);  // row_bcast:15
+  return dpp_add_i32<0x143, 0xC>(x);  // row_bcast:31
+}
+
 // Or and maximum over the wave, in every lane: within rows of 16 lanes by DPP,
 // across them by lane swaps (no LDS round trips).
 template <int CTRL>
@@ -276,42 +282,15 @@ __device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
-// Up to four such loads from base + off[i] (base wave-uniform) to LDS bytes lds
-// + 1024 i + 16 lane.  The instruction's offset moves both sides, so off[i]
-// comes 1024 i short.
-template <bool STREAM, int N>
-__device__ __forceinline__ void tree_load_lds_run(const char* base, const uint32_t* off, uint32_t lds) {
-  static_assert(N == 1 || N == 2 || N == 4, "runs of a wave");
-#define QD_LDS_LOAD(reg, at, policy) "\n\tglobal_load_lds_dwordx4 " reg ", %1 offset:" at policy
-#define QD_LDS_RUN(policy)                                                                                             \
-  if constexpr (N == 1)                                                                                                \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy)::"s"(lds), "s"(base), "v"(off[0])        \
-                 : "memory");                                                                                          \
-  else if constexpr (N == 2)                                                                                           \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy) QD_LDS_LOAD("%3", "1024", policy)::"s"(  \
-                     lds),                                                                                             \
-                 "s"(base), "v"(off[0]), "v"(off[1] - 1024)                                                            \
-                 : "memory");                                                                                          \
-  else                                                                                                                 \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" QD_LDS_LOAD("%2", "0", policy) QD_LDS_LOAD("%3", "1024", policy)        \
-                     QD_LDS_LOAD("%4", "2048", policy) QD_LDS_LOAD("%5", "3072", policy)::"s"(lds),                    \
-                 "s"(base), "v"(off[0]), "v"(off[1] - 1024), "v"(off[2] - 2048), "v"(off[3] - 3072)                    \
-                 : "memory")
-  if constexpr (STREAM) {
-    QD_LDS_RUN(" nt");
-  } else {
-    QD_LDS_RUN("");
-  }
-#undef QD_LDS_RUN
-#undef QD_LDS_LOAD
-}
-
-// All loads of a wave for K or V of a tile.
-template <bool STREAM, int LOADS>
-__device__ __forceinline__ void tree_load_lds_rows(const char* base, const uint32_t (&off)[LOADS], uint32_t lds) {
-#pragma unroll
-  for (int i = 0; i < LOADS; i += LOADS < 4 ? LOADS : 4)
-    tree_load_lds_run<STREAM, (LOADS < 4 ? LOADS : 4)>(base, off + i, lds + 1024 * i);
+// The same from base + off, base wave-uniform.
+template <bool STREAM>
+__device__ __forceinline__ void tree_load_lds(const char* base, uint32_t off, uint32_t lds) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory");
 }
 
 __device__ __forceinline__ uint32_t tree_lds_address(const char* p) {
@@ -370,11 +349,11 @@ struct Span {
 __device__ __forceinline__ Span span_of(const TreeParams& p, int len) {
   Span s;
   s.len = len;
-  s.nd = p.mask ? static_cast<int>(min(static_cast<int64_t>(p.T), capacity(p) - s.len)) : 0;
+  s.nd = p.mask ? min(p.T, p.capacity - s.len) : 0;
   // The first query's window is the earliest: position len, or len - 1
   // without a mask.
-  const int64_t lo = p.window > 0 ? static_cast<int64_t>(s.len) + (p.mask ? 1 : 0) - p.window : 0;
-  s.seen_lo = static_cast<int>(lo < 0 ? 0 : lo < s.len ? lo : s.len);
+  const int lo = p.window > 0 ? s.len + (p.mask ? 1 : 0) - p.window : 0;
+  s.seen_lo = min(max(lo, 0), s.len);
   s.seen_sinks = min(p.sinks, s.seen_lo);
   s.lo = s.seen_lo;
   s.sinks = s.seen_sinks;
@@ -409,16 +388,20 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   // those at the window's edge (bit i: token seen_lo + i).
   unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * 2 * Sh::kTile);
   int32_t* pages = reinterpret_cast<int32_t*>(bad_words + 4);
-  int64_t* incl = reinterpret_cast<int64_t*>(smem + Sh::kLds);
+  int32_t* incl = reinterpret_cast<int32_t*>(smem + Sh::kLds);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r16 = lane & 15, g4 = lane >> 4;
   const int wr = wv / WT, wt = wv % WT;
   const int per_seq = p.Hkv * p.chunks;
-  const int row_bytes = p.D * ES;
-
   auto process = [&](int b, int hc, const Span& sp, int t0, int t1, bool whole, int64_t slot) {
+    // Opaque copies: what is derived from them (masks and offsets per column)
+    // would otherwise be computed ahead of the first item and kept in registers
+    // from item to item.
+    int dim = p.D, lane = static_cast<int>(threadIdx.x) & 63;
+    asm volatile("" : "+s"(dim), "+v"(lane));
+    int r16 = lane & 15, g4 = lane >> 4;
+    const int row_bytes = dim * ES;
     const int h = hc / p.chunks;
     const int row0 = (hc % p.chunks) * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.R - row0);
@@ -450,16 +433,27 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     };
     const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
     const bool grouped = p.P % 16 == 0;
-    // Fills the page list from a tile on; returns the first tile that it does
-    // not cover.
-    auto list_pages = [&](int tile) {
-      const int each = grouped ? 16 : 1;
+    // The page list from a tile on: read, then put into LDS; it covers
+    // list_tiles tiles.
+    constexpr int kEach = kTreePages / (64 * NW);
+    const int each = grouped ? 16 : 1, list_tiles = kTreePages * each / Sh::TT;
+    struct Pages {
+      int32_t id[kEach];
+    };
+    auto read_pages = [&](int tile) {
       const int until = min(sp.n, Sh::TT * t1);
-      for (int i = tid; i < kTreePages; i += 64 * NW) {
-        const int v = Sh::TT * tile + each * i;
-        if (v < until) pages[i] = min(max(table[page_of(token(v))], 0), p.last_block);
+      Pages x;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int v = Sh::TT * tile + each * (64 * NW * i + tid);
+        x.id[i] = 0;
+        if (v < until) x.id[i] = table[page_of(token(v))];
       }
-      return tile + kTreePages * each / Sh::TT;
+      return x;
+    };
+    auto put_pages = [&](const Pages& x) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) pages[64 * NW * i + tid] = min(max(x.id[i], 0), p.last_block);
     };
     // Place of this wave's rows of a tile in the list that starts at tile
     // `base`.  Groups past the last token take its page.
@@ -467,47 +461,56 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       const int at = Sh::TT * (tile - base) + Sh::kLoadRows * wv;
       return grouped ? min(at, sp.n - 1 - Sh::TT * base) / 16 : at;
     };
-    // Starts the loads of this wave's rows of a tile, from page `phys` (grouped)
-    // or from the listed ones (`at`: this wave's first).  Rows past the last
+    // Loads of this wave's rows of a tile, from page `phys` (grouped) or from the
+    // listed ones (`at`: this wave's first), piece by piece.  Rows past the last
     // token and drafted tokens that no row sees are loaded from some page of
     // the pool; they are cleared before they are used.
-    auto load_tile = [&](int tile, int slot, int32_t phys, int at) {
-      const int v0 = Sh::TT * tile + Sh::kLoadRows * wv;
-      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
+    struct TileLoad {
+      const char* k;
+      const char* v;
+      int v0, at;
+      uint32_t to;
+    };
+    auto tile_load = [&](int tile, int slot, int32_t phys, int at) {
+      TileLoad x;
+      x.v0 = Sh::TT * tile + Sh::kLoadRows * wv;
+      x.at = at;
+      x.to = __builtin_amdgcn_readfirstlane(lds_wave + slot * 2 * Sh::kTile);
+      x.k = static_cast<const char*>(p.k);
+      x.v = static_cast<const char*>(p.v);
       if (grouped) {
-        const int tok0 = token(v0);
+        const int tok0 = token(x.v0);
         const int64_t off = readlane_i64(  // the same in all lanes: scalar registers
             static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(phys)) * page_bytes +
                                  static_cast<uint32_t>(p.pshift >= 0 ? tok0 & (p.P - 1) : tok0 % p.P) * tok_bytes),
             0);
-        const char* k = static_cast<const char*>(p.k) + off;
-        const char* v = static_cast<const char*>(p.v) + off;
-        if (padded) {
-#pragma unroll
-          for (int i = 0; i < Sh::kLoads; ++i)
-            if (inside(i)) {
-              tree_load_lds<true>(k + lane_off[i], to + 1024 * i);
-              tree_load_lds<true>(v + lane_off[i], to + Sh::kTile + 1024 * i);
-            }
-        } else if (p.chunks == 1) {
-          tree_load_lds_rows<true>(k, lane_off, to);
-          tree_load_lds_rows<true>(v, lane_off, to + Sh::kTile);
+        x.k += off;
+        x.v += off;
+      }
+      return x;
+    };
+    auto load_piece = [&](const TileLoad& x, int i) {
+      const uint32_t to = x.to + 1024 * i;
+      if (grouped && !padded) {
+        if (p.chunks == 1) {
+          tree_load_lds<true>(x.k, lane_off[i], to);
+          tree_load_lds<true>(x.v, lane_off[i], to + Sh::kTile);
         } else {  // the other chunks read the same rows
-          tree_load_lds_rows<false>(k, lane_off, to);
-          tree_load_lds_rows<false>(v, lane_off, to + Sh::kTile);
+          tree_load_lds<false>(x.k, lane_off[i], to);
+          tree_load_lds<false>(x.v, lane_off[i], to + Sh::kTile);
         }
         return;
       }
-#pragma unroll
-      for (int i = 0; i < Sh::kLoads; ++i) {
+      uint64_t off = lane_off[i];
+      if (!grouped) {
         const int r = (64 * i + lane) / Sh::kSlots;
-        const int v = min(v0 + r, sp.n - 1), tok = token(v);
-        const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(pages[at + v - v0])) * page_bytes +
-                             static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes + (lane_off[i] - r * tok_bytes);
-        if (inside(i)) {
-          tree_load_lds<true>(static_cast<const char*>(p.k) + off, to + 1024 * i);
-          tree_load_lds<true>(static_cast<const char*>(p.v) + off, to + Sh::kTile + 1024 * i);
-        }
+        const int v = min(x.v0 + r, sp.n - 1), tok = token(v);
+        off += static_cast<uint64_t>(static_cast<uint32_t>(pages[x.at + v - x.v0])) * page_bytes +
+               static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes - r * tok_bytes;
+      }
+      if (inside(i)) {
+        tree_load_lds<true>(x.k + off, to);
+        tree_load_lds<true>(x.v + off, to + Sh::kTile);
       }
     };
 
@@ -539,8 +542,11 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
         *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
     }
-    int listed = 0, list_base = t0;  // the list covers tiles [list_base, listed)
-    if (!grouped && t0 < t1) listed = list_pages(t0);
+    int list_base = grouped ? t0 + Sh::kBufs - 1 : t0;
+    const Pages listed = read_pages(list_base);
+    uint64_t my_mask = 0;
+    if (p.mask && q0 + lane <= q1) my_mask = draft_bits(p, b, q0 + lane);
+    if (!grouped) put_pages(listed);
     if (padded || !grouped) tree_barrier();
     for (int i = 0; i < Sh::kBufs - 1; ++i)
       if (t0 + i < t1) {
@@ -548,20 +554,19 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         if (grouped)
           phys = min(max(tree_scalar_load(table + min(page_of(token(Sh::TT * (t0 + i) + Sh::kLoadRows * wv)), last_page)), 0),
                      p.last_block);
-        load_tile(t0 + i, i, phys, list_at(t0 + i, t0));
+        const TileLoad x = tile_load(t0 + i, i, phys, list_at(t0 + i, t0));
+#pragma unroll
+        for (int j = 0; j < Sh::kLoads; ++j) load_piece(x, j);
       }
-    if (grouped && t0 + Sh::kBufs - 1 < t1) {
-      list_base = t0 + Sh::kBufs - 1;
-      listed = list_pages(list_base);
-    }
+    if (grouped) put_pages(listed);
     // Lane t: what query q0 + t sees (at most 64 queries).
     Row mine;
     mine.len = mine.lo = mine.sinks = 0;
     mine.seen = 0;
     bool sees = false;
     if (q0 + lane <= q1) {
-      sees = !p.mask || draft_bits(p, b, q0 + lane) != 0;
-      if (sees) mine = row_view(p, b, q0 + lane);
+      sees = !p.mask || my_mask != 0;
+      if (sees) mine = row_view(p, b, sp.len, my_mask);
     }
     auto bits_or = [](uint32_t x, uint32_t y) { return x | y; };
     const uint32_t seen_low = __builtin_amdgcn_readfirstlane(tree_wave_reduce(static_cast<uint32_t>(mine.seen), bits_or));
@@ -595,14 +600,16 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         tree_barrier_loads<4 * Sh::kLoads>();
       const int next = tile + Sh::kBufs - 1;
       if (next < t1) {
-        if (next >= listed) {
+        if (next >= list_base + list_tiles) {
           list_base = next;
-          listed = list_pages(next);
+          put_pages(read_pages(next));
           tree_barrier();
         }
         const int at = list_at(next, list_base);
-        load_tile(next, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1,
-                  grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
+        const TileLoad x = tile_load(next, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1,
+                                     grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
+#pragma unroll
+        for (int j = 0; j < Sh::kLoads; ++j) load_piece(x, j);
       }
       char* buf = smem + slot_now * 2 * Sh::kTile;
       slot_now = slot_now == Sh::kBufs - 1 ? 0 : slot_now + 1;
@@ -669,7 +676,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
             }
           }
           if (st + Sh::kQkAhead < Sh::kSteps) read_k(st + Sh::kQkAhead);
-          if (Sh::kQkAhead < Sh::kSteps) __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_sched_barrier(0);
         }
         // V^T of the first columns, in flight during the softmax.
         const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
@@ -810,6 +817,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     }
 
     // The waves' parts of the same rows.
+    asm volatile("" : "+s"(dim), "+v"(lane), "+v"(r16), "+v"(g4));
     tree_barrier();
     if constexpr (WT > 1) {
       constexpr int kPart = NB * Sh::kCols * 1024 + NB * 512;  // acc, m, l of a wave
@@ -876,7 +884,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int d = 16 * c + 4 * g4 + i;
-                if (d >= p.D) continue;
+                if (d >= dim) continue;
                 const float val = E::to_f(reinterpret_cast<const S*>(src)[d]);
                 if (!(fabsf(val) < INFINITY)) acc[c][nb][i] += val;
               }
@@ -898,7 +906,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
             const int d = 16 * c + 4 * g4;
-            if (d >= p.D) continue;
+            if (d >= dim) continue;
             const f32x4 y = has ? acc[c][nb] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
             if constexpr (k16)
               *reinterpret_cast<u32x2*>(out + d * ES) =
@@ -907,55 +915,63 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
               *reinterpret_cast<f32x4*>(out + d * ES) = y;
           }
         } else {
-          float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (p.D + 2));
+          float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (dim + 2));
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
             const int d = 16 * c + 4 * g4;
-            if (d < p.D)
-              *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(rr) * p.D + d) =
+            if (d < dim)
+              *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(rr) * dim + d) =
                   has ? acc[c][nb] : f32x4{0.f, 0.f, 0.f, 0.f};
           }
           if (g4 == 0)
-            *reinterpret_cast<f32x2*>(part + static_cast<int64_t>(Sh::kRows) * p.D + 2 * rr) =
+            *reinterpret_cast<f32x2*>(part + static_cast<int64_t>(Sh::kRows) * dim + 2 * rr) =
                 has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
         }
       }
     }
   };
 
-  // Balanced: the costs of all items in a row, cut into equal ranges.  Up to 64
-  // sequences, every wave keeps the prefix of the costs in its lanes.
-  int64_t total = 0, used = 1, pos = 0, end = 1, mine_incl = 0;
-  const int64_t w = blockIdx.x;
+  // Balanced: the costs of all items in a row (below 2^31: the host sees to
+  // it), cut into equal ranges.  Up to 64 sequences, every wave keeps the prefix
+  // of the costs in its lanes.
+  int total = 0, used = 1, pos = 0, end = 1, mine_incl = 0;
+  const int w = static_cast<int>(blockIdx.x);
   int b = 0;
   const bool in_lanes = p.B <= 64;
-  auto prefix = [&](int i) { return readlane_i64(in_lanes ? mine_incl : incl[i], in_lanes ? i : 0); };
+  auto prefix = [&](int i) {
+    return in_lanes ? __builtin_amdgcn_readlane(mine_incl, i) : __builtin_amdgcn_readfirstlane(incl[i]);
+  };
+  // a n / d below 2^31; a n is below 2^42, so that the rounded quotient of
+  // doubles is never on the wrong side of an integer.
+  auto part_of = [](int a, int n, int d) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(a) * n / d));
+  };
   if (p.W > 0) {
-    auto cost_of = [&](int i) -> int64_t {
+    auto cost_of = [&](int i) {
       const int tiles = span_tiles<Sh::TT>(item_span(p, i));
-      return tiles > 0 ? static_cast<int64_t>(tiles + kTreeItemCost) * per_seq : 0;
+      return tiles > 0 ? (tiles + kTreeItemCost) * per_seq : 0;
     };
     if (in_lanes) {
-      mine_incl = wave_incl_scan_small(lane < p.B ? cost_of(lane) : 0, lane);
+      mine_incl = tree_wave_scan(lane < p.B ? cost_of(lane) : 0);
     } else {
       for (int i = tid; i < p.B; i += 64 * NW) incl[i] = cost_of(i);
       __syncthreads();
       if (wv == 0) {
-        int64_t carry = 0;
+        int carry = 0;
         for (int base = 0; base < p.B; base += 64) {
           const int i = base + lane;
-          const int64_t v = carry + wave_incl_scan_small(i < p.B ? incl[i] : 0, lane);
+          const int v = carry + tree_wave_scan(i < p.B ? incl[i] : 0);
           if (i < p.B) incl[i] = v;
-          carry = readlane_i64(v, 63);
+          carry = __builtin_amdgcn_readlane(v, 63);
         }
       }
       __syncthreads();
     }
     total = prefix(p.B - 1);
-    used = min(static_cast<int64_t>(p.W), max<int64_t>(1, total / kTreeMinCost));
+    used = min(p.W, max(1, total / kTreeMinCost));
     if (w >= used) return;
-    pos = div_nonneg(w * total, used);
-    end = div_nonneg((w + 1) * total, used);
+    pos = part_of(w, total, used);
+    end = part_of(w + 1, total, used);
     if (in_lanes) {
       b = __builtin_popcountll(__ballot(lane < p.B && mine_incl <= pos));
     } else {
@@ -974,21 +990,23 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     Span sp;
     if (p.W > 0) {
       while (prefix(b) <= pos) ++b;
-      const int64_t before = b > 0 ? prefix(b - 1) : 0;
-      const int cost = static_cast<int>(div_nonneg(prefix(b) - before, per_seq));
-      hc = static_cast<int>(div_nonneg(pos - before, cost));
-      const int off = static_cast<int>((pos - before) - static_cast<int64_t>(hc) * cost);
-      const int stop = static_cast<int>(min(static_cast<int64_t>(cost), off + (end - pos)));
+      const int before = b > 0 ? prefix(b - 1) : 0;
+      const int cost = static_cast<int>(static_cast<uint32_t>(prefix(b) - before) / static_cast<uint32_t>(per_seq));
+      hc = static_cast<int>(static_cast<uint32_t>(pos - before) / static_cast<uint32_t>(cost));
+      const int off = pos - before - hc * cost;
+      const int stop = min(cost, off + (end - pos));
       t0 = max(0, off - kTreeItemCost);
       t1 = max(0, stop - kTreeItemCost);
       tiles = cost - kTreeItemCost;
       step = stop - off;
       if (t1 > t0 && t0 == 0 && tid == 0) {
-        const int64_t first = before + static_cast<int64_t>(hc) * cost + kTreeItemCost;  // the item's first tile
-        const int64_t last = div_nonneg((first + tiles) * used - 1, total);              // holder of its last tile
+        // The workgroup w that holds a place x: w total / used <= x.
+        const int x = before + hc * cost + cost - 1;  // the item's last tile
+        int last = part_of(x, used, total);
+        while (last + 1 < used && part_of(last + 1, total, used) <= x) ++last;
         int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * per_seq + hc);
-        meta[0] = static_cast<int32_t>(w);
-        meta[1] = static_cast<int32_t>(last - w + 1);
+        meta[0] = w;
+        meta[1] = last - w + 1;
       }
       sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
     } else {
@@ -996,7 +1014,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
       t1 = tiles = span_tiles<Sh::TT>(sp);
     }
-    if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * w + (t0 == 0 ? 1 : 0));
+    if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
     pos += step;
   }
 }
@@ -1051,7 +1069,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
 template <int DT, int DP, int NB, int WR, int NW>
 hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
   using Sh = TreeShape<DT, DP, NB, WR, NW>;
-  const size_t lds = Sh::kLds + (p.W > 0 ? sizeof(int64_t) * static_cast<size_t>(p.B) : 0);
+  const size_t lds = Sh::kLds + (p.W > 0 ? sizeof(int32_t) * static_cast<size_t>(p.B) : 0);
   void (*fn)(TreeParams) = tree_mfma_kernel<DT, DP, NB, WR, NW>;
   static std::atomic<uint64_t> allowed{0};  // devices on which more than 64 KB of LDS were asked for
   int dev = 0;
@@ -1059,7 +1077,7 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
   const uint64_t bit = uint64_t{1} << (dev & 63);
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             Sh::kLds + 8 * kTreeMaxBalanced);
+                                             Sh::kLds + 4 * kTreeMaxBalanced);
     if (e != hipSuccess) return e;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
