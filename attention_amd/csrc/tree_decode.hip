@@ -203,8 +203,24 @@ struct TreePlan {
   size_t meta_bytes, bytes;
 };
 
-// Contexts of at most this many tiles are not split over workgroups.
-constexpr int kTreeDirectTiles = 4;
+// One workgroup per item, without a merge, or the items' tiles cut into equal
+// ranges, one per resident workgroup, with a merge kernel (about 5 us, and a
+// start of 4 tiles for every item that a range begins)?  By what is left idle
+// if every context fills its table or window, in units of 64 tokens per
+// resident workgroup, and by how uneven contexts without a window can be.
+// bf16, 8 kv-heads of 128, one workgroup per item against equal ranges, us:
+// 512 items of 18 units (a window of 1024) 48.6 / 54.6, 320 of them 40.0 / 38.9,
+// 128 of them 32.7 / 25.1; 1024 items of 9 units 56.4 / 60.1, 1600 of them 98 /
+// 93.6; without a window, 512 items of 2 to 16 units 40.5 / 52.6, 1024 items of
+// 2 to 32 units 126 / 115, 256 items of 8 to 64 units 107 / 77.
+constexpr int kTreeIdleUnits = 5;
+constexpr int kTreeUnevenUnits = 20;
+
+bool tree_direct(int64_t items, int64_t units, int64_t resident, bool windowed) {
+  const int64_t rounds = (items + resident - 1) / resident;
+  if (!windowed && rounds * units > kTreeUnevenUnits) return false;
+  return rounds * units * resident - items * units <= kTreeIdleUnits * resident;
+}
 
 TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim, int block_size, int max_pages,
                    int has_mask, int window, int sinks, int dtype, int flags) {
@@ -229,11 +245,12 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
   const int tt = tree_tile(slots, wv.nw);
   const int64_t tiles = (cap + tt - 1) / tt;
-  if (tiles <= kTreeDirectTiles || batch > kTreeMaxBalanced || items * (tiles + kTreeItemCost) > INT32_MAX) {
+  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
+  if (batch > kTreeMaxBalanced || items * (tiles + kTreeItemCost) > INT32_MAX ||
+      tree_direct(items, std::max<int64_t>(1, tiles * tt / 64), resident, window > 0)) {
     pl.grid = static_cast<int>(items);
     return pl;
   }
-  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
   pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / kTreeMinCost)));
   pl.grid = pl.W;
   pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;

@@ -1043,21 +1043,35 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
   const int64_t slot_floats = static_cast<int64_t>(KROWS) * (p.D + 2);
   auto part = [&](int s) { return p.part + (2 * static_cast<int64_t>(first + s) + (s == 0 ? 1 : 0)) * slot_floats; };
   auto stat = [&](int s) { return *reinterpret_cast<const f32x2*>(part(s) + static_cast<int64_t>(KROWS) * p.D + 2 * rr); };
+  // Four partials at a time, statistics and values in flight together.
   const int l16 = threadIdx.x & 15;
-  float mx = -INFINITY;
-  for (int s = l16; s < count; s += 16) mx = fmaxf(mx, stat(s)[0]);
-  for (int off = 8; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-  const float ref = mx == -INFINITY ? 0.f : mx;
   for (int d = 4 * l16; d < p.D; d += 64) {
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < count; ++s) {
-      const f32x2 ml = stat(s);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(part(s) + static_cast<int64_t>(rr) * p.D + d);
-      const float f = fast_exp2(ml[0] - ref);
-      sum += f * ml[1];
-      a += f * x;
+    float mx = -INFINITY, sum = 0.f;
+    for (int s0 = 0; s0 < count; s0 += 4) {
+      f32x2 ml[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = min(s0 + i, count - 1);
+        ml[i] = stat(s);
+        x[i] = *reinterpret_cast<const f32x4*>(part(s) + static_cast<int64_t>(rr) * p.D + d);
+      }
+      float most = mx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, ml[i][0]);
+      const float ref = most == -INFINITY ? 0.f : most;
+      const float old = fast_exp2(mx - ref);
+      sum *= old;
+      a *= old;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s0 + i >= count) continue;
+        const float f = fast_exp2(ml[i][0] - ref);
+        sum += f * ml[i][1];
+        a += f * x[i];
+      }
+      mx = most;
     }
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
