@@ -311,6 +311,14 @@ __device__ __forceinline__ u32x2 tree_tr_read(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
 }
 
+template <int DT>
+__device__ __forceinline__ uint32_t tree_pack(float x, float y) {
+  if constexpr (DT == QD_DTYPE_F32)
+    return 0;  // not called
+  else
+    return MfmaOps<DT>::pack2(x, y);
+}
+
 // Zeroes the elements of x that are Inf or NaN; returns whether there were any.
 template <int DT>
 __device__ __forceinline__ bool drop_not_finite(u32x4& x) {
@@ -646,6 +654,9 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // The matrix cores' phases go before another wave's softmax (64 drafts x
+        // 64 heads: 277 -> 270 us).
+        __builtin_amdgcn_s_setprio(1);
         // Operands are read ahead of their products: a product takes 16 cycles,
         // an LDS read here well over 100.  The scheduling barriers keep the
         // distance.
@@ -678,6 +689,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
           if (st + Sh::kQkAhead < Sh::kSteps) read_k(st + Sh::kQkAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         // V^T of the first columns, in flight during the softmax.
         const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
         const int vr = 4 * g4 + (k16 ? r16 >> 2 : 0);
@@ -771,6 +783,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
                   if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           }
           __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int c = 0; c < Sh::kCols; ++c) {
             const u32x2* f = vf[c % Sh::kPvAhead];
@@ -813,128 +826,136 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
             }
           }
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     }
 
-    // The waves' parts of the same rows.
+    // The item's end: its rows' sums, and the output or a partial.
     asm volatile("" : "+s"(dim), "+v"(lane), "+v"(r16), "+v"(g4));
     tree_barrier();
+    float sum[NB], scale[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) sum[nb] = tree_sum_groups(l[nb]);
+    float share[NB][WT];  // factors of the waves' parts of the same rows
     if constexpr (WT > 1) {
-      constexpr int kPart = NB * Sh::kCols * 1024 + NB * 512;  // acc, m, l of a wave
-      static_assert(WR * (WT - 1) * kPart <= Sh::kBufs * 2 * Sh::kTile, "the waves' parts fit the tile buffers");
-      char* base = smem + (wr * (WT - 1) + wt - 1) * kPart;
-      if (wt > 0) {
+      // Every wave leaves its part in LDS, {m, l} of its rows where the page
+      // list was, and takes up a share of the columns.
+      static_assert(NW * NB * Sh::kCols * 1024 <= Sh::kBufs * 2 * Sh::kTile && NW * NB * 128 <= 4 * kTreePages,
+                    "the waves' parts fit the tile buffers and the page list");
+      f32x2* stats = reinterpret_cast<f32x2*>(pages);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c)
-            *reinterpret_cast<f32x4*>(base + (nb * Sh::kCols + c) * 1024 + 16 * lane) = acc[c][nb];
-          *reinterpret_cast<f32x2*>(base + NB * Sh::kCols * 1024 + nb * 512 + 8 * lane) = f32x2{m[nb], l[nb]};
-        }
+        for (int c = 0; c < Sh::kCols; ++c)
+          *reinterpret_cast<f32x4*>(smem + ((wv * NB + nb) * Sh::kCols + c) * 1024 + 16 * lane) = acc[c][nb];
+        if (g4 == 0) stats[(wv * NB + nb) * 16 + r16] = f32x2{m[nb], sum[nb]};
       }
       tree_barrier();
-      if (wt == 0) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float mx = m[nb];
-          f32x2 ml[WT];
+      for (int nb = 0; nb < NB; ++nb) {
+        f32x2 ml[WT];
+        float mx = -INFINITY;
 #pragma unroll
-          for (int w = 1; w < WT; ++w) {
-            const char* part = smem + (wr * (WT - 1) + w - 1) * kPart;
-            ml[w] = *reinterpret_cast<const f32x2*>(part + NB * Sh::kCols * 1024 + nb * 512 + 8 * lane);
-            mx = fmaxf(mx, ml[w][0]);
-          }
-          const float ref = mx == -INFINITY ? 0.f : mx;
-          float f = fast_exp2(m[nb] - ref);
-          l[nb] *= f;
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= f;
-#pragma unroll
-          for (int w = 1; w < WT; ++w) {
-            const char* part = smem + (wr * (WT - 1) + w - 1) * kPart;
-            f = fast_exp2(ml[w][0] - ref);
-            l[nb] += f * ml[w][1];
-#pragma unroll
-            for (int c = 0; c < Sh::kCols; ++c)
-              acc[c][nb] += f * *reinterpret_cast<const f32x4*>(part + (nb * Sh::kCols + c) * 1024 + 16 * lane);
-          }
-          m[nb] = mx;
+        for (int w = 0; w < WT; ++w) {
+          ml[w] = stats[((wr * WT + w) * NB + nb) * 16 + r16];
+          mx = fmaxf(mx, ml[w][0]);
         }
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        sum[nb] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+          share[nb][w] = ml[w][0] == mx && mx != -INFINITY ? 1.f : fast_exp2(ml[w][0] - ref);
+          sum[nb] += share[nb][w] * ml[w][1];
+        }
+        m[nb] = mx;
       }
     }
-    if (wt == 0) {
-      // Inf and NaN that only some rows see: whatever their weight, the sum is
-      // no longer finite.
+    bool has[NB];
+    char* to[NB];  // the row of the output or of the partial
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      has[nb] = __shfl(static_cast<int>(sees), query[nb] - q0) != 0 && (sum[nb] > 0.f || sum[nb] != sum[nb]);
+      scale[nb] = has[nb] ? (whole ? 1.f / sum[nb] : 1.f) : 0.f;
+      const int rr = 16 * (NB * wr + nb) + r16;
+      if (whole) {
+        to[nb] = static_cast<char*>(p.out) +
+                 ((static_cast<int64_t>(b) * p.T + query[nb]) * p.Hq + static_cast<int64_t>(h) * p.G +
+                  (row0 + rr - query[nb] * p.G)) *
+                     row_bytes;
+      } else {
+        float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (dim + 2));
+        to[nb] = reinterpret_cast<char*>(part + static_cast<int64_t>(rr) * dim);
+        if (wt == 0 && g4 == 0 && real[nb])
+          *reinterpret_cast<f32x2*>(part + static_cast<int64_t>(Sh::kRows) * dim + 2 * rr) =
+              has[nb] ? f32x2{m[nb], sum[nb]} : f32x2{-INFINITY, 0.f};
+      }
+    }
+    const uint64_t bad_drafts = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad_words[0]), 0));
+    const uint64_t bad_edge = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad_words[1]), 0));
+    auto finish = [&](int c, f32x4 (&y)[NB]) {
+      const int d = 16 * c + 4 * g4;
+      if (bad_drafts | bad_edge) {
+        // Inf and NaN that only some rows see: whatever their weight, the sum
+        // is no longer finite.
 #pragma unroll 1
-      for (int kind = 0; kind < 2; ++kind) {
-        uint64_t bad = static_cast<uint64_t>(readlane_i64(static_cast<int64_t>(bad_words[kind]), 0));
-        while (bad) {
-          const int x = __builtin_ctzll(bad);
-          bad &= bad - 1;
-          const int tok = kind == 0 ? sp.len + x : sp.seen_lo + x;
-          const char* src = static_cast<const char*>(p.v) + (pool_row(p, b, tok) * p.Hkv + h) * row_bytes;
+        for (int kind = 0; kind < 2; ++kind) {
+          uint64_t bad = kind == 0 ? bad_drafts : bad_edge;
+#pragma unroll 1
+          while (bad) {
+            const int x = __builtin_ctzll(bad);
+            bad &= bad - 1;
+            const int tok = kind == 0 ? sp.len + x : sp.seen_lo + x;
+            const S* src = reinterpret_cast<const S*>(static_cast<const char*>(p.v) +
+                                                      (pool_row(p, b, tok) * p.Hkv + h) * row_bytes);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const int from = query[nb] - q0;
-            const int lo = __shfl(mine.lo, from), sinks = __shfl(mine.sinks, from);
-            const uint64_t seen = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), from));
-            if (!(kind == 0 ? ((seen >> x) & 1) != 0 : tok < sinks || tok >= lo)) continue;
+            for (int nb = 0; nb < NB; ++nb) {
+              const int from = query[nb] - q0;
+              const int lo = __shfl(mine.lo, from), sinks = __shfl(mine.sinks, from);
+              const uint64_t seen = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), from));
+              if (d < dim && (kind == 0 ? ((seen >> x) & 1) != 0 : tok < sinks || tok >= lo))
 #pragma unroll
-            for (int c = 0; c < Sh::kCols; ++c)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d = 16 * c + 4 * g4 + i;
-                if (d >= dim) continue;
-                const float val = E::to_f(reinterpret_cast<const S*>(src)[d]);
-                if (!(fabsf(val) < INFINITY)) acc[c][nb][i] += val;
-              }
+                for (int i = 0; i < 4; ++i) {
+                  const float val = E::to_f(src[d + i]);
+                  if (!(fabsf(val) < INFINITY)) y[nb][i] += val;
+                }
+            }
           }
         }
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const float sum = tree_sum_groups(l[nb]);
-        const bool has = __shfl(static_cast<int>(sees), query[nb] - q0) != 0 && (sum > 0.f || sum != sum);
-        if (!real[nb]) continue;
-        const int rr = 16 * (NB * wr + nb) + r16;
-        if (whole) {
-          const float inv = has ? 1.f / sum : 0.f;
-          char* out = static_cast<char*>(p.out) +
-                      ((static_cast<int64_t>(b) * p.T + query[nb]) * p.Hq + static_cast<int64_t>(h) * p.G +
-                       (row0 + rr - query[nb] * p.G)) *
-                          row_bytes;
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) {
-            const int d = 16 * c + 4 * g4;
-            if (d >= dim) continue;
-            const f32x4 y = has ? acc[c][nb] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
-            if constexpr (k16)
-              *reinterpret_cast<u32x2*>(out + d * ES) =
-                  u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
-            else
-              *reinterpret_cast<f32x4*>(out + d * ES) = y;
-          }
-        } else {
-          float* part = p.part + slot * (static_cast<int64_t>(Sh::kRows) * (dim + 2));
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) {
-            const int d = 16 * c + 4 * g4;
-            if (d < dim)
-              *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(rr) * dim + d) =
-                  has ? acc[c][nb] : f32x4{0.f, 0.f, 0.f, 0.f};
-          }
-          if (g4 == 0)
-            *reinterpret_cast<f32x2*>(part + static_cast<int64_t>(Sh::kRows) * dim + 2 * rr) =
-                has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
-        }
+        if (!real[nb] || d >= dim) continue;
+        const f32x4 z = has[nb] ? y[nb] * scale[nb] : f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k16 && whole)
+          *reinterpret_cast<u32x2*>(to[nb] + d * 2) = u32x2{tree_pack<DT>(z[0], z[1]), tree_pack<DT>(z[2], z[3])};
+        else
+          *reinterpret_cast<f32x4*>(to[nb] + d * 4) = z;
       }
+    };
+    if constexpr (WT > 1) {
+#pragma unroll 2
+      for (int c = wt * Sh::kCols / WT; c < (wt + 1) * Sh::kCols / WT; ++c) {
+        f32x4 y[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          y[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < WT; ++w)
+            y[nb] += share[nb][w] * *reinterpret_cast<const f32x4*>(
+                                        smem + (((wr * WT + w) * NB + nb) * Sh::kCols + c) * 1024 + 16 * lane);
+        }
+        finish(c, y);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < Sh::kCols; ++c) finish(c, acc[c]);
     }
   };
 
   // Balanced: the costs of all items in a row (below 2^31: the host sees to
   // it), cut into equal ranges.  Up to 64 sequences, every wave keeps the prefix
   // of the costs in its lanes.
-  int total = 0, used = 1, pos = 0, end = 1, mine_incl = 0;
+  int total = 0, used = 1, pos = 0, end = 1, mine_incl = 0, mine_len = 0;
   const int w = static_cast<int>(blockIdx.x);
   int b = 0;
   const bool in_lanes = p.B <= 64;
@@ -947,14 +968,15 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(a) * n / d));
   };
   if (p.W > 0) {
-    auto cost_of = [&](int i) {
-      const int tiles = span_tiles<Sh::TT>(item_span(p, i));
+    auto cost_of = [&](int len) {
+      const int tiles = span_tiles<Sh::TT>(span_of(p, len));
       return tiles > 0 ? (tiles + kTreeItemCost) * per_seq : 0;
     };
     if (in_lanes) {
-      mine_incl = tree_wave_scan(lane < p.B ? cost_of(lane) : 0);
+      if (lane < p.B) mine_len = context_len(p, lane);
+      mine_incl = tree_wave_scan(lane < p.B ? cost_of(mine_len) : 0);
     } else {
-      for (int i = tid; i < p.B; i += 64 * NW) incl[i] = cost_of(i);
+      for (int i = tid; i < p.B; i += 64 * NW) incl[i] = cost_of(context_len(p, i));
       __syncthreads();
       if (wv == 0) {
         int carry = 0;
@@ -1008,7 +1030,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         meta[0] = w;
         meta[1] = last - w + 1;
       }
-      sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
+      sp = span_of(p, in_lanes ? __builtin_amdgcn_readlane(mine_len, b) : clamp_len(p, tree_scalar_load(p.lens + b)));
     } else {
       hc = static_cast<int>(blockIdx.x) % per_seq;
       sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
