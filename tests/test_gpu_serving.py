@@ -223,6 +223,49 @@ def test_long_contexts_match_oracle(gpu, shape):
     check_case(gpu, case, window, sinks, what="default")
 
 
+def shared_pages_case(dtype, B, T, Hq, Hkv, D, P, lens, width, *, branch=2, seed=0):
+    """Many or long sequences on a small pool: their tables name the same pages in different orders."""
+    gen = torch.Generator().manual_seed(seed)
+    pool = 40 if P > 1 else 400
+    table = torch.randint(0, pool, (B, width), generator=gen, dtype=torch.int32)
+    q = torch.randn(*((B, T) if T else (B,)), Hq, D, generator=gen).to(dtype)
+    k, v = (torch.randn(pool, P, Hkv, D, generator=gen).to(dtype) for _ in range(2))
+    masks = tree_masks(gen, B, T, branch, True) if T else None
+    return q, k, v, table, torch.tensor(lens, dtype=torch.int32), masks
+
+
+def lengths(B, hi, *long):
+    return list(long) + [(37 * i) % (hi + 1) for i in range(B - len(long))]
+
+
+MANY_SHAPES = [
+    # dtype, B, T, Hq, Hkv, D, P, lens, width, window, sinks, kind
+    # the prefix of the costs in a wave's lanes, all of them used, and in LDS
+    (BF, 64, 2, 4, 2, 64, 16, lengths(64, 60, 1900, 0, 700), 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    (BF, 65, 2, 4, 2, 64, 16, lengths(65, 60, 1900, 0, 700), 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    (HF, 300, 1, 4, 1, 64, 16, lengths(300, 90, 0, 0, 1500), 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    (FP, 90, 2, 2, 1, 128, 8, lengths(90, 40, 900), 250, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    (BF, 1024, 0, 2, 1, 64, 16, lengths(1024, 30, 3000), 250, 2000, 4, cabi.QD_TREE_MFMA_SPLIT),
+    (BF, 70, 2, 2, 1, 64, 16, [0] * 70, 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    # more sequences than the split takes; a workgroup's page list is refilled: one
+    # id for a token (pages of 12, 1) and for 16 (pages of 32)
+    (BF, 1030, 1, 2, 1, 64, 12, lengths(1030, 20, 2500, 1024, 1025, 0, 2049), 220, 0, 0, cabi.QD_TREE_MFMA),
+    (FP, 1030, 1, 2, 1, 64, 1, lengths(1030, 20, 2500, 1024, 1025, 0, 2049), 2600, 0, 0, cabi.QD_TREE_MFMA),
+    (BF, 1030, 2, 2, 1, 128, 32, lengths(1030, 20, 16500, 16384, 33000, 0), 1040, 0, 0, cabi.QD_TREE_MFMA),
+    (HF, 1030, 0, 2, 1, 64, 1, lengths(1030, 20, 2500, 1024), 2600, 1500, 33, cabi.QD_TREE_MFMA),
+]
+
+
+@pytest.mark.parametrize("shape", MANY_SHAPES, ids=lambda s: f"{str(s[0])[6:]}-B{s[1]}-T{s[2]}-{s[5]}-P{s[6]}-w{s[9]}-n{max(s[7])}")
+def test_many_sequences_match_oracle(gpu, shape):
+    dtype, B, T, Hq, Hkv, D, P, lens, width, window, sinks, kind = shape
+    say(f"many {shape[:7]} {width} {window} {sinks}")
+    assert cabi.gqa_decode_tree_info(B, max(T, 1), Hq, Hkv, D, P, width, int(T > 0), window, sinks,
+                                     cabi.DTYPE[dtype])[0] == kind
+    case = shared_pages_case(dtype, B, T, Hq, Hkv, D, P, lens, width, seed=B + D)
+    check_case(gpu, case, window, sinks, what="default")
+
+
 def test_large_scores_stay_exact(gpu):
     """Scores of a few hundred: one token takes all of the weight."""
     say("large scores")

@@ -141,6 +141,79 @@ def test_tree_launch_batch_zero_is_a_no_op():
     assert cabi.lib().qd_gqa_decode_tree(*a.values()) == 0
 
 
+SHAPES_OF_PLANS = [
+    # B, T, Hq, Hkv, D, P, maxP, has_mask, window, sinks, dtype
+    (1, 1, 1, 1, 8, 16, 1, 1, 0, 0, BF16),
+    (64, 1, 32, 8, 128, 16, 512, 0, 1024, 4, BF16),
+    (64, 1, 32, 8, 128, 16, 512, 0, 8192, 4, BF16),
+    (32, 16, 32, 8, 128, 16, 257, 1, 0, 0, BF16),
+    (8, 64, 64, 8, 128, 64, 257, 1, 0, 0, BF16),
+    (5, 7, 32, 32, 80, 12, 60, 1, 0, 0, F16),
+    (8, 8, 32, 8, 128, 16, 65, 1, 0, 0, F32),
+    (2, 64, 71, 1, 256, 1, 4000, 1, 300, 64, BF16),
+    (1025, 2, 4, 2, 64, 16, 2000, 1, 0, 0, F16),
+    (4, 3, 4, 2, 33, 16, 2000, 1, 0, 0, F32),
+    (1, 1, 8, 1, 128, 16, 1 << 27, 1, 0, 0, BF16),
+    (1, 1, 8, 1, 128, 16, 1 << 27, 0, 2147483647, 2147483647, BF16),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES_OF_PLANS)
+def test_plans_cover_all_rows_and_fit_their_workspace(shape):
+    """Every row has a workgroup, one launch at most fills the card, and the
+    workspace holds both kernels' partials."""
+    B, T, Hq, Hkv, D, P, maxP, has_mask, window, sinks, dtype = shape
+    kind, groups, rows = cabi.gqa_decode_tree_info(*shape)
+    per_head = T * Hq // Hkv
+    chunks = -(-per_head // rows)
+    assert rows >= 1 and groups >= 1
+    need = 0
+    if kind == cabi.QD_TREE_VALU:
+        assert D % 8 and rows == 1 and groups % (B * T * Hq) == 0
+        splits = groups // (B * T * Hq)
+        need = 4 * B * T * Hq * splits * (D + 2) if splits > 1 else 0
+    elif kind == cabi.QD_TREE_MFMA:
+        assert groups == B * Hkv * chunks
+    else:
+        assert B <= 1024 and groups <= 3 * 256
+        need = 8 * B * Hkv * chunks + 4 * 2 * groups * rows * (D + 2)
+    args = (B, T, Hq, Hkv, D, P, maxP, has_mask, window, sinks, dtype)
+    valu = cabi.gqa_decode_tree_info(*args, cabi.QD_FLAG_FORCE_GENERIC)
+    assert valu[0] == cabi.QD_TREE_VALU
+    splits = valu[1] // (B * T * Hq)
+    both = max(need, 4 * B * T * Hq * splits * (D + 2) if splits > 1 else 0)
+    bytes_ = cabi.lib().qd_gqa_decode_tree_workspace_bytes(*args, 0)
+    # Up to 16 rows round up to a block of each wave; nothing near twice the need beyond that.
+    assert both <= bytes_ <= 32 * both + 4096
+
+
+@pytest.mark.parametrize("T,Hq,D,dtype", [(1, 8, 128, BF16), (2, 8, 128, BF16), (8, 8, 128, BF16), (64, 8, 128, BF16),
+                                          (64, 64, 64, F16), (64, 71, 256, BF16), (64, 71, 128, F32),
+                                          (64, 71, 256, F32), (3, 200, 192, F16)])
+def test_rows_are_cut_evenly(T, Hq, D, dtype):
+    kind, _, rows = cabi.gqa_decode_tree_info(2, T, Hq, 1, D, 16, 100, dtype=dtype)
+    es = 4 if dtype == F32 else 2
+    most = 256 if D * es <= 256 else 128 if D * es <= 512 else 32
+    chunks = -(-T * Hq // most)
+    assert kind != cabi.QD_TREE_VALU and rows == -(-T * Hq // chunks) <= most
+
+
+def test_which_contexts_are_split():
+    """One workgroup per item where that leaves little idle, equal ranges of all tiles elsewhere; more sequences
+    than the split's prefix holds are not split."""
+    def kind(B, maxP, window=0, mask=1):
+        return cabi.gqa_decode_tree_info(B, 1, 32, 8, 128, 16, maxP, mask, window, 0, BF16)[0]
+
+    assert kind(64, 512, 1024, 0) == cabi.QD_TREE_MFMA           # 512 items for 512 places
+    assert kind(40, 512, 1024, 0) == cabi.QD_TREE_MFMA_SPLIT     # 320 items
+    assert kind(4, 4) == cabi.QD_TREE_MFMA                       # one unit each
+    assert kind(4, 512) == cabi.QD_TREE_MFMA_SPLIT
+    assert kind(64, 64) == cabi.QD_TREE_MFMA                     # 16 units at most
+    assert kind(64, 100) == cabi.QD_TREE_MFMA_SPLIT              # lengths may differ by 25 units
+    assert kind(1024, 512) == cabi.QD_TREE_MFMA_SPLIT
+    assert kind(1025, 512) == cabi.QD_TREE_MFMA
+
+
 # ---- Norm, rotation and write ------------------------------------------------
 
 
