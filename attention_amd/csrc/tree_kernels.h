@@ -303,12 +303,19 @@ __device__ __forceinline__ int32_t tree_scalar_load(const int32_t* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
+// Reads by LDS byte address: slots of a row are exchanged by an exclusive or of
+// its bits, without a step from address to pointer.
+template <typename X>
+__device__ __forceinline__ X tree_lds_read(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) X*>(at);
+}
+
 // Four transposed 16-bit elements: lane (g4, r16) of the wave gets column r16
 // of the 4 x 16 block whose row r16 / 4, columns 4 (r16 % 4).. this lane
 // addresses.
-__device__ __forceinline__ u32x2 tree_tr_read(const char* p) {
+__device__ __forceinline__ u32x2 tree_tr_read(uint32_t at) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at)));
 }
 
 template <int DT>
@@ -414,9 +421,6 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     const int row0 = (hc % p.chunks) * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.R - row0);
     const int q0 = row0 / p.G, q1 = (row0 + rows - 1) / p.G;  // the chunk's queries
-    auto flip = [](const char* at, int bits) {  // swizzled slots: the chunk's bits are exchanged
-      return smem + (static_cast<uint32_t>(at - smem) ^ bits);
-    };
     const int context = sp.sinks + sp.len - sp.lo;
     auto token = [&](int v) { return v < sp.sinks ? v : sp.lo + (v - sp.sinks); };
     auto page_of = [&](int tok) { return p.pshift >= 0 ? tok >> p.pshift : tok / p.P; };
@@ -648,7 +652,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll 1
       for (int sub = 0; sub < Sh::kSub; ++sub) {
         const int wave_tok = Sh::kTW * wt + 16 * TB * sub;
-        const char* kb = buf + (wave_tok + r16) * Sh::kRow + 16 * (g4 ^ tree_swizzle(Sh::kSlots, r16));
+        const uint32_t at = tree_lds_address(buf) + wave_tok * Sh::kRow;
+        const uint32_t kb = at + r16 * Sh::kRow + 16 * (g4 ^ tree_swizzle(Sh::kSlots, r16));
         f32x4 s[TB][NB];
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb)
@@ -664,7 +669,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         auto read_k = [&](int st) {
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb)
-            ka[st % Sh::kQkAhead][tb] = *reinterpret_cast<const u32x4*>(flip(kb, 64 * st) + 16 * tb * Sh::kRow);
+            ka[st % Sh::kQkAhead][tb] = tree_lds_read<u32x4>((kb ^ (64 * st)) + 16 * tb * Sh::kRow);
         };
 #pragma unroll
         for (int st = 0; st < Sh::kQkAhead; ++st) read_k(st);
@@ -691,23 +696,23 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         }
         __builtin_amdgcn_s_setprio(0);
         // V^T of the first columns, in flight during the softmax.
-        const char* vb = buf + Sh::kTile + wave_tok * Sh::kRow;
+        const uint32_t vb = at + Sh::kTile;
         const int vr = 4 * g4 + (k16 ? r16 >> 2 : 0);
-        const char* va =
+        const uint32_t va =
             k16 ? vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tree_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1) : vb;
         u32x2 vf[Sh::kPvAhead][2 * TB];  // fp32: 4 TB values
         auto read_v = [&](int c) {
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb) {
             if constexpr (k16) {
-              vf[c % Sh::kPvAhead][tb] = tree_tr_read(flip(va, 32 * c) + 16 * tb * Sh::kRow);
+              vf[c % Sh::kPvAhead][tb] = tree_tr_read((va ^ (32 * c)) + 16 * tb * Sh::kRow);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int row = 4 * g4 + i;
-                const char* at = vb + row * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, row)) + 4 * (r16 & 3);
+                const uint32_t col = vb + row * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, row)) + 4 * (r16 & 3);
                 vf[c % Sh::kPvAhead][2 * tb + i / 2][i % 2] =
-                    *reinterpret_cast<const uint32_t*>(flip(at, 64 * c) + 16 * tb * Sh::kRow);
+                    tree_lds_read<uint32_t>((col ^ (64 * c)) + 16 * tb * Sh::kRow);
               }
             }
           }
