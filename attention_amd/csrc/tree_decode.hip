@@ -206,9 +206,11 @@ struct TreePlan {
 // One workgroup per item, without a merge, or the items' tiles cut into equal
 // ranges, one per resident workgroup, with a merge kernel (about 5 us, and a
 // start of 4 tiles for every item that a range begins)?  By what is left idle
-// if every context fills its table or window, in units of 64 tokens per
-// resident workgroup, and by how uneven contexts without a window can be.
-// bf16, 8 kv-heads of 128, one workgroup per item against equal ranges, us:
+// if every context fills its table or window, in units of 64 tokens with rows
+// of 256 bytes per resident workgroup (longer rows count as more units: fp32,
+// 22 items of 230 tokens x 256, 25.5 us in ranges, 38.3 us whole), and by how
+// uneven contexts without a window can be.  bf16, 8 kv-heads of 128, one
+// workgroup per item against equal ranges, us:
 // 512 items of 18 units (a window of 1024) 48.6 / 54.6, 320 of them 40.0 / 38.9,
 // 128 of them 32.7 / 25.1; 1024 items of 9 units 56.4 / 60.1, 1600 of them 98 /
 // 93.6; without a window, 512 items of 2 to 16 units 40.5 / 52.6, 1024 items of
@@ -237,21 +239,32 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   }
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   pl.dp = tree_padded(es, head_dim);
-  const int slots = tree_slots(es, pl.dp), most = tree_most_rows(slots);
+  const int slots = tree_slots(es, pl.dp);
   const int R = q_len * (q_heads / kv_heads);
-  pl.chunks = (R + most - 1) / most;
-  pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
-  const TreeWaves wv = tree_waves(slots, pl.chunk_rows);
-  const int64_t items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
-  const int tt = tree_tile(slots, wv.nw);
-  const int64_t tiles = (cap + tt - 1) / tt;
-  const int64_t resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
+  TreeWaves wv{};
+  int64_t items = 0, tiles = 0, units = 0, resident = 0;
+  // The largest chunks that still give every resident workgroup a tile: K and V
+  // are read once per chunk, but a tile of 256 rows takes 8 times as long as one
+  // of 16 (one sequence of 8000 to 16000 tokens, 24 drafts x 4 heads of 96:
+  // chunks of 16 rows 20.6 us, one chunk 30.5 us; 8 sequences of 489 tokens, 64
+  // drafts x 8 heads of 128: 23.6 us, chunks of 256 rows 41.3 us).
+  for (int most = tree_most_rows(slots);; most /= 2) {
+    pl.chunks = (R + most - 1) / most;
+    pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
+    wv = tree_waves(slots, pl.chunk_rows);
+    const int tt = tree_tile(slots, wv.nw);
+    items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
+    tiles = (cap + tt - 1) / tt;
+    units = std::max<int64_t>(1, tiles * tt / 64) * std::max(1, slots / 16);
+    resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
+    if (pl.chunk_rows <= 16 || items * tiles >= resident) break;
+  }
   if (batch > kTreeMaxBalanced || items * (tiles + kTreeItemCost) > INT32_MAX ||
-      tree_direct(items, std::max<int64_t>(1, tiles * tt / 64), resident, window > 0)) {
+      tree_direct(items, units, resident, window > 0)) {
     pl.grid = static_cast<int>(items);
     return pl;
   }
-  pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / kTreeMinCost)));
+  pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kTreeItemCost) / tree_min_cost(slots))));
   pl.grid = pl.W;
   pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;
   pl.bytes = pl.meta_bytes + sizeof(float) * 2 * static_cast<size_t>(pl.W) * (16 * wv.nb * wv.wr) * (head_dim + 2);

@@ -129,12 +129,14 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 // c ^ tree_swizzle(r), which spreads both the 16 rows of a K operand read and
 // the 32-byte pieces of a transposing V read over the 64 banks.
 
-// Balanced launches: an item costs its tiles and one more (its queries, first
-// round trips and stores take about as long).
+// Balanced launches: an item costs its tiles and this many more (its queries,
+// first round trips and stores take about as long; 2 instead of 4: trees of 16
+// over 32 sequences 75 -> 81 us).
 constexpr int kTreeItemCost = 4;
-// Least cost of a workgroup's range: shorter ones gain less than their
-// partials cost.
-constexpr int kTreeMinCost = 4;
+// Partials of an item, on average, from which the merge gives each row a whole
+// workgroup (one sequence of 20000 tokens, 81 partials: 74.6 -> 38.2 us; 24
+// items with 6 partials of 256 rows: 43.8 -> 50.2 us).
+constexpr int kTreeManyPartials = 8;
 // Sequences whose prefix of costs fits the kernel's LDS.
 constexpr int kTreeMaxBalanced = 1024;
 // Page ids that the kernel keeps in LDS at a time, one for each group of 16
@@ -154,6 +156,11 @@ __host__ __device__ constexpr int tree_slots(int es, int dp) {
 __host__ __device__ constexpr int tree_tile(int slots, int nw) {
   return slots == 64 ? 32 : slots <= 16 && nw == 8 ? 128 : 64;
 }
+// Least cost of a workgroup's range: shorter ones gain less than their
+// partials cost (2 against 4: one sequence of 20000 tokens, rows of 512 bytes,
+// 31.9 / 36.6 us, fp32 trees of 8 over 8 sequences 27.1 / 31.3 us; rows of 256
+// bytes, 8 drafts over 8 sequences of 200 to 400 tokens, 20.6 / 18.8 us).
+__host__ __device__ constexpr int tree_min_cost(int slots) { return slots >= 32 ? 2 : 4; }
 // The most rows of a chunk: what the registers hold.
 __host__ __device__ constexpr int tree_most_rows(int slots) { return slots <= 16 ? 256 : slots == 32 ? 128 : 32; }
 
@@ -995,7 +1002,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       __syncthreads();
     }
     total = prefix(p.B - 1);
-    used = min(p.W, max(1, total / kTreeMinCost));
+    used = min(p.W, max(1, total / tree_min_cost(Sh::kSlots)));
     if (w >= used) return;
     pos = part_of(w, total, used);
     end = part_of(w + 1, total, used);
@@ -1047,10 +1054,11 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 }
 
 // Log-sum-exp merge of the items that a balanced launch split, and the rows of
-// sequences without any token.  A workgroup of 4 waves serves 16 rows of an
-// item: 16 lanes per row, the lanes stride its columns.
+// sequences without any token.  A workgroup of 4 waves serves 16 / LANES rows of
+// an item: LANES x 16 lanes per row, 16 of them stride its columns, LANES its
+// partials.
 // grid (items, row blocks), block 256.
-template <int DT, int KROWS>
+template <int DT, int KROWS, int LANES>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
   using E = Elem<DT>;
   const int per_seq = p.Hkv * p.chunks;
@@ -1062,44 +1070,70 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
   if (count == 1) return;
   const int h = hc / p.chunks, row0 = (hc % p.chunks) * p.chunk_rows;
   const int rows = min(p.chunk_rows, p.R - row0);
-  const int rr = 16 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x >> 4);
-  if (rr >= rows) return;
+  const int l16 = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int rr = 16 / LANES * static_cast<int>(blockIdx.y) + group / LANES, lane = group % LANES;
+  if (rr >= rows) return;  // LANES > 1: the whole workgroup
   const int t = (row0 + rr) / p.G, g = (row0 + rr) % p.G;
   typename E::S* out = static_cast<typename E::S*>(p.out) +
                        ((static_cast<int64_t>(b) * p.T + t) * p.Hq + static_cast<int64_t>(h) * p.G + g) * p.D;
   const int64_t slot_floats = static_cast<int64_t>(KROWS) * (p.D + 2);
   auto part = [&](int s) { return p.part + (2 * static_cast<int64_t>(first + s) + (s == 0 ? 1 : 0)) * slot_floats; };
   auto stat = [&](int s) { return *reinterpret_cast<const f32x2*>(part(s) + static_cast<int64_t>(KROWS) * p.D + 2 * rr); };
-  // Four partials at a time, statistics and values in flight together.
-  const int l16 = threadIdx.x & 15;
-  for (int d = 4 * l16; d < p.D; d += 64) {
+  static_assert(LANES == 1 || LANES == 16, "a row per group of 16 lanes or per workgroup");
+  __shared__ f32x4 values[LANES > 1 ? 16 : 1][16];
+  __shared__ f32x2 stats[16];
+  for (int d0 = 0; d0 < p.D; d0 += 64) {
+    const int d = d0 + 4 * l16;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     float mx = -INFINITY, sum = 0.f;
-    for (int s0 = 0; s0 < count; s0 += 4) {
-      f32x2 ml[4];
-      f32x4 x[4];
+    // Four partials at a time, statistics and values in flight together.
+    if (d < p.D) {
+      for (int s0 = 4 * lane; s0 < count; s0 += 4 * LANES) {
+        f32x2 ml[4];
+        f32x4 x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = min(s0 + i, count - 1);
-        ml[i] = stat(s);
-        x[i] = *reinterpret_cast<const f32x4*>(part(s) + static_cast<int64_t>(rr) * p.D + d);
+        for (int i = 0; i < 4; ++i) {
+          const int s = min(s0 + i, count - 1);
+          ml[i] = stat(s);
+          x[i] = *reinterpret_cast<const f32x4*>(part(s) + static_cast<int64_t>(rr) * p.D + d);
+        }
+        float most = mx;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, ml[i][0]);
+        const float ref = most == -INFINITY ? 0.f : most;
+        const float old = fast_exp2(mx - ref);
+        sum *= old;
+        a *= old;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (s0 + i >= count) continue;
+          const float f = fast_exp2(ml[i][0] - ref);
+          sum += f * ml[i][1];
+          a += f * x[i];
+        }
+        mx = most;
       }
-      float most = mx;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = fmaxf(most, ml[i][0]);
-      const float ref = most == -INFINITY ? 0.f : most;
-      const float old = fast_exp2(mx - ref);
-      sum *= old;
-      a *= old;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (s0 + i >= count) continue;
-        const float f = fast_exp2(ml[i][0] - ref);
-        sum += f * ml[i][1];
-        a += f * x[i];
-      }
-      mx = most;
     }
+    if constexpr (LANES > 1) {
+      if (d0 > 0) __syncthreads();
+      values[group][l16] = a;
+      if (l16 == 0) stats[group] = f32x2{mx, sum};
+      __syncthreads();
+      if (lane > 0) continue;
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) most = fmaxf(most, stats[i][0]);
+      const float ref = most == -INFINITY ? 0.f : most;
+      a = f32x4{0.f, 0.f, 0.f, 0.f};
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) {
+        const float f = fast_exp2(stats[i][0] - ref);
+        sum += f * stats[i][1];
+        a += f * values[i][l16];
+      }
+    }
+    if (d >= p.D) continue;
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[d + i] = E::from_f(sum > 0.f || sum != sum ? a[i] * inv : 0.f);
@@ -1124,8 +1158,10 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
   }
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(64 * NW), lds, st, p);
   if (p.W > 0) {
-    void (*merge)(TreeParams) = tree_merge_kernel<DT, Sh::kRows>;
-    hipLaunchKernelGGL(merge, dim3(static_cast<uint32_t>(p.B * p.Hkv * p.chunks), static_cast<uint32_t>((p.chunk_rows + 15) / 16)),
+    const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * p.chunks;
+    const bool many = p.W >= kTreeManyPartials * items;
+    void (*merge)(TreeParams) = many ? tree_merge_kernel<DT, Sh::kRows, 16> : tree_merge_kernel<DT, Sh::kRows, 1>;
+    hipLaunchKernelGGL(merge, dim3(static_cast<uint32_t>(items), static_cast<uint32_t>(many ? p.chunk_rows : (p.chunk_rows + 15) / 16)),
                        dim3(256), 0, st, p);
   }
   return hipGetLastError();

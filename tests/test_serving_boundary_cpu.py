@@ -191,11 +191,14 @@ def test_plans_cover_all_rows_and_fit_their_workspace(shape):
                                           (64, 64, 64, F16), (64, 71, 256, BF16), (64, 71, 128, F32),
                                           (64, 71, 256, F32), (3, 200, 192, F16)])
 def test_rows_are_cut_evenly(T, Hq, D, dtype):
-    kind, _, rows = cabi.gqa_decode_tree_info(2, T, Hq, 1, D, 16, 100, dtype=dtype)
+    """As many rows as the registers hold where the tiles fill the card, fewer where they do not, 16 at least."""
     es = 4 if dtype == F32 else 2
     most = 256 if D * es <= 256 else 128 if D * es <= 512 else 32
-    chunks = -(-T * Hq // most)
-    assert kind != cabi.QD_TREE_VALU and rows == -(-T * Hq // chunks) <= most
+    R = T * Hq
+    kind, _, rows = cabi.gqa_decode_tree_info(256, T, Hq, 1, D, 16, 1000, dtype=dtype)
+    assert kind != cabi.QD_TREE_VALU and rows == -(-R // -(-R // most)) <= most
+    kind, _, rows = cabi.gqa_decode_tree_info(1, T, Hq, 1, D, 16, 1, dtype=dtype)
+    assert kind != cabi.QD_TREE_VALU and rows == -(-R // -(-R // 16)) <= 16
 
 
 def test_which_contexts_are_split():
