@@ -727,21 +727,26 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
         for (int c = 0; c < Sh::kPvAhead; ++c) read_v(c);
         __builtin_amdgcn_sched_barrier(0);
+        uint32_t vis[TB][NB];  // bits of this lane's 4 tokens of a block that its row sees
         if (!whole_tile) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
             const int src = query[nb] - q0;
-            const int lo = __shfl(mine.lo, src), sinks = __shfl(mine.sinks, src);
+            const int sinks = __shfl(mine.sinks, src);
+            const int lo = __shfl(mine.lo, src) - (sp.lo - sp.sinks);  // as a virtual token
             const uint64_t seen = static_cast<uint64_t>(__shfl(static_cast<long long>(mine.seen), src));
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
+            for (int tb = 0; tb < TB; ++tb) {
+              const int v = first + wave_tok + 16 * tb + 4 * g4;
+              auto below = [&](int end) { return (1u << min(max(end - v, 0), 4)) - 1; };  // tokens before `end`
+              const int j = v - context;
+              const uint32_t drafts = j <= -4 || j >= 64 ? 0u
+                                      : j < 0            ? static_cast<uint32_t>(seen) << -j
+                                                         : static_cast<uint32_t>(seen >> j);
+              vis[tb][nb] = below(sinks) | (below(context) & ~below(lo)) | drafts;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int v = first + wave_tok + 16 * tb + 4 * g4 + i;
-                const int tok = token(v);
-                const bool vis = v >= context ? v < sp.n && ((seen >> (v - context)) & 1) != 0 : tok < sinks || tok >= lo;
-                if (!vis) s[tb][nb][i] = -INFINITY;
-              }
+              for (int i = 0; i < 4; ++i) s[tb][nb][i] = (vis[tb][nb] >> i) & 1 ? s[tb][nb][i] : -INFINITY;
+            }
           }
         }
 #pragma unroll
@@ -791,8 +796,10 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (s[tb][nb][i] == 0.f) lw[tb][nb][i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t two = vis[tb][nb] >> (2 * i);
+                  lw[tb][nb][i] &= (two & 1 ? 0x0000FFFFu : 0u) | (two & 2 ? 0xFFFF0000u : 0u);
+                }
           }
           __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(1);
