@@ -6,8 +6,8 @@
 // What a query sees (Row below): context tokens [0, sinks) and [lo, len), and
 // the drafted tokens of its mask.  The tokens that it sees without the mask
 // are numbered through ("virtual" tokens): v < sinks is token v, the others
-// are lo + v - sinks, so tiles of 64 never cover the gap between the first
-// tokens and the window.
+// are lo + v - sinks, so no tile covers the gap between the first tokens and
+// the window.
 
 #include <hip/hip_runtime.h>
 
@@ -28,7 +28,10 @@ namespace {
 // Any head_dim, alignment and type, on the VALU: a workgroup per (query head,
 // split); its four waves take 64-token blocks in turn, a lane per token for
 // the scores and a lane per 64th column for the values.  Tokens that the query
-// does not see are not read at all.
+// does not see are not read at all.  For what the matrix-core kernel does not
+// take, and as its check: it reads K and V once per query and head, a lane a
+// whole row (8 sequences, trees of 64, 64 heads of 128: 33 ms against 270 us;
+// trees of 16 over 32 sequences 4.5 ms / 75 us; 4 short windows 17.6 / 9.5 us).
 // grid (B * T * Hq, splits), block 256.
 template <int DT>
 __global__ __launch_bounds__(256) void tree_generic_kernel(TreeParams p) {

@@ -125,6 +125,23 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 //            output's own.
 // Waves that share rows (WT > 1) merge at the end of an item through LDS.
 //
+// K and V are read once per chunk of rows, scores never leave registers.  With
+// few rows HBM bounds the kernel, with many the issue of matrix and vector
+// instructions: a 16x16 step of 32 tokens takes 3 matrix instructions of 16
+// cycles per 16 columns (two parts of the weights) and about 50 cycles of vector
+// instructions per score register, and two waves of a SIMD overlap them only
+// in part.  Measured, bf16, heads of 128, pages of 16:
+//   64 sequences, window 1024, 4 rows        48 us, 5.5 TB/s
+//   16 sequences, window 32768, 8 rows       341 us, 6.3 TB/s
+//   32 sequences, trees of 16, 64 rows       75 us, 4.2 TB/s
+//   8 sequences, trees of 64, 512 rows       270 us, 474 TFLOP/s of QK^T and PV
+//   fp32, 8 sequences, trees of 8, 32 rows   27 us
+// Tried without gain: software pipelining of a wave's scores, softmax and values
+// (302 to 340 us for trees of 64: the registers of two steps spill), barriers
+// that make the two waves of a SIMD take turns at products and softmax (356 us),
+// later K operands read under the last products of V (no change), 64-token
+// tiles with eight waves, loads spread over a step.
+//
 // LDS rows are a power of two of 16-byte slots; chunk c of row r lies in slot
 // c ^ tree_swizzle(r), which spreads both the 16 rows of a K operand read and
 // the 32-byte pieces of a transposing V read over the 64 banks.
@@ -511,6 +528,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     auto load_piece = [&](const TileLoad& x, int i) {
       const uint32_t to = x.to + 1024 * i;
       if (grouped && !padded) {
+        // Not kept in the caches where no other chunk reads the rows (316 MB of
+        // K and V 75 us, kept 82 us; 2.1 GB 341 / 381 us).
         if (p.chunks == 1) {
           tree_load_lds<true>(x.k, lane_off[i], to);
           tree_load_lds<true>(x.v, lane_off[i], to + Sh::kTile);
@@ -666,8 +685,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // The matrix cores' phases go before another wave's softmax (64 drafts x
-        // 64 heads: 277 -> 270 us).
+        // The matrix cores' phases go before another wave's softmax (trees of
+        // 64: 277 -> 270 us).
         __builtin_amdgcn_s_setprio(1);
         // Operands are read ahead of their products: a product takes 16 cycles,
         // an LDS read here well over 100.  The scheduling barriers keep the

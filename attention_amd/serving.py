@@ -87,8 +87,9 @@ def kv_compact(caches, block_table, context_lens, accepted):
     moves to token ``context_lens[b] + i``, as if all were read before any is
     written.  ``accepted`` int32 ``[B, A]``, ``A <= 64``: indices of drafted
     tokens, such as the path that was verified; negative entries move nothing.
-    Tokens outside the table and pages outside the pool are skipped.  One
-    launch serves up to 128 caches.
+    Tokens outside the table and pages outside the pool are skipped.  Rows
+    that move must be their sequence's own: pages shared with other sequences
+    may hold context, not drafted tokens.  One launch serves up to 128 caches.
     """
     _require_extension()
     torch.ops.qd_serving.kv_compact(list(caches), block_table, context_lens, accepted)

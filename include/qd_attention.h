@@ -538,7 +538,8 @@ int qd_kv_compact_validate(const qd_tensor_desc* cache, const qd_tensor_desc* bl
  * is written.  count <= 64.  Tokens past the table, page ids outside the pool
  * and negative lengths are skipped (nothing is read or written).  `caches` is
  * a host array of device pointers, read during the call; the caches must not
- * overlap (checked). */
+ * overlap (checked).  Rows that move must be their sequence's own: a row that
+ * one sequence writes is not read or written for another in the same call. */
 int qd_kv_compact(void* const* caches, int num_caches, const int32_t* block_table, const int32_t* context_lens,
                   const int32_t* accepted, int batch, int count, int block_size, int max_pages, int64_t num_blocks,
                   int64_t row_bytes, void* stream);
