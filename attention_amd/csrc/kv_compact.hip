@@ -46,10 +46,10 @@ __device__ __forceinline__ int64_t pool_row(const CompactParams& p, int b, int64
 // of the cache.  Every row moved is read and written once: bound by HBM in large
 // calls, by the launch and three dependent round trips (length, table, row) in
 // small ones.  Measured: 72 caches, 32 sequences of 16 drafts, rows of 2 KB
-// (57.5 MB in and out) 12.8 us, 4.5 TB/s, where a large copy makes 4.9; two
-// caches, 4 sequences of 8 5.4 us.  Registers for 16 rows instead of 64 where
-// that is enough made no difference (15.8 / 15.9 us with cold caches).
-template <typename V>
+// (57.5 MB in and out) 13.5 us, 4.3 TB/s, where a large copy makes 4.9; two
+// caches, 4 sequences of 8 5.4 us.  ROWS rows per wave: registers for 16 rows in
+// all where that is enough, or for 64 (16 drafts: 14.5 / 15.8 us).
+template <typename V, int ROWS>
 __global__ __launch_bounds__(256) void kv_compact_kernel(CompactParams p) {
   const int b = blockIdx.x;
   const int lane = threadIdx.x & 63;
@@ -68,10 +68,9 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(CompactParams p) {
   char* cache = p.caches[blockIdx.y];
   const int64_t col = (static_cast<int64_t>(blockIdx.z) * 64 + lane) * static_cast<int64_t>(sizeof(V));
   const bool inside = col < p.row_bytes;
-  constexpr int kRows = QD_TREE_MAX_DRAFTS / 4;
-  V held[kRows];
+  V held[ROWS];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const int64_t row = readlane_i64(from, wv + 4 * i);
     if (row >= 0 && inside) held[i] = *reinterpret_cast<const V*>(cache + row * p.row_bytes + col);
   }
@@ -79,7 +78,7 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(CompactParams p) {
   wait_memory_retired();
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const int64_t row = readlane_i64(from, wv + 4 * i);
     const int64_t dst = readlane_i64(to, wv + 4 * i);
     if (row >= 0 && inside) *reinterpret_cast<V*>(cache + dst * p.row_bytes + col) = held[i];
@@ -101,7 +100,10 @@ template <typename V>
 void launch_compact(const CompactParams& p, int batch, int caches, hipStream_t st) {
   const int64_t blocks = (p.row_bytes + 64 * static_cast<int64_t>(sizeof(V)) - 1) / (64 * static_cast<int64_t>(sizeof(V)));
   const dim3 grid(static_cast<uint32_t>(batch), static_cast<uint32_t>(caches), static_cast<uint32_t>(blocks));
-  hipLaunchKernelGGL(kv_compact_kernel<V>, grid, dim3(256), 0, st, p);
+  if (p.count <= 16)
+    hipLaunchKernelGGL((kv_compact_kernel<V, 4>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((kv_compact_kernel<V, QD_TREE_MAX_DRAFTS / 4>), grid, dim3(256), 0, st, p);
 }
 
 }  // namespace
