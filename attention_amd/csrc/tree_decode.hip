@@ -259,7 +259,7 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
     items = static_cast<int64_t>(batch) * kv_heads * pl.chunks;
     tiles = (cap + tt - 1) / tt;
     units = std::max<int64_t>(1, tiles * tt / 64) * std::max(1, slots / 16);
-    resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nb, wv.nw);
+    resident = static_cast<int64_t>(tree_cu_count()) * tree_occupancy(slots, wv.nw);
     if (pl.chunk_rows <= 16 || items * tiles >= resident) break;
   }
   if (batch > kTreeMaxBalanced || items * (tiles + kTreeItemCost) > INT32_MAX ||

@@ -111,9 +111,8 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 //
 // An item is a (sequence, kv-head, chunk of its rows); a row is a (query,
 // q-head of the kv-head's group).  A workgroup of NW waves goes through an
-// item's virtual tokens in tiles of TT: K and V rows come straight into a ring
-// of LDS buffers (global_load_lds), up to kBufs - 1 tiles ahead, and wave (wr,
-// wt) multiplies row blocks [16 NB wr, 16 NB (wr + 1)) with tokens [TT / WT
+// item's virtual tokens in tiles of TT: K and V rows come straight into one of
+// two LDS buffers (global_load_lds), one tile ahead, and wave (wr, wt) multiplies row blocks [16 NB wr, 16 NB (wr + 1)) with tokens [TT / WT
 // wt, ...), at most 32 of them at a time:
 //   scores   S^T = K Q^T, 16x16 blocks (A = K rows from LDS, B = Q from
 //            registers): a lane holds one row and 4 tokens per block
@@ -168,7 +167,7 @@ __host__ __device__ constexpr int tree_padded(int es, int d) {
 __host__ __device__ constexpr int tree_slots(int es, int dp) {
   return dp * es <= 128 ? 8 : dp * es <= 256 ? 16 : dp * es <= 512 ? 32 : 64;
 }
-// Tokens of a tile: a wave works on 16, 32 or 64 of them, so that what it does
+// Tokens of a tile: a wave works on 16 to 128 of them, so that what it does
 // once per tile stays small beside its products.
 __host__ __device__ constexpr int tree_tile(int slots, int nw) {
   return slots == 64 ? 32 : slots <= 16 && nw == 8 ? 128 : 64;
@@ -182,8 +181,11 @@ __host__ __device__ constexpr int tree_min_cost(int slots) { return slots >= 32 
 __host__ __device__ constexpr int tree_most_rows(int slots) { return slots <= 16 ? 256 : slots == 32 ? 128 : 32; }
 
 // Row blocks per wave, waves along the rows and waves of a workgroup for a
-// chunk of rows.  Either two workgroups of four waves are resident on a CU or
-// one of eight: one wave's products run under another's softmax.
+// chunk of rows.  Two waves share a SIMD, of two workgroups or of one with eight
+// waves, except where a row of LDS is 512 bytes or longer.  Eight waves on up to
+// 64 rows took 123 us where four take 95 (trees of 16), four on 512 rows 619
+// where eight take 335 (trees of 64); one row block of 16 per wave instead of
+// two doubles the LDS reads per product.
 struct TreeWaves {
   int nb, wr, nw;
 };
@@ -196,14 +198,17 @@ __host__ __device__ constexpr TreeWaves tree_waves(int slots, int rows) {
          : rows <= 128  ? TreeWaves{2, 4, 8}
                         : TreeWaves{2, 8, 8};
 }
-__host__ __device__ constexpr int tree_bufs(int slots, int nw) { return nw == 8 && slots == 8 ? 4 : 2; }
+// Tiles in LDS, of K and V each.  Four where they fit (heads of 64, more than 64
+// rows) made no call faster (64 drafts x 8 heads of 64: 115 us, 108 us with two).
+constexpr int kTreeBufs = 2;
 __host__ __device__ constexpr int tree_lds_bytes(int slots, int nw) {
-  return tree_bufs(slots, nw) * 2 * tree_tile(slots, nw) * slots * 16 + 4 * kTreePages + 32;
+  return kTreeBufs * 2 * tree_tile(slots, nw) * slots * 16 + 4 * kTreePages + 32;
 }
-// Resident workgroups per CU, which the launch bounds ask for.
-__host__ __device__ constexpr int tree_occupancy(int slots, int nb, int nw) {
+// Resident workgroups per CU, which the launch bounds ask for (three of heads
+// of 64 and up to 16 rows: 37.0 us, two 31.2 us, for 128 windows of 512).
+__host__ __device__ constexpr int tree_occupancy(int slots, int nw) {
   const int by_lds = 160 * 1024 / (tree_lds_bytes(slots, nw) + 4 * kTreeMaxBalanced);
-  const int by_regs = nw == 8 ? 1 : slots >= 32 ? 1 : slots == 8 && nb == 1 ? 3 : 2;
+  const int by_regs = nw == 8 || slots >= 32 ? 1 : 2;
   return by_lds < by_regs ? by_lds : by_regs;
 }
 
@@ -219,7 +224,6 @@ struct TreeShape {
   static constexpr int kWT = NW / WR;
   static constexpr int kRow = kSlots * 16;                   // bytes of an LDS row
   static constexpr int kTile = TT * kRow;                    // bytes of K or V
-  static constexpr int kBufs = tree_bufs(kSlots, NW);
   static constexpr int kLoadRows = TT / NW;                  // rows that a wave loads
   static constexpr int kLoads = kLoadRows * kSlots / 64;     // its instructions, for K and for V
   static constexpr int kSteps = DP * kES / 64;
@@ -233,7 +237,7 @@ struct TreeShape {
   static constexpr int kPvAhead = kES == 2 ? 4 : 2;
   static constexpr int kRows = 16 * NB * WR;                 // rows of a workgroup
   static constexpr int kLds = tree_lds_bytes(kSlots, NW);
-  static constexpr int kOcc = tree_occupancy(kSlots, NB, NW);
+  static constexpr int kOcc = tree_occupancy(kSlots, NW);
   static_assert(kTW >= 16 && kLoadRows * kSlots % 64 == 0 && kOcc >= 1, "waves do not fit the tile");
 };
 
@@ -425,7 +429,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   extern __shared__ __align__(16) char smem[];
   // Tokens with non-finite values that not all rows see: drafted ones, and
   // those at the window's edge (bit i: token seen_lo + i).
-  unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + Sh::kBufs * 2 * Sh::kTile);
+  unsigned long long* bad_words = reinterpret_cast<unsigned long long*>(smem + kTreeBufs * 2 * Sh::kTile);
   int32_t* pages = reinterpret_cast<int32_t*>(bad_words + 4);
   int32_t* incl = reinterpret_cast<int32_t*>(smem + Sh::kLds);
   const int tid = static_cast<int>(threadIdx.x);
@@ -572,30 +576,29 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         qf[nb][s] = real[nb] && at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
       }
     }
-    // The first tiles.  Their pages come through the scalar cache where one
-    // page serves a wave's rows; the list takes a barrier.
+    // The first tile.  Its pages come through the scalar cache where one page
+    // serves a wave's rows; the list takes a barrier.
     tree_barrier();  // the previous item's merge and the prefix are done with LDS
     if (tid < 2) bad_words[tid] = 0;
     if (padded) {
-      for (int i = tid; i < Sh::kBufs * Sh::kTile / 16; i += 64 * NW)
+      for (int i = tid; i < kTreeBufs * Sh::kTile / 16; i += 64 * NW)
         *(reinterpret_cast<u32x4*>(smem + i / (Sh::kTile / 16) * 2 * Sh::kTile) + i % (Sh::kTile / 16)) = u32x4{0u, 0u, 0u, 0u};
     }
-    int list_base = grouped ? t0 + Sh::kBufs - 1 : t0;
+    int list_base = grouped ? t0 + 1 : t0;
     const Pages listed = read_pages(list_base);
     uint64_t my_mask = 0;
     if (p.mask && q0 + lane <= q1) my_mask = draft_bits(p, b, q0 + lane);
     if (!grouped) put_pages(listed);
     if (padded || !grouped) tree_barrier();
-    for (int i = 0; i < Sh::kBufs - 1; ++i)
-      if (t0 + i < t1) {
-        int32_t phys = 0;
-        if (grouped)
-          phys = min(max(tree_scalar_load(table + min(page_of(token(Sh::TT * (t0 + i) + Sh::kLoadRows * wv)), last_page)), 0),
-                     p.last_block);
-        const TileLoad x = tile_load(t0 + i, i, phys, list_at(t0 + i, t0));
+    if (t0 < t1) {
+      int32_t phys = 0;
+      if (grouped)
+        phys = min(max(tree_scalar_load(table + min(page_of(token(Sh::TT * t0 + Sh::kLoadRows * wv)), last_page)), 0),
+                   p.last_block);
+      const TileLoad x = tile_load(t0, 0, phys, list_at(t0, t0));
 #pragma unroll
-        for (int j = 0; j < Sh::kLoads; ++j) load_piece(x, j);
-      }
+      for (int j = 0; j < Sh::kLoads; ++j) load_piece(x, j);
+    }
     if (grouped) put_pages(listed);
     // Lane t: what query q0 + t sees (at most 64 queries).
     Row mine;
@@ -629,14 +632,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     int slot_now = 0;
     for (int tile = t0; tile < t1; ++tile) {
       // The tile has arrived, and every wave is done with the one before it.
-      const int left = min(t1 - 1 - tile, Sh::kBufs - 2);
-      if (Sh::kBufs == 2 || left == 0)
-        tree_barrier_loads<0>();
-      else if (left == 1)
-        tree_barrier_loads<2 * Sh::kLoads>();
-      else
-        tree_barrier_loads<4 * Sh::kLoads>();
-      const int next = tile + Sh::kBufs - 1;
+      tree_barrier_loads<0>();
+      const int next = tile + 1;
       if (next < t1) {
         if (next >= list_base + list_tiles) {
           list_base = next;
@@ -644,13 +641,12 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
           tree_barrier();
         }
         const int at = list_at(next, list_base);
-        const TileLoad x = tile_load(next, slot_now == 0 ? Sh::kBufs - 1 : slot_now - 1,
-                                     grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
+        const TileLoad x = tile_load(next, slot_now ^ 1, grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
 #pragma unroll
         for (int j = 0; j < Sh::kLoads; ++j) load_piece(x, j);
       }
       char* buf = smem + slot_now * 2 * Sh::kTile;
-      slot_now = slot_now == Sh::kBufs - 1 ? 0 : slot_now + 1;
+      slot_now ^= 1;
       // Every row of the chunk sees all (existing) tokens of the tile.
       const int first = Sh::TT * tile, stop = first + Sh::TT;
       const bool whole_tile = stop <= sp.seen_sinks || (first >= edge && (stop <= context || (p.T == 1 && stop <= sp.n)));
@@ -878,7 +874,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     if constexpr (WT > 1) {
       // Every wave leaves its part in LDS, {m, l} of its rows where the page
       // list was, and takes up a share of the columns.
-      static_assert(NW * NB * Sh::kCols * 1024 <= Sh::kBufs * 2 * Sh::kTile && NW * NB * 128 <= 4 * kTreePages,
+      static_assert(NW * NB * Sh::kCols * 1024 <= kTreeBufs * 2 * Sh::kTile && NW * NB * 128 <= 4 * kTreePages,
                     "the waves' parts fit the tile buffers and the page list");
       f32x2* stats = reinterpret_cast<f32x2*>(pages);
 #pragma unroll

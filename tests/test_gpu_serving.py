@@ -245,7 +245,8 @@ MANY_SHAPES = [
     (BF, 65, 2, 4, 2, 64, 16, lengths(65, 60, 1900, 0, 700), 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
     (HF, 300, 1, 4, 1, 64, 16, lengths(300, 90, 0, 0, 1500), 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
     (FP, 90, 2, 2, 1, 128, 8, lengths(90, 40, 900), 250, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
-    (BF, 1024, 0, 2, 1, 64, 16, lengths(1024, 30, 3000), 250, 2000, 4, cabi.QD_TREE_MFMA_SPLIT),
+    (BF, 1024, 1, 2, 1, 64, 16, lengths(1024, 30, 3000), 250, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
+    (BF, 1024, 0, 2, 1, 64, 16, lengths(1024, 30, 3000), 250, 2000, 4, cabi.QD_TREE_MFMA),
     (BF, 70, 2, 2, 1, 64, 16, [0] * 70, 130, 0, 0, cabi.QD_TREE_MFMA_SPLIT),
     # more sequences than the split takes; a workgroup's page list is refilled: one
     # id for a token (pages of 12, 1) and for 16 (pages of 32)

@@ -175,7 +175,7 @@ def test_plans_cover_all_rows_and_fit_their_workspace(shape):
     elif kind == cabi.QD_TREE_MFMA:
         assert groups == B * Hkv * chunks
     else:
-        assert B <= 1024 and groups <= 3 * 256
+        assert B <= 1024 and groups <= 2 * 256
         need = 8 * B * Hkv * chunks + 4 * 2 * groups * rows * (D + 2)
     args = (B, T, Hq, Hkv, D, P, maxP, has_mask, window, sinks, dtype)
     valu = cabi.gqa_decode_tree_info(*args, cabi.QD_FLAG_FORCE_GENERIC)
