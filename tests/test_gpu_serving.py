@@ -267,6 +267,22 @@ def test_many_sequences_match_oracle(gpu, shape):
     check_case(gpu, case, window, sinks, what="default")
 
 
+def test_launch_limit_of_sequences(gpu):
+    """Almost 2^24 rows in one call, a workgroup for each: parts of the batch by themselves are bitwise the same."""
+    say("2^24 rows")
+    B = 4_000_000
+    gen = torch.Generator(device=gpu).manual_seed(0)
+    q = torch.randn(B, 4, 8, generator=gen, device=gpu).to(BF)
+    k, v = (torch.randn(50, 16, 4, 8, generator=gen, device=gpu).to(BF) for _ in range(2))
+    table = torch.randint(0, 50, (B, 1), generator=gen, device=gpu, dtype=torch.int32)
+    lens = torch.randint(0, 17, (B,), generator=gen, device=gpu, dtype=torch.int32)
+    whole = attention_amd.gqa_decode_window(q, k, v, table, lens, window=12, sinks=2)
+    for at in (0, 1_500_000, B - 2000):
+        part = slice(at, at + 2000)
+        assert torch.equal(whole[part], attention_amd.gqa_decode_window(q[part], k, v, table[part], lens[part], window=12,
+                                                                        sinks=2))
+
+
 def test_large_scores_stay_exact(gpu):
     """Scores of a few hundred: one token takes all of the weight."""
     say("large scores")
