@@ -183,7 +183,7 @@ def test_plans_cover_all_rows_and_fit_their_workspace(shape):
     splits = valu[1] // (B * T * Hq)
     both = max(need, 4 * B * T * Hq * splits * (D + 2) if splits > 1 else 0)
     bytes_ = cabi.lib().qd_gqa_decode_tree_workspace_bytes(*args, 0)
-    # Up to 16 rows round up to a block of each wave; nothing near twice the need beyond that.
+    # A range has two partials, of whole blocks of 16 rows even for one row.
     assert both <= bytes_ <= 32 * both + 4096
 
 
