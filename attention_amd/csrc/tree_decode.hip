@@ -221,6 +221,14 @@ struct TreePlan {
 constexpr int kTreeIdleUnits = 5;
 constexpr int kTreeUnevenUnits = 20;
 
+// Up to 128 rows run as two chunks on four waves each, rather than as one on
+// eight, while contexts hold at most this many tokens.  Two chunks / one, us: 80
+// rows, 122 sequences of up to 115 tokens 64.1 / 84.9; 128 rows, 64 sequences of
+// 100 to 500 tokens 53.5 / 60.7; 80 rows, 32 sequences of 1000 to 3000 98.9 /
+// 96.2; 128 rows, 8 sequences of 2000 to 8000 76.5 / 72.1; heads of 64, 96 rows,
+// 16 sequences of 2000 to 8000 66.4 / 58.0.
+constexpr int64_t kTreeShortContext = 1024;
+
 bool tree_direct(int64_t items, int64_t units, int64_t resident, bool windowed) {
   const int64_t rounds = (items + resident - 1) / resident;
   if (!windowed && rounds * units > kTreeUnevenUnits) return false;
@@ -251,7 +259,9 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   // of 16 (one sequence of 8000 to 16000 tokens, 24 drafts x 4 heads of 96:
   // chunks of 16 rows 20.6 us, one chunk 30.5 us; 8 sequences of 489 tokens, 64
   // drafts x 8 heads of 128: 23.6 us, chunks of 256 rows 41.3 us).
-  for (int most = tree_most_rows(slots);; most /= 2) {
+  int most = tree_most_rows(slots);
+  if (R <= 128 && cap <= kTreeShortContext) most = std::min(most, 64);
+  for (;; most /= 2) {
     pl.chunks = (R + most - 1) / most;
     pl.chunk_rows = (R + pl.chunks - 1) / pl.chunks;
     wv = tree_waves(slots, pl.chunk_rows);

@@ -187,18 +187,27 @@ def test_plans_cover_all_rows_and_fit_their_workspace(shape):
     assert both <= bytes_ <= 32 * both + 4096
 
 
-@pytest.mark.parametrize("T,Hq,D,dtype", [(1, 8, 128, BF16), (2, 8, 128, BF16), (8, 8, 128, BF16), (64, 8, 128, BF16),
+@pytest.mark.parametrize("T,Hq,D,dtype", [(1, 8, 128, BF16), (2, 8, 128, BF16), (8, 8, 128, BF16), (16, 8, 128, BF16), (11, 8, 64, F16), (17, 8, 128, BF16), (64, 8, 128, BF16),
                                           (64, 64, 64, F16), (64, 71, 256, BF16), (64, 71, 128, F32),
                                           (64, 71, 256, F32), (3, 200, 192, F16)])
 def test_rows_are_cut_evenly(T, Hq, D, dtype):
-    """As many rows as the registers hold where the tiles fill the card, fewer where they do not, 16 at least."""
+    """As many rows as the registers hold where the tiles fill the card (up to 128 rows of 256 bytes and short
+    contexts: 64), fewer where they do not, 16 at least."""
     es = 4 if dtype == F32 else 2
-    most = 256 if D * es <= 256 else 128 if D * es <= 512 else 32
     R = T * Hq
-    kind, _, rows = cabi.gqa_decode_tree_info(256, T, Hq, 1, D, 16, 1000, dtype=dtype)
-    assert kind != cabi.QD_TREE_VALU and rows == -(-R // -(-R // most)) <= most
-    kind, _, rows = cabi.gqa_decode_tree_info(1, T, Hq, 1, D, 16, 1, dtype=dtype)
-    assert kind != cabi.QD_TREE_VALU and rows == -(-R // -(-R // 16)) <= 16
+    most = 256 if D * es <= 256 else 128 if D * es <= 512 else 32
+
+    def rows_of(B, maxP):
+        kind, _, rows = cabi.gqa_decode_tree_info(B, T, Hq, 1, D, 16, maxP, dtype=dtype)
+        assert kind != cabi.QD_TREE_VALU
+        return rows
+
+    def cut(most):
+        return -(-R // -(-R // most))
+
+    assert rows_of(256, 1000) == cut(most) <= most
+    assert rows_of(1000, 64) == cut(min(most, 64) if R <= 128 else most)
+    assert rows_of(1, 1) == cut(16) <= 16
 
 
 def test_which_contexts_are_split():
