@@ -626,6 +626,9 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     }
 
     const int edge = sp.sinks + max(lo_max - sp.lo, 0);  // virtual tokens below: not in every row's window
+    // Tokens between these: in no row's window.  The chunk's only query may be a
+    // later one than the sequence's first.
+    const int lo_all = q0 == q1 ? lo_max : sp.seen_lo, sinks_all = q0 == q1 ? min(p.sinks, lo_max) : sp.seen_sinks;
     // No register load is pending when the loop starts: the compiler would
     // wait for it, and so for the tiles in flight, in every turn.
     __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0)
@@ -658,7 +661,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         for (int i = tid; i < Sh::TT * Sh::kSlots; i += 64 * NW) {
           const int v = first + i / Sh::kSlots, tok = token(v);
           u32x4* at = reinterpret_cast<u32x4*>(buf + Sh::kTile) + i;
-          if (v < context ? tok >= sp.seen_sinks && tok < sp.seen_lo : v >= sp.n || !((any_seen >> (v - context)) & 1)) {
+          if (v < context ? tok >= sinks_all && tok < lo_all : v >= sp.n || !((any_seen >> (v - context)) & 1)) {
             *at = u32x4{0u, 0u, 0u, 0u};
           } else if (q0 != q1 && (v >= context || (tok >= sp.seen_lo && tok < lo_max))) {
             u32x4 x = *at;

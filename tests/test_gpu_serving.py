@@ -345,6 +345,34 @@ def test_hidden_tokens_cannot_reach_a_row(gpu, dtype, T, window, sinks):
             assert not torch.isfinite(out[~keep]).all(-1).any(), "a row that sees NaN must say so"
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FP], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("T,group,window,sinks", [(8, 16, 130, 0), (8, 16, 40, 30), (12, 16, 5, 3), (3, 64, 60, 2),
+                                                  (5, 71, 33, 0), (4, 256, 100, 7), (2, 16, 1, 0)])
+def test_hidden_tokens_where_workgroups_hold_one_query(gpu, dtype, T, group, window, sinks):
+    """As above, with rows cut so that a workgroup serves heads of one query, whose window begins later than the
+    first query's."""
+    say(f"poison {dtype} T{T} group {group} window {window} sinks {sinks}")
+    from oracle.serving_oracle import visible
+    lens, P = [172, 8, 0, 300], 16
+    q, k, v, table, lens, _ = attention_case(dtype, 4, T, 2 * group, 2, 72, P, lens, seed=T)
+    masks = [[(2 << t) - 1 for t in range(T)],                         # a chain
+             [(2 << t) - 1 if t else 0 for t in range(T)],             # whose first token is padding
+             [1 | 1 << t for t in range(T)], [1 << t for t in range(T)]]
+    clean, spread, size = attention_want(q, k, v, table, lens, masks, window, sinks, 0.1)
+    for b in range(4):
+        # One query at a time: everything that it does not see is poisoned.
+        for t in range(T):
+            seen = visible(int(lens[b]), masks[b], T, table.shape[1] * P, window, sinks)[t]
+            used = torch.zeros(k.shape[0], P, dtype=torch.bool)
+            for tok in np.nonzero(seen)[0]:
+                used[int(table[b, tok // P]), tok % P] = True
+            bk, bv = k.clone(), v.clone()
+            bk[~used] = float("nan")
+            bv[~used] = float("inf")
+            out = attend(gpu, (q, bk, bv, table, lens, masks), window, sinks, scale=0.1)
+            attention_check(out[b, t], clean[b, t], spread[b, t], size[b, t], dtype, 72, 400, f"sequence {b} query {t}")
+
+
 def test_hidden_values_in_window_edge(gpu):
     """Infinite values (finite keys) in a token that only the earlier queries' windows hold."""
     say("window edge")
