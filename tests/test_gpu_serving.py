@@ -19,6 +19,7 @@ Below the smallest normal number the rounding step is fixed: 2^-25 for fp16.
 from __future__ import annotations
 
 import math
+import random
 
 import numpy as np
 import pytest
@@ -281,6 +282,42 @@ def test_launch_limit_of_sequences(gpu):
         part = slice(at, at + 2000)
         assert torch.equal(whole[part], attention_amd.gqa_decode_window(q[part], k, v, table[part], lens[part], window=12,
                                                                         sinks=2))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_calls_match_oracle(gpu, seed):
+    """Types, heads, pages, lengths, trees and windows at random; what one random query does not see holds NaN, Inf
+    or large values."""
+    from oracle.serving_oracle import visible
+    rng = random.Random(seed)
+    for n in range(60):
+        dtype, D, P = rng.choice([BF, HF, FP]), rng.choice([8, 40, 64, 72, 80, 96, 112, 128, 160, 192, 256]), \
+            rng.choice([1, 3, 4, 8, 12, 16, 16, 32, 48, 64])
+        Hkv, group = rng.choice([1, 2, 3]), rng.choice([1, 2, 4, 5, 8, 16, 40])
+        T, B = rng.choice([0, 1, 2, 5, 8, 16, 33, 64]), rng.randint(1, 4)
+        lens = [rng.choice([0, 1, rng.randint(0, 40), rng.randint(0, 300), rng.randint(0, 1000)]) for _ in range(B)]
+        window = rng.choice([0, 0, 1, 7, 40, 130, 700]) or (0 if T else 50)
+        sinks = rng.choice([0, 4, 20, 200]) if window else 0
+        if sum(lens) * max(T, 1) * group * Hkv * D > 1e8:
+            lens = [length % 30 for length in lens]
+        say(f"{n}: {dtype} T{T} {group * Hkv}x{Hkv}x{D} P{P} {lens} window {window} sinks {sinks}")
+        q, k, v, table, dl, masks = attention_case(dtype, B, T, group * Hkv, Hkv, D, P, lens, branch=rng.choice([1, 2, 5]),
+                                                   seed=n, spare=rng.choice([1, 2, 40]))
+        if masks and rng.random() < 0.3:
+            masks = [[m if rng.random() < 0.8 else 0 for m in row] for row in masks]
+        want, spread, size = attention_want(q, k, v, table, dl, masks, window, sinks, 1 / math.sqrt(D))
+        b, t = rng.randrange(B), rng.randrange(max(T, 1))
+        sees = visible(lens[b], masks[b] if masks else None, T, table.shape[1] * P, window, sinks)[t]
+        used = torch.zeros(k.shape[0], P, dtype=torch.bool)
+        for tok in np.nonzero(sees)[0]:
+            used[int(table[b, tok // P]), tok % P] = True
+        clean = attend(gpu, (q, k, v, table, dl, masks), window, sinks)
+        attention_check(clean, want, spread, size, dtype, D, max(lens) + 64, "clean")
+        k[~used] = rng.choice([math.nan, math.inf, 1.0, -3e4])
+        v[~used] = rng.choice([math.nan, math.inf, -math.inf, 3e4])
+        out = attend(gpu, (q, k, v, table, dl, masks), window, sinks)
+        at = (b, t) if T else b
+        attention_check(out[at], want[at], spread[at], size[at], dtype, D, max(lens) + 64, "poisoned")
 
 
 def test_large_scores_stay_exact(gpu):
