@@ -37,7 +37,8 @@ struct TreeParams {
   int pshift;    // log2(P), or -1
   int32_t last_block;  // largest page id that a table entry can hold
   // Tokens of a table row; the last 256 below 2^31 are left out, so that token
-  // numbers, their tiles and sums with a window or 64 drafts fit 32 bits.
+  // numbers, the ends of their tiles and sums with 64 drafts fit 32 bits.
+  // Whatever reaches further ahead is compared as a distance.
   int32_t capacity;
 };
 
@@ -481,13 +482,15 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       int32_t id[kEach];
     };
     auto read_pages = [&](int tile) {
-      const int until = min(sp.n, Sh::TT * t1);
+      // The list reaches up to 16 kTreePages tokens past the tile, which may pass
+      // 2^31: only a place below `left` is added to the tile's first token.
+      const int first = Sh::TT * tile, left = min(sp.n, Sh::TT * t1) - first;
       Pages x;
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int v = Sh::TT * tile + each * (64 * NW * i + tid);
+        const int ahead = each * (64 * NW * i + tid);
         x.id[i] = 0;
-        if (v < until) x.id[i] = table[page_of(token(v))];
+        if (ahead < left) x.id[i] = table[page_of(token(first + ahead))];
       }
       return x;
     };

@@ -987,3 +987,39 @@ def test_tree_decode_captured_with_split_contexts(gpu):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("T,P,width", [(0, 1 << 20, 2048), (2, 1 << 20, 2048), (1, (1 << 20) - 4, 2049)], ids=str)
+def test_contexts_up_to_the_clamp(gpu, T, P, width):
+    """Contexts that fill a table of 2^31 tokens and more: the last page's ids are listed, and nothing past the
+    table is read.  Keys of all but a few tokens score 2^-184 of those; the few lie in the last page, some of them
+    closer to the end than a page list is long."""
+    say(f"clamp T{T} P{P}")
+    D, capacity = 8, 2 ** 31 - 256
+    gen = torch.Generator().manual_seed(3)
+    few = [capacity - T - x for x in (1, 2, 17, 64, 300, 1030, 16000, 17000, 100000)]
+    assert min(few) >= (width - 1) * P or P % 16
+    table = torch.zeros(1, width, dtype=torch.int32)
+    last = (capacity - 1) // P
+    table[0, last] = 1
+    few = [tok for tok in few if tok // P == last]
+    assert len(few) > 5
+    k = torch.full((2, P, 1, D), -16.0, dtype=BF)
+    v = torch.full((2, P, 1, D), 9.0, dtype=BF)
+    for tok in few:
+        k[1, tok % P] = torch.rand(1, D, generator=gen).to(BF) / 4
+        v[1, tok % P] = torch.randn(1, D, generator=gen).to(BF)
+    q = torch.ones(*((1, T) if T else (1,)), 1, D, dtype=BF)
+    masks = [[(2 << t) - 1 for t in range(T)]] if T else None
+    lens = torch.tensor([capacity - T if T else 2 ** 31 - 1], dtype=torch.int32)
+    window = 0 if T else 2 ** 31 - 1
+    assert cabi.gqa_decode_tree_info(1, max(T, 1), 1, 1, D, P, width, int(T > 0), window, 0,
+                                     cabi.DTYPE[BF])[0] == cabi.QD_TREE_MFMA_SPLIT
+    got = f64(attend(gpu, (q, k, v, table, lens, masks), window, scale=1.0)).reshape(-1, D)
+    at = [tok % P for tok in few]
+    w = np.exp(f64(k)[1, at, 0].sum(1))
+    w /= w.sum()
+    want, spread = w @ f64(v)[1, at, 0], w @ np.abs(f64(v)[1, at, 0])
+    # Scores up to 2; about 2^31 weights whose parts are at least 2^-133 add less than 2^-90.
+    rel = 2 * (D + 4) * U * 2 + 8 * U + 2 * 64 * U + WEIGHT[BF]
+    assert (np.abs(got - want) <= HALF[BF] * np.abs(want) + rel * spread + 2.0 ** -90).all()
