@@ -167,7 +167,8 @@ bool tree_shape_ok(int batch, int q_len, int q_heads, int kv_heads, int head_dim
 
 // The most tokens that a query of the batch can see.
 int64_t visible_capacity(int q_len, int block_size, int max_pages, int has_mask, int window, int sinks) {
-  const int64_t cap = static_cast<int64_t>(block_size) * max_pages;
+  // As the kernels clamp it: products with the items of a batch fit 64 bits.
+  const int64_t cap = std::min<int64_t>(static_cast<int64_t>(block_size) * max_pages, kTreeCapacity);
   if (window <= 0) return cap;
   // Widened to whole groups of 16 tokens at three ends (item_span).
   return std::min(cap, static_cast<int64_t>(window) + sinks + (has_mask ? q_len : 0) + 48);
@@ -435,7 +436,7 @@ int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, 
   p.chunks = pl.chunks;
   p.chunk_rows = pl.chunk_rows;
   p.W = pl.W;
-  p.capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(block_size) * max_pages, INT32_MAX - 255));
+  p.capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(block_size) * max_pages, kTreeCapacity));
   p.last_block = static_cast<int32_t>(std::min<int64_t>(num_blocks - 1, INT32_MAX));
   p.pshift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);

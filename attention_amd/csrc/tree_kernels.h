@@ -14,6 +14,11 @@
 #include "qd_attention.h"
 #include "qd_device.h"
 
+// Most tokens of a table row; the last 256 below 2^31 are left out, so that
+// token numbers, the ends of their tiles and sums with 64 drafts fit 32 bits.
+// Whatever reaches further ahead is compared as a distance.
+constexpr int32_t kTreeCapacity = INT32_MAX - 255;
+
 // Arguments of the matrix-core kernels, passed between translation units.
 struct TreeParams {
   const void* q;
@@ -36,10 +41,7 @@ struct TreeParams {
   int W;         // workgroups of a balanced launch; 0: one per item
   int pshift;    // log2(P), or -1
   int32_t last_block;  // largest page id that a table entry can hold
-  // Tokens of a table row; the last 256 below 2^31 are left out, so that token
-  // numbers, the ends of their tiles and sums with 64 drafts fit 32 bits.
-  // Whatever reaches further ahead is compared as a distance.
-  int32_t capacity;
+  int32_t capacity;    // tokens of a table row, at most kTreeCapacity
 };
 
 // Runs the matrix-core kernel for padded head_dim dp (tree_mfma_*.hip); grid

@@ -226,6 +226,21 @@ def test_which_contexts_are_split():
     assert kind(1025, 512) == cabi.QD_TREE_MFMA
 
 
+@pytest.mark.parametrize("P", [1 << 20, 1 << 24, 1 << 25, (1 << 25) + 5, (1 << 26) - 1])
+@pytest.mark.parametrize("Hq", [1, 16, 1 << 10, 1 << 17, (1 << 18) - 1])
+def test_plans_of_tables_past_the_clamp(P, Hq):
+    """Lengths are clamped below 2^31 tokens, so wider tables change no plan (their items times tiles pass 2^63)."""
+    tight = -(-(1 << 31) // P)
+    for T, has_mask, window in ((64, 1, 0), (1, 0, 2147483647)):
+        want = cabi.gqa_decode_tree_info(1, T, Hq, 1, 8, P, tight, has_mask, window, 0, BF16)
+        assert want[0] != cabi.QD_TREE_VALU
+        for maxP in (tight + 1, 1 << 20, 2147483647):
+            args = (1, T, Hq, 1, 8, P, maxP, has_mask, window, 0, BF16)
+            assert cabi.gqa_decode_tree_info(*args) == want
+            assert cabi.lib().qd_gqa_decode_tree_workspace_bytes(*args, 0) == \
+                cabi.lib().qd_gqa_decode_tree_workspace_bytes(1, T, Hq, 1, 8, P, tight, has_mask, window, 0, BF16, 0)
+
+
 # ---- Norm, rotation and write ------------------------------------------------
 
 
