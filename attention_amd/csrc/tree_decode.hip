@@ -162,6 +162,7 @@ bool tree_shape_ok(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   return batch >= 0 && q_len >= 1 && q_len <= QD_TREE_MAX_DRAFTS && (has_mask || q_len == 1) && q_heads > 0 &&
          kv_heads > 0 && q_heads % kv_heads == 0 && head_dim >= 1 && head_dim <= 256 && block_size > 0 &&
          max_pages > 0 && window >= 0 && sinks >= 0 && (window > 0 || sinks == 0) && float_dtype(dtype) &&
+         batch < (1 << 24) && q_heads < (1 << 24) &&  // each, so that the product fits 64 bits
          static_cast<int64_t>(batch) * q_len * q_heads < (1 << 24);
 }
 

@@ -241,6 +241,20 @@ def test_plans_of_tables_past_the_clamp(P, Hq):
                 cabi.lib().qd_gqa_decode_tree_workspace_bytes(1, T, Hq, 1, 8, P, tight, has_mask, window, 0, BF16, 0)
 
 
+@pytest.mark.parametrize("over", [dict(B=1 << 30, T=64, Hq=1 << 30), dict(B=1 << 28, T=64, Hq=1 << 30),
+                                  dict(B=1 << 24, T=1, Hq=2), dict(B=2, T=1, Hq=1 << 24),
+                                  dict(B=0, T=64, Hq=1 << 30), dict(B=2147483647, T=64, Hq=2147483647)])
+def test_tree_rows_are_counted_without_overflow(over):
+    """Factors whose product wraps to a small number in 64 bits are refused everywhere."""
+    a = tree_args()
+    a.update(over, Hkv=1)
+    assert cabi.lib().qd_gqa_decode_tree(*a.values()) == 1
+    assert cabi.error_string(1) == "invalid dimensions"
+    shape = (a["B"], a["T"], a["Hq"], 1, 64, 16, 32, 1, 0, 0, BF16)
+    assert cabi.gqa_decode_tree_info(*shape)[0] == -1
+    assert cabi.lib().qd_gqa_decode_tree_workspace_bytes(*shape, 0) == 0
+
+
 # ---- Norm, rotation and write ------------------------------------------------
 
 
