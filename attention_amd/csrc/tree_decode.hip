@@ -243,7 +243,7 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   const int64_t cap = visible_capacity(q_len, block_size, max_pages, has_mask, window, sinks);
   // The matrix-core kernel's page and row offsets are 32 bits wide.
   pl.mfma = head_dim % 8 == 0 && !(flags & QD_FLAG_FORCE_GENERIC) &&
-            static_cast<int64_t>(kv_heads) * head_dim * 4 * std::max(block_size, 16) < (int64_t{1} << 31);
+            static_cast<int64_t>(kv_heads) * head_dim * 4 <= INT32_MAX / std::max(block_size, 16);
   if (!pl.mfma) {
     pl.splits = generic_splits(batch, q_len, q_heads, cap);
     if (pl.splits > 1)

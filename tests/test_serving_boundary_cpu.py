@@ -255,6 +255,16 @@ def test_tree_rows_are_counted_without_overflow(over):
     assert cabi.lib().qd_gqa_decode_tree_workspace_bytes(*shape, 0) == 0
 
 
+@pytest.mark.parametrize("Hkv,D,P,valu", [
+    (1 << 23, 256, 2147483647, True),        # 2^64 - 2^33 bytes, counted at 4 per element
+    (1 << 23, 256, 1 << 30, True), (1 << 14, 256, 128, True),
+    ((1 << 14) - 1, 256, 128, False), (1, 8, (1 << 26) - 1, False),
+    (1, 8, 1 << 26, True), (1 << 17, 256, 1, True)])
+def test_pages_past_32_bits_take_the_valu_kernel(Hkv, D, P, valu):
+    """The matrix-core kernel's offsets within a page (of 16 tokens at least) are 32 bits wide."""
+    assert (cabi.gqa_decode_tree_info(1, 1, Hkv, Hkv, D, P, 1, 1, 0, 0, BF16)[0] == cabi.QD_TREE_VALU) == valu
+
+
 # ---- Norm, rotation and write ------------------------------------------------
 
 
