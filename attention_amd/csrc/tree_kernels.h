@@ -120,7 +120,8 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 //   scores   S^T = K Q^T, 16x16 blocks (A = K rows from LDS, B = Q from
 //            registers): a lane holds one row and 4 tokens per block
 //   softmax  per lane; the reference maximum of a row moves only when a score
-//            exceeds it by 2^8, so most tiles exchange nothing between lanes
+//            exceeds it by 2^8 (fp16: by 2), so most tiles exchange nothing
+//            between lanes
 //   output   O^T += V^T P^T: the score layout is already the B operand, V^T
 //            comes from transposing LDS reads.  16-bit weights go in as two
 //            parts (split2): one rounding would add an error as large as the
@@ -425,10 +426,16 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
   using S = typename E::S;
   constexpr bool k16 = DT != QD_DTYPE_F32;
   constexpr int WT = Sh::kWT, TB = Sh::kTB, ES = Sh::kES;
-  // fp16 weights up to 2^8 above the reference maximum's stay below 2^15, and
-  // their low parts above the smallest subnormal.
-  constexpr float kShift = DT == QD_DTYPE_F16 ? 7.f : 0.f;
-  constexpr float kLazy = 8.f;
+  // A row's reference maximum moves when a score exceeds it by 2^kLazy; weights
+  // are relative to it, times 2^kShift.  fp16 parts of a weight are multiples of
+  // 2^-24, the low one at least that (split2), so what they add to a weight too
+  // small for them is at most 2^-(24 + kShift) of the largest one; kShift + kLazy
+  // = 15 keeps the largest inside fp16.  7 and 8 instead left 2^-31, 3e-5 of the
+  // values of 65536 tokens without a weight (8 sequences, trees of 64, 64 heads
+  // of 128, whose scores spread widely: 290 us, 299 us with 14 and 1; windows and
+  // trees of 16 within 1%).
+  constexpr float kShift = DT == QD_DTYPE_F16 ? 14.f : 0.f;
+  constexpr float kLazy = DT == QD_DTYPE_F16 ? 1.f : 8.f;
   extern __shared__ __align__(16) char smem[];
   // Tokens with non-finite values that not all rows see: drafted ones, and
   // those at the window's edge (bit i: token seen_lo + i).

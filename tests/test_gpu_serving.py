@@ -1023,3 +1023,28 @@ def test_contexts_up_to_the_clamp(gpu, T, P, width):
     # Scores up to 2; about 2^31 weights whose parts are at least 2^-133 add less than 2^-90.
     rel = 2 * (D + 4) * U * 2 + 8 * U + 2 * 64 * U + WEIGHT[BF]
     assert (np.abs(got - want) <= HALF[BF] * np.abs(want) + rel * spread + 2.0 ** -90).all()
+
+
+@pytest.mark.parametrize("T,Hq", [(0, 2), (8, 8), (32, 8)], ids=lambda x: str(x))
+def test_tokens_of_no_weight_do_not_add_up(gpu, T, Hq):
+    """fp16: a first token of value 0 takes all of the weight, 2^58 times that of any of 65536 others, whose values
+    are 1.  Their parts of a weight are at least 2^-24 (a part is never 0 where the weight is not), scaled by 2^14
+    below a reference that the row's largest score exceeds by a factor of 2 at most: each adds up to 2^-38 to the
+    output, and the rounding of a subnormal half a step."""
+    say(f"no weight T{T} Hq{Hq}")
+    B, n, D, P = 1030, 65536, 64, 16                     # more sequences than are split: one workgroup takes all
+    gen = torch.Generator().manual_seed(T)
+    table = torch.randint(1, 30, (B, n // P + 4), generator=gen, dtype=torch.int32)
+    table[0, 0] = 0
+    lens = torch.tensor([n] + [i % 20 for i in range(B - 1)], dtype=torch.int32)
+    q = torch.ones(*((B, T) if T else (B,)), Hq, D, dtype=HF)
+    k = torch.zeros(30, P, 1, D, dtype=HF)
+    v = torch.ones(30, P, 1, D, dtype=HF)
+    k[0, 0], v[0, 0] = 5.0, 0.0                          # a score of 64 x 5 / 8 = 40, 57.7 bits
+    masks = [[(2 << t) - 1 for t in range(T)] for _ in range(B)] if T else None
+    assert cabi.gqa_decode_tree_info(B, max(T, 1), Hq, 1, D, P, table.shape[1], int(T > 0), 0 if T else 1 << 20, 0,
+                                     cabi.DTYPE[HF])[0] == cabi.QD_TREE_MFMA
+    got = f64(attend(gpu, (q, k, v, table, lens, masks), 0 if T else 1 << 20))[0]
+    want = (n + T) * math.exp(-40)
+    print(f"[case] {got.max():.3g}", flush=True)
+    assert (got >= 0).all() and got.max() <= want + (n + T) * 2.0 ** -38 + TINY[HF]
