@@ -406,6 +406,11 @@ int qd_qk_norm_rope_write(const void* q, const void* key, const void* value, con
   if (!q || !key || !value || !positions || !k_cache || !v_cache || !slots || !q_out ||
       (!cos_sin && rotary_dim > 0 && max_positions > 0))
     return rope_fail(nullptr, 0, "null tensor pointer");
+  // A token's key and value would be written to one place by different lanes.
+  const uintptr_t kc = reinterpret_cast<uintptr_t>(k_cache), vc = reinterpret_cast<uintptr_t>(v_cache);
+  const uint64_t row_bytes = static_cast<uint64_t>(kv_heads) * head_dim * (dtype == QD_DTYPE_F32 ? 4 : 2);
+  if ((std::max(kc, vc) - std::min(kc, vc)) / row_bytes < static_cast<uint64_t>(cache_rows))
+    return rope_fail(nullptr, 0, "k_cache and v_cache must not overlap");
   RopeParams p;
   p.q = q;
   p.key = key;

@@ -70,8 +70,9 @@ def qk_norm_rope_write(q, key, value, cos_sin, positions, k_cache, v_cache, slot
     ``positions`` int32 ``[N]``.  ``slot_mapping`` int64 ``[N]`` are flat cache
     rows, as in :func:`latent_kv_write`: distinct, and one outside the cache
     (such as -1 for padding) is skipped.  A position outside the table gives a
-    zero query and writes nothing.  ``q_weight`` and ``k_weight`` ``[D]`` (q's
-    dtype or float32) turn the norms on.  fp32 arithmetic, rounded once.
+    zero query and writes nothing.  The caches must not overlap each other (an
+    error) or the inputs.  ``q_weight`` and ``k_weight`` ``[D]`` (q's dtype or
+    float32) turn the norms on.  fp32 arithmetic, rounded once.
     """
     _require_extension()
     return torch.ops.qd_serving.qk_norm_rope_write(q, key, value, cos_sin, positions, k_cache, v_cache, slot_mapping,

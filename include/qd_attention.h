@@ -515,9 +515,10 @@ int qd_qk_norm_rope_write_validate(const qd_tensor_desc* q, const qd_tensor_desc
  * fp32 arithmetic, one rounding.  q goes to q_out [tokens, q_heads, head_dim]
  * (contiguous), key and value to flat row slots[n] of the caches [cache_rows,
  * kv_heads, head_dim].  q_stride, k_stride and v_stride are the elements from
- * one token to the next.  Outputs and inputs do not overlap.  Slots must be
- * distinct; one outside [0, cache_rows) is skipped.  A position outside the
- * table gives a zero q row and writes nothing to the caches. */
+ * one token to the next.  Outputs and inputs do not overlap, nor the caches
+ * each other (checked).  Slots must be distinct; one outside [0, cache_rows)
+ * is skipped.  A position outside the table gives a zero q row and writes
+ * nothing to the caches. */
 int qd_qk_norm_rope_write(const void* q, const void* key, const void* value, const float* cos_sin,
                           const int32_t* positions, void* k_cache, void* v_cache, const int64_t* slots,
                           const void* q_weight, const void* k_weight, void* q_out, int64_t tokens, int q_heads,

@@ -753,6 +753,24 @@ def test_write_strided_contiguous_and_unaligned_agree(gpu):
     assert torch.equal(same, full) and torch.equal(k2, k3) and torch.equal(v2, v3)
 
 
+def test_write_caches_of_one_allocation(gpu):
+    """Caches side by side in one tensor are written; one tensor for both is refused, before anything is written."""
+    say("write caches")
+    qkv, cs, positions, kc, vc, slots, qw, kw = write_case(BF, BF, 6, 8, 2, 128, 128)
+    want, wk, wv = run_write(gpu, (qkv, cs, positions, kc, vc, slots, qw, kw), 8, 2, 1e-6, False)
+    q, key, value = qkv.to(gpu).split([8, 2, 2], dim=1)
+    rest = [x.to(gpu) for x in (cs, positions)]
+    pool = torch.stack([vc, kc]).to(gpu)
+    out = attention_amd.qk_norm_rope_write(q, key, value, *rest, pool[1], pool[0], slots.to(gpu), q_weight=qw.to(gpu),
+                                           k_weight=kw.to(gpu), eps=1e-6)
+    assert torch.equal(out, want) and torch.equal(pool[1], wk) and torch.equal(pool[0], wv)
+    before = pool.clone()
+    with pytest.raises(RuntimeError, match="k_cache and v_cache must not overlap"):
+        attention_amd.qk_norm_rope_write(q, key, value, *rest, pool[0], pool[0], slots.to(gpu))
+    torch.cuda.synchronize()
+    assert torch.equal(pool, before)
+
+
 # ---- Compaction ------------------------------------------------------------------
 
 

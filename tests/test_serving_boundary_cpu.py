@@ -350,6 +350,16 @@ def test_write_launch_without_tokens_is_a_no_op():
     assert cabi.lib().qd_qk_norm_rope_write(*a.values()) == 0
 
 
+@pytest.mark.parametrize("dtype, kc, vc, rows", [
+    (BF16, 4096, 4096, 144), (BF16, 4096, 4096 + 144 * 256 - 16, 144), (F32, 4096 + 144 * 512 - 16, 4096, 144),
+    (F16, 4096, 1 << 47, 1 << 62)])
+def test_write_refuses_overlapping_caches(dtype, kc, vc, rows):
+    a = write_args()
+    a.update(dtype=dtype, wdtype=dtype, kc=kc, vc=vc, rows=rows)
+    assert cabi.lib().qd_qk_norm_rope_write(*a.values()) == 1
+    assert cabi.error_string(1) == "k_cache and v_cache must not overlap"
+
+
 # ---- Compaction --------------------------------------------------------------
 
 
