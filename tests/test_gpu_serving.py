@@ -268,6 +268,47 @@ def test_many_sequences_match_oracle(gpu, shape):
     check_case(gpu, case, window, sinks, what="default")
 
 
+REFILL_SHAPES = [
+    # dtype, B, T, Hq, Hkv, D, P, longest, window, sinks: ranges of more tokens than a page list holds (1024 ids,
+    # of one token or of 16)
+    (BF, 200, 1, 2, 1, 64, 12, 5200, 0, 0),
+    (FP, 100, 3, 2, 1, 64, 1, 12000, 0, 0),
+    (BF, 60, 2, 24, 2, 72, 12, 9000, 0, 0),
+    (BF, 200, 0, 2, 1, 64, 12, 9000, 5200, 70),
+    (BF, 64, 1, 1, 1, 8, 16, 190000, 0, 0),
+    (FP, 40, 2, 2, 1, 8, 64, 300000, 0, 0),
+    (BF, 64, 0, 1, 1, 8, 32, 220000, 190000, 33),
+]
+
+
+@pytest.mark.parametrize("shape", REFILL_SHAPES, ids=lambda s: f"{str(s[0])[6:]}-B{s[1]}-T{s[2]}-{s[3]}x{s[4]}x{s[5]}-P{s[6]}-w{s[8]}")
+def test_ranges_that_refill_their_page_list(gpu, shape):
+    """Split contexts whose ranges begin inside an item and pass the end of a page list.  About every 50th page
+    holds keys that count, one of 30 such pages; the keys of all others score e^-100 of them, so that each page
+    listed wrongly shows.  Sums round only where something is added: the tokens that count."""
+    dtype, B, T, Hq, Hkv, D, P, longest, window, sinks = shape
+    say(f"refill {shape}")
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(longest * 4 // 5, longest + 1, (B,), generator=gen, dtype=torch.int32)
+    width = -(-(longest + T) // P) + 1
+    kind, groups, _ = cabi.gqa_decode_tree_info(B, max(T, 1), Hq, Hkv, D, P, width, int(T > 0), window, sinks,
+                                                cabi.DTYPE[dtype])
+    assert kind == cabi.QD_TREE_MFMA_SPLIT
+    seen = sum(min(n, window + sinks) if window else n for n in lens.tolist())
+    assert Hkv * seen / groups > 1.1 * 1024 * (16 if P % 16 == 0 else 1)
+    counts = torch.rand(B, width, generator=gen) < 0.02
+    table = torch.where(counts, torch.randint(1, 31, (B, width), generator=gen), 0).int().contiguous()
+    q = (0.5 + torch.rand(*((B, T) if T else (B,)), Hq, D, generator=gen)).to(dtype)
+    k = torch.randn(31, P, Hkv, D, generator=gen).to(dtype)
+    v = torch.randn(31, P, Hkv, D, generator=gen).to(dtype)
+    k[0], v[0] = -105 / math.sqrt(D), 5.0               # a score of -105 times q's mean, about 1
+    masks = [[(2 << t) - 1 for t in range(T)] for _ in range(B)] if T else None
+    want, spread, size = attention_want(q, k, v, table, lens, masks, window, sinks, 1 / math.sqrt(D))
+    out = attend(gpu, (q, k, v, table, lens, masks), window, sinks)
+    most = int(counts.sum(1).max()) * P
+    attention_check(out, want, spread, size, dtype, D, most, f"{groups} ranges, {most} tokens that count")
+
+
 def test_launch_limit_of_sequences(gpu):
     """Almost 2^24 rows in one call, a workgroup for each: parts of the batch by themselves are bitwise the same."""
     say("2^24 rows")
