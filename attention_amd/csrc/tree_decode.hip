@@ -166,7 +166,8 @@ bool tree_shape_ok(int batch, int q_len, int q_heads, int kv_heads, int head_dim
          static_cast<int64_t>(batch) * q_len * q_heads < (1 << 24);
 }
 
-// The most tokens that a query of the batch can see.
+// The most tokens that a query of the batch can see by the width of the table
+// and the window: lengths are not known on the host.
 int64_t visible_capacity(int q_len, int block_size, int max_pages, int has_mask, int window, int sinks) {
   // As the kernels clamp it: products with the items of a batch fit 64 bits.
   const int64_t cap = std::min<int64_t>(static_cast<int64_t>(block_size) * max_pages, kTreeCapacity);
@@ -200,7 +201,14 @@ int tree_cu_count() {
   return n;
 }
 
-// How a call runs.  All from static shapes and the device.
+// How a call runs.  All from static shapes and the device: without a window, the
+// table's width stands for the longest context.  Short contexts in a wide table
+// therefore run as long ones would, us with a table of the longest context's
+// pages / of 2048 pages of 16: 8 sequences of 489 tokens, 64 drafts x 8 heads of
+// 128, 23.7 / 47.5 (rows in chunks of 64 / 256); 122 of up to 115, 20 x 4 heads,
+// 14.5 / 24.3; 64 of 100 to 500, 16 x 8 heads, 24.1 / 31.1; one of 300, 24 x 4
+// heads of 96, 16.7 / 21.0; 32 of 512 to 4096, 16 x 4 heads on 8 kv-heads, 73.2 /
+// 72.5.
 struct TreePlan {
   bool mfma;
   int splits;                                  // VALU kernel
@@ -224,7 +232,7 @@ constexpr int kTreeIdleUnits = 5;
 constexpr int kTreeUnevenUnits = 20;
 
 // Up to 128 rows run as two chunks on four waves each, rather than as one on
-// eight, while contexts hold at most this many tokens.  Two chunks / one, us: 80
+// eight, while the table (or the window) holds at most this many tokens.  Two chunks / one, us: 80
 // rows, 122 sequences of up to 115 tokens 64.1 / 84.9; 128 rows, 64 sequences of
 // 100 to 500 tokens 53.5 / 60.7; 80 rows, 32 sequences of 1000 to 3000 98.9 /
 // 96.2; 128 rows, 8 sequences of 2000 to 8000 76.5 / 72.1; heads of 64, 96 rows,
@@ -256,9 +264,9 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   const int R = q_len * (q_heads / kv_heads);
   TreeWaves wv{};
   int64_t items = 0, tiles = 0, units = 0, resident = 0;
-  // The largest chunks that still give every resident workgroup a tile: K and V
-  // are read once per chunk, but a tile of 256 rows takes 8 times as long as one
-  // of 16 (one sequence of 8000 to 16000 tokens, 24 drafts x 4 heads of 96:
+  // The largest chunks that still give every resident workgroup a tile if the
+  // contexts fill the table or the window: K and V are read once per chunk, but a
+  // tile of 256 rows takes 8 times as long as one of 16 (one sequence of 8000 to 16000 tokens, 24 drafts x 4 heads of 96:
   // chunks of 16 rows 20.6 us, one chunk 30.5 us; 8 sequences of 489 tokens, 64
   // drafts x 8 heads of 128: 23.6 us, chunks of 256 rows 41.3 us).
   int most = tree_most_rows(slots);

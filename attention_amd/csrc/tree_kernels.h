@@ -304,7 +304,9 @@ __device__ __forceinline__ void tree_barrier() { tree_barrier_loads<63>(); }
 // 16 bytes per lane from `src` to LDS bytes lds + 16 lane.  Written in assembly
 // so that the compiler does not wait for it before LDS reads of other buffers:
 // tree_barrier_loads does.  M0 (the LDS side) is written and used within one
-// statement.  At least one lane is active (the loads of a tile are counted).
+// statement; the compiler keeps nothing in it from one statement to another (a
+// reserved register, which a clobber list may not name), and nothing else in
+// these kernels uses it.  At least one lane is active (the loads of a tile are counted).
 // STREAM: not kept in the caches.
 template <bool STREAM>
 __device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
@@ -562,6 +564,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         off += static_cast<uint64_t>(static_cast<uint32_t>(pages[x.at + v - x.v0])) * page_bytes +
                static_cast<uint32_t>(tok - page_of(tok) * p.P) * tok_bytes - r * tok_bytes;
       }
+      // Padded heads and pages of no whole groups: never kept, also where other
+      // chunks read the same rows (not measured against keeping them).
       if (inside(i)) {
         tree_load_lds<true>(x.k + off, to);
         tree_load_lds<true>(x.v + off, to + Sh::kTile);
@@ -669,7 +673,9 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         // Values of tokens that no row sees are cleared.  Where only some rows
         // see a token, a weight of 0 would not hide Inf and NaN from the
         // others: they are left out here and join the rows that do at the
-        // item's end.
+        // item's end.  Slots past a padded head are looked at too: what LDS held
+        // there may list a token in bad_words for nothing, which costs time at
+        // the item's end (only values that are not finite are added).
         for (int i = tid; i < Sh::TT * Sh::kSlots; i += 64 * NW) {
           const int v = first + i / Sh::kSlots, tok = token(v);
           u32x4* at = reinterpret_cast<u32x4*>(buf + Sh::kTile) + i;

@@ -47,6 +47,12 @@ def gqa_decode_tree(q, k_cache, v_cache, block_table, context_lens, tree_mask, *
     all of its context, or with ``window`` what is less than ``window``
     positions before its own, ``context_lens[b] + popcount(mask) - 1``, and the
     first ``sinks`` tokens.  Returns ``[B, T, Hq, D]``.
+
+    Without a window, how the work is cut follows from the width of
+    ``block_table``, since lengths are not read on the host: short contexts are
+    up to twice as fast with a table of the batch's longest context
+    (``block_table[:, :pages].contiguous()``) as with one of the longest that a
+    model allows.
     """
     _require_extension()
     if scale is None:

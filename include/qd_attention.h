@@ -490,6 +490,9 @@ int qd_gqa_decode_tree_info(int batch, int q_len, int q_heads, int kv_heads, int
  * window and sinks are never read.  A query that sees nothing gets a zero
  * row.  Whatever a token holds that a query does not see (NaN included)
  * does not reach that query's row.
+ * Without a window, max_pages * block_size stands for the longest context when
+ * the work is cut: short contexts are up to twice as slow in a table much wider
+ * than they need.
  * flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
 int qd_gqa_decode_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                        const int32_t* context_lens, const int64_t* tree_mask, void* out, void* workspace,
