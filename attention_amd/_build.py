@@ -60,8 +60,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 
 HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla", "tree_decode", "tree_mfma_bf16", "tree_mfma_f16",
-               "tree_mfma_f32", "qk_norm_rope", "kv_compact"]
-TORCH_SOURCES = ["torch_ops", "serving_ops"]
+               "tree_mfma_f32", "qk_norm_rope", "kv_compact", "prefill", "cache_q8", "decode_q8"]
+TORCH_SOURCES = ["torch_ops", "serving_ops", "prompt_ops"]
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 
 # Per-source flags.  mla: MFMA accumulators in VGPRs where the register
@@ -91,6 +91,8 @@ def _stale(name: str) -> bool:
             os.path.join(INCLUDE, "qd_attention.h")]
     if name.startswith("tree_"):
         deps.append(os.path.join(CSRC, "tree_kernels.h"))
+    if name.startswith(("prefill", "cache_q8")):
+        deps += [os.path.join(CSRC, "packed.h"), os.path.join(CSRC, "prefill_kernels.h")]
     return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 
 

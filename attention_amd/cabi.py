@@ -18,6 +18,7 @@ HEADER = os.path.join(os.path.dirname(PKG), "include", "qd_attention.h")
 LIB_PATH = os.path.join(PKG, "lib", "libqd_attention.so")
 
 DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: 3, torch.int64: 4}
+CACHE_DTYPE = {torch.float8_e4m3fn: 5, torch.int8: 6}
 QD_FLAG_FORCE_GENERIC = 1
 QD_FLAG_MLA_STAGED = 2
 QD_FLAG_MLA_WAVE = 4
@@ -132,6 +133,30 @@ def lib():
         L.qd_mla_decode.restype = I
         L.qd_mla_decode.argtypes = ([V] * 11 + [ctypes.c_size_t] + [I] * 9 + [I64] + [I] * 3 + [F]
                                     + [I, I, V])
+        L.qd_gqa_prefill_validate.restype = I
+        L.qd_gqa_prefill_validate.argtypes = [P] * 5 + [ctypes.c_double, I64, I64] + MSG
+        L.qd_gqa_prefill_info.restype = I
+        L.qd_gqa_prefill_info.argtypes = [I, I64, I64, I, I, I, I, I] + [ctypes.POINTER(I)] * 2
+        L.qd_gqa_prefill_workspace_bytes.restype = ctypes.c_size_t
+        L.qd_gqa_prefill_workspace_bytes.argtypes = [I, I64, I64] + [I] * 6
+        L.qd_gqa_prefill.restype = I
+        L.qd_gqa_prefill.argtypes = ([V] * 7 + [ctypes.c_size_t, I, I64, I64, I, I, I, I64, I64, I64, I, F, I, I, I, V])
+        L.qd_kv_append_q8_validate.restype = I
+        L.qd_kv_append_q8_validate.argtypes = [P] * 9 + MSG
+        L.qd_kv_append_q8.restype = I
+        L.qd_kv_append_q8.argtypes = [V] * 9 + [I, I64, I, I, I, I, I64, I64, I64, I, I, V]
+        L.qd_kv_gather_q8_validate.restype = I
+        L.qd_kv_gather_q8_validate.argtypes = [P] * 9 + MSG
+        L.qd_kv_gather_q8.restype = I
+        L.qd_kv_gather_q8.argtypes = [V] * 9 + [I, I64, I, I, I, I, I64, I64, I64, I, I, V]
+        L.qd_gqa_decode_q8_validate.restype = I
+        L.qd_gqa_decode_q8_validate.argtypes = [P] * 7 + [ctypes.c_double] + MSG
+        L.qd_gqa_decode_q8_workspace_bytes.restype = ctypes.c_size_t
+        L.qd_gqa_decode_q8_workspace_bytes.argtypes = [I] * 8
+        L.qd_gqa_decode_q8_info.restype = I
+        L.qd_gqa_decode_q8_info.argtypes = [I] * 8 + [ctypes.POINTER(I)]
+        L.qd_gqa_decode_q8.restype = I
+        L.qd_gqa_decode_q8.argtypes = [V] * 9 + [ctypes.c_size_t] + [I] * 6 + [I64, I, I, F, I, V]
         L.qd_gqa_decode_tree_validate.restype = I
         L.qd_gqa_decode_tree_validate.argtypes = [P] * 6 + [ctypes.c_double, I64, I64] + MSG
         L.qd_gqa_decode_tree_workspace_bytes.restype = ctypes.c_size_t
@@ -431,3 +456,63 @@ def kv_compact(caches, table, lens, accepted, stream=None):
     return lib().qd_kv_compact(pointers, len(caches), table.data_ptr(), lens.data_ptr(), accepted.data_ptr(),
                                accepted.shape[0], accepted.shape[1], c.shape[1], table.shape[1], c.shape[0],
                                c[0, 0].numel() * c.element_size(), _stream(c, stream))
+
+
+def validate_gqa_prefill(q, key, value, cu, cu_k=None, scale=0.1, window=0, sinks=0):
+    return _msg_call(lib().qd_gqa_prefill_validate, *(ctypes.byref(d) for d in (q, key, value, cu)), _ref(cu_k), scale,
+                     window, sinks)
+
+
+def gqa_prefill_info(B, Tq, Tk, Hq, Hkv, D, dtype=2, flags=0):
+    """(kind, workgroups, rows per workgroup) from qd_gqa_prefill_info."""
+    w, r = ctypes.c_int(), ctypes.c_int()
+    kind = lib().qd_gqa_prefill_info(B, Tq, Tk, Hq, Hkv, D, dtype, flags, ctypes.byref(w), ctypes.byref(r))
+    return kind, w.value, r.value
+
+
+def gqa_prefill(q, key, value, cu, cu_k, out, *, scale, window=0, sinks=0, flags=0, workspace=None, stream=None):
+    """Calls qd_gqa_prefill on torch device tensors (no validation)."""
+    (Tq, Hq, D), (Tk, Hkv, _), B = q.shape, key.shape, cu.numel() - 1
+    n = lib().qd_gqa_prefill_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, DTYPE[q.dtype], window, flags)
+    if workspace is None and n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+    return lib().qd_gqa_prefill(
+        q.data_ptr(), key.data_ptr(), value.data_ptr(), cu.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
+        out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() if workspace is not None else 0, B, Tq, Tk, Hq, Hkv, D, q.stride(0), key.stride(0),
+        value.stride(0), DTYPE[q.dtype], float(scale), window, sinks, flags, _stream(q, stream))
+
+
+def validate_kv_append_q8(key, value, kc, vc, ks, vs, table, positions, cu=None):
+    return _msg_call(lib().qd_kv_append_q8_validate,
+                     *(ctypes.byref(d) for d in (key, value, kc, vc, ks, vs, table, positions)), _ref(cu))
+
+
+def validate_kv_gather_q8(key, value, kc, vc, ks, vs, table, lens, cu=None):
+    return _msg_call(lib().qd_kv_gather_q8_validate,
+                     *(ctypes.byref(d) for d in (key, value, kc, vc, ks, vs, table, lens)), _ref(cu))
+
+
+def validate_gqa_decode_q8(q, kc, vc, ks, vs, table, lens, scale=0.1):
+    return _msg_call(lib().qd_gqa_decode_q8_validate, *(ctypes.byref(d) for d in (q, kc, vc, ks, vs, table, lens)),
+                     scale)
+
+
+def gqa_decode_q8_info(B, Hq, Hkv, D, P, maxP, dtype=2, flags=0):
+    """(kind, workgroups) from qd_gqa_decode_q8_info."""
+    w = ctypes.c_int()
+    kind = lib().qd_gqa_decode_q8_info(B, Hq, Hkv, D, P, maxP, dtype, flags, ctypes.byref(w))
+    return kind, w.value
+
+
+def gqa_decode_q8(q, kc, vc, ks, vs, table, lens, out, *, scale, flags=0, workspace=None, stream=None):
+    """Calls qd_gqa_decode_q8 on torch device tensors (no validation)."""
+    (B, Hq, D), (N, P, Hkv, _), maxP = q.shape, kc.shape, table.shape[1]
+    n = lib().qd_gqa_decode_q8_workspace_bytes(B, Hq, Hkv, D, P, maxP, DTYPE[q.dtype], flags)
+    if workspace is None and n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+    return lib().qd_gqa_decode_q8(
+        q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() if workspace is not None else 0, B, Hq, Hkv, D, P, maxP, N, DTYPE[q.dtype],
+        CACHE_DTYPE[kc.dtype], float(scale), flags, _stream(q, stream))

@@ -51,6 +51,9 @@ enum {
   QD_DTYPE_BF16 = 2,
   QD_DTYPE_I32 = 3,
   QD_DTYPE_I64 = 4,
+  /* Elements of an 8-bit cache (kv_append_q8 and what reads it, only). */
+  QD_DTYPE_E4M3 = 5,
+  QD_DTYPE_I8 = 6,
   QD_DTYPE_OTHER = -1
 };
 
@@ -547,6 +550,128 @@ int qd_kv_compact_validate(const qd_tensor_desc* cache, const qd_tensor_desc* bl
 int qd_kv_compact(void* const* caches, int num_caches, const int32_t* block_table, const int32_t* context_lens,
                   const int32_t* accepted, int batch, int count, int block_size, int max_pages, int64_t num_blocks,
                   int64_t row_bytes, void* stream);
+
+/* ---- Prompts, and a cache held in 8 bits -----------------------------
+ * No counterpart in the reference: attention over whole prompts, and a paged
+ * cache of half the bytes.
+ *   qd_gqa_prefill    packed prompts attend to their keys
+ *   qd_kv_append_q8   writes prompts or single tokens to the 8-bit cache
+ *   qd_gqa_decode_q8  attention of one token per sequence over it
+ *   qd_kv_gather_q8   reads it back as packed rows: keys of a later chunk's
+ *                     qd_gqa_prefill
+ * An 8-bit cache is [num_blocks, block_size, kv_heads, head_dim] of
+ * QD_DTYPE_E4M3 (OCP, finite, largest value 448) or QD_DTYPE_I8, with a
+ * float32 scale per page and head, [num_blocks, kv_heads], for keys and
+ * another for values: an element stands for itself times its scale.
+ * Sequences are packed: cu[0] is 0 (and not read), sequence b has rows
+ * [cu[b], cu[b + 1]) of q, key or value.  Metadata are caller-owned; values
+ * outside their range are clamped, so that no access leaves a tensor.  Nothing
+ * here allocates, synchronizes or reads metadata on the host. */
+
+/* Checks of qd_gqa_prefill in order.  `contiguous` of q, key and value means
+ * that the rows of one token are.  cu_k undefined or NULL: cu. */
+int qd_gqa_prefill_validate(const qd_tensor_desc* q, const qd_tensor_desc* key, const qd_tensor_desc* value,
+                            const qd_tensor_desc* cu, const qd_tensor_desc* cu_k, double scale, int64_t window,
+                            int64_t sinks, char* msg, size_t msg_cap);
+
+/* What qd_gqa_prefill runs for these sizes on aligned tensors: QD_PREFILL_*,
+ * or -1 for invalid sizes, with *workgroups and *rows of one workgroup
+ * (queries x q-heads of a kv-head).  Output pointers may be NULL. */
+enum { QD_PREFILL_VALU = 0, QD_PREFILL_MFMA = 1 };
+int qd_gqa_prefill_info(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads, int head_dim,
+                        int dtype, int flags, int* workgroups, int* rows);
+
+/* Workspace bytes of qd_gqa_prefill (fp32 partials of keys split over
+ * workgroups); 0 when none is needed.  16-byte aligned, no zeroing needed.
+ * Calls that can overlap need different workspaces. */
+size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads,
+                                      int head_dim, int dtype, int window, int flags);
+
+/* out = softmax(q . k * scale) . v over the keys that a query sees.  Query i of
+ * the nq of a sequence with nk keys lies at position p = nk - nq + i and sees
+ * key j iff j <= p and (window == 0 or j > p - window or j < sinks); one that
+ * sees nothing gets a zero row, and so do rows behind the last sequence.
+ * Whatever a key or value holds that a query does not see (NaN included)
+ * does not reach that query's row.  q [q_tokens, q_heads, head_dim], key and
+ * value [k_tokens, kv_heads, head_dim], their tokens q_stride, k_stride and
+ * v_stride elements apart; out is contiguous.
+ * flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
+int qd_gqa_prefill(const void* q, const void* key, const void* value, const int32_t* cu, const int32_t* cu_k,
+                   void* out, void* workspace, size_t workspace_bytes, int batch, int64_t q_tokens, int64_t k_tokens,
+                   int q_heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                   int dtype, float scale, int window, int sinks, int flags, void* stream);
+
+/* Checks of qd_kv_append_q8 in order.  `contiguous` of key and value means
+ * that the rows of one token are.  cu undefined or NULL: one token per
+ * sequence. */
+int qd_kv_append_q8_validate(const qd_tensor_desc* key, const qd_tensor_desc* value, const qd_tensor_desc* k_cache,
+                             const qd_tensor_desc* v_cache, const qd_tensor_desc* k_scales,
+                             const qd_tensor_desc* v_scales, const qd_tensor_desc* block_table,
+                             const qd_tensor_desc* positions, const qd_tensor_desc* cu, char* msg, size_t msg_cap);
+
+/* Writes row cu[b] + i of key and value to token positions[b] + i of sequence
+ * b's cache.  For each page and head that the call writes to, a is the largest
+ * |x| of the new rows and s = 2^e the smallest power of two with a <= s * 448
+ * (e4m3) or a <= s * 127 (int8), at least 2^-100.  If the call begins the page
+ * (its first new row is the page's first), its scale becomes s; else the larger
+ * of s and the old one, and if that is s, the rows before are rounded to it.
+ * Elements are x / scale rounded to nearest, ties to even.  With an Inf or NaN
+ * among the new rows, or if s would pass 2^100, the scale becomes NaN, and the
+ * elements are unspecified.
+ * Other rows keep their elements.  Sequences with a negative position write
+ * nothing, nor do tokens past the table or in pages outside the pool.  Pages
+ * that are written to must be their sequence's own.  Caches, scales and inputs
+ * must not overlap (the caches and the scales are checked). */
+int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_cache, float* k_scales,
+                    float* v_scales, const int32_t* block_table, const int32_t* positions, const int32_t* cu,
+                    int batch, int64_t tokens, int kv_heads, int head_dim, int block_size, int max_pages,
+                    int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype, int cache_dtype, void* stream);
+
+/* Checks of qd_kv_gather_q8 in order, `contiguous` of key and value as above. */
+int qd_kv_gather_q8_validate(const qd_tensor_desc* key, const qd_tensor_desc* value, const qd_tensor_desc* k_cache,
+                             const qd_tensor_desc* v_cache, const qd_tensor_desc* k_scales,
+                             const qd_tensor_desc* v_scales, const qd_tensor_desc* block_table,
+                             const qd_tensor_desc* context_lens, const qd_tensor_desc* cu, char* msg, size_t msg_cap);
+
+/* Row cu[b] + i of key and value becomes token i of sequence b's cache, for
+ * every i < context_lens[b] inside the sequence's rows and its table; other
+ * rows are left as they were.  Page ids are clamped to the pool. */
+int qd_kv_gather_q8(void* key, void* value, const void* k_cache, const void* v_cache, const float* k_scales,
+                    const float* v_scales, const int32_t* block_table, const int32_t* context_lens,
+                    const int32_t* cu, int batch, int64_t tokens, int kv_heads, int head_dim, int block_size,
+                    int max_pages, int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype,
+                    int cache_dtype, void* stream);
+
+/* Checks of qd_gqa_decode_q8 in order. */
+int qd_gqa_decode_q8_validate(const qd_tensor_desc* q, const qd_tensor_desc* k_cache, const qd_tensor_desc* v_cache,
+                              const qd_tensor_desc* k_scales, const qd_tensor_desc* v_scales,
+                              const qd_tensor_desc* block_table, const qd_tensor_desc* context_lens, double scale,
+                              char* msg, size_t msg_cap);
+
+/* Workspace bytes of qd_gqa_decode_q8 (partials of split contexts); 0 when
+ * none is needed.  16-byte aligned, no zeroing needed: every call writes what it
+ * reads.  Calls that can overlap need different workspaces.  Depends on the
+ * current device, like the launch. */
+size_t qd_gqa_decode_q8_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int block_size,
+                                        int max_pages, int dtype, int flags);
+
+/* What qd_gqa_decode_q8 runs for these shapes on aligned tensors: QD_Q8_*, or
+ * -1 for invalid shapes, with *workgroups of the attention kernel. */
+enum { QD_Q8_VALU = 0, QD_Q8_MFMA = 1, QD_Q8_MFMA_SPLIT = 2 };
+int qd_gqa_decode_q8_info(int batch, int q_heads, int kv_heads, int head_dim, int block_size, int max_pages,
+                          int dtype, int flags, int* workgroups);
+
+/* qd_gqa_decode_auto over an 8-bit cache: out [batch, q_heads, head_dim] =
+ * softmax(q . (s_k k) * scale) . (s_v v) over the context_lens[b] tokens of
+ * each sequence; q and out are 16-bit.  Lengths are clamped to [0, max_pages *
+ * block_size] (0: a zero row), page ids to the pool.  Scales may be any float32
+ * of a magnitude in [2^-100, 2^100], or 0; a NaN one (qd_kv_append_q8) makes the
+ * rows that see its page NaN.  flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
+int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scales,
+                     const float* v_scales, const int32_t* block_table, const int32_t* context_lens, void* out,
+                     void* workspace, size_t workspace_bytes, int batch, int q_heads, int kv_heads, int head_dim,
+                     int block_size, int max_pages, int64_t num_blocks, int dtype, int cache_dtype, float scale,
+                     int flags, void* stream);
 
 #ifdef __cplusplus
 }
