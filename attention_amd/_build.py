@@ -60,16 +60,18 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 
 HIP_SOURCES = ["gqa_decode", "kv_append", "validate", "mla", "tree_decode", "tree_mfma_bf16", "tree_mfma_f16",
-               "tree_mfma_f32", "qk_norm_rope", "kv_compact", "prefill", "cache_q8", "decode_q8"]
+               "tree_mfma_f32", "qk_norm_rope", "kv_compact", "prefill", "prefill_mfma_bf16",
+               "prefill_mfma_f16", "prefill_mfma_f32", "cache_q8", "decode_q8"]
 TORCH_SOURCES = ["torch_ops", "serving_ops", "prompt_ops"]
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 
 # Per-source flags.  mla: MFMA accumulators in VGPRs where the register
 # budget allows (one wave per SIMD gives 512); with the default AGPR form the
 # attention kernels moved hundreds of registers between the two files per
-# cache tile.  The matrix-core tree kernels likewise.
+# cache tile.  The matrix-core tree and prompt kernels likewise.
 _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-SOURCE_FLAGS = {n: _VGPR_FORM for n in ("mla", "tree_mfma_bf16", "tree_mfma_f16", "tree_mfma_f32")}
+SOURCE_FLAGS = {n: _VGPR_FORM for n in ("mla", "tree_mfma_bf16", "tree_mfma_f16", "tree_mfma_f32", "prefill_mfma_bf16",
+                                      "prefill_mfma_f16", "prefill_mfma_f32")}
 
 
 def hip_object_cmd(name: str) -> list[str]:
@@ -90,9 +92,11 @@ def _stale(name: str) -> bool:
     deps = [os.path.join(CSRC, f"{name}.hip"), os.path.join(CSRC, "qd_device.h"),
             os.path.join(INCLUDE, "qd_attention.h")]
     if name.startswith("tree_"):
-        deps.append(os.path.join(CSRC, "tree_kernels.h"))
-    if name.startswith(("prefill", "cache_q8")):
-        deps += [os.path.join(CSRC, "packed.h"), os.path.join(CSRC, "prefill_kernels.h")]
+        deps += [os.path.join(CSRC, h) for h in ("tree_kernels.h", "tile_device.h")]
+    if name.startswith("prefill"):
+        deps += [os.path.join(CSRC, h) for h in ("prefill_kernels.h", "packed.h", "tile_device.h")]
+    if name == "cache_q8":
+        deps.append(os.path.join(CSRC, "packed.h"))
     return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 
 

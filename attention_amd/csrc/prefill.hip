@@ -121,16 +121,26 @@ bool prefill_shape_ok(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads
 
 struct PrefillPlan {
   bool mfma;
+  int dp;        // padded head_dim
   int rows;      // rows of a workgroup
   int64_t grid;  // workgroups
 };
 
-PrefillPlan prefill_plan(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads, int head_dim,
-                         int dtype, int flags) {
-  (void)batch, (void)k_tokens, (void)kv_heads, (void)head_dim, (void)dtype, (void)flags;
+PrefillPlan prefill_plan(int batch, int64_t q_tokens, int q_heads, int kv_heads, int head_dim, int dtype, int flags) {
   PrefillPlan pl{};
   pl.rows = 1;
   pl.grid = q_tokens * q_heads;
+  const int group = q_heads / kv_heads;
+  const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
+  if (head_dim * es % 16 != 0 || (flags & QD_FLAG_FORCE_GENERIC)) return pl;
+  const auto grid_of = [&](int rows) { return (q_tokens * group / rows + batch + 1) * kv_heads; };
+  pl.dp = es == 4 ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256)
+                  : (head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 ? 192 : 256);
+  const int rows = es == 2 && pl.dp <= 128 && q_tokens * q_heads >= 256 * 256 ? 256 : 128;
+  if (grid_of(rows) > INT32_MAX) return pl;
+  pl.mfma = true;
+  pl.rows = rows;
+  pl.grid = grid_of(rows);
   return pl;
 }
 
@@ -190,7 +200,7 @@ int qd_gqa_prefill_validate(const qd_tensor_desc* q, const qd_tensor_desc* key, 
 int qd_gqa_prefill_info(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads, int head_dim,
                         int dtype, int flags, int* workgroups, int* rows) {
   if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype)) return -1;
-  const PrefillPlan pl = prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, flags);
+  const PrefillPlan pl = prefill_plan(batch, q_tokens, q_heads, kv_heads, head_dim, dtype, flags);
   if (workgroups) *workgroups = static_cast<int>(pl.grid);
   if (rows) *rows = pl.rows;
   return pl.mfma ? QD_PREFILL_MFMA : QD_PREFILL_VALU;
@@ -207,7 +217,7 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
                    void* out, void* workspace, size_t workspace_bytes, int batch, int64_t q_tokens, int64_t k_tokens,
                    int q_heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                    int dtype, float scale, int window, int sinks, int flags, void* stream) {
-  (void)workspace, (void)workspace_bytes, (void)flags;
+  (void)workspace, (void)workspace_bytes;
   if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype) || q_stride < 0 ||
       k_stride < 0 || v_stride < 0 || (!cu_k && k_tokens != q_tokens))
     return prefill_fail(nullptr, 0, "invalid dimensions");
@@ -216,6 +226,16 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
     return prefill_fail(nullptr, 0, "sinks must not be negative and need a window");
   if (q_tokens == 0) return QD_OK;
   if (!q || !cu || !out || (k_tokens > 0 && (!key || !value))) return prefill_fail(nullptr, 0, "null tensor pointer");
+  const int64_t es = dtype == QD_DTYPE_F32 ? 4 : 2;
+  // The matrix-core kernel loads 16 bytes at a time, at 32-bit offsets within a
+  // tile of at most 64 tokens.
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value) |
+        reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(q_stride * es) |
+        static_cast<uintptr_t>(k_stride * es) | static_cast<uintptr_t>(v_stride * es)) &
+       15u) != 0 ||
+      std::max(k_stride, v_stride) > (int64_t{1} << 24))
+    flags |= QD_FLAG_FORCE_GENERIC;
+  const PrefillPlan pl = prefill_plan(batch, q_tokens, q_heads, kv_heads, head_dim, dtype, flags);
   PrefillParams p;
   p.q = q;
   p.k = key;
@@ -238,12 +258,20 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
   p.sl2 = scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
-  switch (dtype) {
-    case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;
-    case QD_DTYPE_F16: launch_generic<QD_DTYPE_F16>(p, st); break;
-    default: launch_generic<QD_DTYPE_BF16>(p, st); break;
+  hipError_t e = hipSuccess;
+  if (pl.mfma) {
+    const auto run = dtype == QD_DTYPE_F32   ? qd_prefill_mfma_launch_f32
+                     : dtype == QD_DTYPE_F16 ? qd_prefill_mfma_launch_f16
+                                             : qd_prefill_mfma_launch_bf16;
+    e = static_cast<hipError_t>(run(p, pl.dp, pl.rows, static_cast<uint32_t>(pl.grid), stream));
+  } else {
+    switch (dtype) {
+      case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;
+      case QD_DTYPE_F16: launch_generic<QD_DTYPE_F16>(p, st); break;
+      default: launch_generic<QD_DTYPE_BF16>(p, st); break;
+    }
+    e = hipGetLastError();
   }
-  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     qd_set_last_error(static_cast<int>(e), std::string("gqa_prefill kernel launch failed: ") + hipGetErrorString(e));
     return static_cast<int>(e);

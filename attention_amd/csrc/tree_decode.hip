@@ -260,7 +260,7 @@ TreePlan tree_plan(int batch, int q_len, int q_heads, int kv_heads, int head_dim
   }
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   pl.dp = tree_padded(es, head_dim);
-  const int slots = tree_slots(es, pl.dp);
+  const int slots = tile_slots(es, pl.dp);
   const int R = q_len * (q_heads / kv_heads);
   TreeWaves wv{};
   int64_t items = 0, tiles = 0, units = 0, resident = 0;

@@ -13,6 +13,7 @@
 
 #include "qd_attention.h"
 #include "qd_device.h"
+#include "tile_device.h"
 
 // Most tokens of a table row; the last 256 below 2^31 are left out, so that
 // token numbers, the ends of their tiles and sums with 64 drafts fit 32 bits.
@@ -145,10 +146,6 @@ __device__ __forceinline__ int64_t pool_row(const TreeParams& p, int b, int tok)
 // later K operands read under the last products of V (no change), 64-token
 // tiles with eight waves, loads spread over a step.
 //
-// LDS rows are a power of two of 16-byte slots; chunk c of row r lies in slot
-// c ^ tree_swizzle(r), which spreads both the 16 rows of a K operand read and
-// the 32-byte pieces of a transposing V read over the 64 banks.
-
 // Balanced launches: an item costs its tiles and this many more (its queries,
 // first round trips and stores take about as long; 2 instead of 4: trees of 16
 // over 32 sequences 75 -> 81 us).
@@ -166,10 +163,6 @@ constexpr int kTreePages = 1024;
 // Padded head_dim of an instance; es: element size.
 __host__ __device__ constexpr int tree_padded(int es, int d) {
   return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 && es == 2 ? 192 : 256;
-}
-// 16-byte slots of an LDS row.
-__host__ __device__ constexpr int tree_slots(int es, int dp) {
-  return dp * es <= 128 ? 8 : dp * es <= 256 ? 16 : dp * es <= 512 ? 32 : 64;
 }
 // Tokens of a tile: a wave works on 16 to 128 of them, so that what it does
 // once per tile stays small beside its products.
@@ -216,14 +209,10 @@ __host__ __device__ constexpr int tree_occupancy(int slots, int nw) {
   return by_lds < by_regs ? by_lds : by_regs;
 }
 
-__device__ __forceinline__ int tree_swizzle(int slots, int row) {
-  return slots == 8 ? 2 * ((row >> 1) & 3) + ((row >> 3) & 1) : 2 * (row & 7) + ((row >> 3) & 1);
-}
-
 template <int DT, int DP, int NB, int WR, int NW>
 struct TreeShape {
   static constexpr int kES = DT == QD_DTYPE_F32 ? 4 : 2;
-  static constexpr int kSlots = tree_slots(kES, DP);
+  static constexpr int kSlots = tile_slots(kES, DP);
   static constexpr int TT = tree_tile(kSlots, NW);
   static constexpr int kWT = NW / WR;
   static constexpr int kRow = kSlots * 16;                   // bytes of an LDS row
@@ -286,70 +275,6 @@ __device__ __forceinline__ uint32_t tree_wave_reduce(uint32_t x, F&& f) {
   x = f(a[0], a[1]);
   const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   return f(b[0], b[1]);
-}
-
-// Workgroup barrier for LDS traffic: waits for this wave's LDS operations and
-// for all but the last kLeft of its loads into LDS.
-template <int kLeft>
-__device__ __forceinline__ void tree_barrier_loads() {
-  static_assert(kLeft >= 0 && kLeft < 64, "vmcnt is 6 bits");
-  constexpr int imm = (kLeft & 0xF) | ((kLeft >> 4) << 14) | (0x7 << 4) | (0x0 << 8);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(imm);
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void tree_barrier() { tree_barrier_loads<63>(); }
-
-// 16 bytes per lane from `src` to LDS bytes lds + 16 lane.  Written in assembly
-// so that the compiler does not wait for it before LDS reads of other buffers:
-// tree_barrier_loads does.  M0 (the LDS side) is written and used within one
-// statement; the compiler keeps nothing in it from one statement to another (a
-// reserved register, which a clobber list may not name), and nothing else in
-// these kernels uses it.  At least one lane is active (the loads of a tile are counted).
-// STREAM: not kept in the caches.
-template <bool STREAM>
-__device__ __forceinline__ void tree_load_lds(const char* src, uint32_t lds) {
-  if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
-}
-
-// The same from base + off, base wave-uniform.
-template <bool STREAM>
-__device__ __forceinline__ void tree_load_lds(const char* base, uint32_t off, uint32_t lds) {
-  if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory");
-}
-
-__device__ __forceinline__ uint32_t tree_lds_address(const char* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
-}
-
-// A table entry at a wave-uniform place, through the scalar cache: a vector
-// load would complete only after the tiles in flight.
-__device__ __forceinline__ int32_t tree_scalar_load(const int32_t* p) {
-  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
-}
-
-// Reads by LDS byte address: slots of a row are exchanged by an exclusive or of
-// its bits, without a step from address to pointer.
-template <typename X>
-__device__ __forceinline__ X tree_lds_read(uint32_t at) {
-  return *reinterpret_cast<const __attribute__((address_space(3))) X*>(at);
-}
-
-// Four transposed 16-bit elements: lane (g4, r16) of the wave gets column r16
-// of the 4 x 16 block whose row r16 / 4, columns 4 (r16 % 4).. this lane
-// addresses.
-__device__ __forceinline__ u32x2 tree_tr_read(uint32_t at) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at)));
 }
 
 template <int DT>
@@ -477,13 +402,13 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     for (int i = 0; i < Sh::kLoads; ++i) {
       const int r = (64 * i + lane) / Sh::kSlots;
       lane_off[i] = r * tok_bytes + h * row_bytes +
-                    16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r));
+                    16 * ((lane & (Sh::kSlots - 1)) ^ tile_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r));
     }
     auto inside = [&](int i) {
       const int r = (64 * i + lane) / Sh::kSlots;
-      return 16 * ((lane & (Sh::kSlots - 1)) ^ tree_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
+      return 16 * ((lane & (Sh::kSlots - 1)) ^ tile_swizzle(Sh::kSlots, Sh::kLoadRows * wv + r)) < row_bytes;
     };
-    const uint32_t lds_wave = tree_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
+    const uint32_t lds_wave = tile_lds_address(smem) + Sh::kLoadRows * wv * Sh::kRow;
     const bool grouped = p.P % 16 == 0;
     // The page list from a tile on: read, then put into LDS; it covers
     // list_tiles tiles.
@@ -549,11 +474,11 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         // Not kept in the caches where no other chunk reads the rows (316 MB of
         // K and V 75 us, kept 82 us; 2.1 GB 341 / 381 us).
         if (p.chunks == 1) {
-          tree_load_lds<true>(x.k, lane_off[i], to);
-          tree_load_lds<true>(x.v, lane_off[i], to + Sh::kTile);
+          tile_load_lds<true>(x.k, lane_off[i], to);
+          tile_load_lds<true>(x.v, lane_off[i], to + Sh::kTile);
         } else {  // the other chunks read the same rows
-          tree_load_lds<false>(x.k, lane_off[i], to);
-          tree_load_lds<false>(x.v, lane_off[i], to + Sh::kTile);
+          tile_load_lds<false>(x.k, lane_off[i], to);
+          tile_load_lds<false>(x.v, lane_off[i], to + Sh::kTile);
         }
         return;
       }
@@ -567,8 +492,8 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
       // Padded heads and pages of no whole groups: never kept, also where other
       // chunks read the same rows (not measured against keeping them).
       if (inside(i)) {
-        tree_load_lds<true>(x.k + off, to);
-        tree_load_lds<true>(x.v + off, to + Sh::kTile);
+        tile_load_lds<true>(x.k + off, to);
+        tile_load_lds<true>(x.v + off, to + Sh::kTile);
       }
     };
 
@@ -594,7 +519,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     }
     // The first tile.  Its pages come through the scalar cache where one page
     // serves a wave's rows; the list takes a barrier.
-    tree_barrier();  // the previous item's merge and the prefix are done with LDS
+    tile_barrier();  // the previous item's merge and the prefix are done with LDS
     if (tid < 2) bad_words[tid] = 0;
     if (padded) {
       for (int i = tid; i < kTreeBufs * Sh::kTile / 16; i += 64 * NW)
@@ -605,11 +530,11 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     uint64_t my_mask = 0;
     if (p.mask && q0 + lane <= q1) my_mask = draft_bits(p, b, q0 + lane);
     if (!grouped) put_pages(listed);
-    if (padded || !grouped) tree_barrier();
+    if (padded || !grouped) tile_barrier();
     if (t0 < t1) {
       int32_t phys = 0;
       if (grouped)
-        phys = min(max(tree_scalar_load(table + min(page_of(token(Sh::TT * t0 + Sh::kLoadRows * wv)), last_page)), 0),
+        phys = min(max(tile_scalar_load(table + min(page_of(token(Sh::TT * t0 + Sh::kLoadRows * wv)), last_page)), 0),
                    p.last_block);
       const TileLoad x = tile_load(t0, 0, phys, list_at(t0, t0));
 #pragma unroll
@@ -651,13 +576,13 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
     int slot_now = 0;
     for (int tile = t0; tile < t1; ++tile) {
       // The tile has arrived, and every wave is done with the one before it.
-      tree_barrier_loads<0>();
+      tile_barrier_loads<0>();
       const int next = tile + 1;
       if (next < t1) {
         if (next >= list_base + list_tiles) {
           list_base = next;
           put_pages(read_pages(next));
-          tree_barrier();
+          tile_barrier();
         }
         const int at = list_at(next, list_base);
         const TileLoad x = tile_load(next, slot_now ^ 1, grouped ? __builtin_amdgcn_readfirstlane(pages[at]) : 0, at);
@@ -689,14 +614,14 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
             }
           }
         }
-        tree_barrier();
+        tile_barrier();
       }
 
 #pragma unroll 1
       for (int sub = 0; sub < Sh::kSub; ++sub) {
         const int wave_tok = Sh::kTW * wt + 16 * TB * sub;
-        const uint32_t at = tree_lds_address(buf) + wave_tok * Sh::kRow;
-        const uint32_t kb = at + r16 * Sh::kRow + 16 * (g4 ^ tree_swizzle(Sh::kSlots, r16));
+        const uint32_t at = tile_lds_address(buf) + wave_tok * Sh::kRow;
+        const uint32_t kb = at + r16 * Sh::kRow + 16 * (g4 ^ tile_swizzle(Sh::kSlots, r16));
         f32x4 s[TB][NB];
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb)
@@ -712,7 +637,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         auto read_k = [&](int st) {
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb)
-            ka[st % Sh::kQkAhead][tb] = tree_lds_read<u32x4>((kb ^ (64 * st)) + 16 * tb * Sh::kRow);
+            ka[st % Sh::kQkAhead][tb] = tile_lds_read<u32x4>((kb ^ (64 * st)) + 16 * tb * Sh::kRow);
         };
 #pragma unroll
         for (int st = 0; st < Sh::kQkAhead; ++st) read_k(st);
@@ -742,20 +667,20 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         const uint32_t vb = at + Sh::kTile;
         const int vr = 4 * g4 + (k16 ? r16 >> 2 : 0);
         const uint32_t va =
-            k16 ? vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tree_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1) : vb;
+            k16 ? vb + vr * Sh::kRow + 16 * (((r16 >> 1) & 1) ^ tile_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1) : vb;
         u32x2 vf[Sh::kPvAhead][2 * TB];  // fp32: 4 TB values
         auto read_v = [&](int c) {
 #pragma unroll
           for (int tb = 0; tb < TB; ++tb) {
             if constexpr (k16) {
-              vf[c % Sh::kPvAhead][tb] = tree_tr_read((va ^ (32 * c)) + 16 * tb * Sh::kRow);
+              vf[c % Sh::kPvAhead][tb] = tile_tr_read((va ^ (32 * c)) + 16 * tb * Sh::kRow);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int row = 4 * g4 + i;
-                const uint32_t col = vb + row * Sh::kRow + 16 * ((r16 >> 2) ^ tree_swizzle(Sh::kSlots, row)) + 4 * (r16 & 3);
+                const uint32_t col = vb + row * Sh::kRow + 16 * ((r16 >> 2) ^ tile_swizzle(Sh::kSlots, row)) + 4 * (r16 & 3);
                 vf[c % Sh::kPvAhead][2 * tb + i / 2][i % 2] =
-                    tree_lds_read<uint32_t>((col ^ (64 * c)) + 16 * tb * Sh::kRow);
+                    tile_lds_read<uint32_t>((col ^ (64 * c)) + 16 * tb * Sh::kRow);
               }
             }
           }
@@ -887,7 +812,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
 
     // The item's end: its rows' sums, and the output or a partial.
     asm volatile("" : "+s"(dim), "+v"(lane), "+v"(r16), "+v"(g4));
-    tree_barrier();
+    tile_barrier();
     float sum[NB], scale[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) sum[nb] = tree_sum_groups(l[nb]);
@@ -905,7 +830,7 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
           *reinterpret_cast<f32x4*>(smem + ((wv * NB + nb) * Sh::kCols + c) * 1024 + 16 * lane) = acc[c][nb];
         if (g4 == 0) stats[(wv * NB + nb) * 16 + r16] = f32x2{m[nb], sum[nb]};
       }
-      tree_barrier();
+      tile_barrier();
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         f32x2 ml[WT];
@@ -1085,10 +1010,10 @@ __global__ __launch_bounds__(64 * NW, (TreeShape<DT, DP, NB, WR, NW>::kOcc * NW 
         meta[0] = w;
         meta[1] = last - w + 1;
       }
-      sp = span_of(p, in_lanes ? __builtin_amdgcn_readlane(mine_len, b) : clamp_len(p, tree_scalar_load(p.lens + b)));
+      sp = span_of(p, in_lanes ? __builtin_amdgcn_readlane(mine_len, b) : clamp_len(p, tile_scalar_load(p.lens + b)));
     } else {
       hc = static_cast<int>(blockIdx.x) % per_seq;
-      sp = span_of(p, clamp_len(p, tree_scalar_load(p.lens + b)));
+      sp = span_of(p, clamp_len(p, tile_scalar_load(p.lens + b)));
       t1 = tiles = span_tiles<Sh::TT>(sp);
     }
     if (t1 > t0 || p.W == 0) process(b, hc, sp, t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
@@ -1212,7 +1137,7 @@ hipError_t tree_launch(const TreeParams& p, int grid, hipStream_t st) {
 
 template <int DT, int DP, int ROWS>
 hipError_t tree_launch_rows(const TreeParams& p, int grid, hipStream_t st) {
-  constexpr int kSlots = tree_slots(DT == QD_DTYPE_F32 ? 4 : 2, DP);
+  constexpr int kSlots = tile_slots(DT == QD_DTYPE_F32 ? 4 : 2, DP);
   if constexpr (ROWS <= tree_most_rows(kSlots)) {
     if (p.chunk_rows <= ROWS) {
       constexpr TreeWaves w = tree_waves(kSlots, ROWS);
