@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void prefill_generic_kernel(PrefillParams p) {
   const int q0 = packed_start(p.cu, b, p.Tq), q1 = packed_start(p.cu, b + 1, p.Tq);
   const int k0 = packed_start(p.cu_k, b, p.Tk), k1 = packed_start(p.cu_k, b + 1, p.Tk);
   // Keys [0, sinks) and [lo, at] are seen; none by rows outside the sequences.
-  const int at = t < q1 ? max(k1 - k0, 0) - (q1 - q0) + (t - q0) : -1;
+  const int at = t < q1 ? max(max(k1 - k0, 0) - (q1 - q0) + (t - q0), -1) : -1;
   const int lo = p.window > 0 ? max(at - p.window + 1, 0) : 0;
   const int sinks = min(p.sinks, lo);
   const int count = sinks + max(at + 1 - lo, 0);

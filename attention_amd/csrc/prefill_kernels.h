@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "packed.h"
 #include "qd_attention.h"
@@ -57,6 +58,15 @@ struct PrefillShape {
   static constexpr int kLds = 4 * kTile + 16;
   static_assert(kLoadRows * kSlots % 64 == 0 && DP % 32 == 0, "waves do not fit the tile");
 };
+
+// As tile_swizzle, for operands of 32 rows: a transposing V read takes 4 rows of 64
+// neighbouring bytes for each half of the wave, which have to be 4 different 64
+// bytes of the 64 banks (with tile_swizzle they were the same 128: a third of the
+// LDS cycles in conflicts).
+__device__ __forceinline__ int prefill_swizzle(int slots, int row) {
+  return slots == 8 ? 4 * ((row >> 1) & 1) + 2 * ((row >> 2) & 1) + ((row >> 3) & 1)
+                    : 4 * (row & 3) + 2 * ((row >> 2) & 1) + ((row >> 3) & 1);
+}
 
 __device__ __forceinline__ float prefill_max_halves(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -113,323 +123,187 @@ __device__ __forceinline__ bool prefill_finite(u32x4 x) {
 // An item is a (sequence, kv-head, kRows of its rows); a row is a (query, q-head
 // of the kv-head's group), numbered query by query, so that the heads that share
 // K and V share a workgroup's reads of them and the rows of a workgroup span few
-// positions.  The workgroup goes through the tokens that its rows see in tiles of
-// TT: K and V rows come straight into one of two LDS buffers, one tile ahead, and
-// each wave multiplies its 32 NB rows with them:
-//   scores   S^T = K Q^T, 32x32 blocks (A = K rows from LDS, B = Q from
-//            registers): a lane holds one row and 16 of 32 tokens
-//   softmax  per lane; the reference maximum of a row moves only when a score
-//            exceeds it by 2^kLazy, so most tiles exchange nothing between lanes
-//   output   O^T += V^T P^T: the score layout is already the B operand (the
-//            products sum over tokens in the order that the lanes hold them in),
-//            V^T comes from transposing LDS reads.
-// 16-bit weights are rounded to nearest once: half a step of the output's type,
-// which a sum over many values averages out.
-template <int DT, int DP, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 && DT != QD_DTYPE_F32 ? 2 : 1)) void prefill_mfma_kernel(PrefillParams p) {
-  using Sh = PrefillShape<DT, DP, NB, NW>;
-  using E = Elem<DT>;
-  using S = typename E::S;
-  constexpr bool k16 = DT != QD_DTYPE_F32;
-  constexpr int ES = Sh::kES, TT = Sh::TT, TB = Sh::kTB;
-  // fp16 weights are multiples of 2^-24 and the largest of a row is at least
-  // 2^kShift: what that grid adds is at most 2^-32 of it.
-  constexpr float kShift = DT == QD_DTYPE_F16 ? 7.f : 0.f;
-  constexpr float kLazy = 8.f;
-  extern __shared__ __align__(16) char smem[];
-  int* bad_word = reinterpret_cast<int*>(smem + 4 * Sh::kTile);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n32 = lane & 31, half = lane >> 5;
-  const int h = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.Hkv));
+// positions.  Positions below 0 (more queries than keys) see nothing: -1.
+struct PrefillItem {
+  int h, q0, row0, rows;   // rows of the workgroup, of sequence rows from query q0 on
+  int k0, nk, before;      // keys, position of query 0
+  int p_min, p_max;        // positions of the first and the last row
+  int lo_tile, sink_tiles, tiles;  // tiles [0, sink_tiles), then from lo_tile on
+};
+
+template <int ROWS, int TT>
+__device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem& x) {
+  x.h = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.Hkv));
   // The last rows of a sequence see most: first.
   const int64_t u = gridDim.x / static_cast<uint32_t>(p.Hkv) - 1 - blockIdx.x / static_cast<uint32_t>(p.Hkv);
-  const int b = packed_find(p.cu, p.B + 1, p.Tq, p.G, Sh::kRows, 1, u);
-  const bool tail = b == p.B;  // rows behind the last sequence
-  const int q0 = packed_start(p.cu, b, p.Tq), q1 = tail ? p.Tq : packed_start(p.cu, b + 1, p.Tq);
-  const int rows_all = max(q1 - q0, 0) * p.G;  // below 2^31: Tq Hq is
-  const int64_t row0_64 = (u - packed_base(p.cu, b, p.Tq, p.G, Sh::kRows, 1)) * Sh::kRows;
-  if (row0_64 >= rows_all) return;
-  const int row0 = static_cast<int>(row0_64);
-  const int rows = min(Sh::kRows, rows_all - row0);
-  const int k0 = tail ? 0 : packed_start(p.cu_k, b, p.Tk);
-  const int nk = tail ? 0 : max(packed_start(p.cu_k, b + 1, p.Tk) - k0, 0);
-  const int before = nk - (q1 - q0);  // position of query 0
-  const int row_bytes = p.D * ES;
-  // Positions of the workgroup's rows, and of this wave's.
-  const int p_min = before + row0 / p.G, p_max = before + (row0 + rows - 1) / p.G;
-  const int wave_row = 32 * NB * wv;
-  const int w_min = before + min(row0 + wave_row, row0 + rows - 1) / p.G;
-  const int w_max = before + min(row0 + wave_row + 32 * NB - 1, row0 + rows - 1) / p.G;
-  const bool wave_real = wave_row < rows;
-  // Tiles [0, sink_tiles) and from lo_tile on.
-  const int end = min(p_max + 1, nk);
-  const int lo = p.window > 0 ? max(p_min - p.window + 1, 0) : 0;
-  const int lo_tile = lo / TT;
-  const int sink_tiles = min((min(p.sinks, lo) + TT - 1) / TT, lo_tile);
-  const int tiles = end > 0 ? sink_tiles + (end + TT - 1) / TT - lo_tile : 0;
-  auto first_of = [&](int i) { return TT * (i < sink_tiles ? i : i - sink_tiles + lo_tile); };
-
-  const char* k_base = static_cast<const char*>(p.k) + (k0 * p.k_stride + static_cast<int64_t>(h) * p.D) * ES;
-  const char* v_base = static_cast<const char*>(p.v) + (k0 * p.v_stride + static_cast<int64_t>(h) * p.D) * ES;
-  const uint32_t k_bytes = static_cast<uint32_t>(p.k_stride * ES), v_bytes = static_cast<uint32_t>(p.v_stride * ES);
-  const bool padded = row_bytes < Sh::kRow;
-  uint32_t col[Sh::kLoads];
-  int load_row[Sh::kLoads];
-#pragma unroll
-  for (int i = 0; i < Sh::kLoads; ++i) {
-    load_row[i] = Sh::kLoadRows * wv + (64 * i + lane) / Sh::kSlots;
-    col[i] = 16 * ((lane & (Sh::kSlots - 1)) ^ tile_swizzle(Sh::kSlots, load_row[i]));
+  int b, q1, k1;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  if (p.B < 64) {
+    // Lane b holds sequence b's starts: one round trip.
+    const int at = min(lane, p.B);
+    const int qs = packed_start(p.cu, at, p.Tq), ks = packed_start(p.cu_k, at, p.Tk);
+    const int64_t base = static_cast<int64_t>(qs) * p.G / ROWS + lane;
+    b = 63 - __builtin_clzll(__ballot(lane == 0 || (lane <= p.B && base <= u)));
+    const int next = min(b + 1, p.B);
+    x.q0 = __builtin_amdgcn_readlane(qs, b);
+    q1 = __builtin_amdgcn_readlane(qs, next);
+    x.k0 = __builtin_amdgcn_readlane(ks, b);
+    k1 = __builtin_amdgcn_readlane(ks, next);
+  } else {
+    b = packed_find(p.cu, p.B + 1, p.Tq, p.G, ROWS, 1, u);
+    const int next = min(b + 1, p.B);
+    x.q0 = packed_start(p.cu, b, p.Tq);
+    q1 = packed_start(p.cu, next, p.Tq);
+    x.k0 = packed_start(p.cu_k, b, p.Tk);
+    k1 = packed_start(p.cu_k, next, p.Tk);
   }
-  const uint32_t lds0 = tile_lds_address(smem);
-  const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds0 + Sh::kLoadRows * wv * Sh::kRow);
-  // Rows past the last key repeat it: they are hidden from every query.
-  auto load_tile = [&](int first, int slot) {
-    const char* k = k_base + static_cast<int64_t>(first) * k_bytes;
-    const char* v = v_base + static_cast<int64_t>(first) * v_bytes;
-    const uint32_t to = lds_wave + slot * 2 * Sh::kTile;
-    const int last = nk - 1 - first;
+  const bool tail = b == p.B;  // rows behind the last sequence
+  if (tail) q1 = p.Tq;
+  const int rows_all = max(q1 - x.q0, 0) * p.G;  // below 2^31: Tq Hq is
+  const int64_t row0 = (u - static_cast<int64_t>(x.q0) * p.G / ROWS - b) * ROWS;
+  if (row0 >= rows_all) return false;
+  x.row0 = static_cast<int>(row0);
+  x.rows = min(ROWS, rows_all - x.row0);
+  x.nk = tail ? 0 : max(k1 - x.k0, 0);
+  x.before = x.nk - (q1 - x.q0);
+  x.p_min = max(x.before + x.row0 / p.G, -1);
+  x.p_max = max(x.before + (x.row0 + x.rows - 1) / p.G, -1);
+  const int end = x.p_max + 1;  // at most nk
+  const int lo = p.window > 0 ? max(x.p_min - p.window + 1, 0) : 0;
+  x.lo_tile = lo / TT;
+  x.sink_tiles = min((min(p.sinks, lo) + TT - 1) / TT, x.lo_tile);
+  x.tiles = end > 0 ? x.sink_tiles + (end + TT - 1) / TT - x.lo_tile : 0;
+  return true;
+}
+
+template <int TT>
+__device__ __forceinline__ int prefill_first(const PrefillItem& x, int i) {
+  return TT * (i < x.sink_tiles ? i : i - x.sink_tiles + x.lo_tile);
+}
+
+// Whether rows at positions lowest .. highest all see tokens first .. last.
+__device__ __forceinline__ bool prefill_sees_all(const PrefillParams& p, int first, int last, int lowest, int highest) {
+  return last <= lowest && (p.window == 0 || first > highest - p.window || last < p.sinks);
+}
+
+// Bit-free view of a lane's tokens: those from `token` on that a row at `place`
+// sees are o <= hi with o > lo or o < sinks, o counted from `token`.
+struct PrefillView {
+  int hi, lo, sinks;
+  __device__ __forceinline__ bool operator()(int o) const {
+    return static_cast<bool>(static_cast<int>(o <= hi) & (static_cast<int>(o > lo) | static_cast<int>(o < sinks)));
+  }
+};
+__device__ __forceinline__ PrefillView prefill_view(const PrefillParams& p, int place, int token) {
+  PrefillView v;
+  v.hi = place - token;
+  v.lo = p.window > 0 ? max(place - p.window, token - 1) - token : -1;
+  v.sinks = p.sinks - token;
+  return v;
+}
+
+// Loads of K and V rows into LDS: a wave's rows of a tile, one instruction at a
+// time.  What lies past the last key is taken from the end of its row instead:
+// no query sees it.
+template <typename Sh>
+struct PrefillLoads {
+  const char* base[2];  // K, V
+  uint32_t bytes[2];
+  int row_bytes, nk;
+  uint32_t off[2][Sh::kLoads], lds_wave;
+  bool inside[Sh::kLoads];
+  __device__ __forceinline__ PrefillLoads(const PrefillParams& p, const PrefillItem& x, uint32_t lds, int wv, int lane) {
+    row_bytes = p.D * Sh::kES;
+    nk = x.nk;
+    base[0] = static_cast<const char*>(p.k) + (x.k0 * p.k_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES;
+    base[1] = static_cast<const char*>(p.v) + (x.k0 * p.v_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES;
+    bytes[0] = static_cast<uint32_t>(p.k_stride * Sh::kES);
+    bytes[1] = static_cast<uint32_t>(p.v_stride * Sh::kES);
 #pragma unroll
     for (int i = 0; i < Sh::kLoads; ++i) {
-      const uint32_t r = min(load_row[i], last);
-      if (!padded || static_cast<int>(col[i]) < row_bytes) {
-        tile_load_lds<false>(k, r * k_bytes + col[i], to + 1024 * i);
-        tile_load_lds<false>(v, r * v_bytes + col[i], to + Sh::kTile + 1024 * i);
-      }
+      const int row = Sh::kLoadRows * wv + (64 * i + lane) / Sh::kSlots;
+      const int col = 16 * ((lane & (Sh::kSlots - 1)) ^ prefill_swizzle(Sh::kSlots, row));
+      inside[i] = col < row_bytes;  // false only in padded rows
+      off[0][i] = row * bytes[0] + col;
+      off[1][i] = row * bytes[1] + col;
     }
-  };
-
-  if (padded) {  // products run over the slots past the head
-    for (int i = tid; i < 4 * Sh::kTile / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
-    tile_barrier();
+    lds_wave = __builtin_amdgcn_readfirstlane(lds + Sh::kLoadRows * wv * Sh::kRow);
   }
-  if (tiles > 0) load_tile(first_of(0), 0);
-
-  // This lane's rows.
-  int place[NB];  // position of its query
-  u32x4 qf[NB][Sh::kSteps];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = row0 + min(wave_row + 32 * nb + n32, rows - 1);
-    const int query = row / p.G;
-    place[nb] = before + query;
-    const char* src = static_cast<const char*>(p.q) +
-                      ((q0 + query) * p.q_stride + (static_cast<int64_t>(h) * p.G + (row - query * p.G)) * p.D) * ES;
-#pragma unroll
-    for (int st = 0; st < Sh::kSteps; ++st) {
-      const int at = 32 * st + 16 * half;
-      qf[nb][st] = at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
-    }
+  // Load i of K (which 0) or V (1) of the tile at token `first`; `to`: the
+  // buffer's place in LDS.
+  __device__ __forceinline__ void one(int which, int i, int first, uint32_t to) const {
+    const int64_t from = static_cast<int64_t>(first) * bytes[which];
+    const char* src = base[which] + readlane_i64(from, 0);  // the same in all lanes: scalar registers
+    const uint32_t most = static_cast<uint32_t>(min(nk - 1 - first, Sh::TT - 1)) * bytes[which] + row_bytes - 16;
+    if (row_bytes == Sh::kRow || inside[i])
+      tile_load_lds<false>(src, min(off[which][i], most), lds_wave + to + 1024 * i);
   }
-  f32x16 acc[Sh::kCols][NB];
-  float m[NB], l[NB];
+  __device__ __forceinline__ void operator()(int which, int first, uint32_t to) const {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m[nb] = -INFINITY;
-    l[nb] = 0.f;
-#pragma unroll
-    for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] = f32x16{};
+    for (int i = 0; i < Sh::kLoads; ++i) one(which, i, first, to);
   }
-  // Addresses of operands within a tile (bytes).
-  const uint32_t k_at = n32 * Sh::kRow + 16 * (half ^ tile_swizzle(Sh::kSlots, n32));
-  const int r16 = lane & 15;
-  const int vr = 4 * half + (k16 ? r16 >> 2 : 0);
-  const uint32_t v_at = k16 ? vr * Sh::kRow + 16 * ((2 * ((lane >> 4) & 1) + ((r16 >> 1) & 1)) ^ tile_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1)
-                            : 4 * half * Sh::kRow + 16 * (n32 >> 2) + 4 * (n32 & 3);
-  __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0): no register load is pending in the loop
+};
 
-  auto visible = [&](int nb, int token) {
-    return token <= place[nb] && (p.window == 0 || token > place[nb] - p.window || token < p.sinks);
-  };
-  // V^T operand of 16 tokens (16-bit) for columns 32 c..
-  auto read_v16 = [&](uint32_t at, int ks, int c) {
-    const uint32_t a = at + v_at + 16 * ks * Sh::kRow;
-    const u32x2 x = tile_tr_read(a ^ (64 * c)), y = tile_tr_read((a + 8 * Sh::kRow) ^ (64 * c) ^ 16);
-    return u32x4{x[0], x[1], y[0], y[1]};
-  };
-  // V[token 32 tb + 8 (i / 4) + 4 half + i % 4][32 c + n32] (fp32).
-  auto read_v32 = [&](uint32_t at, int tb, int i, int c) {
-    const int row = 32 * tb + 8 * (i / 4) + i % 4;
-    return tile_lds_read<float>((at + v_at + row * Sh::kRow) ^ (128 * c) ^ (16 * (8 * half)) ^ (16 * (2 * (i % 4) + ((i / 4) & 1))));
-  };
-
-  for (int i = 0; i < tiles; ++i) {
-    // The tile has arrived, and every wave is done with the one before it.
-    tile_barrier_loads<0>();
-    const int first = first_of(i), slot = i & 1;
-    if (i + 1 < tiles) load_tile(first_of(i + 1), slot ^ 1);
-    const uint32_t at = lds0 + slot * 2 * Sh::kTile, vt = at + Sh::kTile;
-    char* tile = smem + slot * 2 * Sh::kTile;
-    const int last = first + TT - 1;
-    // Every row of the workgroup (of the wave) sees all of the tile.
-    auto sees_all = [&](int lowest, int highest) {
-      return last <= lowest && (p.window == 0 || first > highest - p.window || last < p.sinks);
-    };
-    const bool whole = sees_all(p_min, p_max);
-    bool bad = false;
-    if (!whole) {
-      // Where only some rows see a token, a weight of 0 would not hide Inf and
-      // NaN from the others.
-      if (tid == 0) *bad_word = 0;
-      tile_barrier();
-      bool found = false;
-      for (int x = tid; x < Sh::kTile / 16; x += 64 * NW)
-        found |= !prefill_finite<DT>(reinterpret_cast<const u32x4*>(tile + Sh::kTile)[x]);
-      if (found) *bad_word = 1;
-      tile_barrier();
-      bad = __builtin_amdgcn_readfirstlane(*bad_word) != 0;
-    }
-    const bool none = !wave_real || first > w_max || (p.window > 0 && last <= w_min - p.window && first >= p.sinks);
-    if (none && !bad) continue;
-    const bool masked = !sees_all(w_min, w_max);
-
-    f32x16 s[TB][NB];
+// Puts zeros in place of values that are not finite; whether this thread found
+// any.
+template <int DT, int PIECES, int STEP>
+__device__ __forceinline__ bool prefill_drop_bad(char* v, int tid) {
+  using S = typename Elem<DT>::S;
+  constexpr int kEach = 16 / static_cast<int>(sizeof(S));
+  bool found = false;
+#pragma unroll 4
+  for (int i = tid; i < PIECES; i += STEP) {
+    u32x4* at = reinterpret_cast<u32x4*>(v) + i;
+    if (prefill_finite<DT>(*at)) continue;
+    found = true;
+    S* val = reinterpret_cast<S*>(at);
 #pragma unroll
-    for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[tb][nb] = f32x16{};
-#pragma unroll
-    for (int st = 0; st < Sh::kSteps; ++st)
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb) {
-        const u32x4 a = tile_lds_read<u32x4>((at + k_at + 32 * tb * Sh::kRow) ^ (32 * st));
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[tb][nb] = PrefillMma<DT>::mma(a, qf[nb][st], s[tb][nb]);
-      }
-    if (masked) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[tb][nb][e] = visible(nb, first + 32 * tb + 8 * (e / 4) + 4 * half + e % 4) ? s[tb][nb][e] : -INFINITY;
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][nb][e]);
-      if (__ballot(mx * p.sl2 > m[nb] + kLazy)) {
-        const float mn = fmaxf(m[nb], prefill_max_halves(mx) * p.sl2);
-        const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
-        m[nb] = mn;
-        l[nb] *= alpha;
-#pragma unroll
-        for (int c = 0; c < Sh::kCols; ++c) acc[c][nb] *= alpha;
-      }
-      const float ref = m[nb] == -INFINITY ? kShift : kShift - m[nb];
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[tb][nb][e] = fast_exp2(fmaf(s[tb][nb][e], p.sl2, ref));
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          l[nb] += (s[tb][nb][e] + s[tb][nb][e + 1]) + (s[tb][nb][e + 2] + s[tb][nb][e + 3]);
-    }
-    if (bad) {
-      // Values that are not finite: which rows see which of them by a product of
-      // what is visible with their flags (in K's place, which is done with),
-      // and zeros in their place.
-      tile_barrier();
-      for (int x = tid; x < Sh::kTile / 16; x += 64 * NW) {
-        constexpr int kEach = 16 / ES;
-        S* val = reinterpret_cast<S*>(tile + Sh::kTile) + x * kEach;
-        S* flag = reinterpret_cast<S*>(tile) + x * kEach;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const float f = prefill_flag<DT>(val[e]);
-          flag[e] = E::from_f(f);
-          if (f != 0.f) val[e] = E::from_f(0.f);
-        }
-      }
-      tile_barrier();
-#pragma unroll 1
-      for (int nb_at = 0; nb_at < NB; ++nb_at)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          if (nb != nb_at || !wave_real) continue;
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) {
-            f32x16 seen = f32x16{};
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-              for (int ks = 0; ks < 2; ++ks) {
-                auto one = [&](int e) {
-                  return visible(nb, first + 32 * tb + 8 * (e / 4) + 4 * half + e % 4) ? 1.f : 0.f;
-                };
-                if constexpr (k16) {
-                  u32x4 w;
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) w[j] = MfmaOps<DT>::pack2(one(8 * ks + 2 * j), one(8 * ks + 2 * j + 1));
-                  seen = PrefillMma<DT>::mma(read_v16(at, 2 * tb + ks, c), w, seen);
-                } else {
-#pragma unroll
-                  for (int e = 8 * ks; e < 8 * ks + 8; ++e)
-                    seen = __builtin_amdgcn_mfma_f32_32x32x2f32(read_v32(at, tb, e, c), one(e), seen, 0, 0, 0);
-                }
-              }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float minus = floorf(seen[e] / kPrefillMinusInf), plus = seen[e] - minus * kPrefillMinusInf;
-              if (seen[e] >= kPrefillNan) {
-                acc[c][nb][e] = NAN;
-              } else {
-                if (plus > 0.f) acc[c][nb][e] += INFINITY;
-                if (minus > 0.f) acc[c][nb][e] -= INFINITY;
-              }
-            }
-          }
-        }
-    }
-    if constexpr (k16) {
-#pragma unroll
-      for (int ks = 0; ks < TT / 16; ++ks) {
-        u32x4 w[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[nb][j] = MfmaOps<DT>::pack2(s[ks / 2][nb][8 * (ks & 1) + 2 * j], s[ks / 2][nb][8 * (ks & 1) + 2 * j + 1]);
-#pragma unroll
-        for (int c = 0; c < Sh::kCols; ++c) {
-          const u32x4 a = read_v16(vt, ks, c);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) acc[c][nb] = PrefillMma<DT>::mma(a, w[nb], acc[c][nb]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-#pragma unroll
-          for (int c = 0; c < Sh::kCols; ++c) {
-            const float a = read_v32(vt, tb, e, c);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-              acc[c][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[tb][nb][e], acc[c][nb], 0, 0, 0);
-          }
-    }
+    for (int e = 0; e < kEach; ++e)
+      if (prefill_flag<DT>(val[e]) != 0.f) val[e] = Elem<DT>::from_f(0.f);
   }
+  return found;
+}
 
+// Flags in place of all values.
+template <int DT, int PIECES, int STEP>
+__device__ __forceinline__ void prefill_to_flags(char* v, int tid) {
+  using S = typename Elem<DT>::S;
+  constexpr int kEach = 16 / static_cast<int>(sizeof(S));
+  for (int i = tid; i < PIECES; i += STEP) {
+    S* val = reinterpret_cast<S*>(v) + i * kEach;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) val[e] = Elem<DT>::from_f(prefill_flag<DT>(val[e]));
+  }
+}
+
+// y plus the values that a sum of flags stands for.
+__device__ __forceinline__ float prefill_add_bad(float y, float seen) {
+  if (seen >= kPrefillNan) return NAN;
+  const float minus = floorf(seen / kPrefillMinusInf), plus = seen - minus * kPrefillMinusInf;
+  if (plus > 0.f) y += INFINITY;
+  if (minus > 0.f) y -= INFINITY;
+  return y;
+}
+
+// out rows of a lane: acc of column block c, element e is column 32 c + 8 (e / 4) +
+// 4 half + e % 4 of row wave_row + 32 nb + lane % 32.
+template <int DT, int DP, int NB>
+__device__ __forceinline__ void prefill_store(const PrefillParams& p, const PrefillItem& x, int wave_row,
+                                              const f32x16 (&acc)[DP / 32][NB], const float (&l)[NB]) {
+  constexpr int ES = DT == QD_DTYPE_F32 ? 4 : 2;
+  const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const float sum = prefill_sum_halves(l[nb]);
     const bool has = sum > 0.f || sum != sum;
     const float scale = has ? 1.f / sum : 0.f;
-    const int rr = wave_row + 32 * nb + n32;
-    if (rr >= rows) continue;
-    const int row = row0 + rr, query = row / p.G;
+    const int rr = wave_row + 32 * nb + (lane & 31);
+    if (rr >= x.rows) continue;
+    const int row = x.row0 + rr, query = row / p.G;
     char* to = static_cast<char*>(p.out) +
-               ((static_cast<int64_t>(q0 + query) * p.Hq + static_cast<int64_t>(h) * p.G + (row - query * p.G)) * p.D) * ES;
+               ((static_cast<int64_t>(x.q0 + query) * p.Hq + static_cast<int64_t>(x.h) * p.G + (row - query * p.G)) * p.D) * ES;
 #pragma unroll
-    for (int c = 0; c < Sh::kCols; ++c)
+    for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const int d = 32 * c + 2 * e + 4 * half;
@@ -437,7 +311,7 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 && DT != QD_DTYPE_F3
         f32x4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = has ? acc[c][nb][e + j] * scale : 0.f;
-        if constexpr (k16)
+        if constexpr (DT != QD_DTYPE_F32)
           *reinterpret_cast<u32x2*>(to + d * ES) = u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
         else
           *reinterpret_cast<f32x4*>(to + d * ES) = y;
@@ -445,10 +319,500 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 && DT != QD_DTYPE_F3
   }
 }
 
+// Q as the B operand, and the positions of this lane's rows.
+template <typename Sh, int NB>
+__device__ __forceinline__ void prefill_load_q(const PrefillParams& p, const PrefillItem& x, int wave_row, int (&place)[NB],
+                                               u32x4 (&qf)[NB][Sh::kSteps]) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int row_bytes = p.D * Sh::kES;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = x.row0 + min(wave_row + 32 * nb + (lane & 31), x.rows - 1);
+    const int query = row / p.G;
+    place[nb] = max(x.before + query, -1);
+    const char* src = static_cast<const char*>(p.q) +
+                      ((x.q0 + query) * p.q_stride + (static_cast<int64_t>(x.h) * p.G + (row - query * p.G)) * p.D) * Sh::kES;
+#pragma unroll
+    for (int st = 0; st < Sh::kSteps; ++st) {
+      const int at = 32 * st + 16 * (lane >> 5);
+      qf[nb][st] = at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+}
+
+// The workgroup goes through the tokens that its rows see in tiles of TT: K and V
+// rows come straight into LDS, a tile ahead, and each wave multiplies its 32 NB
+// rows with them, 32 tokens at a time:
+//   scores   S^T = K Q^T, 32x32 blocks (A = K rows from LDS, B = Q from
+//            registers): a lane holds one row and 16 of 32 tokens
+//   softmax  per lane, weights 2^(s - m) with a reference m of the row that
+//            was one of its scores.  m moves only when a lane's weights of a
+//            step sum to more than 2^kLazy (which every weight beyond that
+//            does): the maximum is not computed otherwise, and lanes exchange
+//            nothing.
+//   output   O^T += V^T P^T: the score layout is already the B operand (the
+//            products sum over tokens in the order that the lanes hold them in),
+//            V^T comes from transposing LDS reads.
+// 16-bit weights are rounded to nearest once: half a step of the output's type,
+// which a sum over many values averages out; their sum is that of the rounded
+// ones.
+//
+// Three steps are in work at once, in one stream of instructions: the scores of
+// the next 32 tokens, the softmax of these, the values of the ones before.  A
+// 32x32x16 product takes 32 cycles, in which a wave issues up to seven vector
+// instructions; per product there is one element's worth of softmax (a
+// multiply-add, an exponential that counts as two, halves of a conversion and of
+// a sum), so the matrix cores go on without a pause.
+template <int DT, int DP, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefill_pipe_kernel(PrefillParams p) {
+  using Sh = PrefillShape<DT, DP, NB, NW>;
+  static_assert(DT != QD_DTYPE_F32 && Sh::TT == 64, "16-bit types");
+  // fp16 weights are multiples of 2^-24 and the largest of a row is at least
+  // 2^kShift: what that grid adds is at most 2^-32 of it.
+  constexpr float kShift = DT == QD_DTYPE_F16 ? 7.f : 0.f;
+  constexpr float kMost = DT == QD_DTYPE_F16 ? 32768.f : 256.f;  // 2^(kShift + kLazy)
+  constexpr int kN = Sh::kSteps;      // steps of the scores, and (token 16, column 32) pairs of the output
+  constexpr int kCols = Sh::kCols;
+  constexpr int kRing = kN % 4 == 0 ? 4 : 3;  // operands in registers, all but one of them read ahead
+  constexpr int kPairs = 8 * NB;      // packed pairs of weights
+  constexpr int kSlots = kN * NB;     // slots of one product each of scores and output
+  extern __shared__ __align__(16) char smem[];
+  // K in two buffers, V in two, a word.
+  int* word = reinterpret_cast<int*>(smem + 4 * Sh::kTile);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, half = lane >> 5, r16 = lane & 15;
+  PrefillItem x;
+  if (!prefill_item<Sh::kRows, Sh::TT>(p, x)) return;
+  const int wave_row = 32 * NB * wv;
+  const int w_min = max(x.before + min(x.row0 + wave_row, x.row0 + x.rows - 1) / p.G, -1);
+  const int w_max = max(x.before + min(x.row0 + wave_row + 32 * NB - 1, x.row0 + x.rows - 1) / p.G, -1);
+  const uint32_t lds0 = tile_lds_address(smem);
+  const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
+  auto k_buf = [](int t) { return static_cast<uint32_t>((t & 1) * Sh::kTile); };
+  auto v_buf = [](int t) { return static_cast<uint32_t>((2 + (t & 1)) * Sh::kTile); };
+  if (load.row_bytes < Sh::kRow) {  // products run over the slots past the head
+    for (int i = tid; i < 4 * Sh::kTile / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    tile_barrier();
+  }
+  if (x.tiles > 0) {
+    load(0, prefill_first<64>(x, 0), k_buf(0));
+    load(1, prefill_first<64>(x, 0), v_buf(0));
+  }
+  if (x.tiles > 1) load(0, prefill_first<64>(x, 1), k_buf(1));
+  int place[NB];
+  u32x4 qf[NB][kN];
+  prefill_load_q<Sh, NB>(p, x, wave_row, place, qf);
+  f32x16 acc[kCols][NB];
+  float m[NB], l[NB], ref[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = -INFINITY;
+    ref[nb] = INFINITY;  // the first step finds its maximum
+    l[nb] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c][nb] = f32x16{};
+  }
+  // Operands' places in LDS, in the buffers that the next step reads: step st of
+  // a K row, columns 32 c.. of V's token rows 4 half.. and 8 further.
+  uint32_t k_at[kN], v_at[kCols][2];
+#pragma unroll
+  for (int st = 0; st < kN; ++st)
+    k_at[st] = lds0 + n32 * Sh::kRow + (16 * (half ^ prefill_swizzle(Sh::kSlots, n32)) ^ (32 * st));
+  const int vr = 4 * half + (r16 >> 2);
+#pragma unroll
+  for (int c = 0; c < kCols; ++c)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v_at[c][i] = lds0 + v_buf(1) + (vr + 8 * i) * Sh::kRow +
+                   ((16 * ((2 * ((lane >> 4) & 1) + ((r16 >> 1) & 1)) ^ prefill_swizzle(Sh::kSlots, vr)) + 8 * (r16 & 1)) ^
+                    (64 * c) ^ (16 * i));
+  auto read_k = [&](int token, int st) { return tile_lds_read<u32x4>(k_at[st] + token * Sh::kRow); };
+  // V^T of 16 tokens from `token` on, columns 32 c..
+  auto read_v = [&](int token, int c) {
+    const u32x2 a = tile_tr_read(v_at[c][0] + token * Sh::kRow), b = tile_tr_read(v_at[c][1] + token * Sh::kRow);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  };
+  auto next_buffers = [&]() {
+#pragma unroll
+    for (int st = 0; st < kN; ++st) k_at[st] ^= Sh::kTile;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      v_at[c][0] ^= Sh::kTile;
+      v_at[c][1] ^= Sh::kTile;
+    }
+  };
+  auto sum2 = [](uint32_t w, float c) {
+    if constexpr (DT == QD_DTYPE_BF16)
+      return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), c, false);
+    else
+      return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3C003C00u), c, false);
+  };
+  struct Weights {
+    u32x4 w[2][NB];  // 16 tokens each
+  };
+
+  u32x4 ka[kRing], va[kRing];  // operands read ahead of their products
+  // The scores of the 32 tokens from `at` on in K's buffer, the weights of `cur`,
+  // the products of the weights `prev` with those from `at` on in V's.  `midway`
+  // runs when the last operands of the step are on their way, and the next step's
+  // first ones, from 32 - `at` on, follow; `aside(i)` runs beside the products i.
+  auto step = [&](f32x16 (&cur)[NB], f32x16 (&next)[NB], const Weights& prev, Weights& now, auto at, auto&& midway,
+                  auto&& aside) {
+    float arg[kPairs][2], val[kPairs][2], sum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) sum[nb] = 0.f;
+    // Pair j: elements 2 (j / NB), + 1 of row block j % NB.  The empty statements
+    // keep each stage in its slot.
+    auto scale2 = [&](int j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        arg[j][e] = fmaf(cur[j % NB][2 * (j / NB) + e], p.sl2, ref[j % NB]);
+        asm volatile("" : "+v"(arg[j][e]));
+      }
+    };
+    auto exp2 = [&](int j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        val[j][e] = fast_exp2(arg[j][e]);
+        asm volatile("" : "+v"(val[j][e]));
+      }
+    };
+    auto pack = [&](int j) {
+      uint32_t w = MfmaOps<DT>::pack2(val[j][0], val[j][1]);
+      asm volatile("" : "+v"(w));
+      now.w[(j / NB) >> 2][j % NB][(j / NB) & 3] = w;
+      sum[j % NB] = sum2(w, sum[j % NB]);
+    };
+    // Stages of a pair, a slot apart.
+    auto from = [](int slot) { return slot < 0 ? 0 : slot >= kSlots ? kPairs : slot * kPairs / kSlots; };
+#pragma unroll
+    for (int j = 0; j < from(2); ++j) scale2(j);
+#pragma unroll
+    for (int j = 0; j < from(1); ++j) exp2(j);
+#pragma unroll
+    for (int slot = 0; slot < kSlots; ++slot) {
+      const int i = slot / NB, nb = slot % NB;
+      if (nb == 0) {
+        const int ahead = i + kRing - 1;
+        if (ahead == kN) midway();
+        const int token = ahead < kN ? at : 32 - at;
+        ka[ahead % kRing] = read_k(token, ahead % kN);
+        va[ahead % kRing] = read_v(token + 16 * (ahead % kN / kCols), ahead % kCols);
+      }
+      next[nb] = PrefillMma<DT>::mma(ka[i % kRing], qf[nb][i], i == 0 ? f32x16{} : next[nb]);
+      acc[i % kCols][nb] = PrefillMma<DT>::mma(va[i % kRing], prev.w[i / kCols][nb], acc[i % kCols][nb]);
+#pragma unroll
+      for (int j = from(slot + 2); j < from(slot + 3); ++j) scale2(j);
+#pragma unroll
+      for (int j = from(slot + 1); j < from(slot + 2); ++j) exp2(j);
+#pragma unroll
+      for (int j = from(slot); j < from(slot + 1); ++j) pack(j);
+      if (nb == 0) aside(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // NaN sums too.
+    bool move = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) move |= !(sum[nb] <= kMost);
+    if (__ballot(move)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        asm volatile("" : "+v"(cur[nb]));  // nothing of this is computed ahead of the branch
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, cur[nb][e]);
+        const float mn = fmaxf(m[nb], prefill_max_halves(mx) * p.sl2);
+        const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
+        m[nb] = mn;
+        ref[nb] = mn == -INFINITY ? kShift : kShift - mn;
+        l[nb] *= alpha;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[c][nb] *= alpha;
+        sum[nb] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        scale2(j);
+        exp2(j);
+        pack(j);
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        if (m[nb] == -INFINITY) ref[nb] = INFINITY;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) l[nb] += sum[nb];
+  };
+  // Hides the scores of 32 tokens from `first` on that rows do not see.
+  auto hide = [&](f32x16 (&s)[NB], int first) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const PrefillView sees = prefill_view(p, place[nb], first + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[nb][e] = sees(8 * (e / 4) + e % 4) ? s[nb][e] : -INFINITY;
+    }
+  };
+
+  if (x.tiles > 0) {
+    f32x16 s0[NB], s1[NB];
+    Weights w0, w1;
+    // The first step has no tokens before it: no weights, and values of 0.
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) w1.w[0][nb] = w1.w[1][nb] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < Sh::kTile / 32; i += 64 * NW)
+      reinterpret_cast<u32x4*>(smem + v_buf(1) + Sh::kTile / 2)[i] = u32x4{0u, 0u, 0u, 0u};
+    tile_barrier_loads<0>();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) s0[nb] = f32x16{};
+#pragma unroll
+    for (int st = 0; st < kN; ++st) {
+      const u32x4 a = read_k(0, st);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s0[nb] = PrefillMma<DT>::mma(a, qf[nb][st], s0[nb]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) {
+      ka[i] = read_k(32, i);
+      va[i] = read_v(32 + 16 * (i / kCols), i % kCols);
+    }
+    using Lower = std::integral_constant<int, 0>;
+    using Upper = std::integral_constant<int, 32>;
+    bool found = false;
+#pragma unroll 1
+    for (int t = 0; t < x.tiles; ++t) {
+      const int first = prefill_first<64>(x, t);
+      const bool masked = !prefill_sees_all(p, first, first + 63, w_min, w_max);
+      if (masked) hide(s0, first);
+      step(
+          s0, s1, w1, w0, Upper{},
+          [&]() {
+            // This V and the next K have arrived, and every wave has read what it
+            // needs of this K and the V before.
+            tile_barrier_loads<0>();
+            next_buffers();
+            // Where only some rows see a token, a weight of 0 would not hide Inf
+            // and NaN from the others: they are left out here and added at the end.
+            if (!prefill_sees_all(p, first, first + 63, x.p_min, x.p_max)) {
+              found |= prefill_drop_bad<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(t), tid);
+              tile_barrier();
+            }
+          },
+          [](int) {});
+      if (masked) hide(s1, first + 32);
+      // After the last tile: scores of no use.
+      const int k_next = prefill_first<64>(x, min(t + 2, x.tiles - 1)), v_next = prefill_first<64>(x, min(t + 1, x.tiles - 1));
+      step(
+          s1, s0, w0, w1, Lower{}, []() {},
+          [&](int i) {
+#pragma unroll
+            for (int j = 2 * Sh::kLoads * i / kN; j < 2 * Sh::kLoads * (i + 1) / kN; ++j) {
+              if (j < Sh::kLoads) {
+                if (t + 2 < x.tiles) load.one(0, j, k_next, k_buf(t));
+              } else {
+                if (t + 1 < x.tiles) load.one(1, j - Sh::kLoads, v_next, v_buf(t + 1));
+              }
+            }
+          });
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const u32x4 a = i < kRing - 1 ? va[i] : read_v(32 + 16 * (i / kCols), i % kCols);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) acc[i % kCols][nb] = PrefillMma<DT>::mma(a, w1.w[i / kCols][nb], acc[i % kCols][nb]);
+    }
+    tile_barrier();
+    if (tid == 0) *word = 0;
+    tile_barrier();
+    if (found) *word = 1;
+    tile_barrier();
+    if (__builtin_amdgcn_readfirstlane(*word) != 0) {
+      // Values that are not finite: a product of what is visible with their
+      // flags tells which rows see which of them.
+      if (x.tiles & 1) next_buffers();  // to V's second buffer
+#pragma unroll 1
+      for (int t = 0; t < x.tiles; ++t) {
+        const int first = prefill_first<64>(x, t);
+        if (prefill_sees_all(p, first, first + 63, x.p_min, x.p_max)) continue;
+        tile_barrier();
+        load(1, first, v_buf(1));
+        tile_barrier_loads<0>();
+        prefill_to_flags<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(1), tid);
+        tile_barrier();
+#pragma unroll 1
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const PrefillView sees = prefill_view(p, place[nb], first + 16 * ks + 4 * half);
+            u32x4 one;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int o = 8 * (j >> 1) + 2 * (j & 1);
+              one[j] = MfmaOps<DT>::pack2(sees(o) ? 1.f : 0.f, sees(o + 1) ? 1.f : 0.f);
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const f32x16 seen = PrefillMma<DT>::mma(read_v(16 * ks, c), one, f32x16{});
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[c][nb][e] = prefill_add_bad(acc[c][nb][e], seen[e]);
+            }
+          }
+      }
+    }
+  }
+  prefill_store<DT, DP, NB>(p, x, wave_row, acc, l);
+}
+
+// fp32: the same products on the fp32 matrix cores, tile by tile, without the
+// overlap: they take eight times as long as the 16-bit ones, and hide the rest.
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p) {
+  using Sh = PrefillShape<QD_DTYPE_F32, DP, 1, NW>;
+  constexpr int TT = Sh::TT, TB = Sh::kTB;
+  constexpr float kLazy = 8.f;
+  extern __shared__ __align__(16) char smem[];
+  int* word = reinterpret_cast<int*>(smem + 4 * Sh::kTile);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, half = lane >> 5;
+  PrefillItem x;
+  if (!prefill_item<Sh::kRows, TT>(p, x)) return;
+  const int wave_row = 32 * wv;
+  const int w_min = max(x.before + min(x.row0 + wave_row, x.row0 + x.rows - 1) / p.G, -1);
+  const int w_max = max(x.before + min(x.row0 + wave_row + 31, x.row0 + x.rows - 1) / p.G, -1);
+  const uint32_t lds0 = tile_lds_address(smem);
+  const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
+  if (load.row_bytes < Sh::kRow) {  // products run over the slots past the head
+    for (int i = tid; i < 4 * Sh::kTile / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    tile_barrier();
+  }
+  auto load_tile = [&](int i) {
+    const uint32_t to = (i & 1) * 2 * Sh::kTile;
+    load(0, prefill_first<TT>(x, i), to);
+    load(1, prefill_first<TT>(x, i), to + Sh::kTile);
+  };
+  if (x.tiles > 0) load_tile(0);
+  int place[1];
+  u32x4 qf[1][Sh::kSteps];
+  prefill_load_q<Sh, 1>(p, x, wave_row, place, qf);
+  f32x16 acc[Sh::kCols][1];
+  float m = -INFINITY, l[1] = {0.f};
+#pragma unroll
+  for (int c = 0; c < Sh::kCols; ++c) acc[c][0] = f32x16{};
+  const uint32_t k_at = n32 * Sh::kRow + 16 * (half ^ prefill_swizzle(Sh::kSlots, n32));
+  const uint32_t v_at = (4 * half * Sh::kRow + 16 * (n32 >> 2) + 4 * (n32 & 3)) ^ (32 * half);
+  // V[token 32 tb + 8 (e / 4) + 4 half + e % 4][32 c + n32].
+  auto read_v = [&](uint32_t at, int tb, int e, int c) {
+    const int row = 32 * tb + 8 * (e / 4) + e % 4;
+    return tile_lds_read<float>((at + v_at + row * Sh::kRow) ^ (128 * c) ^ (16 * (4 * (e % 4) + ((e / 4) & 1))));
+  };
+  __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0): no register load is pending in the loop
+  bool found = false;
+#pragma unroll 1
+  for (int i = 0; i < x.tiles; ++i) {
+    // The tile has arrived, and every wave is done with the one before it.
+    tile_barrier_loads<0>();
+    const int first = prefill_first<TT>(x, i), last = first + TT - 1;
+    if (i + 1 < x.tiles) load_tile(i + 1);
+    char* tile = smem + (i & 1) * 2 * Sh::kTile;
+    const uint32_t at = lds0 + (i & 1) * 2 * Sh::kTile, vt = at + Sh::kTile;
+    // As in the 16-bit kernel.
+    if (!prefill_sees_all(p, first, last, x.p_min, x.p_max)) {
+      found |= prefill_drop_bad<QD_DTYPE_F32, Sh::kTile / 16, 64 * NW>(tile + Sh::kTile, tid);
+      tile_barrier();
+    }
+    const bool none = wave_row >= x.rows || first > w_max || (p.window > 0 && last <= w_min - p.window && first >= p.sinks);
+    if (none) continue;
+    f32x16 s[TB];
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb) s[tb] = f32x16{};
+#pragma unroll
+    for (int st = 0; st < Sh::kSteps; ++st)
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+        s[tb] = PrefillMma<QD_DTYPE_F32>::mma(tile_lds_read<u32x4>((at + k_at + 32 * tb * Sh::kRow) ^ (32 * st)), qf[0][st], s[tb]);
+    if (!prefill_sees_all(p, first, last, w_min, w_max)) {
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb) {
+        const PrefillView sees = prefill_view(p, place[0], first + 32 * tb + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[tb][e] = sees(8 * (e / 4) + e % 4) ? s[tb][e] : -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][e]);
+    // The reference maximum moves when a score exceeds it by 2^kLazy.
+    if (__ballot(mx * p.sl2 > m + kLazy)) {
+      const float mn = fmaxf(m, prefill_max_halves(mx) * p.sl2);
+      const float alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      l[0] *= alpha;
+#pragma unroll
+      for (int c = 0; c < Sh::kCols; ++c) acc[c][0] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[tb][e] = fast_exp2(fmaf(s[tb][e], p.sl2, ref));
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) l[0] += (s[tb][e] + s[tb][e + 1]) + (s[tb][e + 2] + s[tb][e + 3]);
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int c = 0; c < Sh::kCols; ++c)
+          acc[c][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(read_v(vt, tb, e, c), s[tb][e], acc[c][0], 0, 0, 0);
+  }
+  tile_barrier();
+  if (tid == 0) *word = 0;
+  tile_barrier();
+  if (found) *word = 1;
+  tile_barrier();
+  if (__builtin_amdgcn_readfirstlane(*word) != 0) {
+#pragma unroll 1
+    for (int i = 0; i < x.tiles; ++i) {
+      const int first = prefill_first<TT>(x, i);
+      if (prefill_sees_all(p, first, first + TT - 1, x.p_min, x.p_max)) continue;
+      tile_barrier();
+      load(1, first, 0);
+      tile_barrier_loads<0>();
+      prefill_to_flags<QD_DTYPE_F32, Sh::kTile / 16, 64 * NW>(smem, tid);
+      tile_barrier();
+#pragma unroll 1
+      for (int tb = 0; tb < TB; ++tb) {
+        const PrefillView sees = prefill_view(p, place[0], first + 32 * tb + 4 * half);
+#pragma unroll
+        for (int c = 0; c < Sh::kCols; ++c) {
+          f32x16 seen = f32x16{};
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            seen = __builtin_amdgcn_mfma_f32_32x32x2f32(read_v(lds0 + 32 * tb * Sh::kRow, 0, e, c),
+                                                        sees(8 * (e / 4) + e % 4) ? 1.f : 0.f, seen, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c][0][e] = prefill_add_bad(acc[c][0][e], seen[e]);
+        }
+      }
+    }
+  }
+  prefill_store<QD_DTYPE_F32, DP, 1>(p, x, wave_row, acc, l);
+}
+
 template <int DT, int DP, int NB, int NW>
 hipError_t prefill_launch(const PrefillParams& p, uint32_t grid, hipStream_t st) {
   using Sh = PrefillShape<DT, DP, NB, NW>;
-  void (*fn)(PrefillParams) = prefill_mfma_kernel<DT, DP, NB, NW>;
+  void (*fn)(PrefillParams);
+  if constexpr (DT == QD_DTYPE_F32)
+    fn = prefill_f32_kernel<DP, NW>;
+  else
+    fn = prefill_pipe_kernel<DT, DP, NB, NW>;
   static std::atomic<uint64_t> allowed{0};  // devices on which more than 64 KB of LDS were asked for
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
