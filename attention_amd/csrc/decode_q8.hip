@@ -35,8 +35,13 @@ struct Q8Params {
   int64_t num_blocks;
   int B, Hq, Hkv, D, P, maxP, G;
   int32_t capacity;
-  int splits;
-  float sl2;  // scale * log2(e)
+  int splits;                    // VALU kernel
+  float sl2;                     // scale * log2(e)
+  // Matrix-core kernel.
+  int32_t* meta;                 // {first workgroup, workgroups} per item
+  int chunks, per;               // virtual kv-heads per kv-head and their q-heads (16 at most)
+  int hw, groups;                // virtual heads of a workgroup, workgroups that share a sequence's tokens
+  int W;                         // workgroups of a balanced launch; 0: one per item
 };
 
 __device__ __forceinline__ int q8_len(const Q8Params& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
@@ -160,6 +165,522 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(Q8Params p) {
   static_cast<typename E::S*>(p.out)[row * p.D + d] = E::from_f(sum > 0.f || sum != sum ? a / sum : 0.f);
 }
 
+// ----------------------------------------------------------------------------
+// The matrix-core kernel
+// ----------------------------------------------------------------------------
+//
+// A wave serves up to 16 q-heads of a kv-head (a virtual kv-head) over 32 tokens
+// at a time, straight from registers:
+//   scores   S^T = K Q^T, 16x16x32 in fp16: a lane's 16 bytes of a K row become
+//            operands of two products as they lie (the order of the head's
+//            elements is the queries' too)
+//   softmax  per lane; a token's weight is p = 2^(s - m) and goes into the values'
+//            product as p s_v, whose running reference m is that of s + log2 |s_v|:
+//            whatever the pages' scales, the largest p s_v of a row is near 2^kShift
+//            and fp16 holds the rest as far below it as fp16 goes.
+//   output   O^T += V^T (p s_v)^T, 16x16x32 in fp16: a lane reads E = DP / 16
+//            neighbouring elements of 8 tokens' V rows and exchanges bytes
+//            between token pairs in registers.
+// Elements of both types are exact in fp16 (4 and 8 significant bits within 2^-9
+// .. 448), and so are 16-bit queries, bf16 ones times a power of two that puts the
+// largest of a head just inside fp16's range: 2^-24 of 2^14 is the least that
+// they keep.  Weights are rounded to nearest once, 2^-12 on average.
+//
+// Half the bytes of 16-bit caches come in, and HBM should bound the kernel still:
+// per 32 tokens x 128 a wave moves 8 KB and issues about 200 (e4m3) or 300 (int8)
+// vector instructions, where the SIMD has 2500 cycles at 8 TB/s.
+//
+// Up to four waves of a workgroup take neighbouring virtual heads at the same
+// tokens (whole rows of memory), or, with fewer heads, neighbouring 32 tokens.
+
+constexpr float kQ8Shift = 7.f, kQ8Lazy = 8.f;
+// Balanced launches: what an item's start costs, in tiles, and the least cost of a
+// workgroup's range.
+constexpr int kQ8ItemCost = 2;
+constexpr int kQ8MinCost = 2;
+// Sequences whose prefix of costs fits the kernel's LDS.
+constexpr int kQ8MaxBalanced = 1024;
+
+__host__ __device__ constexpr int q8_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+__device__ __forceinline__ float q8_max_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float q8_sum_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// fp16 pairs (0, 1) and (2, 3) of a word's elements.
+template <int KIND>
+__device__ __forceinline__ u32x2 q8_unpack(uint32_t w) {
+  if constexpr (KIND == QD_DTYPE_E4M3) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true))};
+  } else {
+    // x + 128 as the low byte of 0x6400 is 1024 + 128 + x in fp16.
+    const uint32_t y = w ^ 0x80808080u;
+    const f16x2 off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, y, 0x04010400u)) + off,
+                b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, y, 0x04030402u)) + off;
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+  }
+}
+
+// Element e of words a and b as an fp16 pair, for e = 0 .. 3.
+template <int KIND>
+__device__ __forceinline__ void q8_pairs(uint32_t a, uint32_t b, uint32_t (&out)[4]) {
+  if constexpr (KIND == QD_DTYPE_E4M3) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u), hi = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const u32x2 x = q8_unpack<KIND>(lo), y = q8_unpack<KIND>(hi);
+    out[0] = x[0];
+    out[1] = x[1];
+    out[2] = y[0];
+    out[3] = y[1];
+  } else {
+    const f16x2 off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    const uint32_t w[4] = {__builtin_amdgcn_perm(b, a, 0x0C040C00u), __builtin_amdgcn_perm(b, a, 0x0C050C01u),
+                           __builtin_amdgcn_perm(b, a, 0x0C060C02u), __builtin_amdgcn_perm(b, a, 0x0C070C03u)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out[e] = __builtin_bit_cast(uint32_t, static_cast<f16x2>(__builtin_bit_cast(f16x2, w[e] ^ 0x64806480u) + off));
+  }
+}
+
+template <int DP>
+struct Q8Shape {
+  static constexpr int E = DP / 16;       // V elements of a lane per token
+  static constexpr int kPieces = DP / 64; // 16-byte pieces of a K row per lane
+  static constexpr int kFrags = DP / 32;  // operands of the queries
+  static constexpr int kLds = 4 * E * 1024 + 4 * 16 * 8;  // parts of waves that share heads, {m, l} of their rows
+};
+
+template <int DT, int KIND, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Params p) {
+  using Sh = Q8Shape<DP>;
+  using Ops = MfmaOps<QD_DTYPE_F16>;
+  constexpr int E = Sh::E;
+  extern __shared__ __align__(16) char smem[];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tw_count = 4 / p.hw;              // waves along the tokens
+  const int wh = wv % p.hw, tw = wv / p.hw;
+  const int vheads = p.Hkv * p.chunks;
+  const int64_t row_bytes = static_cast<int64_t>(p.Hkv) * p.D;
+
+  auto process = [&](int b, int hg, int len, int t0, int t1, bool whole, int64_t slot) {
+    const int v = hg * p.hw + wh;  // below vheads: hw divides it
+    const int h = v / p.chunks, g0 = (v - h * p.chunks) * p.per;
+    const int heads = min(p.per, p.G - g0);
+    const bool real = r16 < heads;
+    const int64_t q_row = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G + g0 + (real ? r16 : 0);
+    // Blocks of 16 tokens of this wave's tiles, 64 at a time: lane i holds the
+    // page of block 2 (tile of pair i / 2) + i % 2 and its scales.
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.maxP;
+    const int last_block = (len - 1) >> 4;  // len > 0
+    int64_t at_lane = 0;                    // byte of the block's first row in the pool
+    float ks_lane = 0.f, vs_lane = 0.f, lv_lane = 0.f;
+    auto window = [&](int tile) {
+      const int64_t want = 2 * ((static_cast<int64_t>(tile) + (lane >> 1)) * tw_count + tw) + (lane & 1);
+      const int tok = static_cast<int>(min(want, static_cast<int64_t>(last_block))) * 16;
+      const int page = tok / p.P;
+      const int64_t id = table[page];
+      const int64_t phys = min(max(id, int64_t{0}), p.num_blocks - 1);
+      at_lane = (phys * p.P + (tok - page * p.P)) * row_bytes + static_cast<int64_t>(h) * p.D;
+      ks_lane = p.ks[phys * p.Hkv + h] * p.sl2;
+      vs_lane = p.vs[phys * p.Hkv + h];
+      lv_lane = __builtin_amdgcn_logf(fmaxf(fabsf(vs_lane), 0x1p-100f));
+    };
+    window(t0);
+
+    struct Raw {
+      u32x4 k[2][Sh::kPieces];
+      uint32_t v[2][4][E / 4];
+    };
+    const uint32_t k_off = r16 * static_cast<uint32_t>(row_bytes) + 16 * g4;
+    const uint32_t v_off = 4 * g4 * static_cast<uint32_t>(row_bytes) + E * r16;
+    const bool v_in = E * r16 < p.D;
+    auto load = [&](Raw& x, int i) {  // tile i of the window
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+        const int64_t at = readlane_i64(at_lane, 2 * i + tb);
+        const char* k = reinterpret_cast<const char*>(p.k) + at;
+        const char* v = reinterpret_cast<const char*>(p.v) + at;
+#pragma unroll
+        for (int j = 0; j < Sh::kPieces; ++j) {
+          x.k[tb][j] = u32x4{0u, 0u, 0u, 0u};
+          if (DP == p.D || 64 * j + 16 * g4 < p.D) x.k[tb][j] = stream_load16(k + k_off + 64 * j);
+        }
+#pragma unroll
+        for (int i2 = 0; i2 < 4; ++i2) {
+          const char* src = v + v_off + i2 * row_bytes;
+#pragma unroll
+          for (int e = 0; e < E / 4; ++e) x.v[tb][i2][e] = 0;
+          if (DP == p.D || v_in) {
+            if constexpr (E == 4) {
+              x.v[tb][i2][0] = stream_load4(src);
+            } else if constexpr (E == 8) {
+              const u32x2 y = stream_load8(src);
+              x.v[tb][i2][0] = y[0];
+              x.v[tb][i2][1] = y[1];
+            } else {
+              const u32x4 y = stream_load16(src);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x.v[tb][i2][e] = y[e];
+            }
+          }
+        }
+      }
+    };
+    Raw raw[2];
+    int base = t0;  // the window's first tile
+    if (t0 < t1) load(raw[0], 0);
+
+    // Queries: operand 2 j + u holds elements 64 j + 16 g4 + 8 u .. of this
+    // lane's head.
+    u32x4 qf[Sh::kFrags];
+    float q_inv = 1.f;
+    {
+      const char* src = static_cast<const char*>(p.q) + q_row * p.D * 2;
+#pragma unroll
+      for (int f = 0; f < Sh::kFrags; ++f) {
+        const int d = 64 * (f >> 1) + 16 * g4 + 8 * (f & 1);
+        qf[f] = real && d < p.D ? *reinterpret_cast<const u32x4*>(src + 2 * d) : u32x4{0u, 0u, 0u, 0u};
+      }
+      if constexpr (DT == QD_DTYPE_BF16) {
+        float mx = 0.f;
+#pragma unroll
+        for (int f = 0; f < Sh::kFrags; ++f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x2 x = MfmaOps<QD_DTYPE_BF16>::unpack2(qf[f][i]);
+            mx = fmaxf(mx, fmaxf(fabsf(x[0]), fabsf(x[1])));
+          }
+        mx = q8_max_groups(mx);
+        const int e = static_cast<int>(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= mx
+        const int up = mx > 0.f && e < 255 ? min(max(14 - (e - 127), -120), 120) : 0;
+        const float mul = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        q_inv = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+        for (int f = 0; f < Sh::kFrags; ++f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x2 x = MfmaOps<QD_DTYPE_BF16>::unpack2(qf[f][i]);
+            qf[f][i] = Ops::pack2(x[0] * mul, x[1] * mul);
+          }
+      }
+    }
+    f32x4 acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    auto compute = [&](Raw& x, int i, int tile) {
+      const int first = (tile * tw_count + tw) * 32;
+      f32x4 s[2];
+      float mx = -INFINITY, vs[2], ksc[2];
+      const bool cut = first + 32 > len;
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+        s[tb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < Sh::kPieces; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 a = q8_unpack<KIND>(x.k[tb][j][2 * u]), c = q8_unpack<KIND>(x.k[tb][j][2 * u + 1]);
+            s[tb] = Ops::mma32(u32x4{a[0], a[1], c[0], c[1]}, qf[2 * j + u], s[tb]);
+          }
+        vs[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_lane), 2 * i + tb));
+        ksc[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), 2 * i + tb)) * q_inv;
+        const float lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lv_lane), 2 * i + tb));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[tb][e] *= ksc[tb];
+        if (cut) {
+          // Behind the last token: no weight, and no value (a NaN x 0).
+          const int left = len - first - 16 * tb - 4 * g4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[tb][e] = e < left ? s[tb][e] : -INFINITY;
+#pragma unroll
+            for (int w = 0; w < E / 4; ++w) x.v[tb][e][w] = e < left ? x.v[tb][e][w] : 0u;
+          }
+        }
+        mx = fmaxf(mx, fmaxf(fmaxf(s[tb][0], s[tb][1]), fmaxf(s[tb][2], s[tb][3])) + lv);
+      }
+      if (__ballot(mx > m + kQ8Lazy)) {
+        const float mn = fmaxf(m, q8_max_groups(mx));
+        const float alpha = mn == m ? 1.f : fast_exp2(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= alpha;
+      }
+      const float ref = m == -INFINITY ? kQ8Shift : kQ8Shift - m;
+      u32x4 w;
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[tb][e] = fast_exp2(s[tb][e] + ref);
+        l += (s[tb][0] + s[tb][1]) + (s[tb][2] + s[tb][3]);
+        w[2 * tb] = Ops::pack2(s[tb][0] * vs[tb], s[tb][1] * vs[tb]);
+        w[2 * tb + 1] = Ops::pack2(s[tb][2] * vs[tb], s[tb][3] * vs[tb]);
+      }
+#pragma unroll
+      for (int word = 0; word < E / 4; ++word) {
+        uint32_t a[4][4];  // token pair, element
+#pragma unroll
+        for (int pair = 0; pair < 4; ++pair)
+          q8_pairs<KIND>(x.v[pair >> 1][2 * (pair & 1)][word], x.v[pair >> 1][2 * (pair & 1) + 1][word], a[pair]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[4 * word + e] = Ops::mma32(u32x4{a[0][e], a[1][e], a[2][e], a[3][e]}, w, acc[4 * word + e]);
+      }
+    };
+    for (int tile = t0; tile < t1; tile += 2) {
+      // 32 tiles of a window: both halves of the loop stay within it (its first
+      // tile is a multiple of two from t0).
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int now = tile + half;
+        if (now >= t1) break;
+        const int i = now - base;
+        const bool more = now + 1 < t1, over = i == 31;
+        if (more && !over) load(raw[half ^ 1], i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(raw[half], i, now);
+        if (more && over) {
+          base = now + 1;
+          window(base);
+          load(raw[half ^ 1], 0);
+        }
+      }
+    }
+
+    float sum = q8_sum_groups(l);
+    if (tw_count > 1) {
+      // Waves of the same heads: each leaves its part in LDS, the first of them
+      // takes them up.
+      __syncthreads();
+      f32x2* stats = reinterpret_cast<f32x2*>(smem + 4 * E * 1024);
+      f32x4* parts = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+      for (int e = 0; e < E; ++e) parts[(wv * E + e) * 64 + lane] = acc[e];
+      if (g4 == 0) stats[wv * 16 + r16] = f32x2{m, sum};
+      __syncthreads();
+      if (tw == 0) {
+        float most = -INFINITY;
+        for (int w = 0; w < tw_count; ++w) most = fmaxf(most, stats[(w * p.hw + wh) * 16 + r16][0]);
+        const float ref = most == -INFINITY ? 0.f : most;
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < tw_count; ++w) {
+          const f32x2 ml = stats[(w * p.hw + wh) * 16 + r16];
+          const float f = fast_exp2(ml[0] - ref);
+          sum += f * ml[1];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += f * parts[((w * p.hw + wh) * E + e) * 64 + lane];
+        }
+        m = most;
+      }
+      __syncthreads();
+      if (tw != 0) return;
+    }
+    if (!real) return;
+    const bool has = sum > 0.f || sum != sum;
+    if (whole) {
+      const float inv = has ? 1.f / sum : 0.f;
+      char* to = static_cast<char*>(p.out) + q_row * p.D * 2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = E * (4 * g4 + i);
+        if (d >= p.D) continue;
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = has ? acc[e][i] * inv : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<u32x2*>(to + 2 * (d + e)) =
+              u32x2{MfmaOps<DT>::pack2(y[e], y[e + 1]), MfmaOps<DT>::pack2(y[e + 2], y[e + 3])};
+      }
+    } else {
+      float* part = p.part + (slot * p.hw * 16 + wh * 16 + r16) * (p.D + 4);
+      if (g4 == 0) *reinterpret_cast<f32x2*>(part) = has ? f32x2{m, sum} : f32x2{-INFINITY, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = E * (4 * g4 + i);
+        if (d >= p.D) continue;
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<f32x4*>(part + 4 + d + e) =
+              has ? f32x4{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]} : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  };
+
+  const int tile_tokens = 32 * tw_count;
+  auto zero_rows = [&](int b, int hg) {  // a sequence without tokens
+    const int first = hg * p.hw;
+    for (int i = tid; i < p.hw * p.per * p.D; i += 256) {
+      const int v = first + i / (p.per * p.D), x = i % (p.per * p.D);
+      const int h = v / p.chunks, g = (v % p.chunks) * p.per + x / p.D;
+      if (v < vheads && g < p.G)
+        static_cast<uint16_t*>(p.out)[(static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.D + x % p.D] = 0;
+    }
+  };
+  if (p.W == 0) {
+    const int b = static_cast<int>(blockIdx.x) / p.groups, hg = static_cast<int>(blockIdx.x) % p.groups;
+    const int len = q8_len(p, b);
+    if (len == 0)
+      zero_rows(b, hg);
+    else
+      process(b, hg, len, 0, (len + tile_tokens - 1) / tile_tokens, true, 0);
+    return;
+  }
+  // Balanced: the costs of all items in a row (below 2^31: the host sees to it),
+  // cut into equal ranges.
+  int32_t* incl = reinterpret_cast<int32_t*>(smem + (tw_count > 1 ? Sh::kLds : 0));
+  auto cost_of = [&](int len) { return len > 0 ? ((len + tile_tokens - 1) / tile_tokens + kQ8ItemCost) * p.groups : 0; };
+  for (int i = tid; i < p.B; i += 256) incl[i] = cost_of(q8_len(p, i));
+  __syncthreads();
+  if (wv == 0) {
+    int carry = 0;
+    for (int from = 0; from < p.B; from += 64) {
+      const int i = from + lane;
+      int x = i < p.B ? incl[i] : 0;
+      x = dpp_add_i32<0x111, 0xF>(x);  // row_shr:1
+      x = dpp_add_i32<0x112, 0xF>(x);  // row_shr:2
+      x = dpp_add_i32<0x114, 0xF>(x);  // row_shr:4
+      x = dpp_add_i32<0x118, 0xF>(x);  // row_shr:8
+      x = dpp_add_i32<0x142, 0xA>(x);  // row_bcast:15
+      x = dpp_add_i32<0x143, 0xC>(x);  // row_bcast:31
+      x += carry;
+      if (i < p.B) incl[i] = x;
+      carry = __builtin_amdgcn_readlane(x, 63);
+    }
+  }
+  __syncthreads();
+  const int total = __builtin_amdgcn_readfirstlane(incl[p.B - 1]);
+  const int used = min(p.W, max(1, total / kQ8MinCost));
+  const int w = static_cast<int>(blockIdx.x);
+  if (w >= used) return;
+  // a n / d below 2^31; a n is below 2^42, so that the rounded quotient of doubles
+  // is never on the wrong side of an integer.
+  auto part_of = [](int a, int n, int d) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(a) * n / d));
+  };
+  int pos = part_of(w, total, used);
+  const int end = part_of(w + 1, total, used);
+  int lo = 0, hi = p.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+  }
+  int b = __builtin_amdgcn_readfirstlane(lo);
+  while (pos < end) {
+    while (__builtin_amdgcn_readfirstlane(incl[b]) <= pos) ++b;  // pos < total: ends
+    const int before = b > 0 ? __builtin_amdgcn_readfirstlane(incl[b - 1]) : 0;
+    const int cost = (__builtin_amdgcn_readfirstlane(incl[b]) - before) / p.groups;
+    const int hg = (pos - before) / cost, off = pos - before - hg * cost;
+    const int stop = min(cost, off + (end - pos));
+    const int t0 = max(0, off - kQ8ItemCost), t1 = max(0, stop - kQ8ItemCost), tiles = cost - kQ8ItemCost;
+    if (t1 > t0) {
+      if (t0 == 0 && tid == 0) {
+        const int x = before + hg * cost + cost - 1;  // the item's last tile
+        int last = part_of(x, used, total);
+        while (last + 1 < used && part_of(last + 1, total, used) <= x) ++last;
+        int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * p.groups + hg);
+        meta[0] = w;
+        meta[1] = last - w + 1;
+      }
+      process(b, hg, q8_len(p, b), t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
+    }
+    pos += stop - off;
+  }
+}
+
+// Log-sum-exp merge of the items that a balanced launch split, and the rows of
+// sequences without tokens: a wave per row, LANES lanes stride its columns four at
+// a time, the others its partials.
+// grid (items, ceil(hw per / 4)), block 256.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
+  constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, TEAMS = 64 / LANES, STEP = 4 * LANES;
+  const int item = blockIdx.x, b = item / p.groups, hg = item % p.groups;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int row = 4 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x >> 6);
+  if (row >= p.hw * p.per) return;
+  const int wh = row / p.per, n = row - wh * p.per;
+  const int v = hg * p.hw + wh, h = v / p.chunks, g = (v - h * p.chunks) * p.per + n;
+  if (g >= p.G) return;
+  const bool empty = q8_len(p, b) == 0;
+  const int first = empty ? 0 : p.meta[2 * static_cast<int64_t>(item)];
+  const int count = empty ? 0 : p.meta[2 * static_cast<int64_t>(item) + 1];
+  if (count == 1) return;
+  const int team = lane / LANES, l = lane % LANES;
+  const int64_t slot_floats = static_cast<int64_t>(p.hw) * 16 * (p.D + 4);
+  auto part = [&](int s) {
+    return p.part + (2 * static_cast<int64_t>(first + s) + (s == 0 ? 1 : 0)) * slot_floats + (wh * 16 + n) * (p.D + 4);
+  };
+  char* out = static_cast<char*>(p.out) + (static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G + g) * p.D * 2;
+  for (int d0 = 0; d0 < p.D; d0 += STEP) {
+    const int d = d0 + 4 * l;
+    float mx = -INFINITY, sum = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    // Four partials at a time, statistics and values in flight together.
+    for (int s0 = 4 * team; s0 < count; s0 += 4 * TEAMS) {
+      f32x2 ml[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* src = part(min(s0 + i, count - 1));
+        ml[i] = *reinterpret_cast<const f32x2*>(src);
+        x[i] = d < p.D ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      float most = mx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, ml[i][0]);
+      const float ref = most == -INFINITY ? 0.f : most;
+      const float old = fast_exp2(mx - ref);
+      sum *= old;
+      a *= old;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s0 + i >= count) continue;
+        const float f = fast_exp2(ml[i][0] - ref);
+        sum += f * ml[i][1];
+        a += f * x[i];
+      }
+      mx = most;
+    }
+#pragma unroll
+    for (int off = LANES; off < 64; off <<= 1) {
+      const float om = __shfl_xor(mx, off), os = __shfl_xor(sum, off);
+      f32x4 oa;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) oa[i] = __shfl_xor(a[i], off);
+      const float most = fmaxf(mx, om), ref = most == -INFINITY ? 0.f : most;
+      const float f = fast_exp2(mx - ref), of = fast_exp2(om - ref);
+      sum = f * sum + of * os;
+      a = f * a + of * oa;
+      mx = most;
+    }
+    if (team == 0 && d < p.D) {
+      const bool has = sum > 0.f || sum != sum;
+      const float inv = has ? 1.f / sum : 0.f;
+      if (!has) a = f32x4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<u32x2*>(out + 2 * d) =
+          u32x2{MfmaOps<DT>::pack2(a[0] * inv, a[1] * inv), MfmaOps<DT>::pack2(a[2] * inv, a[3] * inv)};
+    }
+  }
+}
+
 int q8_fail(char* msg, size_t cap, const char* text) {
   qd_set_last_error(QD_ERR_INVALID_VALUE, text);
   if (msg && cap) {
@@ -189,16 +710,94 @@ int generic_splits(int batch, int q_heads, int64_t capacity) {
   return static_cast<int>(std::max<int64_t>(1, std::min({want, (capacity + 511) / 512, int64_t{64}})));
 }
 
+int q8_cu_count() {
+  static std::atomic<int> cached[16];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) {
+    (void)hipGetLastError();
+    dev = 0;
+  }
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) {
+    (void)hipGetLastError();
+    return 256;  // no device: MI355X
+  }
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// How a call runs.  All from static shapes and the device: the table's width
+// stands for the longest context.
 struct Q8Plan {
-  int splits;  // VALU kernel
-  size_t bytes;
+  bool mfma;
+  int splits;                            // VALU kernel
+  int chunks, per, hw, groups, W, grid;  // matrix-core kernel
+  size_t meta_bytes, bytes;
 };
 
-Q8Plan q8_plan(int batch, int q_heads, int head_dim, int block_size, int max_pages) {
+Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int head_dim, int block_size, int max_pages, int flags) {
   Q8Plan pl{};
-  pl.splits = generic_splits(batch, q_heads, q8_capacity(block_size, max_pages));
-  if (pl.splits > 1) pl.bytes = sizeof(float) * static_cast<size_t>(batch) * q_heads * pl.splits * (head_dim + 2);
+  const int64_t cap = q8_capacity(block_size, max_pages);
+  // Rows of a block at 32-bit offsets.
+  pl.mfma = head_dim % 16 == 0 && block_size % 16 == 0 && !(flags & QD_FLAG_FORCE_GENERIC) &&
+            static_cast<int64_t>(kv_heads) * head_dim <= INT32_MAX / 32;
+  if (!pl.mfma) {
+    pl.splits = generic_splits(batch, q_heads, cap);
+    if (pl.splits > 1) pl.bytes = sizeof(float) * static_cast<size_t>(batch) * q_heads * pl.splits * (head_dim + 2);
+    return pl;
+  }
+  const int group = q_heads / kv_heads;
+  pl.chunks = (group + 15) / 16;
+  pl.per = (group + pl.chunks - 1) / pl.chunks;
+  pl.chunks = (group + pl.per - 1) / pl.per;
+  const int vheads = kv_heads * pl.chunks;
+  pl.hw = vheads % 4 == 0 ? 4 : vheads % 2 == 0 ? 2 : 1;
+  pl.groups = vheads / pl.hw;
+  const int64_t items = static_cast<int64_t>(batch) * pl.groups;
+  const int tile = 32 * (4 / pl.hw);
+  const int64_t tiles = (cap + tile - 1) / tile;
+  const int64_t resident = static_cast<int64_t>(q8_cu_count()) * (q8_padded(head_dim) == 256 ? 1 : 2);
+  pl.grid = static_cast<int>(items);
+  // One workgroup per item where a range would not be shorter, and where the
+  // items' costs do not fit the kernel's LDS or 31 bits.
+  if (batch > kQ8MaxBalanced || items * (tiles + kQ8ItemCost) > INT32_MAX || tiles <= 2) return pl;
+  pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kQ8ItemCost) / kQ8MinCost)));
+  pl.grid = pl.W;
+  pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;
+  pl.bytes = pl.meta_bytes + sizeof(float) * 2 * static_cast<size_t>(pl.W) * pl.hw * 16 * (head_dim + 4);
   return pl;
+}
+
+template <int DT, int KIND, int DP>
+hipError_t launch_mfma(const Q8Params& p, int grid, hipStream_t st) {
+  const size_t lds = (p.hw < 4 ? Q8Shape<DP>::kLds : 0) + (p.W > 0 ? sizeof(int32_t) * static_cast<size_t>(p.B) : 0);
+  void (*fn)(Q8Params) = q8_mfma_kernel<DT, KIND, DP>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which more than 64 KB of LDS were asked for
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             Q8Shape<DP>::kLds + 4 * kQ8MaxBalanced);
+    if (e != hipSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(256), lds, st, p);
+  if (p.W > 0)
+    hipLaunchKernelGGL((q8_merge_kernel<DT, DP>),
+                       dim3(static_cast<uint32_t>(p.B * p.groups), static_cast<uint32_t>((p.hw * p.per + 3) / 4)), dim3(256),
+                       0, st, p);
+  return hipGetLastError();
+}
+
+template <int DT, int KIND>
+hipError_t launch_padded(const Q8Params& p, int grid, hipStream_t st) {
+  switch (q8_padded(p.D)) {
+    case 64: return launch_mfma<DT, KIND, 64>(p, grid, st);
+    case 128: return launch_mfma<DT, KIND, 128>(p, grid, st);
+    default: return launch_mfma<DT, KIND, 256>(p, grid, st);
+  }
 }
 
 template <int DT>
@@ -272,17 +871,18 @@ int qd_gqa_decode_q8_validate(const qd_tensor_desc* q, const qd_tensor_desc* k_c
 
 size_t qd_gqa_decode_q8_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int block_size,
                                         int max_pages, int dtype, int flags) {
-  (void)flags;
   if (!q8_shape_ok(batch, q_heads, kv_heads, head_dim, block_size, max_pages, dtype) || batch == 0) return 0;
-  return q8_plan(batch, q_heads, head_dim, block_size, max_pages).bytes;
+  // Unaligned tensors take the VALU kernel.
+  return std::max(q8_plan(batch, q_heads, kv_heads, head_dim, block_size, max_pages, flags).bytes,
+                  q8_plan(batch, q_heads, kv_heads, head_dim, block_size, max_pages, QD_FLAG_FORCE_GENERIC).bytes);
 }
 
 int qd_gqa_decode_q8_info(int batch, int q_heads, int kv_heads, int head_dim, int block_size, int max_pages,
                           int dtype, int flags, int* workgroups) {
-  (void)flags;
   if (!q8_shape_ok(batch, q_heads, kv_heads, head_dim, block_size, max_pages, dtype)) return -1;
-  if (workgroups) *workgroups = batch * q_heads * q8_plan(batch, q_heads, head_dim, block_size, max_pages).splits;
-  return QD_Q8_VALU;
+  const Q8Plan pl = q8_plan(batch, q_heads, kv_heads, head_dim, block_size, max_pages, flags);
+  if (workgroups) *workgroups = pl.mfma ? pl.grid : batch * q_heads * pl.splits;
+  return !pl.mfma ? QD_Q8_VALU : pl.W > 0 ? QD_Q8_MFMA_SPLIT : QD_Q8_MFMA;
 }
 
 int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scales,
@@ -290,7 +890,6 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
                      void* workspace, size_t workspace_bytes, int batch, int q_heads, int kv_heads, int head_dim,
                      int block_size, int max_pages, int64_t num_blocks, int dtype, int cache_dtype, float scale,
                      int flags, void* stream) {
-  (void)flags;
   if (!q8_shape_ok(batch, q_heads, kv_heads, head_dim, block_size, max_pages, dtype) || num_blocks <= 0 ||
       num_blocks > INT32_MAX || (cache_dtype != QD_DTYPE_E4M3 && cache_dtype != QD_DTYPE_I8))
     return q8_fail(nullptr, 0, "invalid dimensions");
@@ -298,7 +897,11 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
   if (batch == 0) return QD_OK;
   if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !block_table || !context_lens || !out)
     return q8_fail(nullptr, 0, "null tensor pointer");
-  const Q8Plan pl = q8_plan(batch, q_heads, head_dim, block_size, max_pages);
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+        reinterpret_cast<uintptr_t>(out)) &
+       15u) != 0)
+    flags |= QD_FLAG_FORCE_GENERIC;
+  const Q8Plan pl = q8_plan(batch, q_heads, kv_heads, head_dim, block_size, max_pages, flags);
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return q8_fail(nullptr, 0, "workspace too small or not 16-byte aligned");
   Q8Params p;
@@ -310,7 +913,13 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
   p.table = block_table;
   p.lens = context_lens;
   p.out = out;
-  p.part = static_cast<float*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.meta_bytes);
+  p.meta = static_cast<int32_t*>(workspace);
+  p.chunks = pl.chunks;
+  p.per = pl.per;
+  p.hw = pl.hw;
+  p.groups = pl.groups;
+  p.W = pl.W;
   p.num_blocks = num_blocks;
   p.B = batch;
   p.Hq = q_heads;
@@ -324,11 +933,22 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
   p.sl2 = scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
-  if (dtype == QD_DTYPE_F16)
-    launch_generic<QD_DTYPE_F16>(p, cache_dtype, st);
-  else
-    launch_generic<QD_DTYPE_BF16>(p, cache_dtype, st);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (pl.mfma) {
+    const bool e4m3 = cache_dtype == QD_DTYPE_E4M3;
+    if (dtype == QD_DTYPE_F16)
+      e = e4m3 ? launch_padded<QD_DTYPE_F16, QD_DTYPE_E4M3>(p, pl.grid, st)
+               : launch_padded<QD_DTYPE_F16, QD_DTYPE_I8>(p, pl.grid, st);
+    else
+      e = e4m3 ? launch_padded<QD_DTYPE_BF16, QD_DTYPE_E4M3>(p, pl.grid, st)
+               : launch_padded<QD_DTYPE_BF16, QD_DTYPE_I8>(p, pl.grid, st);
+  } else {
+    if (dtype == QD_DTYPE_F16)
+      launch_generic<QD_DTYPE_F16>(p, cache_dtype, st);
+    else
+      launch_generic<QD_DTYPE_BF16>(p, cache_dtype, st);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) {
     qd_set_last_error(static_cast<int>(e), std::string("gqa_decode_q8 kernel launch failed: ") + hipGetErrorString(e));
     return static_cast<int>(e);
