@@ -136,7 +136,9 @@ PrefillPlan prefill_plan(int batch, int64_t q_tokens, int q_heads, int kv_heads,
   const auto grid_of = [&](int rows) { return (q_tokens * group / rows + batch + 1) * kv_heads; };
   pl.dp = es == 4 ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256)
                   : (head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 ? 192 : 256);
-  const int rows = es == 2 && pl.dp <= 128 && q_tokens * q_heads >= 256 * 256 ? 256 : 128;
+  // 64 rows per wave where the registers hold two such waves per SIMD, and the
+  // rows are there to fill the card: K and V are read from LDS half as often.
+  const int rows = es == 2 && pl.dp == 64 && q_tokens * q_heads >= 256 * 512 ? 256 : 128;
   if (grid_of(rows) > INT32_MAX) return pl;
   pl.mfma = true;
   pl.rows = rows;

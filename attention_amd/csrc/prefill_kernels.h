@@ -133,9 +133,13 @@ struct PrefillItem {
 
 template <int ROWS, int TT>
 __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem& x) {
-  x.h = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.Hkv));
+  // Quotients come from the vector units: back to scalar registers, or all that
+  // follows from them stays with those too.
+  auto scalar = [](int y) { return __builtin_amdgcn_readfirstlane(y); };
+  const int group = scalar(static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.Hkv)));
+  x.h = static_cast<int>(blockIdx.x) - group * p.Hkv;
   // The last rows of a sequence see most: first.
-  const int64_t u = gridDim.x / static_cast<uint32_t>(p.Hkv) - 1 - blockIdx.x / static_cast<uint32_t>(p.Hkv);
+  const int64_t u = scalar(static_cast<int>(gridDim.x / static_cast<uint32_t>(p.Hkv))) - 1 - group;
   int b, q1, k1;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   if (p.B < 64) {
@@ -166,8 +170,8 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   x.rows = min(ROWS, rows_all - x.row0);
   x.nk = tail ? 0 : max(k1 - x.k0, 0);
   x.before = x.nk - (q1 - x.q0);
-  x.p_min = max(x.before + x.row0 / p.G, -1);
-  x.p_max = max(x.before + (x.row0 + x.rows - 1) / p.G, -1);
+  x.p_min = max(x.before + scalar(x.row0 / p.G), -1);
+  x.p_max = max(x.before + scalar((x.row0 + x.rows - 1) / p.G), -1);
   const int end = x.p_max + 1;  // at most nk
   const int lo = p.window > 0 ? max(x.p_min - p.window + 1, 0) : 0;
   x.lo_tile = lo / TT;
@@ -176,9 +180,32 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   return true;
 }
 
+// Position of a row of the workgroup (wave-uniform), or of its last one.
+__device__ __forceinline__ int prefill_place(const PrefillParams& p, const PrefillItem& x, int row) {
+  return max(x.before + __builtin_amdgcn_readfirstlane((x.row0 + min(row, x.rows - 1)) / p.G), -1);
+}
+
 template <int TT>
 __device__ __forceinline__ int prefill_first(const PrefillItem& x, int i) {
   return TT * (i < x.sink_tiles ? i : i - x.sink_tiles + x.lo_tile);
+}
+
+// The places in the list of tiles whose tokens rows at positions lowest .. highest
+// all see: from, .. from + count - 1.  Tiles of the first tokens are not among
+// them.
+struct PrefillWhole {
+  int from;
+  uint32_t count;
+  __device__ __forceinline__ bool operator()(int i) const { return static_cast<uint32_t>(i - from) < count; }
+};
+template <int TT>
+__device__ __forceinline__ PrefillWhole prefill_whole(const PrefillParams& p, const PrefillItem& x, int lowest, int highest) {
+  const int shift = x.sink_tiles - x.lo_tile;
+  const int lo = p.window > 0 && highest >= p.window ? (highest - p.window) / TT + 1 : 0;
+  PrefillWhole w;
+  w.from = __builtin_amdgcn_readfirstlane(max(lo, x.lo_tile) + shift);
+  w.count = __builtin_amdgcn_readfirstlane(max((lowest + 1) / TT + shift - w.from, 0));
+  return w;
 }
 
 // Whether rows at positions lowest .. highest all see tokens first .. last.
@@ -229,18 +256,29 @@ struct PrefillLoads {
     }
     lds_wave = __builtin_amdgcn_readfirstlane(lds + Sh::kLoadRows * wv * Sh::kRow);
   }
-  // Load i of K (which 0) or V (1) of the tile at token `first`; `to`: the
-  // buffer's place in LDS.
-  __device__ __forceinline__ void one(int which, int i, int first, uint32_t to) const {
-    const int64_t from = static_cast<int64_t>(first) * bytes[which];
-    const char* src = base[which] + readlane_i64(from, 0);  // the same in all lanes: scalar registers
-    const uint32_t most = static_cast<uint32_t>(min(nk - 1 - first, Sh::TT - 1)) * bytes[which] + row_bytes - 16;
-    if (row_bytes == Sh::kRow || inside[i])
-      tile_load_lds<false>(src, min(off[which][i], most), lds_wave + to + 1024 * i);
+  // K (which 0) or V (1) of the tile at token `first`, to the buffer at `to` in
+  // LDS.
+  struct Tile {
+    const char* src;
+    uint32_t most, to;
+  };
+  __device__ __forceinline__ Tile tile(int which, int first, uint32_t to) const {
+    return {base[which] + static_cast<int64_t>(first) * bytes[which],
+            static_cast<uint32_t>(min(nk - 1 - first, Sh::TT - 1)) * bytes[which] + row_bytes - 16, lds_wave + to};
+  }
+  __device__ __forceinline__ void one(int which, int i, const Tile& x) const {
+    const uint32_t at = min(off[which][i], x.most);
+    if (row_bytes == Sh::kRow) {
+      tile_load_lds<false>(x.src, at, x.to + 1024 * i);
+    } else if (inside[i]) {
+      asm volatile("; padded rows");  // keeps the two apart: no mask for whole rows
+      tile_load_lds<false>(x.src, at, x.to + 1024 * i);
+    }
   }
   __device__ __forceinline__ void operator()(int which, int first, uint32_t to) const {
+    const Tile x = tile(which, first, to);
 #pragma unroll
-    for (int i = 0; i < Sh::kLoads; ++i) one(which, i, first, to);
+    for (int i = 0; i < Sh::kLoads; ++i) one(which, i, x);
   }
 };
 
@@ -364,7 +402,7 @@ __device__ __forceinline__ void prefill_load_q(const PrefillParams& p, const Pre
 // multiply-add, an exponential that counts as two, halves of a conversion and of
 // a sum), so the matrix cores go on without a pause.
 template <int DT, int DP, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefill_pipe_kernel(PrefillParams p) {
+__global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pipe_kernel(PrefillParams p) {
   using Sh = PrefillShape<DT, DP, NB, NW>;
   static_assert(DT != QD_DTYPE_F32 && Sh::TT == 64, "16-bit types");
   // fp16 weights are multiples of 2^-24 and the largest of a row is at least
@@ -373,7 +411,7 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
   constexpr float kMost = DT == QD_DTYPE_F16 ? 32768.f : 256.f;  // 2^(kShift + kLazy)
   constexpr int kN = Sh::kSteps;      // steps of the scores, and (token 16, column 32) pairs of the output
   constexpr int kCols = Sh::kCols;
-  constexpr int kRing = kN % 4 == 0 ? 4 : 3;  // operands in registers, all but one of them read ahead
+  constexpr int kRing = NB == 2 ? 2 : kN % 4 == 0 ? 4 : 3;  // operands in registers, read ahead
   constexpr int kPairs = 8 * NB;      // packed pairs of weights
   constexpr int kSlots = kN * NB;     // slots of one product each of scores and output
   extern __shared__ __align__(16) char smem[];
@@ -385,8 +423,7 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
   PrefillItem x;
   if (!prefill_item<Sh::kRows, Sh::TT>(p, x)) return;
   const int wave_row = 32 * NB * wv;
-  const int w_min = max(x.before + min(x.row0 + wave_row, x.row0 + x.rows - 1) / p.G, -1);
-  const int w_max = max(x.before + min(x.row0 + wave_row + 32 * NB - 1, x.row0 + x.rows - 1) / p.G, -1);
+  const int w_min = prefill_place(p, x, wave_row), w_max = prefill_place(p, x, wave_row + 32 * NB - 1);
   const uint32_t lds0 = tile_lds_address(smem);
   const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
   auto k_buf = [](int t) { return static_cast<uint32_t>((t & 1) * Sh::kTile); };
@@ -456,10 +493,11 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
   // The scores of the 32 tokens from `at` on in K's buffer, the weights of `cur`,
   // the products of the weights `prev` with those from `at` on in V's.  `midway`
   // runs when the last operands of the step are on their way, and the next step's
-  // first ones, from 32 - `at` on, follow; `aside(i)` runs beside the products i.
+  // first ones, from 32 - `at` on, follow; `aside` runs beside every slot's products.
   auto step = [&](f32x16 (&cur)[NB], f32x16 (&next)[NB], const Weights& prev, Weights& now, auto at, auto&& midway,
                   auto&& aside) {
     float arg[kPairs][2], val[kPairs][2], sum[NB];
+    uint64_t move = 0;  // lanes whose weights outgrow their reference
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) sum[nb] = 0.f;
     // Pair j: elements 2 (j / NB), + 1 of row block j % NB.  The empty statements
@@ -484,8 +522,17 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
       now.w[(j / NB) >> 2][j % NB][(j / NB) & 3] = w;
       sum[j % NB] = sum2(w, sum[j % NB]);
     };
-    // Stages of a pair, a slot apart.
-    auto from = [](int slot) { return slot < 0 ? 0 : slot >= kSlots ? kPairs : slot * kPairs / kSlots; };
+    // Stages of a pair, a slot apart; the last one is done before the last slot, so
+    // that the sums are there at the end.
+    auto from = [](int slot) { return slot < 0 ? 0 : slot >= kSlots - 1 ? kPairs : slot * kPairs / (kSlots - 1); };
+    auto score = [&](int i, int nb) {
+      next[nb] = PrefillMma<DT>::mma(ka[i % kRing], qf[nb][i], i == 0 ? f32x16{} : next[nb]);
+    };
+    // Scores go a slot ahead of the values: what the next step needs first is not
+    // what this one does last.
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) score(0, nb);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < from(2); ++j) scale2(j);
 #pragma unroll
@@ -494,13 +541,20 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
     for (int slot = 0; slot < kSlots; ++slot) {
       const int i = slot / NB, nb = slot % NB;
       if (nb == 0) {
-        const int ahead = i + kRing - 1;
-        if (ahead == kN) midway();
-        const int token = ahead < kN ? at : 32 - at;
-        ka[ahead % kRing] = read_k(token, ahead % kN);
-        va[ahead % kRing] = read_v(token + 16 * (ahead % kN / kCols), ahead % kCols);
+        // The places of K's operand i and V's i - 1 are free.
+        const int v = i + kRing - 1, k = i + kRing;
+        va[v % kRing] = read_v((v < kN ? at : 32 - at) + 16 * (v % kN / kCols), v % kCols);
+        if (k == kN) midway();
+        ka[k % kRing] = read_k(k < kN ? at : 32 - at, k % kN);
       }
-      next[nb] = PrefillMma<DT>::mma(ka[i % kRing], qf[nb][i], i == 0 ? f32x16{} : next[nb]);
+      if (i + 1 < kN) score(i + 1, nb);
+      if (slot == kSlots - 1) {  // NaN sums too
+        bool over = false;
+#pragma unroll
+        for (int x = 0; x < NB; ++x) over |= !(sum[x] <= kMost);
+        move = __ballot(over);
+        asm volatile("" : "+s"(move));
+      }
       acc[i % kCols][nb] = PrefillMma<DT>::mma(va[i % kRing], prev.w[i / kCols][nb], acc[i % kCols][nb]);
 #pragma unroll
       for (int j = from(slot + 2); j < from(slot + 3); ++j) scale2(j);
@@ -508,14 +562,10 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
       for (int j = from(slot + 1); j < from(slot + 2); ++j) exp2(j);
 #pragma unroll
       for (int j = from(slot); j < from(slot + 1); ++j) pack(j);
-      if (nb == 0) aside(i);
+      aside(slot);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // NaN sums too.
-    bool move = false;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) move |= !(sum[nb] <= kMost);
-    if (__ballot(move)) {
+    if (__builtin_expect(move != 0, 0)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         asm volatile("" : "+v"(cur[nb]));  // nothing of this is computed ahead of the branch
@@ -555,6 +605,7 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
     }
   };
 
+  const PrefillWhole whole = prefill_whole<64>(p, x, x.p_min, x.p_max), wave_whole = prefill_whole<64>(p, x, w_min, w_max);
   if (x.tiles > 0) {
     f32x16 s0[NB], s1[NB];
     Weights w0, w1;
@@ -573,18 +624,17 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
       for (int nb = 0; nb < NB; ++nb) s0[nb] = PrefillMma<DT>::mma(a, qf[nb][st], s0[nb]);
     }
 #pragma unroll
-    for (int i = 0; i < kRing - 1; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       ka[i] = read_k(32, i);
-      va[i] = read_v(32 + 16 * (i / kCols), i % kCols);
+      if (i < kRing - 1) va[i] = read_v(32 + 16 * (i / kCols), i % kCols);
     }
     using Lower = std::integral_constant<int, 0>;
     using Upper = std::integral_constant<int, 32>;
     bool found = false;
 #pragma unroll 1
     for (int t = 0; t < x.tiles; ++t) {
-      const int first = prefill_first<64>(x, t);
-      const bool masked = !prefill_sees_all(p, first, first + 63, w_min, w_max);
-      if (masked) hide(s0, first);
+      const bool masked = !wave_whole(t);
+      if (__builtin_expect(masked, 0)) hide(s0, prefill_first<64>(x, t));
       step(
           s0, s1, w1, w0, Upper{},
           [&]() {
@@ -594,25 +644,37 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
             next_buffers();
             // Where only some rows see a token, a weight of 0 would not hide Inf
             // and NaN from the others: they are left out here and added at the end.
-            if (!prefill_sees_all(p, first, first + 63, x.p_min, x.p_max)) {
+            if (__builtin_expect(!whole(t), 0)) {
               found |= prefill_drop_bad<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(t), tid);
               tile_barrier();
             }
           },
           [](int) {});
-      if (masked) hide(s1, first + 32);
+      if (__builtin_expect(masked, 0)) hide(s1, prefill_first<64>(x, t) + 32);
       // After the last tile: scores of no use.
-      const int k_next = prefill_first<64>(x, min(t + 2, x.tiles - 1)), v_next = prefill_first<64>(x, min(t + 1, x.tiles - 1));
+      const bool more_v = t + 1 < x.tiles, more_k = t + 2 < x.tiles;
+      const auto k_next = load.tile(0, prefill_first<64>(x, more_k ? t + 2 : t), k_buf(t));
+      const auto v_next = load.tile(1, prefill_first<64>(x, more_v ? t + 1 : t), v_buf(t + 1));
       step(
           s1, s0, w0, w1, Lower{}, []() {},
-          [&](int i) {
-#pragma unroll
-            for (int j = 2 * Sh::kLoads * i / kN; j < 2 * Sh::kLoads * (i + 1) / kN; ++j) {
+          [&](int slot) {
+            // Where there are two slots per load, every other wave takes the second:
+            // the loads of all at once would wait for each other.
+            constexpr int kAll = 2 * Sh::kLoads;
+            const int begin = slot * kAll / kSlots, end = (slot + 1) * kAll / kSlots;
+            auto issue = [&](int j) {
               if (j < Sh::kLoads) {
-                if (t + 2 < x.tiles) load.one(0, j, k_next, k_buf(t));
+                if (more_k) load.one(0, j, k_next);
               } else {
-                if (t + 1 < x.tiles) load.one(1, j - Sh::kLoads, v_next, v_buf(t + 1));
+                if (more_v) load.one(1, j - Sh::kLoads, v_next);
               }
+            };
+            if constexpr (kSlots % (2 * kAll) == 0) {
+              constexpr int kEvery = kSlots / kAll;
+              if (slot % kEvery < 2 && (wv & 1) == slot % kEvery) issue(slot / kEvery);
+            } else {
+#pragma unroll
+              for (int j = begin; j < end; ++j) issue(j);
             }
           });
     }
@@ -633,8 +695,8 @@ __global__ __launch_bounds__(64 * NW, (NB == 1 && DP <= 128 ? 2 : 1)) void prefi
       if (x.tiles & 1) next_buffers();  // to V's second buffer
 #pragma unroll 1
       for (int t = 0; t < x.tiles; ++t) {
+        if (whole(t)) continue;
         const int first = prefill_first<64>(x, t);
-        if (prefill_sees_all(p, first, first + 63, x.p_min, x.p_max)) continue;
         tile_barrier();
         load(1, first, v_buf(1));
         tile_barrier_loads<0>();
@@ -679,8 +741,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
   PrefillItem x;
   if (!prefill_item<Sh::kRows, TT>(p, x)) return;
   const int wave_row = 32 * wv;
-  const int w_min = max(x.before + min(x.row0 + wave_row, x.row0 + x.rows - 1) / p.G, -1);
-  const int w_max = max(x.before + min(x.row0 + wave_row + 31, x.row0 + x.rows - 1) / p.G, -1);
+  const int w_min = prefill_place(p, x, wave_row), w_max = prefill_place(p, x, wave_row + 31);
   const uint32_t lds0 = tile_lds_address(smem);
   const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
   if (load.row_bytes < Sh::kRow) {  // products run over the slots past the head

@@ -8,8 +8,8 @@ namespace {
 template <int DP>
 hipError_t run(const PrefillParams& p, int rows, uint32_t grid, hipStream_t st) {
   if (rows == 128) return prefill_launch<QD_DTYPE_F16, DP, 1, 4>(p, grid, st);
-  if constexpr (DP <= 128)
-    if (rows == 256) return prefill_launch<QD_DTYPE_F16, DP, 1, 8>(p, grid, st);
+  if constexpr (DP == 64)
+    if (rows == 256) return prefill_launch<QD_DTYPE_F16, DP, 2, 4>(p, grid, st);
   return hipErrorInvalidValue;
 }
 
