@@ -138,7 +138,7 @@ def lib():
         L.qd_gqa_prefill_info.restype = I
         L.qd_gqa_prefill_info.argtypes = [I, I64, I64, I, I, I, I, I] + [ctypes.POINTER(I)] * 2
         L.qd_gqa_prefill_workspace_bytes.restype = ctypes.c_size_t
-        L.qd_gqa_prefill_workspace_bytes.argtypes = [I, I64, I64] + [I] * 6
+        L.qd_gqa_prefill_workspace_bytes.argtypes = [I, I64, I64] + [I] * 7
         L.qd_gqa_prefill.restype = I
         L.qd_gqa_prefill.argtypes = ([V] * 7 + [ctypes.c_size_t, I, I64, I64, I, I, I, I64, I64, I64, I, F, I, I, I, V])
         L.qd_kv_append_q8_validate.restype = I
@@ -473,7 +473,7 @@ def gqa_prefill_info(B, Tq, Tk, Hq, Hkv, D, dtype=2, flags=0):
 def gqa_prefill(q, key, value, cu, cu_k, out, *, scale, window=0, sinks=0, flags=0, workspace=None, stream=None):
     """Calls qd_gqa_prefill on torch device tensors (no validation)."""
     (Tq, Hq, D), (Tk, Hkv, _), B = q.shape, key.shape, cu.numel() - 1
-    n = lib().qd_gqa_prefill_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, DTYPE[q.dtype], window, flags)
+    n = lib().qd_gqa_prefill_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, DTYPE[q.dtype], window, sinks, flags)
     if workspace is None and n:
         workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
     return lib().qd_gqa_prefill(

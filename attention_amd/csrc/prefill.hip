@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "prefill_kernels.h"
@@ -123,11 +124,32 @@ struct PrefillPlan {
   bool mfma;
   int dp;        // padded head_dim
   int rows;      // rows of a workgroup
-  int64_t grid;  // workgroups
+  int64_t grid;  // workgroups, of which `splits` share an item's keys
+  int splits;
+  size_t bytes;
 };
 
-PrefillPlan prefill_plan(int batch, int64_t q_tokens, int q_heads, int kv_heads, int head_dim, int dtype, int flags) {
+int prefill_cu_count() {
+  static std::atomic<int> cached[16];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) {
+    (void)hipGetLastError();
+    dev = 0;
+  }
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) {
+    (void)hipGetLastError();
+    return 256;  // no device: MI355X
+  }
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+PrefillPlan prefill_plan(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads, int head_dim, int dtype,
+                         int window, int sinks, int flags) {
   PrefillPlan pl{};
+  pl.splits = 1;
   pl.rows = 1;
   pl.grid = q_tokens * q_heads;
   const int group = q_heads / kv_heads;
@@ -143,6 +165,17 @@ PrefillPlan prefill_plan(int batch, int64_t q_tokens, int q_heads, int kv_heads,
   pl.mfma = true;
   pl.rows = rows;
   pl.grid = grid_of(rows);
+  if (es == 4) return pl;
+  // Few rows with many keys: the items' keys are split until the card has a
+  // workgroup per CU, as long as each keeps 512 of them on average.
+  int64_t keys = k_tokens / std::max(batch, 1);
+  if (window > 0) keys = std::min(keys, static_cast<int64_t>(window) + sinks + rows / group);
+  const int64_t splits = std::min({prefill_cu_count() / pl.grid, keys / 512, int64_t{64}});
+  if (splits >= 2) {
+    pl.splits = static_cast<int>(splits);
+    pl.grid *= splits;
+    pl.bytes = sizeof(float) * static_cast<size_t>(splits) * q_tokens * q_heads * (head_dim + 4);
+  }
   return pl;
 }
 
@@ -202,24 +235,22 @@ int qd_gqa_prefill_validate(const qd_tensor_desc* q, const qd_tensor_desc* key, 
 int qd_gqa_prefill_info(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads, int head_dim,
                         int dtype, int flags, int* workgroups, int* rows) {
   if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype)) return -1;
-  const PrefillPlan pl = prefill_plan(batch, q_tokens, q_heads, kv_heads, head_dim, dtype, flags);
+  const PrefillPlan pl = prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, 0, 0, flags);
   if (workgroups) *workgroups = static_cast<int>(pl.grid);
   if (rows) *rows = pl.rows;
   return pl.mfma ? QD_PREFILL_MFMA : QD_PREFILL_VALU;
 }
 
 size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads,
-                                      int head_dim, int dtype, int window, int flags) {
-  (void)window, (void)flags;
-  if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype)) return 0;
-  return 0;
+                                      int head_dim, int dtype, int window, int sinks, int flags) {
+  if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype) || window < 0 || sinks < 0) return 0;
+  return prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, window, sinks, flags).bytes;
 }
 
 int qd_gqa_prefill(const void* q, const void* key, const void* value, const int32_t* cu, const int32_t* cu_k,
                    void* out, void* workspace, size_t workspace_bytes, int batch, int64_t q_tokens, int64_t k_tokens,
                    int q_heads, int kv_heads, int head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                    int dtype, float scale, int window, int sinks, int flags, void* stream) {
-  (void)workspace, (void)workspace_bytes;
   if (!prefill_shape_ok(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype) || q_stride < 0 ||
       k_stride < 0 || v_stride < 0 || (!cu_k && k_tokens != q_tokens))
     return prefill_fail(nullptr, 0, "invalid dimensions");
@@ -230,14 +261,17 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
   if (!q || !cu || !out || (k_tokens > 0 && (!key || !value))) return prefill_fail(nullptr, 0, "null tensor pointer");
   const int64_t es = dtype == QD_DTYPE_F32 ? 4 : 2;
   // The matrix-core kernel loads 16 bytes at a time, at 32-bit offsets within a
-  // tile of at most 64 tokens.
+  // tile of at most 256 tokens.
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value) |
         reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(q_stride * es) |
         static_cast<uintptr_t>(k_stride * es) | static_cast<uintptr_t>(v_stride * es)) &
        15u) != 0 ||
-      std::max(k_stride, v_stride) > (int64_t{1} << 24))
+      std::max({q_stride, k_stride, v_stride}) > (int64_t{1} << 22))
     flags |= QD_FLAG_FORCE_GENERIC;
-  const PrefillPlan pl = prefill_plan(batch, q_tokens, q_heads, kv_heads, head_dim, dtype, flags);
+  const PrefillPlan pl =
+      prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, window, sinks, flags);
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+    return prefill_fail(nullptr, 0, "workspace too small or not 16-byte aligned");
   PrefillParams p;
   p.q = q;
   p.k = key;
@@ -258,6 +292,12 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
   p.window = window;
   p.sinks = sinks;
   p.sl2 = scale * kLog2e;
+  p.inv_g = 1.f / static_cast<float>(p.G);
+  p.by_g = prefill_divide_by(static_cast<uint32_t>(p.G));
+  p.by_hkv = prefill_divide_by(static_cast<uint32_t>(kv_heads));
+  p.groups = pl.mfma ? static_cast<int>(pl.grid / pl.splits / kv_heads) : 0;
+  p.splits = pl.splits;
+  p.part = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   hipError_t e = hipSuccess;
@@ -265,7 +305,7 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
     const auto run = dtype == QD_DTYPE_F32   ? qd_prefill_mfma_launch_f32
                      : dtype == QD_DTYPE_F16 ? qd_prefill_mfma_launch_f16
                                              : qd_prefill_mfma_launch_bf16;
-    e = static_cast<hipError_t>(run(p, pl.dp, pl.rows, static_cast<uint32_t>(pl.grid), stream));
+    e = static_cast<hipError_t>(run(p, pl.dp, pl.rows, static_cast<uint32_t>(pl.grid / pl.splits), stream));
   } else {
     switch (dtype) {
       case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;

@@ -15,6 +15,19 @@
 #include "qd_device.h"
 #include "tile_device.h"
 
+// n / d for n < 2^31 as (n m) >> s, on the scalar units: m = ceil(2^s / d) with s =
+// 31 + ceil(log2 d) exceeds 2^s / d by less than 1, and so n m / 2^s exceeds n / d
+// by less than n / 2^s < 1 / d.
+struct PrefillDivide {
+  uint32_t m;
+  int s;
+};
+inline PrefillDivide prefill_divide_by(uint32_t d) {
+  int bits = 0;
+  while ((uint64_t{1} << bits) < d) ++bits;
+  return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + d - 1) / d), 31 + bits};
+}
+
 // Arguments of the kernels, passed between translation units.
 struct PrefillParams {
   const void* q;
@@ -26,7 +39,12 @@ struct PrefillParams {
   int64_t q_stride, k_stride, v_stride;  // elements from token to token
   int B, Tq, Tk, Hq, Hkv, D, G;          // G q-heads per kv-head
   int window, sinks;
-  float sl2;  // scale * log2(e)
+  float sl2;    // scale * log2(e)
+  float inv_g;  // 1 / G
+  PrefillDivide by_g, by_hkv;
+  int groups;   // workgroups per kv-head (and split)
+  int splits;   // workgroups that share an item's tiles; more than 1: partials in `part`
+  float* part;  // [splits][Tq Hq][D + 4]: {m, l, -, -, acc[D]}
 };
 
 // Runs the matrix-core kernel for padded head_dim dp with workgroups of `rows`
@@ -55,7 +73,14 @@ struct PrefillShape {
   static constexpr int kTB = TT / 32;                     // blocks of 32 tokens
   static constexpr int kCols = DP / 32;
   static constexpr int kRows = 32 * NB * NW;
-  static constexpr int kLds = 4 * kTile + 16;
+  // A wave's rows (its queries, later its output) in LDS: over K's and V's second
+  // buffers where both halves of the workgroup fit, else behind all four.
+  static constexpr bool kOver = kRows * kRow == 2 * kTile;
+  __host__ __device__ static constexpr int rows_at(int wv) {
+    return 32 * NB * kRow * wv + (!kOver ? 4 * kTile : 2 * wv < NW ? kTile : 2 * kTile);
+  }
+  static constexpr int kWord = kES == 2 && !kOver ? 4 * kTile + kRows * kRow : 4 * kTile;
+  static constexpr int kLds = kWord + 16;
   static_assert(kLoadRows * kSlots % 64 == 0 && DP % 32 == 0, "waves do not fit the tile");
 };
 
@@ -125,21 +150,42 @@ __device__ __forceinline__ bool prefill_finite(u32x4 x) {
 // K and V share a workgroup's reads of them and the rows of a workgroup span few
 // positions.  Positions below 0 (more queries than keys) see nothing: -1.
 struct PrefillItem {
-  int h, q0, row0, rows;   // rows of the workgroup, of sequence rows from query q0 on
-  int k0, nk, before;      // keys, position of query 0
+  int h, q0, rows;         // rows of the workgroup: from q-head `rest` of query q0 on
+  int rest;
+  int k0, nk, at0;         // keys, position of query q0
   int p_min, p_max;        // positions of the first and the last row
-  int lo_tile, sink_tiles, tiles;  // tiles [0, sink_tiles), then from lo_tile on
+  // Tiles [0, sink_tiles), then from lo_tile on; the workgroup's are `tiles` from
+  // the place `skip` of that list on.
+  int lo_tile, sink_tiles, skip, tiles;
 };
+
+// Query (counted from q0) and q-head of the group of a row.
+struct PrefillRow {
+  int query, g;
+};
+__device__ __forceinline__ PrefillRow prefill_row(const PrefillParams& p, const PrefillItem& x, int row) {
+  const int y = x.rest + row;  // below G + 256
+  PrefillRow r;
+  // y + 1/2 is at least 1/2 away from multiples of G: exact in fp32.
+  r.query = p.G > 4096 ? static_cast<int>(y >= p.G) : static_cast<int>((static_cast<float>(y) + 0.5f) * p.inv_g);
+  r.g = y - r.query * p.G;
+  return r;
+}
+// Position of a row of the workgroup, or of its last one.
+__device__ __forceinline__ int prefill_place(const PrefillParams& p, const PrefillItem& x, int row) {
+  return max(x.at0 + prefill_row(p, x, min(row, x.rows - 1)).query, -1);
+}
 
 template <int ROWS, int TT>
 __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem& x) {
-  // Quotients come from the vector units: back to scalar registers, or all that
-  // follows from them stays with those too.
+  // What comes from the vector units goes back to scalar registers, or all that
+  // follows from it stays with those too.
   auto scalar = [](int y) { return __builtin_amdgcn_readfirstlane(y); };
-  const int group = scalar(static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.Hkv)));
+  auto divide = [](uint32_t n, PrefillDivide d) { return static_cast<int>((static_cast<uint64_t>(n) * d.m) >> d.s); };
+  const int group = divide(blockIdx.x, p.by_hkv);
   x.h = static_cast<int>(blockIdx.x) - group * p.Hkv;
   // The last rows of a sequence see most: first.
-  const int64_t u = scalar(static_cast<int>(gridDim.x / static_cast<uint32_t>(p.Hkv))) - 1 - group;
+  const int64_t u = p.groups - 1 - group;
   int b, q1, k1;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   if (p.B < 64) {
@@ -166,27 +212,35 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   const int rows_all = max(q1 - x.q0, 0) * p.G;  // below 2^31: Tq Hq is
   const int64_t row0 = (u - static_cast<int64_t>(x.q0) * p.G / ROWS - b) * ROWS;
   if (row0 >= rows_all) return false;
-  x.row0 = static_cast<int>(row0);
-  x.rows = min(ROWS, rows_all - x.row0);
+  x.rows = min(ROWS, rows_all - static_cast<int>(row0));
+  const int query0 = divide(static_cast<uint32_t>(row0), p.by_g);
+  x.rest = static_cast<int>(row0) - query0 * p.G;
   x.nk = tail ? 0 : max(k1 - x.k0, 0);
-  x.before = x.nk - (q1 - x.q0);
-  x.p_min = max(x.before + scalar(x.row0 / p.G), -1);
-  x.p_max = max(x.before + scalar((x.row0 + x.rows - 1) / p.G), -1);
+  x.at0 = x.nk - (q1 - x.q0) + query0;
+  x.q0 += query0;
+  x.p_min = max(x.at0, -1);
+  x.p_max = scalar(prefill_place(p, x, ROWS));
   const int end = x.p_max + 1;  // at most nk
   const int lo = p.window > 0 ? max(x.p_min - p.window + 1, 0) : 0;
   x.lo_tile = lo / TT;
   x.sink_tiles = min((min(p.sinks, lo) + TT - 1) / TT, x.lo_tile);
-  x.tiles = end > 0 ? x.sink_tiles + (end + TT - 1) / TT - x.lo_tile : 0;
+  const int all = end > 0 ? x.sink_tiles + (end + TT - 1) / TT - x.lo_tile : 0;
+  x.skip = 0;
+  x.tiles = all;
+  if (p.splits > 1) {
+    // At most 2^25 tiles and 64 splits.
+    const uint32_t n = all, parts = p.splits;
+    x.skip = scalar(static_cast<int>(n * blockIdx.y / parts));
+    x.tiles = scalar(static_cast<int>(n * (blockIdx.y + 1) / parts)) - x.skip;
+  }
+  for (int* y : {&x.q0, &x.rows, &x.rest, &x.k0, &x.nk, &x.at0, &x.p_min, &x.p_max, &x.lo_tile, &x.sink_tiles, &x.skip, &x.tiles})
+    *y = scalar(*y);
   return true;
-}
-
-// Position of a row of the workgroup (wave-uniform), or of its last one.
-__device__ __forceinline__ int prefill_place(const PrefillParams& p, const PrefillItem& x, int row) {
-  return max(x.before + __builtin_amdgcn_readfirstlane((x.row0 + min(row, x.rows - 1)) / p.G), -1);
 }
 
 template <int TT>
 __device__ __forceinline__ int prefill_first(const PrefillItem& x, int i) {
+  i += x.skip;
   return TT * (i < x.sink_tiles ? i : i - x.sink_tiles + x.lo_tile);
 }
 
@@ -200,10 +254,10 @@ struct PrefillWhole {
 };
 template <int TT>
 __device__ __forceinline__ PrefillWhole prefill_whole(const PrefillParams& p, const PrefillItem& x, int lowest, int highest) {
-  const int shift = x.sink_tiles - x.lo_tile;
+  const int shift = x.sink_tiles - x.lo_tile - x.skip;
   const int lo = p.window > 0 && highest >= p.window ? (highest - p.window) / TT + 1 : 0;
   PrefillWhole w;
-  w.from = __builtin_amdgcn_readfirstlane(max(lo, x.lo_tile) + shift);
+  w.from = __builtin_amdgcn_readfirstlane(max(max(lo, x.lo_tile) + shift, 0));
   w.count = __builtin_amdgcn_readfirstlane(max((lowest + 1) / TT + shift - w.from, 0));
   return w;
 }
@@ -229,6 +283,11 @@ __device__ __forceinline__ PrefillView prefill_view(const PrefillParams& p, int 
   return v;
 }
 
+// A wave-uniform pointer, in scalar registers.
+__device__ __forceinline__ const char* prefill_scalar(const char* x) {
+  return reinterpret_cast<const char*>(readlane_i64(static_cast<int64_t>(reinterpret_cast<uintptr_t>(x)), 0));
+}
+
 // Loads of K and V rows into LDS: a wave's rows of a tile, one instruction at a
 // time.  What lies past the last key is taken from the end of its row instead:
 // no query sees it.
@@ -242,8 +301,8 @@ struct PrefillLoads {
   __device__ __forceinline__ PrefillLoads(const PrefillParams& p, const PrefillItem& x, uint32_t lds, int wv, int lane) {
     row_bytes = p.D * Sh::kES;
     nk = x.nk;
-    base[0] = static_cast<const char*>(p.k) + (x.k0 * p.k_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES;
-    base[1] = static_cast<const char*>(p.v) + (x.k0 * p.v_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES;
+    base[0] = prefill_scalar(static_cast<const char*>(p.k) + (x.k0 * p.k_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES);
+    base[1] = prefill_scalar(static_cast<const char*>(p.v) + (x.k0 * p.v_stride + static_cast<int64_t>(x.h) * p.D) * Sh::kES);
     bytes[0] = static_cast<uint32_t>(p.k_stride * Sh::kES);
     bytes[1] = static_cast<uint32_t>(p.v_stride * Sh::kES);
 #pragma unroll
@@ -316,30 +375,41 @@ __device__ __forceinline__ void prefill_to_flags(char* v, int tid) {
 
 // y plus the values that a sum of flags stands for.
 __device__ __forceinline__ float prefill_add_bad(float y, float seen) {
-  if (seen >= kPrefillNan) return NAN;
-  const float minus = floorf(seen / kPrefillMinusInf), plus = seen - minus * kPrefillMinusInf;
-  if (plus > 0.f) y += INFINITY;
-  if (minus > 0.f) y -= INFINITY;
-  return y;
+  const float negative = __builtin_amdgcn_fractf(seen / kPrefillMinusInf) == 0.f && seen < kPrefillNan ? -INFINITY : NAN;
+  return y + (seen >= kPrefillMinusInf ? negative : seen > 0.f ? INFINITY : 0.f);
 }
 
-// out rows of a lane: acc of column block c, element e is column 32 c + 8 (e / 4) +
-// 4 half + e % 4 of row wave_row + 32 nb + lane % 32.
+// out rows of a lane, or their partials: acc of column block c, element e is
+// column 32 c + 8 (e / 4) + 4 half + e % 4 of row wave_row + 32 nb + lane % 32.
 template <int DT, int DP, int NB>
 __device__ __forceinline__ void prefill_store(const PrefillParams& p, const PrefillItem& x, int wave_row,
-                                              const f32x16 (&acc)[DP / 32][NB], const float (&l)[NB]) {
+                                              const f32x16 (&acc)[DP / 32][NB], const float (&m)[NB], const float (&l)[NB]) {
   constexpr int ES = DT == QD_DTYPE_F32 ? 4 : 2;
   const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const float sum = prefill_sum_halves(l[nb]);
     const bool has = sum > 0.f || sum != sum;
-    const float scale = has ? 1.f / sum : 0.f;
     const int rr = wave_row + 32 * nb + (lane & 31);
     if (rr >= x.rows) continue;
-    const int row = x.row0 + rr, query = row / p.G;
-    char* to = static_cast<char*>(p.out) +
-               ((static_cast<int64_t>(x.q0 + query) * p.Hq + static_cast<int64_t>(x.h) * p.G + (row - query * p.G)) * p.D) * ES;
+    const PrefillRow row = prefill_row(p, x, rr);
+    const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
+    if (p.splits > 1) {
+      float* to = p.part + (blockIdx.y * (static_cast<int64_t>(p.Tq) * p.Hq) + at) * (p.D + 4);
+      if (half == 0) *reinterpret_cast<f32x2*>(to) = has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int d = 32 * c + 2 * e + 4 * half;
+          if (d < p.D)
+            *reinterpret_cast<f32x4*>(to + 4 + d) =
+                f32x4{acc[c][nb][e], acc[c][nb][e + 1], acc[c][nb][e + 2], acc[c][nb][e + 3]};
+        }
+      continue;
+    }
+    const float scale = has ? 1.f / sum : 0.f;
+    char* to = static_cast<char*>(p.out) + at * p.D * ES;
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
@@ -349,31 +419,93 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
         f32x4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = has ? acc[c][nb][e + j] * scale : 0.f;
-        if constexpr (DT != QD_DTYPE_F32)
-          *reinterpret_cast<u32x2*>(to + d * ES) = u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
-        else
-          *reinterpret_cast<f32x4*>(to + d * ES) = y;
+        *reinterpret_cast<f32x4*>(to + d * ES) = y;
       }
   }
 }
 
-// Q as the B operand, and the positions of this lane's rows.
-template <typename Sh, int NB>
-__device__ __forceinline__ void prefill_load_q(const PrefillParams& p, const PrefillItem& x, int wave_row, int (&place)[NB],
-                                               u32x4 (&qf)[NB][Sh::kSteps]) {
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  const int row_bytes = p.D * Sh::kES;
+// 16-bit rows: through the wave's place in LDS, so that whole rows are stored (as
+// they lie in registers, a store reaches 16 bytes of 32 rows).
+template <typename Sh, int DT, int DP, int NB>
+__device__ __forceinline__ void prefill_store_rows(const PrefillParams& p, const PrefillItem& x, int wave_row, char* place,
+                                                   const f32x16 (&acc)[DP / 32][NB], const float (&l)[NB]) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5, n32 = lane & 31;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int row = x.row0 + min(wave_row + 32 * nb + (lane & 31), x.rows - 1);
-    const int query = row / p.G;
-    place[nb] = max(x.before + query, -1);
-    const char* src = static_cast<const char*>(p.q) +
-                      ((x.q0 + query) * p.q_stride + (static_cast<int64_t>(x.h) * p.G + (row - query * p.G)) * p.D) * Sh::kES;
+    const float sum = prefill_sum_halves(l[nb]);
+    const bool has = sum > 0.f || sum != sum;
+    const float scale = has ? 1.f / sum : 0.f;
+    char* row = place + (32 * nb + n32) * Sh::kRow;
+    const int swizzle = 16 * prefill_swizzle(Sh::kSlots, n32);
 #pragma unroll
-    for (int st = 0; st < Sh::kSteps; ++st) {
-      const int at = 32 * st + 16 * (lane >> 5);
-      qf[nb][st] = at < row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        f32x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = has ? acc[c][nb][e + j] * scale : 0.f;
+        // Column 32 c + 2 e + 4 half.
+        *reinterpret_cast<u32x2*>(row + ((64 * c + 4 * e) ^ swizzle) + 8 * half) =
+            u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
+      }
+  }
+  const int row_bytes = 2 * p.D;
+#pragma unroll
+  for (int i = 0; i < NB * Sh::kSlots / 2; ++i) {
+    const int r = (64 * i + lane) / Sh::kSlots;
+    const int slot = lane & (Sh::kSlots - 1), col = 16 * (slot ^ prefill_swizzle(Sh::kSlots, r));
+    const u32x4 y = *reinterpret_cast<const u32x4*>(place + r * Sh::kRow + 16 * slot);
+    if (wave_row + r >= x.rows || col >= row_bytes) continue;
+    const PrefillRow row = prefill_row(p, x, wave_row + r);
+    const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
+    *reinterpret_cast<u32x4*>(static_cast<char*>(p.out) + at * row_bytes + col) = y;
+  }
+}
+
+// Log-sum-exp merge of split items: a wave per row, LANES lanes stride its columns
+// four at a time, the others its partials.
+// grid ceil(Tq Hq / 4), block 256.
+template <int DT>
+__global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
+  constexpr int LANES = 16, TEAMS = 4;
+  const int64_t rows = static_cast<int64_t>(p.Tq) * p.Hq;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = static_cast<int>(threadIdx.x) & 63, team = lane / LANES, l = lane % LANES;
+  auto part = [&](int s) { return p.part + (s * rows + row) * (p.D + 4); };
+  for (int d = 4 * l; d < p.D + 4 * l; d += 4 * LANES) {
+    const bool in = d < p.D;
+    float mx = -INFINITY, sum = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int s = team; s < p.splits; s += TEAMS) {
+      const float* src = part(s);
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(src);
+      const f32x4 x = in ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+      const float most = fmaxf(mx, ml[0]), ref = most == -INFINITY ? 0.f : most;
+      const float f = fast_exp2(mx - ref), g = fast_exp2(ml[0] - ref);
+      sum = f * sum + g * ml[1];
+      // A part without weight has no say, whatever it holds.
+      a = ml[0] == -INFINITY ? a : f * a + g * x;
+      mx = most;
+    }
+#pragma unroll
+    for (int off = LANES; off < 64; off <<= 1) {
+      const float om = __shfl_xor(mx, off), os = __shfl_xor(sum, off);
+      f32x4 oa;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) oa[i] = __shfl_xor(a[i], off);
+      const float most = fmaxf(mx, om), ref = most == -INFINITY ? 0.f : most;
+      const float f = fast_exp2(mx - ref), g = fast_exp2(om - ref);
+      sum = f * sum + g * os;
+      a = f * a + g * oa;
+      mx = most;
+    }
+    if (team == 0 && in) {
+      const bool has = sum > 0.f || sum != sum;
+      const float inv = has ? 1.f / sum : 0.f;
+      if (!has) a = f32x4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<u32x2*>(static_cast<char*>(p.out) + (row * p.D + d) * 2) =
+          u32x2{MfmaOps<DT>::pack2(a[0] * inv, a[1] * inv), MfmaOps<DT>::pack2(a[2] * inv, a[3] * inv)};
     }
   }
 }
@@ -415,41 +547,67 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   constexpr int kPairs = 8 * NB;      // packed pairs of weights
   constexpr int kSlots = kN * NB;     // slots of one product each of scores and output
   extern __shared__ __align__(16) char smem[];
-  // K in two buffers, V in two, a word.
-  int* word = reinterpret_cast<int*>(smem + 4 * Sh::kTile);
+  // K in two buffers, V in two, queries and output over or behind them, a word.
+  int* word = reinterpret_cast<int*>(smem + Sh::kWord);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, half = lane >> 5, r16 = lane & 15;
   PrefillItem x;
   if (!prefill_item<Sh::kRows, Sh::TT>(p, x)) return;
   const int wave_row = 32 * NB * wv;
-  const int w_min = prefill_place(p, x, wave_row), w_max = prefill_place(p, x, wave_row + 32 * NB - 1);
   const uint32_t lds0 = tile_lds_address(smem);
   const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
   auto k_buf = [](int t) { return static_cast<uint32_t>((t & 1) * Sh::kTile); };
   auto v_buf = [](int t) { return static_cast<uint32_t>((2 + (t & 1)) * Sh::kTile); };
   if (load.row_bytes < Sh::kRow) {  // products run over the slots past the head
-    for (int i = tid; i < 4 * Sh::kTile / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < Sh::kWord / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     tile_barrier();
   }
-  if (x.tiles > 0) {
-    load(0, prefill_first<64>(x, 0), k_buf(0));
-    load(1, prefill_first<64>(x, 0), v_buf(0));
-  }
-  if (x.tiles > 1) load(0, prefill_first<64>(x, 1), k_buf(1));
-  int place[NB];
-  u32x4 qf[NB][kN];
-  prefill_load_q<Sh, NB>(p, x, wave_row, place, qf);
+  if (tid == 0) *word = 0;
   f32x16 acc[kCols][NB];
   float m[NB], l[NB], ref[NB];
+  auto clear = [&]() {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m[nb] = -INFINITY;
-    ref[nb] = INFINITY;  // the first step finds its maximum
-    l[nb] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = -INFINITY;
+      ref[nb] = INFINITY;  // the first step finds its maximum
+      l[nb] = 0.f;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c][nb] = f32x16{};
+      for (int c = 0; c < kCols; ++c) acc[c][nb] = f32x16{};
+    }
+  };
+  clear();
+  if (x.tiles == 0) {  // the same for all waves
+    if (p.splits > 1)
+      prefill_store<DT, DP, NB>(p, x, wave_row, acc, m, l);
+    else
+      prefill_store_rows<Sh, DT, DP, NB>(p, x, wave_row, smem + Sh::rows_at(wv), acc, l);
+    return;
   }
+  // Each wave's queries go through LDS too: as operands straight from memory they
+  // would come in pieces of 32 bytes.
+  load(0, prefill_first<64>(x, 0), k_buf(0));
+  load(1, prefill_first<64>(x, 0), v_buf(0));
+  {
+    const char* base = prefill_scalar(static_cast<const char*>(p.q) +
+                                      (x.q0 * p.q_stride + static_cast<int64_t>(x.h) * p.G * p.D) * Sh::kES);
+    const uint32_t q_bytes = static_cast<uint32_t>(p.q_stride * Sh::kES);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + Sh::rows_at(wv));
+#pragma unroll
+    for (int i = 0; i < NB * Sh::kSlots / 2; ++i) {
+      const int r = (64 * i + lane) / Sh::kSlots;
+      const uint32_t col = 16 * ((lane & (Sh::kSlots - 1)) ^ prefill_swizzle(Sh::kSlots, r));
+      const PrefillRow row = prefill_row(p, x, min(wave_row + r, x.rows - 1));
+      if (static_cast<int>(col) < load.row_bytes)
+        tile_load_lds<false>(base, row.query * q_bytes + row.g * load.row_bytes + col, to + 1024 * i);
+    }
+  }
+  int place[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) place[nb] = prefill_place(p, x, wave_row + 32 * nb + n32);
+  const int w_min = __builtin_amdgcn_readfirstlane(prefill_place(p, x, wave_row));
+  const int w_max = __builtin_amdgcn_readfirstlane(prefill_place(p, x, wave_row + 32 * NB - 1));
+  const PrefillWhole whole = prefill_whole<64>(p, x, x.p_min, x.p_max), wave_whole = prefill_whole<64>(p, x, w_min, w_max);
   // Operands' places in LDS, in the buffers that the next step reads: step st of
   // a K row, columns 32 c.. of V's token rows 4 half.. and 8 further.
   uint32_t k_at[kN], v_at[kCols][2];
@@ -487,6 +645,22 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   };
   struct Weights {
     u32x4 w[2][NB];  // 16 tokens each
+  };
+  u32x4 qf[NB][kN];
+  __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0)
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int st = 0; st < kN; ++st)
+      qf[nb][st] = tile_lds_read<u32x4>(k_at[st] + Sh::rows_at(wv) + 32 * nb * Sh::kRow);
+
+  // The largest score of a row, or m.
+  auto largest = [&](const f32x16& s, float m) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    return fmaxf(m, prefill_max_halves(mx) * p.sl2);
   };
 
   u32x4 ka[kRing], va[kRing];  // operands read ahead of their products
@@ -569,10 +743,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         asm volatile("" : "+v"(cur[nb]));  // nothing of this is computed ahead of the branch
-        float mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, cur[nb][e]);
-        const float mn = fmaxf(m[nb], prefill_max_halves(mx) * p.sl2);
+        const float mn = largest(cur[nb], m[nb]);
         const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
         m[nb] = mn;
         ref[nb] = mn == -INFINITY ? kShift : kShift - mn;
@@ -595,34 +766,60 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) l[nb] += sum[nb];
   };
+  // An opaque copy: what is derived from it is not computed ahead of the loops and
+  // kept in registers.
+  auto apart = [](int y) {
+    asm volatile("" : "+v"(y));
+    return y;
+  };
   // Hides the scores of 32 tokens from `first` on that rows do not see.
   auto hide = [&](f32x16 (&s)[NB], int first) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const PrefillView sees = prefill_view(p, place[nb], first + 4 * half);
+      const PrefillView sees = prefill_view(p, apart(place[nb]), apart(first + 4 * half));
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[nb][e] = sees(8 * (e / 4) + e % 4) ? s[nb][e] : -INFINITY;
     }
   };
 
-  const PrefillWhole whole = prefill_whole<64>(p, x, x.p_min, x.p_max), wave_whole = prefill_whole<64>(p, x, w_min, w_max);
-  if (x.tiles > 0) {
+  // A value that is not finite reaches rows that do not see it as 0 x NaN.  What
+  // comes out not finite is computed again, with care: where only some rows see a
+  // token, such values are left out (zeros) and joined to the rows that do see
+  // them at the end.
+#pragma unroll 1
+  for (bool careful = false;; careful = true) {
     f32x16 s0[NB], s1[NB];
     Weights w0, w1;
+    // The first tile has arrived, and every wave has its queries.
+    tile_barrier_loads<0>();
+    if (x.tiles > 1) load(0, prefill_first<64>(x, 1), k_buf(1));
     // The first step has no tokens before it: no weights, and values of 0.
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) w1.w[0][nb] = w1.w[1][nb] = u32x4{0u, 0u, 0u, 0u};
-    for (int i = tid; i < Sh::kTile / 32; i += 64 * NW)
+    for (int i = apart(tid); i < Sh::kTile / 32; i += 64 * NW)
       reinterpret_cast<u32x4*>(smem + v_buf(1) + Sh::kTile / 2)[i] = u32x4{0u, 0u, 0u, 0u};
-    tile_barrier_loads<0>();
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) s0[nb] = f32x16{};
+    {
+      u32x4 a[kN < 8 ? kN : 8];
+      constexpr int kFirst = kN < 8 ? kN : 8;  // reads ahead of the first product
 #pragma unroll
-    for (int st = 0; st < kN; ++st) {
-      const u32x4 a = read_k(0, st);
+      for (int st = 0; st < kFirst; ++st) a[st] = read_k(0, st);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s0[nb] = PrefillMma<DT>::mma(a, qf[nb][st], s0[nb]);
+      for (int st = 0; st < kN; ++st) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s0[nb] = PrefillMma<DT>::mma(a[st % kFirst], qf[nb][st], s0[nb]);
+        if (st + kFirst < kN) a[st % kFirst] = read_k(0, st + kFirst);
+      }
     }
+    if (!wave_whole(0)) hide(s0, prefill_first<64>(x, 0));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = largest(s0[nb], -INFINITY);
+      if (m[nb] != -INFINITY) ref[nb] = kShift - m[nb];
+    }
+    tile_barrier();  // the zeros are there
 #pragma unroll
     for (int i = 0; i < kRing; ++i) {
       ka[i] = read_k(32, i);
@@ -630,11 +827,8 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
     }
     using Lower = std::integral_constant<int, 0>;
     using Upper = std::integral_constant<int, 32>;
-    bool found = false;
 #pragma unroll 1
     for (int t = 0; t < x.tiles; ++t) {
-      const bool masked = !wave_whole(t);
-      if (__builtin_expect(masked, 0)) hide(s0, prefill_first<64>(x, t));
       step(
           s0, s1, w1, w0, Upper{},
           [&]() {
@@ -642,15 +836,13 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
             // needs of this K and the V before.
             tile_barrier_loads<0>();
             next_buffers();
-            // Where only some rows see a token, a weight of 0 would not hide Inf
-            // and NaN from the others: they are left out here and added at the end.
-            if (__builtin_expect(!whole(t), 0)) {
-              found |= prefill_drop_bad<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(t), tid);
+            if (__builtin_expect(careful && !whole(t), 0)) {
+              prefill_drop_bad<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(t), apart(tid));
               tile_barrier();
             }
           },
           [](int) {});
-      if (__builtin_expect(masked, 0)) hide(s1, prefill_first<64>(x, t) + 32);
+      if (__builtin_expect(!wave_whole(t), 0)) hide(s1, prefill_first<64>(x, t) + 32);
       // After the last tile: scores of no use.
       const bool more_v = t + 1 < x.tiles, more_k = t + 2 < x.tiles;
       const auto k_next = load.tile(0, prefill_first<64>(x, more_k ? t + 2 : t), k_buf(t));
@@ -677,6 +869,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
               for (int j = begin; j < end; ++j) issue(j);
             }
           });
+      if (__builtin_expect(!wave_whole(t + 1), 0)) hide(s0, prefill_first<64>(x, t + 1));
     }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -684,46 +877,63 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) acc[i % kCols][nb] = PrefillMma<DT>::mma(a, w1.w[i / kCols][nb], acc[i % kCols][nb]);
     }
-    tile_barrier();
-    if (tid == 0) *word = 0;
-    tile_barrier();
-    if (found) *word = 1;
-    tile_barrier();
-    if (__builtin_amdgcn_readfirstlane(*word) != 0) {
-      // Values that are not finite: a product of what is visible with their
-      // flags tells which rows see which of them.
-      if (x.tiles & 1) next_buffers();  // to V's second buffer
-#pragma unroll 1
-      for (int t = 0; t < x.tiles; ++t) {
-        if (whole(t)) continue;
-        const int first = prefill_first<64>(x, t);
-        tile_barrier();
-        load(1, first, v_buf(1));
-        tile_barrier_loads<0>();
-        prefill_to_flags<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(1), tid);
-        tile_barrier();
-#pragma unroll 1
-        for (int ks = 0; ks < 4; ++ks)
+    if (x.tiles & 1) next_buffers();  // as at the start: K's first, V's second
+    if (!careful) {
+      float test[4] = {0.f, 0.f, 0.f, 0.f};  // NaN if anything is not finite
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const PrefillView sees = prefill_view(p, place[nb], first + 16 * ks + 4 * half);
-            u32x4 one;
+      for (int nb = 0; nb < NB; ++nb) {
+        test[0] = fmaf(l[nb], 0.f, test[0]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int o = 8 * (j >> 1) + 2 * (j & 1);
-              one[j] = MfmaOps<DT>::pack2(sees(o) ? 1.f : 0.f, sees(o + 1) ? 1.f : 0.f);
-            }
+        for (int c = 0; c < kCols; ++c)
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              const f32x16 seen = PrefillMma<DT>::mma(read_v(16 * ks, c), one, f32x16{});
-#pragma unroll
-              for (int e = 0; e < 16; ++e) acc[c][nb][e] = prefill_add_bad(acc[c][nb][e], seen[e]);
-            }
-          }
+          for (int e = 0; e < 16; ++e) test[e % 4] = fmaf(acc[c][nb][e], 0.f, test[e % 4]);
       }
+      const float all = (test[0] + test[1]) + (test[2] + test[3]);
+      if (all != all) *word = 1;
+      tile_barrier();
+      if (__builtin_amdgcn_readfirstlane(*word) == 0) break;
+      clear();
+      load(0, prefill_first<64>(x, 0), k_buf(0));
+      load(1, prefill_first<64>(x, 0), v_buf(0));
+      continue;
     }
+    // A product of what is visible with the flags of values that are not finite.
+#pragma unroll 1
+    for (int t = 0; t < x.tiles; ++t) {
+      if (whole(t)) continue;
+      const int first = prefill_first<64>(x, t);
+      tile_barrier();
+      load(1, first, v_buf(1));
+      tile_barrier_loads<0>();
+      prefill_to_flags<DT, Sh::kTile / 16, 64 * NW>(smem + v_buf(1), apart(tid));
+      tile_barrier();
+#pragma unroll 1
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const PrefillView sees = prefill_view(p, place[nb], first + 16 * ks + 4 * half);
+          u32x4 one;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int o = 8 * (j >> 1) + 2 * (j & 1);
+            one[j] = MfmaOps<DT>::pack2(sees(o) ? 1.f : 0.f, sees(o + 1) ? 1.f : 0.f);
+          }
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            const f32x16 seen = PrefillMma<DT>::mma(read_v(16 * ks, c), one, f32x16{});
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c][nb][e] = prefill_add_bad(acc[c][nb][e], seen[e]);
+          }
+        }
+    }
+    break;
   }
-  prefill_store<DT, DP, NB>(p, x, wave_row, acc, l);
+  if (p.splits > 1) {
+    prefill_store<DT, DP, NB>(p, x, wave_row, acc, m, l);
+    return;
+  }
+  tile_barrier_loads<0>();  // nothing reads or writes LDS any more
+  prefill_store_rows<Sh, DT, DP, NB>(p, x, wave_row, smem + Sh::rows_at(wv), acc, l);
 }
 
 // fp32: the same products on the fp32 matrix cores, tile by tile, without the
@@ -734,14 +944,15 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
   constexpr int TT = Sh::TT, TB = Sh::kTB;
   constexpr float kLazy = 8.f;
   extern __shared__ __align__(16) char smem[];
-  int* word = reinterpret_cast<int*>(smem + 4 * Sh::kTile);
+  int* word = reinterpret_cast<int*>(smem + Sh::kWord);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, half = lane >> 5;
   PrefillItem x;
   if (!prefill_item<Sh::kRows, TT>(p, x)) return;
   const int wave_row = 32 * wv;
-  const int w_min = prefill_place(p, x, wave_row), w_max = prefill_place(p, x, wave_row + 31);
+  const int w_min = __builtin_amdgcn_readfirstlane(prefill_place(p, x, wave_row));
+  const int w_max = __builtin_amdgcn_readfirstlane(prefill_place(p, x, wave_row + 31));
   const uint32_t lds0 = tile_lds_address(smem);
   const PrefillLoads<Sh> load(p, x, lds0, wv, lane);
   if (load.row_bytes < Sh::kRow) {  // products run over the slots past the head
@@ -754,11 +965,20 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
     load(1, prefill_first<TT>(x, i), to + Sh::kTile);
   };
   if (x.tiles > 0) load_tile(0);
-  int place[1];
-  u32x4 qf[1][Sh::kSteps];
-  prefill_load_q<Sh, 1>(p, x, wave_row, place, qf);
+  const int place = prefill_place(p, x, wave_row + n32);
+  u32x4 qf[Sh::kSteps];
+  {
+    const PrefillRow row = prefill_row(p, x, min(wave_row + n32, x.rows - 1));
+    const char* src = static_cast<const char*>(p.q) +
+                      ((x.q0 + row.query) * p.q_stride + (static_cast<int64_t>(x.h) * p.G + row.g) * p.D) * Sh::kES;
+#pragma unroll
+    for (int st = 0; st < Sh::kSteps; ++st) {
+      const int at = 32 * st + 16 * half;
+      qf[st] = at < load.row_bytes ? *reinterpret_cast<const u32x4*>(src + at) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
   f32x16 acc[Sh::kCols][1];
-  float m = -INFINITY, l[1] = {0.f};
+  float m[1] = {-INFINITY}, l[1] = {0.f};
 #pragma unroll
   for (int c = 0; c < Sh::kCols; ++c) acc[c][0] = f32x16{};
   const uint32_t k_at = n32 * Sh::kRow + 16 * (half ^ prefill_swizzle(Sh::kSlots, n32));
@@ -778,7 +998,8 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
     if (i + 1 < x.tiles) load_tile(i + 1);
     char* tile = smem + (i & 1) * 2 * Sh::kTile;
     const uint32_t at = lds0 + (i & 1) * 2 * Sh::kTile, vt = at + Sh::kTile;
-    // As in the 16-bit kernel.
+    // Where only some rows see a token, a weight of 0 would not hide Inf and NaN
+    // from the others: they are left out here and added at the end.
     if (!prefill_sees_all(p, first, last, x.p_min, x.p_max)) {
       found |= prefill_drop_bad<QD_DTYPE_F32, Sh::kTile / 16, 64 * NW>(tile + Sh::kTile, tid);
       tile_barrier();
@@ -792,11 +1013,11 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
     for (int st = 0; st < Sh::kSteps; ++st)
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb)
-        s[tb] = PrefillMma<QD_DTYPE_F32>::mma(tile_lds_read<u32x4>((at + k_at + 32 * tb * Sh::kRow) ^ (32 * st)), qf[0][st], s[tb]);
+        s[tb] = PrefillMma<QD_DTYPE_F32>::mma(tile_lds_read<u32x4>((at + k_at + 32 * tb * Sh::kRow) ^ (32 * st)), qf[st], s[tb]);
     if (!prefill_sees_all(p, first, last, w_min, w_max)) {
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) {
-        const PrefillView sees = prefill_view(p, place[0], first + 32 * tb + 4 * half);
+        const PrefillView sees = prefill_view(p, place, first + 32 * tb + 4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[tb][e] = sees(8 * (e / 4) + e % 4) ? s[tb][e] : -INFINITY;
       }
@@ -807,15 +1028,15 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][e]);
     // The reference maximum moves when a score exceeds it by 2^kLazy.
-    if (__ballot(mx * p.sl2 > m + kLazy)) {
-      const float mn = fmaxf(m, prefill_max_halves(mx) * p.sl2);
-      const float alpha = mn == m ? 1.f : fast_exp2(m - mn);
-      m = mn;
+    if (__ballot(mx * p.sl2 > m[0] + kLazy)) {
+      const float mn = fmaxf(m[0], prefill_max_halves(mx) * p.sl2);
+      const float alpha = mn == m[0] ? 1.f : fast_exp2(m[0] - mn);
+      m[0] = mn;
       l[0] *= alpha;
 #pragma unroll
       for (int c = 0; c < Sh::kCols; ++c) acc[c][0] *= alpha;
     }
-    const float ref = m == -INFINITY ? 0.f : -m;
+    const float ref = m[0] == -INFINITY ? 0.f : -m[0];
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
@@ -849,7 +1070,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
       tile_barrier();
 #pragma unroll 1
       for (int tb = 0; tb < TB; ++tb) {
-        const PrefillView sees = prefill_view(p, place[0], first + 32 * tb + 4 * half);
+        const PrefillView sees = prefill_view(p, place, first + 32 * tb + 4 * half);
 #pragma unroll
         for (int c = 0; c < Sh::kCols; ++c) {
           f32x16 seen = f32x16{};
@@ -863,7 +1084,7 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
       }
     }
   }
-  prefill_store<QD_DTYPE_F32, DP, 1>(p, x, wave_row, acc, l);
+  prefill_store<QD_DTYPE_F32, DP, 1>(p, x, wave_row, acc, m, l);
 }
 
 template <int DT, int DP, int NB, int NW>
@@ -884,7 +1105,11 @@ hipError_t prefill_launch(const PrefillParams& p, uint32_t grid, hipStream_t st)
     if (e != hipSuccess) return e;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL(fn, dim3(grid), dim3(64 * NW), Sh::kLds, st, p);
+  hipLaunchKernelGGL(fn, dim3(grid, static_cast<uint32_t>(p.splits)), dim3(64 * NW), Sh::kLds, st, p);
+  if constexpr (DT != QD_DTYPE_F32)
+    if (p.splits > 1)
+      hipLaunchKernelGGL(prefill_merge_kernel<DT>,
+                         dim3(static_cast<uint32_t>((static_cast<int64_t>(p.Tq) * p.Hq + 3) / 4)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

@@ -54,7 +54,8 @@ at::Tensor gqa_prefill_hip(const at::Tensor& q, const at::Tensor& key, const at:
   if (q.size(0) == 0) return out;
   const int B = static_cast<int>(cu.size(0)) - 1, Hq = static_cast<int>(q.size(1)), Hkv = static_cast<int>(key.size(1)),
             D = static_cast<int>(q.size(2)), win = static_cast<int>(window);
-  const size_t bytes = qd_gqa_prefill_workspace_bytes(B, q.size(0), key.size(0), Hq, Hkv, D, dq.dtype, win, 0);
+  const size_t bytes = qd_gqa_prefill_workspace_bytes(B, q.size(0), key.size(0), Hq, Hkv, D, dq.dtype, win,
+                                                      static_cast<int>(sinks), 0);
   const at::Tensor ws = workspace(q, bytes);
   st = qd_gqa_prefill(q.data_ptr(), key.data_ptr(), value.data_ptr(), cu.data_ptr<int32_t>(),
                       dck.defined ? cu_k->data_ptr<int32_t>() : nullptr, out.data_ptr(),

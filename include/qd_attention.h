@@ -583,9 +583,10 @@ int qd_gqa_prefill_info(int batch, int64_t q_tokens, int64_t k_tokens, int q_hea
 
 /* Workspace bytes of qd_gqa_prefill (fp32 partials of keys split over
  * workgroups); 0 when none is needed.  16-byte aligned, no zeroing needed.
- * Calls that can overlap need different workspaces. */
+ * Calls that can overlap need different workspaces.  Depends on the current
+ * device, like the launch. */
 size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tokens, int q_heads, int kv_heads,
-                                      int head_dim, int dtype, int window, int flags);
+                                      int head_dim, int dtype, int window, int sinks, int flags);
 
 /* out = softmax(q . k * scale) . v over the keys that a query sees.  Query i of
  * the nq of a sequence with nk keys lies at position p = nk - nq + i and sees

@@ -216,6 +216,84 @@ def test_prefill_hidden_values(gpu, bad, dtype, D, Hq, flags):
         assert (np.abs(out - want)[clear] <= tol[clear]).all()
 
 
+SPLIT = [
+    # As above: few rows with many keys, whose keys several workgroups share.
+    (BF, [16], [3000], 4, 2, 128, 0, 0),
+    (HF, [5, 0, 7], [4000, 900, 10], 8, 2, 64, 0, 0),      # one sequence with all of the keys
+    (BF, [40, 3], [20, 6000], 4, 4, 128, 0, 0),            # rows that see nothing beside a long one
+    (BF, [3], [1200], 71, 1, 96, 0, 0),
+    (HF, [30], [2500], 4, 1, 256, 1500, 40),
+    (BF, [20], [9000], 2, 1, 128, 2000, 2100),             # more sinks than a part has keys
+    (HF, [1, 1], [1024, 5000], 2, 2, 192, 1100, 0),
+]
+
+
+@pytest.mark.parametrize("i", range(len(SPLIT)))
+def test_prefill_split_keys(gpu, i):
+    dtype, nq, nk, Hq, Hkv, D, window, sinks = SPLIT[i]
+    say(f"split {i} {SPLIT[i]}")
+    case = prefill_case(dtype, nq, nk, Hq, Hkv, D, seed=50 + i)
+    bytes_ = cabi.lib().qd_gqa_prefill_workspace_bytes(len(nq), case[0].shape[0], case[1].shape[0], Hq, Hkv, D,
+                                                       cabi.DTYPE[dtype], window, sinks, 0)
+    assert bytes_ > 0
+    torch.full((bytes_ // 4,), float("nan"), device=gpu)  # what the workspace holds before
+    out = check_prefill(gpu, case, window, sinks, None, f"split {i}")
+    assert not out[sum(nq):].any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_prefill_split_hidden_values(gpu, bad):
+    """As test_prefill_hidden_values, where the keys are split."""
+    for window, sinks in ((0, 0), (1500, 2)):
+        say(f"split hidden {bad} window {window}")
+        case = prefill_case(BF, [6], [3000], 4, 2, 128, seed=9)
+        q, k, v, cu, cu_k = case
+        want, spread, size = oracle_prefill(f64(q), f64(k), f64(v), cu.tolist(), cu_k.tolist(), window, sinks, 128 ** -0.5)
+        places = ((2997, 0), (1497, 1), (1, 2), (700, 3))
+        for token, col in places:
+            v[token, :, col] = bad
+        out = f64(prefill(gpu, case, window, sinks))
+        hit = np.zeros_like(want, dtype=bool)
+        for t in range(6):
+            at = 2994 + t
+            for token, col in places:
+                hit[t, :, col] |= token <= at and (not window or token > at - window or token < sinks)
+        assert hit.any() and not np.isfinite(out[hit]).any()
+        tol = prefill_tolerance(case, want, spread, size)
+        assert (np.abs(out - want)[~hit] <= tol[~hit]).all()
+
+
+def test_prefill_split_bad_metadata_stays_inside(gpu):
+    say("split bad metadata")
+    q, k, v, _, _ = (x if x is None else x.to(gpu) for x in prefill_case(BF, [10], [3000], 4, 2, 64))
+    for cu, cu_k in (([0, 500], [0, 1 << 30]), ([0, -5], [0, -9]), ([7, 9], [5, 2 ** 31 - 1]), ([-(1 << 31), 2 ** 31 - 1], [9, -(1 << 31)])):
+        cu, cu_k = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in (cu, cu_k))
+        assert cabi.gqa_prefill(q, k, v, cu, cu_k, torch.zeros_like(q), scale=0.1) == 0
+    torch.cuda.synchronize()
+
+
+def test_prefill_large_rows_of_64(gpu):
+    """As many rows as make heads of 64 take twice the rows per wave; parity with the
+    plain kernel, which the oracle has checked."""
+    say("heads of 64, 256 rows")
+    for dtype, window, sinks in ((BF, 0, 0), (HF, 100, 5)):
+        counts = [3000, 1, 0, 1095]
+        case = prefill_case(dtype, counts, None, 32, 4, 64, seed=12, spare=1)
+        assert cabi.gqa_prefill_info(4, 4097, 4097, 32, 4, 64, cabi.DTYPE[dtype])[2] == 256
+        out = prefill(gpu, case, window, sinks)
+        plain = prefill(gpu, case, window, sinks, cabi.QD_FLAG_FORCE_GENERIC)
+        # Both within their tolerance of the truth: spread at most the largest value,
+        # scores of 64 terms at most 64 * 4.5 * 7 / 8.
+        top = float(case[2].abs().max())
+        tol = 2 * (HALF[dtype] + 2 * 68 * U * 252 + 8 * U + 6000 * U + WEIGHT[dtype]) * top + 3000 * 2.0 ** -32 * top
+        assert (out.float() - plain.float()).abs().max().item() <= tol
+        assert not out[4096:].any()
+        # One sequence's rows against the oracle.
+        part = tuple(x[3001:4096] for x in case[:3]) + (torch.tensor([0, 1095], dtype=torch.int32), None)
+        want, spread, size = oracle_prefill(*(f64(x) for x in part[:3]), [0, 1095], None, window, sinks, 0.125)
+        worst_of(f64(out[3001:4096]), want, prefill_tolerance(part, want, spread, size), "the last sequence")
+
+
 def test_prefill_scores_of_all_sizes(gpu):
     """Scores far apart, rising and falling along the keys: the reference maximum moves."""
     for dtype in (BF, HF, FP):

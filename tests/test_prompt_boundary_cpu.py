@@ -127,7 +127,27 @@ def test_prefill_plans_fit_the_launch():
             assert kind >= 0 and 0 < grid < 1 << 31
             if kind == 1:
                 assert rows * (grid // Hkv) >= Tq * (Hq // Hkv)
-            assert cabi.lib().qd_gqa_prefill_workspace_bytes(B, Tq, Tq, Hq, Hkv, D, dtype, 0, 0) < 1 << 40
+            assert cabi.lib().qd_gqa_prefill_workspace_bytes(B, Tq, Tq, Hq, Hkv, D, dtype, 0, 0, 0) < 1 << 40
+
+
+def test_prefill_splits_keys_of_few_rows():
+    size = cabi.lib().qd_gqa_prefill_workspace_bytes
+    assert cabi.gqa_prefill_info(1, 16, 30000, 8, 2, 128, BF16)[1] == 2 * 2 * 58
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 0, 0, 0) == 4 * 58 * 16 * 8 * 132
+    assert size(1, 16, 30000, 8, 2, 128, F32, 0, 0, 0) == 0      # fp32: never
+    assert size(1, 16, 1000, 8, 2, 128, BF16, 0, 0, 0) == 0      # few keys
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 900, 0, 0) == 0   # few that a row sees
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 900, 900, 0) == 4 * 3 * 16 * 8 * 132
+    assert size(1, 1 << 14, 30000, 8, 2, 128, BF16, 0, 0, 0) == 0  # many rows
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 0, 0, cabi.QD_FLAG_FORCE_GENERIC) == 0
+    a = prefill_args()
+    a.update(B=1, Tq=16, Tk=30000, dtype=BF16, window=0, sinks=0)
+    need = size(1, 16, 30000, a["Hq"], a["Hkv"], a["D"], BF16, 0, 0, 0)
+    assert need > 0
+    for over in (dict(ws=None, ws_bytes=need), dict(ws=24, ws_bytes=need), dict(ws=32, ws_bytes=need - 1)):
+        a.update(over)
+        assert cabi.lib().qd_gqa_prefill(*a.values()) == 1
+        assert cabi.error_string(1) == "workspace too small or not 16-byte aligned"
 
 
 # ---- 8-bit caches --------------------------------------------------------------
