@@ -44,6 +44,8 @@ struct CacheParams {
   int64_t k_stride, v_stride, num_blocks;
   int64_t parts;      // append: runs of tokens of one page
   int B, tokens, Hkv, D, P, maxP;
+  PackedDivide by_hkv, by_page, by_row;  // append; by_row: pieces of a row
+  int row_step, col_step;                // append: from a piece to the 64th after it
 };
 
 // VEC elements of a row, as loaded.
@@ -152,64 +154,116 @@ __device__ __forceinline__ f32x4 unpack4(uint32_t w) {
 // they fit (kHold pieces per lane, 1024 in all: 64 tokens of 128 16-bit
 // elements); longer runs are read again, from L2.  What it moves is 2 T rows in
 // and half as many bytes out: HBM bounds it for prompts, the round trips
-// position -> page -> scale for single tokens.
+// position -> page -> scale for single tokens (TOKENS: a row per sequence, read
+// beside the position).
 // grid ceil(2 parts Hkv / 4), block 256; a workgroup's waves have neighbouring
 // heads, whose rows are neighbours in memory.
-template <int DT, int KIND, int VEC>
-__global__ __launch_bounds__(256) void append_q8_kernel(CacheParams p) {
+template <int DT, int KIND, int VEC, bool TOKENS>
+__global__ __launch_bounds__(256, 4) void append_q8_kernel(CacheParams p) {
   using S = typename Elem<DT>::S;
-  constexpr int kHold = 16;
+  constexpr int kHold = !TOKENS ? 16 : VEC == 1 ? 4 : 1;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= 2 * p.parts * p.Hkv) return;
-  const int64_t pair = div_nonneg(item, p.Hkv);
-  const int h = static_cast<int>(item - pair * p.Hkv);
+  const int pair = packed_divide(static_cast<uint32_t>(item), p.by_hkv);
+  const int h = static_cast<int>(item) - pair * p.Hkv;
   const bool is_v = pair & 1;
-  const int64_t u = pair >> 1;
-  int b = static_cast<int>(u), row0 = b, count = 1, page_at = 0;
-  if (p.cu) {
-    b = packed_find(p.cu, p.B, p.tokens, 1, p.P, 2, u);
-    row0 = packed_start(p.cu, b, p.tokens);
-    count = packed_start(p.cu, b + 1, p.tokens) - row0;
-    page_at = static_cast<int>(u - packed_base(p.cu, b, p.tokens, 1, p.P, 2));
+  const int u = pair >> 1;
+  const int64_t stride = is_v ? p.v_stride : p.k_stride;
+  const S* rows_in = static_cast<const S*>(is_v ? p.value : p.key) + static_cast<int64_t>(h) * p.D;
+  // Pieces of a run are numbered row by row; a lane takes every 64th.
+  const int per_row = p.D / VEC;
+  const int lane_row = packed_divide(static_cast<uint32_t>(lane), p.by_row), lane_col = lane - lane_row * per_row;
+  struct Walk {
+    int row, col;
+  };
+  // An opaque copy for each pass over the pieces: their places are computed again,
+  // not kept in registers beside them.
+  auto begin = [&]() {
+    Walk w{lane_row, lane_col};
+    asm volatile("" : "+v"(w.row), "+v"(w.col));
+    return w;
+  };
+  auto next = [&](Walk& w) {
+    w.row += p.row_step;
+    w.col += p.col_step;
+    if (w.col >= per_row) {
+      w.col -= per_row;
+      ++w.row;
+    }
+  };
+  // Loads every piece of `held` that lies within `rows` rows.
+  auto read = [&](auto& held, Walk& w, const S* src, int rows) {
+#pragma unroll
+    for (auto& x : held) {
+      if (w.row < rows) x.load(src + w.row * stride + w.col * VEC);
+      next(w);
+    }
+  };
+  Piece<DT, VEC> held[kHold];
+  int b = u, row0 = u, count = 1, page_at = 0, pos;
+  if constexpr (TOKENS) {
+    pos = p.at[b];
+    Walk w = begin();
+    read(held, w, rows_in + row0 * stride, 1);
+  } else {
+    // Runs begin at start / P + 2 b: a part begun at either end.
+    auto base = [&](int start, int seq) { return static_cast<int64_t>(packed_divide(static_cast<uint32_t>(start), p.by_page)) + 2 * static_cast<int64_t>(seq); };
+    if (p.B < 64) {
+      // Lane b holds what there is of sequence b: one round trip.
+      const int start = packed_start(p.cu, min(lane, p.B), p.tokens), at = p.at[min(lane, p.B - 1)];
+      b = 63 - __builtin_clzll(__ballot(lane == 0 || (lane < p.B && base(start, lane) <= u)));
+      row0 = __builtin_amdgcn_readlane(start, b);
+      count = __builtin_amdgcn_readlane(start, b + 1) - row0;
+      pos = __builtin_amdgcn_readlane(at, b);
+    } else {
+      b = packed_find(p.cu, p.B, p.tokens, 1, p.P, 2, u);
+      row0 = __builtin_amdgcn_readfirstlane(packed_start(p.cu, b, p.tokens));
+      count = __builtin_amdgcn_readfirstlane(packed_start(p.cu, b + 1, p.tokens)) - row0;
+      pos = __builtin_amdgcn_readfirstlane(p.at[b]);
+    }
+    page_at = static_cast<int>(u - base(row0, b));
   }
-  const int pos = p.at[b];
   if (pos < 0 || count <= 0) return;
-  const int64_t page = pos / p.P + static_cast<int64_t>(page_at);
+  const int64_t page = packed_divide(static_cast<uint32_t>(pos), p.by_page) + static_cast<int64_t>(page_at);
   // Tokens [first, last) of the sequence's rows lie in the page.
   const int64_t first = max(page * p.P - pos, int64_t{0});
   const int64_t last = min((page + 1) * p.P - pos, static_cast<int64_t>(count));
   if (first >= last || page >= p.maxP) return;
   const int32_t phys = p.table[static_cast<int64_t>(b) * p.maxP + page];
-  if (phys < 0 || phys >= p.num_blocks) return;
   const int slot0 = static_cast<int>(pos + first - page * p.P);
   const int rows = static_cast<int>(last - first);
-  const int64_t stride = is_v ? p.v_stride : p.k_stride;
-  const S* src = static_cast<const S*>(is_v ? p.value : p.key) + (row0 + first) * stride + static_cast<int64_t>(h) * p.D;
+  const S* src = rows_in + (row0 + first) * stride;
+  const int64_t total = static_cast<int64_t>(rows) * per_row;
+  const bool held_all = TOKENS || total <= 64 * kHold;
+  if (!TOKENS && held_all) {
+    Walk w = begin();
+    read(held, w, src, rows);
+  }
+  if (phys < 0 || phys >= p.num_blocks) return;
   float* scale_at = (is_v ? p.vs : p.ks) + static_cast<int64_t>(phys) * p.Hkv + h;
   uint8_t* page_base = static_cast<uint8_t*>(is_v ? p.vc : p.kc) +
                        (static_cast<int64_t>(phys) * p.P * p.Hkv + h) * p.D;
   const int64_t row_bytes = static_cast<int64_t>(p.Hkv) * p.D;
-  const uint32_t per_row = static_cast<uint32_t>(p.D) / VEC;
-  const int64_t total = static_cast<int64_t>(rows) * per_row;
   const float old = slot0 > 0 ? *scale_at : 0.f;
-  Piece<DT, VEC> held[kHold];
   Largest<DT, VEC> most;
-  auto read = [&](int64_t from) {
+  auto weigh = [&](auto& held, Walk& w) {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int64_t x = from + 64 * i + lane;
-      if (x < total) {
-        const int64_t r = div_nonneg(x, per_row);
-        held[i].load(src + r * stride + (x - r * per_row) * VEC);
-      }
+    for (auto& x : held) {
+      if (w.row < rows) most.add(x);
+      next(w);
     }
   };
-  for (int64_t from = 0; from < total; from += 64 * kHold) {
-    read(from);
-#pragma unroll
-    for (int i = 0; i < kHold; ++i)
-      if (from + 64 * i + lane < total) most.add(held[i]);
+  constexpr int kSome = 4;  // pieces in flight of a longer run
+  Walk all = begin();
+  if (held_all) {
+    weigh(held, all);
+  } else {
+    for (Walk w = all; __ballot(all.row < rows);) {
+      Piece<DT, VEC> some[kSome];
+      read(some, w, src, rows);
+      weigh(some, all);
+    }
   }
   const float fresh = power_scale<KIND>(q8_dpp_max(most.f32_bits()));
   // A NaN on either side stays.
@@ -237,24 +291,40 @@ __global__ __launch_bounds__(256) void append_q8_kernel(CacheParams p) {
   if (lane == 0) *scale_at = scale;
   // x / scale: a product where the scale is a power of two, as this kernel's
   // are; a caller's own may be anything.
-  const bool power = (__float_as_uint(scale) & 0x007FFFFFu) == 0;
-  const float inv = 1.f / scale;
-  for (int64_t from = 0; from < total; from += 64 * kHold) {
-    if (total > 64 * kHold) read(from);
+  uint8_t* to = page_base + slot0 * row_bytes;
+  auto write = [&](auto& held, Walk& w, auto&& scaled) {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int64_t x = from + 64 * i + lane;
-      if (x >= total) continue;
-      const int64_t r = div_nonneg(x, per_row);
-      uint8_t* to = page_base + (slot0 + r) * row_bytes + (x - r * per_row) * VEC;
-      auto at = [&](int e) { return power ? held[i].get(e) * inv : held[i].get(e) / scale; };
-      if constexpr (VEC == 8)
-        *reinterpret_cast<u32x2*>(to) = u32x2{pack4<KIND>(at(0), at(1), at(2), at(3)), pack4<KIND>(at(4), at(5), at(6), at(7))};
-      else if constexpr (VEC == 4)
-        *reinterpret_cast<uint32_t*>(to) = pack4<KIND>(at(0), at(1), at(2), at(3));
-      else
-        *to = static_cast<uint8_t>(pack4<KIND>(at(0), 0.f, 0.f, 0.f));
+    for (auto& x : held) {
+      if (w.row < rows) {
+        auto at = [&](int e) { return scaled(x.get(e)); };
+        uint8_t* y = to + w.row * row_bytes + w.col * VEC;
+        if constexpr (VEC == 8)
+          *reinterpret_cast<u32x2*>(y) = u32x2{pack4<KIND>(at(0), at(1), at(2), at(3)), pack4<KIND>(at(4), at(5), at(6), at(7))};
+        else if constexpr (VEC == 4)
+          *reinterpret_cast<uint32_t*>(y) = pack4<KIND>(at(0), at(1), at(2), at(3));
+        else
+          *y = static_cast<uint8_t>(pack4<KIND>(at(0), 0.f, 0.f, 0.f));
+      }
+      next(w);
     }
+  };
+  auto write_all = [&](auto&& scaled) {
+    Walk w = begin();
+    if (held_all) {
+      write(held, w, scaled);
+    } else {
+      for (Walk r = w; __ballot(w.row < rows);) {
+        Piece<DT, VEC> some[kSome];
+        read(some, r, src, rows);
+        write(some, w, scaled);
+      }
+    }
+  };
+  if (__builtin_amdgcn_readfirstlane(__float_as_uint(scale) & 0x007FFFFFu) == 0) {
+    const float inv = 1.f / scale;
+    write_all([&](float x) { return x * inv; });
+  } else {
+    write_all([&](float x) { return x / scale; });
   }
 }
 
@@ -501,21 +571,32 @@ int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_c
   if (!apart(k_scales, v_scales, 4 * static_cast<uint64_t>(kv_heads)))
     return q8_fail(nullptr, 0, "k_scales and v_scales must not overlap");
   p.parts = cu ? tokens / block_size + 2 * static_cast<int64_t>(batch) : batch;
-  const int64_t grid = (2 * p.parts * kv_heads + 3) / 4;
-  if (grid > INT32_MAX) return q8_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
+  // Rows and items are counted in 32 bits, past their ends.
+  if (tokens > INT32_MAX - 255 || 2 * p.parts * kv_heads > INT32_MAX - 3)
+    return q8_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   const bool vec = (bits_of(key) | bits_of(value) | static_cast<uintptr_t>(head_dim * es) |
                     static_cast<uintptr_t>(k_stride * es) | static_cast<uintptr_t>(v_stride * es)) % 16 == 0 &&
                    (bits_of(k_cache) | bits_of(v_cache)) % 8 == 0;
+  const int per_row = head_dim / (!vec ? 1 : dtype == QD_DTYPE_F32 ? 4 : 8);
+  p.by_hkv = packed_divide_by(static_cast<uint32_t>(kv_heads));
+  p.by_page = packed_divide_by(static_cast<uint32_t>(block_size));
+  p.by_row = packed_divide_by(static_cast<uint32_t>(per_row));
+  p.row_step = 64 / per_row;
+  p.col_step = 64 % per_row;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   by_types(dtype, cache_dtype, [&](auto dt, auto kind) {
-    constexpr int DT = decltype(dt)::value, KIND = decltype(kind)::value;
-    if (vec)
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, DT == QD_DTYPE_F32 ? 4 : 8>), dim3(static_cast<uint32_t>(grid)),
-                         dim3(256), 0, st, p);
+    constexpr int DT = decltype(dt)::value, KIND = decltype(kind)::value, VEC = DT == QD_DTYPE_F32 ? 4 : 8;
+    const dim3 grid(static_cast<uint32_t>((2 * p.parts * kv_heads + 3) / 4));
+    if (vec && cu)
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, false>), grid, dim3(256), 0, st, p);
+    else if (vec)
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, true>), grid, dim3(256), 0, st, p);
+    else if (cu)
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, false>), grid, dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1>), dim3(static_cast<uint32_t>(grid)), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, true>), grid, dim3(256), 0, st, p);
   });
   return launched("kv_append_q8");
 }

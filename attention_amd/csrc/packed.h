@@ -10,6 +10,22 @@
 
 namespace {
 
+// n / d for n < 2^31 as (n m) >> s, on the scalar units: m = ceil(2^s / d) with s =
+// 31 + ceil(log2 d) exceeds 2^s / d by less than 1, and so n m / 2^s exceeds n / d
+// by less than n / 2^s < 1 / d.
+struct PackedDivide {
+  uint32_t m;
+  int s;
+};
+inline PackedDivide packed_divide_by(uint32_t d) {
+  int bits = 0;
+  while ((uint64_t{1} << bits) < d) ++bits;
+  return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + d - 1) / d), 31 + bits};
+}
+__device__ __forceinline__ int packed_divide(uint32_t n, PackedDivide d) {
+  return static_cast<int>((static_cast<uint64_t>(n) * d.m) >> d.s);
+}
+
 __device__ __forceinline__ int packed_start(const int32_t* cu, int b, int total) {
   return b == 0 ? 0 : min(max(cu[b], 0), total);
 }

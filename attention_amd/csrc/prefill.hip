@@ -293,8 +293,8 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
   p.sinks = sinks;
   p.sl2 = scale * kLog2e;
   p.inv_g = 1.f / static_cast<float>(p.G);
-  p.by_g = prefill_divide_by(static_cast<uint32_t>(p.G));
-  p.by_hkv = prefill_divide_by(static_cast<uint32_t>(kv_heads));
+  p.by_g = packed_divide_by(static_cast<uint32_t>(p.G));
+  p.by_hkv = packed_divide_by(static_cast<uint32_t>(kv_heads));
   p.groups = pl.mfma ? static_cast<int>(pl.grid / pl.splits / kv_heads) : 0;
   p.splits = pl.splits;
   p.part = static_cast<float*>(workspace);

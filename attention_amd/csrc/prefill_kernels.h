@@ -15,19 +15,6 @@
 #include "qd_device.h"
 #include "tile_device.h"
 
-// n / d for n < 2^31 as (n m) >> s, on the scalar units: m = ceil(2^s / d) with s =
-// 31 + ceil(log2 d) exceeds 2^s / d by less than 1, and so n m / 2^s exceeds n / d
-// by less than n / 2^s < 1 / d.
-struct PrefillDivide {
-  uint32_t m;
-  int s;
-};
-inline PrefillDivide prefill_divide_by(uint32_t d) {
-  int bits = 0;
-  while ((uint64_t{1} << bits) < d) ++bits;
-  return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + d - 1) / d), 31 + bits};
-}
-
 // Arguments of the kernels, passed between translation units.
 struct PrefillParams {
   const void* q;
@@ -41,7 +28,7 @@ struct PrefillParams {
   int window, sinks;
   float sl2;    // scale * log2(e)
   float inv_g;  // 1 / G
-  PrefillDivide by_g, by_hkv;
+  PackedDivide by_g, by_hkv;
   int groups;   // workgroups per kv-head (and split)
   int splits;   // workgroups that share an item's tiles; more than 1: partials in `part`
   float* part;  // [splits][Tq Hq][D + 4]: {m, l, -, -, acc[D]}
@@ -181,8 +168,7 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   // What comes from the vector units goes back to scalar registers, or all that
   // follows from it stays with those too.
   auto scalar = [](int y) { return __builtin_amdgcn_readfirstlane(y); };
-  auto divide = [](uint32_t n, PrefillDivide d) { return static_cast<int>((static_cast<uint64_t>(n) * d.m) >> d.s); };
-  const int group = divide(blockIdx.x, p.by_hkv);
+  const int group = packed_divide(blockIdx.x, p.by_hkv);
   x.h = static_cast<int>(blockIdx.x) - group * p.Hkv;
   // The last rows of a sequence see most: first.
   const int64_t u = p.groups - 1 - group;
@@ -213,7 +199,7 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   const int64_t row0 = (u - static_cast<int64_t>(x.q0) * p.G / ROWS - b) * ROWS;
   if (row0 >= rows_all) return false;
   x.rows = min(ROWS, rows_all - static_cast<int>(row0));
-  const int query0 = divide(static_cast<uint32_t>(row0), p.by_g);
+  const int query0 = packed_divide(static_cast<uint32_t>(row0), p.by_g);
   x.rest = static_cast<int>(row0) - query0 * p.G;
   x.nk = tail ? 0 : max(k1 - x.k0, 0);
   x.at0 = x.nk - (q1 - x.q0) + query0;
