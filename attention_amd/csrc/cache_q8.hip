@@ -44,7 +44,8 @@ struct CacheParams {
   int64_t k_stride, v_stride, num_blocks;
   int64_t parts;      // append: runs of tokens of one page
   int B, tokens, Hkv, D, P, maxP;
-  PackedDivide by_hkv, by_page, by_row;  // append; by_row: pieces of a row
+  PackedDivide by_page;
+  PackedDivide by_hkv, by_row;  // append; by_row: pieces of a row
   int row_step, col_step;                // append: from a piece to the 64th after it
 };
 
@@ -149,6 +150,30 @@ __device__ __forceinline__ f32x4 unpack4(uint32_t w) {
   }
 }
 
+// The sequence that part u of `per` tokens lies in (base: its first part), its rows
+// and its entry of `at`; for fewer than 64 sequences all in one round trip.
+struct Packed {
+  int b, start, count, at;
+};
+template <typename Base>
+__device__ __forceinline__ Packed packed_at(const CacheParams& p, int per, int spare, Base&& base, int64_t u) {
+  Packed x;
+  if (p.B < 64) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int start = packed_start(p.cu, min(lane, p.B), p.tokens), at = p.at[min(lane, p.B - 1)];
+    x.b = 63 - __builtin_clzll(__ballot(lane == 0 || (lane < p.B && base(start, lane) <= u)));
+    x.start = __builtin_amdgcn_readlane(start, x.b);
+    x.count = __builtin_amdgcn_readlane(start, x.b + 1) - x.start;
+    x.at = __builtin_amdgcn_readlane(at, x.b);
+  } else {
+    x.b = packed_find(p.cu, p.B, p.tokens, 1, per, spare, u);
+    x.start = __builtin_amdgcn_readfirstlane(packed_start(p.cu, x.b, p.tokens));
+    x.count = __builtin_amdgcn_readfirstlane(packed_start(p.cu, x.b + 1, p.tokens)) - x.start;
+    x.at = __builtin_amdgcn_readfirstlane(p.at[x.b]);
+  }
+  return x;
+}
+
 // A wave writes a run (the new tokens of one page) of one head's keys or values:
 // largest value, scale, elements, with the rows in registers in between where
 // they fit (kHold pieces per lane, 1024 in all: 64 tokens of 128 16-bit
@@ -207,21 +232,13 @@ __global__ __launch_bounds__(256, 4) void append_q8_kernel(CacheParams p) {
     Walk w = begin();
     read(held, w, rows_in + row0 * stride, 1);
   } else {
-    // Runs begin at start / P + 2 b: a part begun at either end.
-    auto base = [&](int start, int seq) { return static_cast<int64_t>(packed_divide(static_cast<uint32_t>(start), p.by_page)) + 2 * static_cast<int64_t>(seq); };
-    if (p.B < 64) {
-      // Lane b holds what there is of sequence b: one round trip.
-      const int start = packed_start(p.cu, min(lane, p.B), p.tokens), at = p.at[min(lane, p.B - 1)];
-      b = 63 - __builtin_clzll(__ballot(lane == 0 || (lane < p.B && base(start, lane) <= u)));
-      row0 = __builtin_amdgcn_readlane(start, b);
-      count = __builtin_amdgcn_readlane(start, b + 1) - row0;
-      pos = __builtin_amdgcn_readlane(at, b);
-    } else {
-      b = packed_find(p.cu, p.B, p.tokens, 1, p.P, 2, u);
-      row0 = __builtin_amdgcn_readfirstlane(packed_start(p.cu, b, p.tokens));
-      count = __builtin_amdgcn_readfirstlane(packed_start(p.cu, b + 1, p.tokens)) - row0;
-      pos = __builtin_amdgcn_readfirstlane(p.at[b]);
-    }
+    // Parts of P tokens, with a spare one for a run begun at either end.
+    auto base = [&](int start, int seq) { return packed_divide(static_cast<uint32_t>(start), p.by_page) + int64_t{2} * seq; };
+    const Packed x = packed_at(p, p.P, 2, base, u);
+    b = x.b;
+    row0 = x.start;
+    count = x.count;
+    pos = x.at;
     page_at = static_cast<int>(u - base(row0, b));
   }
   if (pos < 0 || count <= 0) return;
@@ -332,8 +349,11 @@ __global__ __launch_bounds__(256, 4) void append_q8_kernel(CacheParams p) {
 constexpr int kGatherRows = 32;
 
 // A workgroup reads kGatherRows tokens of one sequence, keys or values, VEC
-// elements per lane at a time; a lane keeps its column, and so its head.  Bound
-// by HBM: one byte in and an element out.
+// elements per lane at a time; a lane keeps its column, and so its head.  Bound by
+// HBM: one byte in and an element out.  Lanes write 16 neighbouring bytes each (16
+// elements per lane, written in two halves: 111 us instead of 104 for 16 contexts
+// of 1000 to 9000 tokens, 8 heads of 128), past the caches (104 -> 100 us, 5.3 TB/s):
+// what reads the rows next mostly runs behind another L2.
 // grid (tokens / kGatherRows + B, 2), block 256.
 template <int DT, int KIND, int VEC>
 __global__ __launch_bounds__(256) void gather_q8_kernel(CacheParams p) {
@@ -344,15 +364,15 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(CacheParams p) {
   const int tid = static_cast<int>(threadIdx.x);
   const bool is_v = blockIdx.y != 0;
   const int64_t u = blockIdx.x;
-  const int b = packed_find(p.cu, p.B, p.tokens, 1, kGatherRows, 1, u);
-  const int start = packed_start(p.cu, b, p.tokens), end = packed_start(p.cu, b + 1, p.tokens);
-  const int64_t first = (u - packed_base(p.cu, b, p.tokens, 1, kGatherRows, 1)) * kGatherRows;
-  const int64_t have = min(static_cast<int64_t>(max(p.at[b], 0)), static_cast<int64_t>(p.maxP) * p.P);
-  const int rows = static_cast<int>(min(min(have, static_cast<int64_t>(end - start)) - first, int64_t{kGatherRows}));
+  auto base = [](int start, int seq) { return int64_t{start / kGatherRows} + seq; };
+  const Packed x = packed_at(p, kGatherRows, 1, base, u);
+  const int64_t first = (u - base(x.start, x.b)) * kGatherRows;
+  const int64_t have = min(static_cast<int64_t>(max(x.at, 0)), static_cast<int64_t>(p.maxP) * p.P);
+  const int rows = static_cast<int>(min(min(have, static_cast<int64_t>(x.count)) - first, int64_t{kGatherRows}));
   if (rows <= 0) return;
   if (tid < rows) {
-    const int tok = static_cast<int>(first) + tid, page = tok / p.P;
-    const int32_t id = p.table[static_cast<int64_t>(b) * p.maxP + page];
+    const int tok = static_cast<int>(first) + tid, page = packed_divide(static_cast<uint32_t>(tok), p.by_page);
+    const int32_t id = p.table[static_cast<int64_t>(x.b) * p.maxP + page];
     const int64_t phys = min(max(static_cast<int64_t>(id), int64_t{0}), p.num_blocks - 1);
     pages[tid] = static_cast<int32_t>(phys);
     from[tid] = phys * p.P + (tok - page * p.P);
@@ -365,8 +385,8 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(CacheParams p) {
   const uint8_t* cache = static_cast<const uint8_t*>(is_v ? p.vc : p.kc);
   const float* scales = is_v ? p.vs : p.ks;
   const int64_t stride = is_v ? p.v_stride : p.k_stride, row_bytes = static_cast<int64_t>(p.Hkv) * p.D;
-  S* out = static_cast<S*>(is_v ? p.value : p.key) + (start + first) * stride;
-  constexpr int kAhead = 4;  // rows in flight
+  S* out = static_cast<S*>(is_v ? p.value : p.key) + (x.start + first) * stride;
+  constexpr int kAhead = 8;  // rows in flight
   constexpr int kWords = VEC >= 4 ? VEC / 4 : 1;
   for (int c = tid - team * width; c < per_row; c += width) {
     const int h = c / (p.D / VEC);
@@ -377,14 +397,12 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(CacheParams p) {
       for (int i = 0; i < kAhead; ++i) {
         const int r = min(r0 + i * teams, rows - 1);
         const uint8_t* src = cache + from[r] * row_bytes + static_cast<int64_t>(c) * VEC;
-        if constexpr (VEC == 16) {
-          const u32x4 x = stream_load16(reinterpret_cast<const char*>(src));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[i][j] = x[j];
-        } else if constexpr (VEC == 8) {
+        if constexpr (VEC == 8) {
           const u32x2 x = stream_load8(reinterpret_cast<const char*>(src));
           w[i][0] = x[0];
           w[i][1] = x[1];
+        } else if constexpr (VEC == 4) {
+          w[i][0] = stream_load4(reinterpret_cast<const char*>(src));
         } else {
           w[i][0] = *src;
         }
@@ -397,19 +415,13 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(CacheParams p) {
         S* to = out + r * stride + static_cast<int64_t>(c) * VEC;
         if constexpr (VEC == 1) {
           *to = E::from_f(unpack4<KIND>(w[i][0])[0] * scale[i]);
+        } else if constexpr (VEC == 4) {
+          __builtin_nontemporal_store(unpack4<KIND>(w[i][0]) * scale[i], reinterpret_cast<f32x4*>(to));
         } else {
-#pragma unroll
-          for (int j = 0; j < kWords; j += 2) {
-            const f32x4 x = unpack4<KIND>(w[i][j]) * scale[i], y = unpack4<KIND>(w[i][j + 1]) * scale[i];
-            if constexpr (DT == QD_DTYPE_F32) {
-              *reinterpret_cast<f32x4*>(to + 4 * j) = x;
-              *reinterpret_cast<f32x4*>(to + 4 * j + 4) = y;
-            } else {
-              *reinterpret_cast<u32x4*>(to + 4 * j) =
-                  u32x4{MfmaOps<DT>::pack2(x[0], x[1]), MfmaOps<DT>::pack2(x[2], x[3]), MfmaOps<DT>::pack2(y[0], y[1]),
-                        MfmaOps<DT>::pack2(y[2], y[3])};
-            }
-          }
+          const f32x4 y = unpack4<KIND>(w[i][0]) * scale[i], z = unpack4<KIND>(w[i][1]) * scale[i];
+          __builtin_nontemporal_store(u32x4{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3]),
+                                            MfmaOps<DT>::pack2(z[0], z[1]), MfmaOps<DT>::pack2(z[2], z[3])},
+                                      reinterpret_cast<u32x4*>(to));
         }
       }
     }
@@ -623,6 +635,7 @@ int qd_kv_gather_q8(void* key, void* value, const void* k_cache, const void* v_c
   if (bad != QD_OK) return bad;
   if (batch == 0 || tokens == 0) return QD_OK;
   p.parts = tokens / kGatherRows + batch;
+  p.by_page = packed_divide_by(static_cast<uint32_t>(block_size));
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   const bool out16 = (bits_of(key) | bits_of(value) | static_cast<uintptr_t>(k_stride * es) |
                       static_cast<uintptr_t>(v_stride * es)) % 16 == 0;
@@ -632,10 +645,9 @@ int qd_kv_gather_q8(void* key, void* value, const void* k_cache, const void* v_c
   const dim3 grid(static_cast<uint32_t>(p.parts), 2);
   by_types(dtype, cache_dtype, [&](auto dt, auto kind) {
     constexpr int DT = decltype(dt)::value, KIND = decltype(kind)::value;
-    if (out16 && in % 16 == 0)
-      hipLaunchKernelGGL((gather_q8_kernel<DT, KIND, 16>), grid, dim3(256), 0, st, p);
-    else if (out16 && in % 8 == 0)
-      hipLaunchKernelGGL((gather_q8_kernel<DT, KIND, 8>), grid, dim3(256), 0, st, p);
+    constexpr int VEC = DT == QD_DTYPE_F32 ? 4 : 8;
+    if (out16 && in % VEC == 0)
+      hipLaunchKernelGGL((gather_q8_kernel<DT, KIND, VEC>), grid, dim3(256), 0, st, p);
     else
       hipLaunchKernelGGL((gather_q8_kernel<DT, KIND, 1>), grid, dim3(256), 0, st, p);
   });
