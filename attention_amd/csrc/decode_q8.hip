@@ -12,6 +12,7 @@
 #include <string>
 #include <type_traits>
 
+#include "packed.h"
 #include "qd_device.h"
 
 void qd_set_last_error(int status, const std::string& msg);
@@ -42,6 +43,7 @@ struct Q8Params {
   int chunks, per;               // virtual kv-heads per kv-head and their q-heads (16 at most)
   int hw, groups;                // virtual heads of a workgroup, workgroups that share a sequence's tokens
   int W;                         // workgroups of a balanced launch; 0: one per item
+  PackedDivide by_page, by_groups, by_chunks;
 };
 
 __device__ __forceinline__ int q8_len(const Q8Params& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
@@ -269,14 +271,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tw_count = 4 / p.hw;              // waves along the tokens
-  const int wh = wv % p.hw, tw = wv / p.hw;
+  const int hw_log = p.hw >> 1;               // of 1, 2, 4
+  const int tw_count = 4 >> hw_log;           // waves along the tokens
+  const int wh = wv & (p.hw - 1), tw = wv >> hw_log;
   const int vheads = p.Hkv * p.chunks;
   const int64_t row_bytes = static_cast<int64_t>(p.Hkv) * p.D;
 
   auto process = [&](int b, int hg, int len, int t0, int t1, bool whole, int64_t slot) {
     const int v = hg * p.hw + wh;  // below vheads: hw divides it
-    const int h = v / p.chunks, g0 = (v - h * p.chunks) * p.per;
+    const int h = packed_divide(static_cast<uint32_t>(v), p.by_chunks), g0 = (v - h * p.chunks) * p.per;
     const int heads = min(p.per, p.G - g0);
     const bool real = r16 < heads;
     const int64_t q_row = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G + g0 + (real ? r16 : 0);
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     auto window = [&](int tile) {
       const int64_t want = 2 * ((static_cast<int64_t>(tile) + (lane >> 1)) * tw_count + tw) + (lane & 1);
       const int tok = static_cast<int>(min(want, static_cast<int64_t>(last_block))) * 16;
-      const int page = tok / p.P;
+      const int page = packed_divide(static_cast<uint32_t>(tok), p.by_page);
       const int64_t id = table[page];
       const int64_t phys = min(max(id, int64_t{0}), p.num_blocks - 1);
       at_lane = (phys * p.P + (tok - page * p.P)) * row_bytes + static_cast<int64_t>(h) * p.D;
@@ -535,71 +538,94 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     }
   };
   if (p.W == 0) {
-    const int b = static_cast<int>(blockIdx.x) / p.groups, hg = static_cast<int>(blockIdx.x) % p.groups;
-    const int len = q8_len(p, b);
+    const int b = packed_divide(blockIdx.x, p.by_groups), hg = static_cast<int>(blockIdx.x) - b * p.groups;
+    const int len = __builtin_amdgcn_readfirstlane(q8_len(p, b));
     if (len == 0)
       zero_rows(b, hg);
     else
-      process(b, hg, len, 0, (len + tile_tokens - 1) / tile_tokens, true, 0);
+      process(b, hg, len, 0, (len + tile_tokens - 1) >> (7 - hw_log), true, 0);
     return;
   }
   // Balanced: the costs of all items in a row (below 2^31: the host sees to it),
-  // cut into equal ranges.
+  // cut into equal ranges.  A lane holds a sequence's sum of costs up to its end;
+  // more than 64 of them are in LDS.
+  auto cost_of = [&](int len) { return len > 0 ? (((len + tile_tokens - 1) >> (7 - hw_log)) + kQ8ItemCost) * p.groups : 0; };
+  auto scan = [](int x) {
+    x = dpp_add_i32<0x111, 0xF>(x);     // row_shr:1
+    x = dpp_add_i32<0x112, 0xF>(x);     // row_shr:2
+    x = dpp_add_i32<0x114, 0xF>(x);     // row_shr:4
+    x = dpp_add_i32<0x118, 0xF>(x);     // row_shr:8
+    x = dpp_add_i32<0x142, 0xA>(x);     // row_bcast:15
+    return dpp_add_i32<0x143, 0xC>(x);  // row_bcast:31
+  };
   int32_t* incl = reinterpret_cast<int32_t*>(smem + (tw_count > 1 ? Sh::kLds : 0));
-  auto cost_of = [&](int len) { return len > 0 ? ((len + tile_tokens - 1) / tile_tokens + kQ8ItemCost) * p.groups : 0; };
-  for (int i = tid; i < p.B; i += 256) incl[i] = cost_of(q8_len(p, i));
-  __syncthreads();
-  if (wv == 0) {
-    int carry = 0;
-    for (int from = 0; from < p.B; from += 64) {
-      const int i = from + lane;
-      int x = i < p.B ? incl[i] : 0;
-      x = dpp_add_i32<0x111, 0xF>(x);  // row_shr:1
-      x = dpp_add_i32<0x112, 0xF>(x);  // row_shr:2
-      x = dpp_add_i32<0x114, 0xF>(x);  // row_shr:4
-      x = dpp_add_i32<0x118, 0xF>(x);  // row_shr:8
-      x = dpp_add_i32<0x142, 0xA>(x);  // row_bcast:15
-      x = dpp_add_i32<0x143, 0xC>(x);  // row_bcast:31
-      x += carry;
-      if (i < p.B) incl[i] = x;
-      carry = __builtin_amdgcn_readlane(x, 63);
+  const bool in_lanes = p.B <= 64;
+  int len_lane = 0, incl_lane = 0, total;
+  if (in_lanes) {
+    if (lane < p.B) len_lane = q8_len(p, lane);
+    incl_lane = scan(cost_of(len_lane));
+    total = __builtin_amdgcn_readlane(incl_lane, 63);
+  } else {
+    for (int i = tid; i < p.B; i += 256) incl[i] = cost_of(q8_len(p, i));
+    __syncthreads();
+    if (wv == 0) {
+      int carry = 0;
+      for (int from = 0; from < p.B; from += 64) {
+        const int i = from + lane;
+        const int x = scan(i < p.B ? incl[i] : 0) + carry;
+        if (i < p.B) incl[i] = x;
+        carry = __builtin_amdgcn_readlane(x, 63);
+      }
     }
+    __syncthreads();
+    total = __builtin_amdgcn_readfirstlane(incl[p.B - 1]);
   }
-  __syncthreads();
-  const int total = __builtin_amdgcn_readfirstlane(incl[p.B - 1]);
   const int used = min(p.W, max(1, total / kQ8MinCost));
   const int w = static_cast<int>(blockIdx.x);
   if (w >= used) return;
-  // a n / d below 2^31; a n is below 2^42, so that the rounded quotient of doubles
-  // is never on the wrong side of an integer.
-  auto part_of = [](int a, int n, int d) {
-    return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(a) * n / d));
-  };
-  int pos = part_of(w, total, used);
-  const int end = part_of(w + 1, total, used);
-  int lo = 0, hi = p.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+  // The first `rem` ranges have a cost of `each` + 1.
+  const int each = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(used)));
+  const int rem = total - each * used;
+  int pos = w * each + min(w, rem);
+  const int end = pos + each + (w < rem ? 1 : 0);
+  int b = 0;
+  if (!in_lanes) {
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
   }
-  int b = __builtin_amdgcn_readfirstlane(lo);
   while (pos < end) {
-    while (__builtin_amdgcn_readfirstlane(incl[b]) <= pos) ++b;  // pos < total: ends
-    const int before = b > 0 ? __builtin_amdgcn_readfirstlane(incl[b - 1]) : 0;
-    const int cost = (__builtin_amdgcn_readfirstlane(incl[b]) - before) / p.groups;
-    const int hg = (pos - before) / cost, off = pos - before - hg * cost;
+    // The first sequence that ends behind pos (pos < total: there is one).
+    int upto, before, len;
+    if (in_lanes) {
+      b = __builtin_popcountll(__ballot(incl_lane <= pos));
+      upto = __builtin_amdgcn_readlane(incl_lane, b);
+      before = b > 0 ? __builtin_amdgcn_readlane(incl_lane, b - 1) : 0;
+      len = __builtin_amdgcn_readlane(len_lane, b);
+    } else {
+      while (__builtin_amdgcn_readfirstlane(incl[b]) <= pos) ++b;
+      upto = __builtin_amdgcn_readfirstlane(incl[b]);
+      before = b > 0 ? __builtin_amdgcn_readfirstlane(incl[b - 1]) : 0;
+      len = __builtin_amdgcn_readfirstlane(q8_len(p, b));
+    }
+    const int cost = packed_divide(static_cast<uint32_t>(upto - before), p.by_groups);
+    const int hg = p.groups == 1 ? 0 : __builtin_amdgcn_readfirstlane((pos - before) / cost);
+    const int off = pos - before - hg * cost;
     const int stop = min(cost, off + (end - pos));
     const int t0 = max(0, off - kQ8ItemCost), t1 = max(0, stop - kQ8ItemCost), tiles = cost - kQ8ItemCost;
     if (t1 > t0) {
       if (t0 == 0 && tid == 0) {
-        const int x = before + hg * cost + cost - 1;  // the item's last tile
-        int last = part_of(x, used, total);
-        while (last + 1 < used && part_of(last + 1, total, used) <= x) ++last;
+        // The range of the item's last tile.
+        const uint32_t x = before + hg * cost + cost - 1, low = static_cast<uint32_t>(rem) * (each + 1);
+        const int last = x < low ? x / (each + 1) : rem + (x - low) / each;
         int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * p.groups + hg);
         meta[0] = w;
         meta[1] = last - w + 1;
       }
-      process(b, hg, q8_len(p, b), t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
+      process(b, hg, len, t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
     }
     pos += stop - off;
   }
@@ -612,16 +638,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
   constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, TEAMS = 64 / LANES, STEP = 4 * LANES;
-  const int item = blockIdx.x, b = item / p.groups, hg = item % p.groups;
+  const int item = static_cast<int>(blockIdx.x), b = packed_divide(blockIdx.x, p.by_groups), hg = item - b * p.groups;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int row = 4 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x >> 6);
   if (row >= p.hw * p.per) return;
   const int wh = row / p.per, n = row - wh * p.per;
   const int v = hg * p.hw + wh, h = v / p.chunks, g = (v - h * p.chunks) * p.per + n;
   if (g >= p.G) return;
+  // One round trip (an empty sequence's entry was not written: not used).
+  const int32_t first_of = p.meta[2 * static_cast<int64_t>(item)], count_of = p.meta[2 * static_cast<int64_t>(item) + 1];
   const bool empty = q8_len(p, b) == 0;
-  const int first = empty ? 0 : p.meta[2 * static_cast<int64_t>(item)];
-  const int count = empty ? 0 : p.meta[2 * static_cast<int64_t>(item) + 1];
+  const int first = empty ? 0 : first_of, count = empty ? 0 : count_of;
   if (count == 1) return;
   const int team = lane / LANES, l = lane % LANES;
   const int64_t slot_floats = static_cast<int64_t>(p.hw) * 16 * (p.D + 4);
@@ -633,25 +660,26 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
     const int d = d0 + 4 * l;
     float mx = -INFINITY, sum = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    // Four partials at a time, statistics and values in flight together.
-    for (int s0 = 4 * team; s0 < count; s0 += 4 * TEAMS) {
-      f32x2 ml[4];
-      f32x4 x[4];
+    // Eight partials at a time, statistics and values in flight together.
+    constexpr int kAhead = 8;
+    for (int s0 = kAhead * team; s0 < count; s0 += kAhead * TEAMS) {
+      f32x2 ml[kAhead];
+      f32x4 x[kAhead];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kAhead; ++i) {
         const float* src = part(min(s0 + i, count - 1));
         ml[i] = *reinterpret_cast<const f32x2*>(src);
         x[i] = d < p.D ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
       float most = mx;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most = fmaxf(most, ml[i][0]);
+      for (int i = 0; i < kAhead; ++i) most = fmaxf(most, ml[i][0]);
       const float ref = most == -INFINITY ? 0.f : most;
       const float old = fast_exp2(mx - ref);
       sum *= old;
       a *= old;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kAhead; ++i) {
         if (s0 + i >= count) continue;
         const float f = fast_exp2(ml[i][0] - ref);
         sum += f * ml[i][1];
@@ -920,6 +948,9 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
   p.hw = pl.hw;
   p.groups = pl.groups;
   p.W = pl.W;
+  p.by_page = packed_divide_by(static_cast<uint32_t>(block_size));
+  p.by_groups = packed_divide_by(static_cast<uint32_t>(std::max(pl.groups, 1)));
+  p.by_chunks = packed_divide_by(static_cast<uint32_t>(std::max(pl.chunks, 1)));
   p.num_blocks = num_blocks;
   p.B = batch;
   p.Hq = q_heads;
