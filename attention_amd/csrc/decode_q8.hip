@@ -283,24 +283,29 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     const int heads = min(p.per, p.G - g0);
     const bool real = r16 < heads;
     const int64_t q_row = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G + g0 + (real ? r16 : 0);
-    // Blocks of 16 tokens of this wave's tiles, 64 at a time: lane i holds the
-    // page of block 2 (tile of pair i / 2) + i % 2 and its scales.
+    // Blocks of 16 tokens of this wave's tiles, 64 at a time (a window): lane i holds
+    // block 2 (tile of pair i / 2) + i % 2, its page's scales, and ahead of need the
+    // page of the next window's.
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.maxP;
     const int last_block = (len - 1) >> 4;  // len > 0
     int64_t at_lane = 0;                    // byte of the block's first row in the pool
-    float ks_lane = 0.f, vs_lane = 0.f, lv_lane = 0.f;
-    auto window = [&](int tile) {
+    float ks_lane = 0.f, vs_lane = 0.f;
+    int32_t id_lane = 0;
+    auto token_of = [&](int tile) {
       const int64_t want = 2 * ((static_cast<int64_t>(tile) + (lane >> 1)) * tw_count + tw) + (lane & 1);
-      const int tok = static_cast<int>(min(want, static_cast<int64_t>(last_block))) * 16;
-      const int page = packed_divide(static_cast<uint32_t>(tok), p.by_page);
-      const int64_t id = table[page];
-      const int64_t phys = min(max(id, int64_t{0}), p.num_blocks - 1);
-      at_lane = (phys * p.P + (tok - page * p.P)) * row_bytes + static_cast<int64_t>(h) * p.D;
-      ks_lane = p.ks[phys * p.Hkv + h] * p.sl2;
-      vs_lane = p.vs[phys * p.Hkv + h];
-      lv_lane = __builtin_amdgcn_logf(fmaxf(fabsf(vs_lane), 0x1p-100f));
+      return static_cast<int>(min(want, static_cast<int64_t>(last_block))) * 16;
     };
-    window(t0);
+    auto find = [&](int tile) { id_lane = table[packed_divide(static_cast<uint32_t>(token_of(tile)), p.by_page)]; };
+    // The window that find() was called for.
+    auto window = [&](int tile, float& ks, float& vs) {
+      const int tok = token_of(tile), page = packed_divide(static_cast<uint32_t>(tok), p.by_page);
+      const int64_t phys = min(max(static_cast<int64_t>(id_lane), int64_t{0}), p.num_blocks - 1);
+      at_lane = (phys * p.P + (tok - page * p.P)) * row_bytes + static_cast<int64_t>(h) * p.D;
+      ks = p.ks[phys * p.Hkv + h];
+      vs = p.vs[phys * p.Hkv + h];
+    };
+    find(t0);
+    window(t0, ks_lane, vs_lane);
 
     struct Raw {
       u32x4 k[2][Sh::kPieces];
@@ -344,6 +349,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     Raw raw[2];
     int base = t0;  // the window's first tile
     if (t0 < t1) load(raw[0], 0);
+    if (t0 + 32 < t1) find(t0 + 32);
 
     // Queries: operand 2 j + u holds elements 64 j + 16 g4 + 8 u .. of this
     // lane's head.
@@ -400,8 +406,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
             s[tb] = Ops::mma32(u32x4{a[0], a[1], c[0], c[1]}, qf[2 * j + u], s[tb]);
           }
         vs[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_lane), 2 * i + tb));
-        ksc[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), 2 * i + tb)) * q_inv;
-        const float lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lv_lane), 2 * i + tb));
+        ksc[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), 2 * i + tb)) * (p.sl2 * q_inv);
+        const float lv = __builtin_amdgcn_logf(fmaxf(fabsf(vs[tb]), 0x1p-100f));
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[tb][e] *= ksc[tb];
         if (cut) {
@@ -454,13 +460,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
         if (now >= t1) break;
         const int i = now - base;
         const bool more = now + 1 < t1, over = i == 31;
-        if (more && !over) load(raw[half ^ 1], i + 1);
+        float ks = 0.f, vs = 0.f;
+        if (more) {
+          if (over) window(now + 1, ks, vs);
+          load(raw[half ^ 1], over ? 0 : i + 1);
+        }
         __builtin_amdgcn_sched_barrier(0);
         compute(raw[half], i, now);
         if (more && over) {
           base = now + 1;
-          window(base);
-          load(raw[half ^ 1], 0);
+          ks_lane = ks;
+          vs_lane = vs;
+          if (base + 32 < t1) find(base + 32);
         }
       }
     }
