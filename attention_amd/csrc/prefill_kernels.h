@@ -572,8 +572,6 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   }
   // Each wave's queries go through LDS too: as operands straight from memory they
   // would come in pieces of 32 bytes.
-  load(0, prefill_first<64>(x, 0), k_buf(0));
-  load(1, prefill_first<64>(x, 0), v_buf(0));
   {
     const char* base = prefill_scalar(static_cast<const char*>(p.q) +
                                       (x.q0 * p.q_stride + static_cast<int64_t>(x.h) * p.G * p.D) * Sh::kES);
@@ -588,6 +586,8 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
         tile_load_lds<false>(base, row.query * q_bytes + row.g * load.row_bytes + col, to + 1024 * i);
     }
   }
+  load(0, prefill_first<64>(x, 0), k_buf(0));
+  load(1, prefill_first<64>(x, 0), v_buf(0));  // needed last
   int place[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) place[nb] = prefill_place(p, x, wave_row + 32 * nb + n32);
@@ -633,8 +633,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
     u32x4 w[2][NB];  // 16 tokens each
   };
   u32x4 qf[NB][kN];
-  __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt(0)
-  asm volatile("" ::: "memory");
+  tile_wait_loads<2 * Sh::kLoads>();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -776,8 +775,8 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   for (bool careful = false;; careful = true) {
     f32x16 s0[NB], s1[NB];
     Weights w0, w1;
-    // The first tile has arrived, and every wave has its queries.
-    tile_barrier_loads<0>();
+    // The first K has arrived, and every wave has its queries.
+    tile_barrier_loads<Sh::kLoads>();
     if (x.tiles > 1) load(0, prefill_first<64>(x, 1), k_buf(1));
     // The first step has no tokens before it: no weights, and values of 0.
 #pragma unroll

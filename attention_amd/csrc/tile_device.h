@@ -33,6 +33,14 @@ __device__ __forceinline__ void tile_barrier_loads() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// This wave's part of it only.
+template <int kLeft>
+__device__ __forceinline__ void tile_wait_loads() {
+  static_assert(kLeft >= 0 && kLeft < 64, "vmcnt is 6 bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((kLeft & 0xF) | ((kLeft >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+  asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ void tile_barrier() { tile_barrier_loads<63>(); }
 
 // 16 bytes per lane from `src` to LDS bytes lds + 16 lane.  Written in assembly
