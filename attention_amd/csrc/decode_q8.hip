@@ -39,11 +39,13 @@ struct Q8Params {
   int splits;                    // VALU kernel
   float sl2;                     // scale * log2(e)
   // Matrix-core kernel.
-  int32_t* meta;                 // {first workgroup, workgroups} per item
+  int32_t* meta;                 // {first workgroup, last workgroup} per item
   int chunks, per;               // virtual kv-heads per kv-head and their q-heads (16 at most)
   int hw, groups;                // virtual heads of a workgroup, workgroups that share a sequence's tokens
   int W;                         // workgroups of a balanced launch; 0: one per item
   PackedDivide by_page, by_groups, by_chunks;
+  int last_page;                 // num_blocks - 1
+  int64_t page_bytes;
 };
 
 __device__ __forceinline__ int q8_len(const Q8Params& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
   const int tw_count = 4 >> hw_log;           // waves along the tokens
   const int wh = wv & (p.hw - 1), tw = wv >> hw_log;
   const int vheads = p.Hkv * p.chunks;
-  const int64_t row_bytes = static_cast<int64_t>(p.Hkv) * p.D;
+  const int row_bytes = p.Hkv * p.D;  // below 2^26
 
   auto process = [&](int b, int hg, int len, int t0, int t1, bool whole, int64_t slot) {
     const int v = hg * p.hw + wh;  // below vheads: hw divides it
@@ -291,18 +293,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     int64_t at_lane = 0;                    // byte of the block's first row in the pool
     float ks_lane = 0.f, vs_lane = 0.f;
     int32_t id_lane = 0;
-    auto token_of = [&](int tile) {
-      const int64_t want = 2 * ((static_cast<int64_t>(tile) + (lane >> 1)) * tw_count + tw) + (lane & 1);
-      return static_cast<int>(min(want, static_cast<int64_t>(last_block))) * 16;
+    auto token_of = [&](int tile) {  // blocks are below 2^27
+      return 16 * min(2 * ((tile + (lane >> 1)) * tw_count + tw) + (lane & 1), last_block);
     };
     auto find = [&](int tile) { id_lane = table[packed_divide(static_cast<uint32_t>(token_of(tile)), p.by_page)]; };
     // The window that find() was called for.
     auto window = [&](int tile, float& ks, float& vs) {
       const int tok = token_of(tile), page = packed_divide(static_cast<uint32_t>(tok), p.by_page);
-      const int64_t phys = min(max(static_cast<int64_t>(id_lane), int64_t{0}), p.num_blocks - 1);
-      at_lane = (phys * p.P + (tok - page * p.P)) * row_bytes + static_cast<int64_t>(h) * p.D;
-      ks = p.ks[phys * p.Hkv + h];
-      vs = p.vs[phys * p.Hkv + h];
+      const int phys = min(max(id_lane, 0), p.last_page);
+      at_lane = phys * p.page_bytes + (static_cast<int64_t>(tok - page * p.P) * row_bytes + h * p.D);
+      const int64_t scale_at = static_cast<int64_t>(phys) * p.Hkv + h;
+      ks = p.ks[scale_at];
+      vs = p.vs[scale_at];
     };
     find(t0);
     window(t0, ks_lane, vs_lane);
@@ -311,8 +313,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
       u32x4 k[2][Sh::kPieces];
       uint32_t v[2][4][E / 4];
     };
-    const uint32_t k_off = r16 * static_cast<uint32_t>(row_bytes) + 16 * g4;
-    const uint32_t v_off = 4 * g4 * static_cast<uint32_t>(row_bytes) + E * r16;
+    const uint32_t k_off = r16 * row_bytes + 16 * g4, v_off = 4 * g4 * row_bytes + E * r16;
     const bool v_in = E * r16 < p.D;
     auto load = [&](Raw& x, int i) {  // tile i of the window
 #pragma unroll
@@ -548,15 +549,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
         static_cast<uint16_t*>(p.out)[(static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.D + x % p.D] = 0;
     }
   };
-  if (p.W == 0) {
-    const int b = packed_divide(blockIdx.x, p.by_groups), hg = static_cast<int>(blockIdx.x) - b * p.groups;
-    const int len = __builtin_amdgcn_readfirstlane(q8_len(p, b));
-    if (len == 0)
-      zero_rows(b, hg);
-    else
-      process(b, hg, len, 0, (len + tile_tokens - 1) >> (7 - hw_log), true, 0);
-    return;
-  }
   // Balanced: the costs of all items in a row (below 2^31: the host sees to it),
   // cut into equal ranges.  A lane holds a sequence's sum of costs up to its end;
   // more than 64 of them are in LDS.
@@ -571,74 +563,85 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
   };
   int32_t* incl = reinterpret_cast<int32_t*>(smem + (tw_count > 1 ? Sh::kLds : 0));
   const bool in_lanes = p.B <= 64;
-  int len_lane = 0, incl_lane = 0, total;
-  if (in_lanes) {
-    if (lane < p.B) len_lane = q8_len(p, lane);
-    incl_lane = scan(cost_of(len_lane));
-    total = __builtin_amdgcn_readlane(incl_lane, 63);
-  } else {
-    for (int i = tid; i < p.B; i += 256) incl[i] = cost_of(q8_len(p, i));
-    __syncthreads();
-    if (wv == 0) {
-      int carry = 0;
-      for (int from = 0; from < p.B; from += 64) {
-        const int i = from + lane;
-        const int x = scan(i < p.B ? incl[i] : 0) + carry;
-        if (i < p.B) incl[i] = x;
-        carry = __builtin_amdgcn_readlane(x, 63);
-      }
-    }
-    __syncthreads();
-    total = __builtin_amdgcn_readfirstlane(incl[p.B - 1]);
-  }
-  const int used = min(p.W, max(1, total / kQ8MinCost));
   const int w = static_cast<int>(blockIdx.x);
-  if (w >= used) return;
-  // The first `rem` ranges have a cost of `each` + 1.
-  const int each = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(used)));
-  const int rem = total - each * used;
-  int pos = w * each + min(w, rem);
-  const int end = pos + each + (w < rem ? 1 : 0);
-  int b = 0;
-  if (!in_lanes) {
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+  int len_lane = 0, incl_lane = 0, b = 0, pos = 0, end = 1;
+  if (p.W > 0) {
+    int total;
+    if (in_lanes) {
+      if (lane < p.B) len_lane = q8_len(p, lane);
+      incl_lane = scan(cost_of(len_lane));
+      total = __builtin_amdgcn_readlane(incl_lane, 63);
+    } else {
+      for (int i = tid; i < p.B; i += 256) incl[i] = cost_of(q8_len(p, i));
+      __syncthreads();
+      if (wv == 0) {
+        int carry = 0;
+        for (int from = 0; from < p.B; from += 64) {
+          const int i = from + lane;
+          const int x = scan(i < p.B ? incl[i] : 0) + carry;
+          if (i < p.B) incl[i] = x;
+          carry = __builtin_amdgcn_readlane(x, 63);
+        }
+      }
+      __syncthreads();
+      total = __builtin_amdgcn_readfirstlane(incl[p.B - 1]);
     }
-    b = __builtin_amdgcn_readfirstlane(lo);
+    const int used = min(p.W, max(1, total / kQ8MinCost));
+    if (w >= used) return;
+    // The first `rem` ranges have a cost of `each` + 1.
+    const int each = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(used)));
+    const int rem = total - each * used;
+    pos = w * each + min(w, rem);
+    end = pos + each + (w < rem ? 1 : 0);
+    if (!in_lanes) {
+      int lo = 0, hi = p.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (incl[mid] > pos) hi = mid; else lo = mid + 1;
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
+    }
   }
   while (pos < end) {
-    // The first sequence that ends behind pos (pos < total: there is one).
-    int upto, before, len;
-    if (in_lanes) {
-      b = __builtin_popcountll(__ballot(incl_lane <= pos));
-      upto = __builtin_amdgcn_readlane(incl_lane, b);
-      before = b > 0 ? __builtin_amdgcn_readlane(incl_lane, b - 1) : 0;
-      len = __builtin_amdgcn_readlane(len_lane, b);
-    } else {
-      while (__builtin_amdgcn_readfirstlane(incl[b]) <= pos) ++b;
-      upto = __builtin_amdgcn_readfirstlane(incl[b]);
-      before = b > 0 ? __builtin_amdgcn_readfirstlane(incl[b - 1]) : 0;
+    int len, hg, t0, t1, tiles;
+    if (p.W == 0) {
+      b = packed_divide(blockIdx.x, p.by_groups);
+      hg = w - b * p.groups;
       len = __builtin_amdgcn_readfirstlane(q8_len(p, b));
-    }
-    const int cost = packed_divide(static_cast<uint32_t>(upto - before), p.by_groups);
-    const int hg = p.groups == 1 ? 0 : __builtin_amdgcn_readfirstlane((pos - before) / cost);
-    const int off = pos - before - hg * cost;
-    const int stop = min(cost, off + (end - pos));
-    const int t0 = max(0, off - kQ8ItemCost), t1 = max(0, stop - kQ8ItemCost), tiles = cost - kQ8ItemCost;
-    if (t1 > t0) {
-      if (t0 == 0 && tid == 0) {
-        // The range of the item's last tile.
-        const uint32_t x = before + hg * cost + cost - 1, low = static_cast<uint32_t>(rem) * (each + 1);
-        const int last = x < low ? x / (each + 1) : rem + (x - low) / each;
-        int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * p.groups + hg);
-        meta[0] = w;
-        meta[1] = last - w + 1;
+      if (len == 0) zero_rows(b, hg);
+      t0 = 0;
+      tiles = t1 = (len + tile_tokens - 1) >> (7 - hw_log);
+      pos = end;
+    } else {
+      // The first sequence that ends behind pos (pos < total: there is one).
+      int upto, before;
+      if (in_lanes) {
+        b = __builtin_popcountll(__ballot(incl_lane <= pos));
+        upto = __builtin_amdgcn_readlane(incl_lane, b);
+        before = b > 0 ? __builtin_amdgcn_readlane(incl_lane, b - 1) : 0;
+        len = __builtin_amdgcn_readlane(len_lane, b);
+      } else {
+        while (__builtin_amdgcn_readfirstlane(incl[b]) <= pos) ++b;
+        upto = __builtin_amdgcn_readfirstlane(incl[b]);
+        before = b > 0 ? __builtin_amdgcn_readfirstlane(incl[b - 1]) : 0;
+        len = __builtin_amdgcn_readfirstlane(q8_len(p, b));
       }
-      process(b, hg, len, t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
+      const uint32_t cost = packed_divide(static_cast<uint32_t>(upto - before), p.by_groups);
+      hg = p.groups == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(pos - before) / cost));
+      const int off = pos - before - hg * static_cast<int>(cost);
+      const int stop = min(static_cast<int>(cost), off + (end - pos));
+      t0 = max(0, off - kQ8ItemCost);
+      t1 = max(0, stop - kQ8ItemCost);
+      tiles = static_cast<int>(cost) - kQ8ItemCost;
+      pos += stop - off;
+      if (t1 > t0 && tid == 0) {
+        int32_t* meta = p.meta + 2 * (static_cast<int64_t>(b) * p.groups + hg);
+        if (t0 == 0) meta[0] = w;
+        if (t1 == tiles) meta[1] = w;
+      }
     }
-    pos += stop - off;
+    if (t1 > t0)
+      process(b, hg, len, t0, t1, t0 == 0 && t1 == tiles, 2 * static_cast<int64_t>(w) + (t0 == 0 ? 1 : 0));
   }
 }
 
@@ -657,9 +660,9 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
   const int v = hg * p.hw + wh, h = v / p.chunks, g = (v - h * p.chunks) * p.per + n;
   if (g >= p.G) return;
   // One round trip (an empty sequence's entry was not written: not used).
-  const int32_t first_of = p.meta[2 * static_cast<int64_t>(item)], count_of = p.meta[2 * static_cast<int64_t>(item) + 1];
+  const int32_t first_of = p.meta[2 * static_cast<int64_t>(item)], last_of = p.meta[2 * static_cast<int64_t>(item) + 1];
   const bool empty = q8_len(p, b) == 0;
-  const int first = empty ? 0 : first_of, count = empty ? 0 : count_of;
+  const int first = empty ? 0 : first_of, count = empty ? 0 : last_of - first_of + 1;
   if (count == 1) return;
   const int team = lane / LANES, l = lane % LANES;
   const int64_t slot_floats = static_cast<int64_t>(p.hw) * 16 * (p.D + 4);
@@ -959,6 +962,8 @@ int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, co
   p.hw = pl.hw;
   p.groups = pl.groups;
   p.W = pl.W;
+  p.last_page = static_cast<int>(num_blocks - 1);
+  p.page_bytes = static_cast<int64_t>(block_size) * kv_heads * head_dim;
   p.by_page = packed_divide_by(static_cast<uint32_t>(block_size));
   p.by_groups = packed_divide_by(static_cast<uint32_t>(std::max(pl.groups, 1)));
   p.by_chunks = packed_divide_by(static_cast<uint32_t>(std::max(pl.chunks, 1)));
