@@ -313,8 +313,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
       u32x4 k[2][Sh::kPieces];
       uint32_t v[2][4][E / 4];
     };
-    const uint32_t k_off = r16 * row_bytes + 16 * g4, v_off = 4 * g4 * row_bytes + E * r16;
-    const bool v_in = E * r16 < p.D;
+    // Columns past the head are read from its first ones: the queries are zero
+    // there, and such columns of the output go nowhere.
+    uint32_t k_off[Sh::kPieces];
+#pragma unroll
+    for (int j = 0; j < Sh::kPieces; ++j) k_off[j] = r16 * row_bytes + (64 * j + 16 * g4 < p.D ? 64 * j + 16 * g4 : 0);
+    const uint32_t v_off = 4 * g4 * row_bytes + (E * r16 < p.D ? E * r16 : 0);
     auto load = [&](Raw& x, int i) {  // tile i of the window
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
@@ -322,27 +326,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
         const char* k = reinterpret_cast<const char*>(p.k) + at;
         const char* v = reinterpret_cast<const char*>(p.v) + at;
 #pragma unroll
-        for (int j = 0; j < Sh::kPieces; ++j) {
-          x.k[tb][j] = u32x4{0u, 0u, 0u, 0u};
-          if (DP == p.D || 64 * j + 16 * g4 < p.D) x.k[tb][j] = stream_load16(k + k_off + 64 * j);
-        }
+        for (int j = 0; j < Sh::kPieces; ++j) x.k[tb][j] = stream_load16(k + k_off[j]);
 #pragma unroll
         for (int i2 = 0; i2 < 4; ++i2) {
           const char* src = v + v_off + i2 * row_bytes;
+          if constexpr (E == 4) {
+            x.v[tb][i2][0] = stream_load4(src);
+          } else if constexpr (E == 8) {
+            const u32x2 y = stream_load8(src);
+            x.v[tb][i2][0] = y[0];
+            x.v[tb][i2][1] = y[1];
+          } else {
+            const u32x4 y = stream_load16(src);
 #pragma unroll
-          for (int e = 0; e < E / 4; ++e) x.v[tb][i2][e] = 0;
-          if (DP == p.D || v_in) {
-            if constexpr (E == 4) {
-              x.v[tb][i2][0] = stream_load4(src);
-            } else if constexpr (E == 8) {
-              const u32x2 y = stream_load8(src);
-              x.v[tb][i2][0] = y[0];
-              x.v[tb][i2][1] = y[1];
-            } else {
-              const u32x4 y = stream_load16(src);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x.v[tb][i2][e] = y[e];
-            }
+            for (int e = 0; e < 4; ++e) x.v[tb][i2][e] = y[e];
           }
         }
       }

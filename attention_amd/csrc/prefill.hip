@@ -165,13 +165,23 @@ PrefillPlan prefill_plan(int batch, int64_t q_tokens, int64_t k_tokens, int q_he
   pl.mfma = true;
   pl.rows = rows;
   pl.grid = grid_of(rows);
-  if (es == 4) return pl;
   // Few rows with many keys: the items' keys are split until the card has a
-  // workgroup per CU, as long as each keeps 512 of them on average.
-  int64_t keys = k_tokens / std::max(batch, 1);
+  // workgroup for every CU, as long as each keeps 128 keys on average, and two where
+  // they fit beside each other (fp32: one after the other), with 256 each.  Items
+  // and keys are what static shapes tell: an item per 128 or 256 rows, at least one
+  // per sequence; the keys that a sequence's queries see on average.  Below 384 keys
+  // the merge's launch costs more than it saves (fp32, eight times slower per key:
+  // 256).  Measured, 32 heads over 8 of 128, bf16: one query over 2000 keys 22 -> 14
+  // us, 16 over 30000 557 -> 35 us, 4 x 64 over 8000 158 -> 58 us; 300 queries over
+  // their own 300 keys would go from 13 to 18 us.
+  const int64_t items = std::max((q_tokens * group + rows - 1) / rows, std::min<int64_t>(batch, q_tokens)) * kv_heads;
+  int64_t keys = std::max<int64_t>(k_tokens - q_tokens / 2, 0) / std::max(batch, 1);
   if (window > 0) keys = std::min(keys, static_cast<int64_t>(window) + sinks + rows / group);
-  const int64_t splits = std::min({prefill_cu_count() / pl.grid, keys / 512, int64_t{64}});
-  if (splits >= 2) {
+  if (keys < (es == 4 ? 256 : 384)) return pl;
+  const int64_t cus = prefill_cu_count(), slots = es == 4 || pl.dp <= 128 ? 2 * cus : cus;
+  const int64_t splits = std::min<int64_t>(std::max(std::min(cus / std::max<int64_t>(items, 1), keys / 128),
+                                                    std::min(slots / std::max<int64_t>(items, 1), keys / 256)), 32);
+  if (splits >= 2 && pl.grid * splits <= INT32_MAX) {
     pl.splits = static_cast<int>(splits);
     pl.grid *= splits;
     pl.bytes = sizeof(float) * static_cast<size_t>(splits) * q_tokens * q_heads * (head_dim + 4);
@@ -297,6 +307,7 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
   p.by_hkv = packed_divide_by(static_cast<uint32_t>(kv_heads));
   p.groups = pl.mfma ? static_cast<int>(pl.grid / pl.splits / kv_heads) : 0;
   p.splits = pl.splits;
+  p.by_splits = packed_divide_by(static_cast<uint32_t>(pl.splits));
   p.part = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
@@ -305,7 +316,7 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
     const auto run = dtype == QD_DTYPE_F32   ? qd_prefill_mfma_launch_f32
                      : dtype == QD_DTYPE_F16 ? qd_prefill_mfma_launch_f16
                                              : qd_prefill_mfma_launch_bf16;
-    e = static_cast<hipError_t>(run(p, pl.dp, pl.rows, static_cast<uint32_t>(pl.grid / pl.splits), stream));
+    e = static_cast<hipError_t>(run(p, pl.dp, pl.rows, static_cast<uint32_t>(pl.grid), stream));
   } else {
     switch (dtype) {
       case QD_DTYPE_F32: launch_generic<QD_DTYPE_F32>(p, st); break;

@@ -28,8 +28,8 @@ struct PrefillParams {
   int window, sinks;
   float sl2;    // scale * log2(e)
   float inv_g;  // 1 / G
-  PackedDivide by_g, by_hkv;
-  int groups;   // workgroups per kv-head (and split)
+  PackedDivide by_g, by_hkv, by_splits;
+  int groups;   // items per kv-head
   int splits;   // workgroups that share an item's tiles; more than 1: partials in `part`
   float* part;  // [splits][Tq Hq][D + 4]: {m, l, -, -, acc[D]}
 };
@@ -144,6 +144,7 @@ struct PrefillItem {
   // Tiles [0, sink_tiles), then from lo_tile on; the workgroup's are `tiles` from
   // the place `skip` of that list on.
   int lo_tile, sink_tiles, skip, tiles;
+  int split;
 };
 
 // Query (counted from q0) and q-head of the group of a row.
@@ -168,8 +169,12 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   // What comes from the vector units goes back to scalar registers, or all that
   // follows from it stays with those too.
   auto scalar = [](int y) { return __builtin_amdgcn_readfirstlane(y); };
-  const int group = packed_divide(blockIdx.x, p.by_hkv);
-  x.h = static_cast<int>(blockIdx.x) - group * p.Hkv;
+  // Parts of one item run on different XCDs: as evenly as there are parts, and no
+  // XCD has all of a head's keys to fetch.
+  const int item = packed_divide(blockIdx.x, p.by_splits);
+  x.split = static_cast<int>(blockIdx.x) - item * p.splits;
+  const int group = packed_divide(static_cast<uint32_t>(item), p.by_hkv);
+  x.h = item - group * p.Hkv;
   // The last rows of a sequence see most: first.
   const int64_t u = p.groups - 1 - group;
   int b, q1, k1;
@@ -214,10 +219,9 @@ __device__ __forceinline__ bool prefill_item(const PrefillParams& p, PrefillItem
   x.skip = 0;
   x.tiles = all;
   if (p.splits > 1) {
-    // At most 2^25 tiles and 64 splits.
-    const uint32_t n = all, parts = p.splits;
-    x.skip = scalar(static_cast<int>(n * blockIdx.y / parts));
-    x.tiles = scalar(static_cast<int>(n * (blockIdx.y + 1) / parts)) - x.skip;
+    const uint32_t n = all;  // below 2^26, and at most 32 parts
+    x.skip = packed_divide(n * x.split, p.by_splits);
+    x.tiles = packed_divide(n * (x.split + 1), p.by_splits) - x.skip;
   }
   for (int* y : {&x.q0, &x.rows, &x.rest, &x.k0, &x.nk, &x.at0, &x.p_min, &x.p_max, &x.lo_tile, &x.sink_tiles, &x.skip, &x.tiles})
     *y = scalar(*y);
@@ -381,7 +385,7 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
     const PrefillRow row = prefill_row(p, x, rr);
     const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
     if (p.splits > 1) {
-      float* to = p.part + (blockIdx.y * (static_cast<int64_t>(p.Tq) * p.Hq) + at) * (p.D + 4);
+      float* to = p.part + (x.split * (static_cast<int64_t>(p.Tq) * p.Hq) + at) * (p.D + 4);
       if (half == 0) *reinterpret_cast<f32x2*>(to) = has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c)
@@ -451,9 +455,9 @@ __device__ __forceinline__ void prefill_store_rows(const PrefillParams& p, const
 // Log-sum-exp merge of split items: a wave per row, LANES lanes stride its columns
 // four at a time, the others its partials.
 // grid ceil(Tq Hq / 4), block 256.
-template <int DT>
+template <int DT, int LANES>
 __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
-  constexpr int LANES = 16, TEAMS = 4;
+  constexpr int TEAMS = 64 / LANES, kAhead = 8;  // partials in flight
   const int64_t rows = static_cast<int64_t>(p.Tq) * p.Hq;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
@@ -463,15 +467,30 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
     const bool in = d < p.D;
     float mx = -INFINITY, sum = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    for (int s = team; s < p.splits; s += TEAMS) {
-      const float* src = part(s);
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(src);
-      const f32x4 x = in ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
-      const float most = fmaxf(mx, ml[0]), ref = most == -INFINITY ? 0.f : most;
-      const float f = fast_exp2(mx - ref), g = fast_exp2(ml[0] - ref);
-      sum = f * sum + g * ml[1];
-      // A part without weight has no say, whatever it holds.
-      a = ml[0] == -INFINITY ? a : f * a + g * x;
+    for (int s0 = kAhead * team; s0 < p.splits; s0 += kAhead * TEAMS) {
+      f32x2 ml[kAhead];
+      f32x4 x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float* src = part(min(s0 + i, p.splits - 1));
+        ml[i] = *reinterpret_cast<const f32x2*>(src);
+        x[i] = in ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      float most = mx;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) most = fmaxf(most, ml[i][0]);
+      const float ref = most == -INFINITY ? 0.f : most;
+      const float old = fast_exp2(mx - ref);
+      sum *= old;
+      a *= old;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        // A part without weight has no say, whatever it holds.
+        if (s0 + i >= p.splits || ml[i][0] == -INFINITY) continue;
+        const float f = fast_exp2(ml[i][0] - ref);
+        sum += f * ml[i][1];
+        a += f * x[i];
+      }
       mx = most;
     }
 #pragma unroll
@@ -490,8 +509,11 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
       const bool has = sum > 0.f || sum != sum;
       const float inv = has ? 1.f / sum : 0.f;
       if (!has) a = f32x4{0.f, 0.f, 0.f, 0.f};
-      *reinterpret_cast<u32x2*>(static_cast<char*>(p.out) + (row * p.D + d) * 2) =
-          u32x2{MfmaOps<DT>::pack2(a[0] * inv, a[1] * inv), MfmaOps<DT>::pack2(a[2] * inv, a[3] * inv)};
+      if constexpr (DT == QD_DTYPE_F32)
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + row * p.D + d) = a * inv;
+      else
+        *reinterpret_cast<u32x2*>(static_cast<char*>(p.out) + (row * p.D + d) * 2) =
+            u32x2{MfmaOps<DT>::pack2(a[0] * inv, a[1] * inv), MfmaOps<DT>::pack2(a[2] * inv, a[3] * inv)};
     }
   }
 }
@@ -1090,11 +1112,10 @@ hipError_t prefill_launch(const PrefillParams& p, uint32_t grid, hipStream_t st)
     if (e != hipSuccess) return e;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL(fn, dim3(grid, static_cast<uint32_t>(p.splits)), dim3(64 * NW), Sh::kLds, st, p);
-  if constexpr (DT != QD_DTYPE_F32)
-    if (p.splits > 1)
-      hipLaunchKernelGGL(prefill_merge_kernel<DT>,
-                         dim3(static_cast<uint32_t>((static_cast<int64_t>(p.Tq) * p.Hq + 3) / 4)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(fn, dim3(grid), dim3(64 * NW), Sh::kLds, st, p);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((prefill_merge_kernel<DT, (DP <= 64 ? 16 : 32)>),
+                       dim3(static_cast<uint32_t>((static_cast<int64_t>(p.Tq) * p.Hq + 3) / 4)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

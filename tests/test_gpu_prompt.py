@@ -225,6 +225,10 @@ SPLIT = [
     (HF, [30], [2500], 4, 1, 256, 1500, 40),
     (BF, [20], [9000], 2, 1, 128, 2000, 2100),             # more sinks than a part has keys
     (HF, [1, 1], [1024, 5000], 2, 2, 192, 1100, 0),
+    (BF, [700, 20], [900, 1400], 16, 4, 128, 0, 0),        # two workgroups per CU
+    (FP, [7], [1500], 4, 2, 64, 0, 0),
+    (FP, [20, 3], [900, 700], 3, 1, 128, 300, 5),
+    (FP, [1], [2000], 2, 1, 256, 0, 0),
 ]
 
 
@@ -241,12 +245,13 @@ def test_prefill_split_keys(gpu, i):
     assert not out[sum(nq):].any()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_prefill_split_hidden_values(gpu, bad):
+def test_prefill_split_hidden_values(gpu, bad, dtype):
     """As test_prefill_hidden_values, where the keys are split."""
     for window, sinks in ((0, 0), (1500, 2)):
-        say(f"split hidden {bad} window {window}")
-        case = prefill_case(BF, [6], [3000], 4, 2, 128, seed=9)
+        say(f"split hidden {dtype} {bad} window {window}")
+        case = prefill_case(dtype, [6], [3000], 4, 2, 128, seed=9)
         q, k, v, cu, cu_k = case
         want, spread, size = oracle_prefill(f64(q), f64(k), f64(v), cu.tolist(), cu_k.tolist(), window, sinks, 128 ** -0.5)
         places = ((2997, 0), (1497, 1), (1, 2), (700, 3))

@@ -132,13 +132,18 @@ def test_prefill_plans_fit_the_launch():
 
 def test_prefill_splits_keys_of_few_rows():
     size = cabi.lib().qd_gqa_prefill_workspace_bytes
-    assert cabi.gqa_prefill_info(1, 16, 30000, 8, 2, 128, BF16)[1] == 2 * 2 * 58
-    assert size(1, 16, 30000, 8, 2, 128, BF16, 0, 0, 0) == 4 * 58 * 16 * 8 * 132
-    assert size(1, 16, 30000, 8, 2, 128, F32, 0, 0, 0) == 0      # fp32: never
-    assert size(1, 16, 1000, 8, 2, 128, BF16, 0, 0, 0) == 0      # few keys
-    assert size(1, 16, 30000, 8, 2, 128, BF16, 900, 0, 0) == 0   # few that a row sees
-    assert size(1, 16, 30000, 8, 2, 128, BF16, 900, 900, 0) == 4 * 3 * 16 * 8 * 132
-    assert size(1, 1 << 14, 30000, 8, 2, 128, BF16, 0, 0, 0) == 0  # many rows
+    assert cabi.gqa_prefill_info(1, 16, 30000, 8, 2, 128, BF16)[1] == 2 * 2 * 32
+    row = 4 * 16 * 8 * 132                                        # bytes of a part
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 0, 0, 0) == 32 * row
+    assert size(1, 16, 1000, 8, 2, 128, BF16, 0, 0, 0) == 7 * row    # of 128 keys or more
+    assert size(1, 16, 391, 8, 2, 128, BF16, 0, 0, 0) == 0           # few keys
+    assert size(1, 16, 391, 8, 2, 128, F32, 0, 0, 0) == 2 * row
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 300, 0, 0) == 0       # few that a row sees
+    assert size(1, 16, 30000, 8, 2, 128, BF16, 900, 900, 0) == 14 * row
+    assert size(1, 3100, 30000, 8, 2, 128, BF16, 0, 0, 0) == 2 * row * 3100 // 16  # two workgroups beside each other
+    assert size(1, 3100, 30000, 8, 2, 256, BF16, 0, 0, 0) == 0       # too wide for that
+    assert size(1, 1 << 14, 30000, 8, 2, 128, BF16, 0, 0, 0) == 0    # many rows
+    assert size(1, 400, 400, 8, 2, 128, BF16, 0, 0, 0) == 0          # a prompt that sees itself
     assert size(1, 16, 30000, 8, 2, 128, BF16, 0, 0, cabi.QD_FLAG_FORCE_GENERIC) == 0
     a = prefill_args()
     a.update(B=1, Tq=16, Tk=30000, dtype=BF16, window=0, sinks=0)
