@@ -158,28 +158,31 @@ PrefillPlan prefill_plan(int batch, int64_t q_tokens, int64_t k_tokens, int q_he
   const auto grid_of = [&](int rows) { return (q_tokens * group / rows + batch + 1) * kv_heads; };
   pl.dp = es == 4 ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256)
                   : (head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 ? 192 : 256);
-  // 64 rows per wave where the registers hold two such waves per SIMD, and the
-  // rows are there to fill the card: K and V are read from LDS half as often.
-  const int rows = es == 2 && pl.dp == 64 && q_tokens * q_heads >= 256 * 512 ? 256 : 128;
+  // 64 rows per wave where the registers hold two such waves per SIMD, and there are
+  // rows for two rounds of workgroups: K and V are read from LDS half as often.
+  // Heads of 64 with 32 / 64 rows per wave: 16 prompts of 1000 tokens, 32 heads, 129 /
+  // 118 us; one of 8192, 16 heads, 180 / 187 us; one of 4096 63 / 92 us.
+  const int rows = es == 2 && pl.dp == 64 && q_tokens * q_heads >= 512 * 512 ? 256 : 128;
   if (grid_of(rows) > INT32_MAX) return pl;
   pl.mfma = true;
   pl.rows = rows;
   pl.grid = grid_of(rows);
   // Few rows with many keys: the items' keys are split until the card has a
-  // workgroup for every CU, as long as each keeps 128 keys on average, and two where
-  // they fit beside each other (fp32: one after the other), with 256 each.  Items
-  // and keys are what static shapes tell: an item per 128 or 256 rows, at least one
-  // per sequence; the keys that a sequence's queries see on average.  Below 384 keys
-  // the merge's launch costs more than it saves (fp32, eight times slower per key:
-  // 256).  Measured, 32 heads over 8 of 128, bf16: one query over 2000 keys 22 -> 14
-  // us, 16 over 30000 557 -> 35 us, 4 x 64 over 8000 158 -> 58 us; 300 queries over
-  // their own 300 keys would go from 13 to 18 us.
+  // workgroup for every CU, as long as each keeps 128 keys on average (fp32, eight
+  // times slower per key: 64), and two where they fit beside each other (fp32: one
+  // after the other), with 256 each.  Items and keys are what static shapes tell: an
+  // item per 128 or 256 rows, at least one per sequence; the keys that a sequence's
+  // queries see on average.  Below 384 keys the merge's launch costs more than it
+  // saves (fp32: 128).  Measured, 32 heads over 8 of 128, bf16: one query over 2000
+  // keys 22 -> 14 us, 16 over 30000 557 -> 35 us, 4 x 64 over 8000 158 -> 58 us; 300
+  // queries over their own 300 keys would go from 13 to 18 us.  fp32, 16 heads over
+  // 4: a prompt of 500 tokens 87 -> 48 us.
   const int64_t items = std::max((q_tokens * group + rows - 1) / rows, std::min<int64_t>(batch, q_tokens)) * kv_heads;
   int64_t keys = std::max<int64_t>(k_tokens - q_tokens / 2, 0) / std::max(batch, 1);
   if (window > 0) keys = std::min(keys, static_cast<int64_t>(window) + sinks + rows / group);
-  if (keys < (es == 4 ? 256 : 384)) return pl;
+  if (keys < (es == 4 ? 128 : 384)) return pl;
   const int64_t cus = prefill_cu_count(), slots = es == 4 || pl.dp <= 128 ? 2 * cus : cus;
-  const int64_t splits = std::min<int64_t>(std::max(std::min(cus / std::max<int64_t>(items, 1), keys / 128),
+  const int64_t splits = std::min<int64_t>(std::max(std::min(cus / std::max<int64_t>(items, 1), keys / (es == 4 ? 64 : 128)),
                                                     std::min(slots / std::max<int64_t>(items, 1), keys / 256)), 32);
   if (splits >= 2 && pl.grid * splits <= INT32_MAX) {
     pl.splits = static_cast<int>(splits);

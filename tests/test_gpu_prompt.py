@@ -283,8 +283,8 @@ def test_prefill_large_rows_of_64(gpu):
     say("heads of 64, 256 rows")
     for dtype, window, sinks in ((BF, 0, 0), (HF, 100, 5)):
         counts = [3000, 1, 0, 1095]
-        case = prefill_case(dtype, counts, None, 32, 4, 64, seed=12, spare=1)
-        assert cabi.gqa_prefill_info(4, 4097, 4097, 32, 4, 64, cabi.DTYPE[dtype])[2] == 256
+        case = prefill_case(dtype, counts, None, 64, 8, 64, seed=12, spare=1)
+        assert cabi.gqa_prefill_info(4, 4097, 4097, 64, 8, 64, cabi.DTYPE[dtype])[2] == 256
         out = prefill(gpu, case, window, sinks)
         plain = prefill(gpu, case, window, sinks, cabi.QD_FLAG_FORCE_GENERIC)
         # Both within their tolerance of the truth: spread at most the largest value,
