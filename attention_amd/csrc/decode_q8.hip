@@ -190,16 +190,23 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(Q8Params p) {
 // largest of a head just inside fp16's range: 2^-24 of 2^14 is the least that
 // they keep.  Weights are rounded to nearest once, 2^-12 on average.
 //
-// Half the bytes of 16-bit caches come in, and HBM should bound the kernel still:
-// per 32 tokens x 128 a wave moves 8 KB and issues about 200 (e4m3) or 300 (int8)
-// vector instructions, where the SIMD has 2500 cycles at 8 TB/s.
+// Half the bytes of 16-bit caches come in, and HBM bounds the kernel still: 48
+// sequences of 2000 to 30000 tokens, 64 heads over 8 of 128, fp16 over int8, take 260 us, 5.9
+// TB/s (reading alone reaches 6.9).  Per 32 tokens x 128 a wave moves 8 KB and
+// issues about 200 (e4m3) or 300 (int8) vector instructions, where the SIMD has
+// 2500 cycles.  Two tiles in registers, two waves per SIMD; three waves in 168
+// registers spill (312 us).  Small batches are bound by their start: length,
+// ranges, page and rows follow each other (5.8 us of 28 for 32 sequences of 512 to
+// 4096 tokens, 32 heads), and by the merge's launch (4.6 us).
 //
 // Up to four waves of a workgroup take neighbouring virtual heads at the same
 // tokens (whole rows of memory), or, with fewer heads, neighbouring 32 tokens.
 
 constexpr float kQ8Shift = 7.f, kQ8Lazy = 8.f;
 // Balanced launches: what an item's start costs, in tiles, and the least cost of a
-// workgroup's range.
+// workgroup's range.  Starts of 1 or 4 tiles: 256 sequences of 50 to 200 tokens 28.0
+// us for 26.7; ranges of 4: one sequence of 1500 tokens 12.2 for 11.5, 16 sequences
+// of up to 2000 with one kv-head 15.8 for 12.2.
 constexpr int kQ8ItemCost = 2;
 constexpr int kQ8MinCost = 2;
 // Sequences whose prefix of costs fits the kernel's LDS.
@@ -798,9 +805,14 @@ Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int head_dim, int block_siz
   const int64_t tiles = (cap + tile - 1) / tile;
   const int64_t resident = static_cast<int64_t>(q8_cu_count()) * (q8_padded(head_dim) == 256 ? 1 : 2);
   pl.grid = static_cast<int>(items);
-  // One workgroup per item where a range would not be shorter, and where the
-  // items' costs do not fit the kernel's LDS or 31 bits.
-  if (batch > kQ8MaxBalanced || items * (tiles + kQ8ItemCost) > INT32_MAX || tiles <= 2) return pl;
+  // One workgroup per item, without a merge, where contexts are short (up to 8 tiles,
+  // or 16 with items for every workgroup that the card holds), and where the items'
+  // costs do not fit the kernel's LDS or 31 bits.  us, ranges / items, 32 heads over 8
+  // of 128: 256 sequences of 50 to 200 tokens 27.2 / 19.6, of 100 to 500 44.2 / 40.0,
+  // of 100 to 1000 67.4 / 71.5; 64 of 100 to 250 15.2 / 13.0, of 100 to 500 17.8 /
+  // 20.9; 4 of 100 11.5 / 8.9.
+  if (batch > kQ8MaxBalanced || items * (tiles + kQ8ItemCost) > INT32_MAX || tiles <= (items >= resident ? 16 : 8))
+    return pl;
   pl.W = static_cast<int>(std::max<int64_t>(1, std::min(resident, items * (tiles + kQ8ItemCost) / kQ8MinCost)));
   pl.grid = pl.W;
   pl.meta_bytes = (8 * static_cast<size_t>(items) + 15) / 16 * 16;

@@ -257,8 +257,8 @@ __device__ __forceinline__ bool prefill_sees_all(const PrefillParams& p, int fir
   return last <= lowest && (p.window == 0 || first > highest - p.window || last < p.sinks);
 }
 
-// Bit-free view of a lane's tokens: those from `token` on that a row at `place`
-// sees are o <= hi with o > lo or o < sinks, o counted from `token`.
+// The tokens from `token` on that a row at `place` sees: o <= hi with o > lo or o <
+// sinks, o counted from `token`.
 struct PrefillView {
   int hi, lo, sinks;
   __device__ __forceinline__ bool operator()(int o) const {
@@ -537,10 +537,21 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
 //
 // Three steps are in work at once, in one stream of instructions: the scores of
 // the next 32 tokens, the softmax of these, the values of the ones before.  A
-// 32x32x16 product takes 32 cycles, in which a wave issues up to seven vector
-// instructions; per product there is one element's worth of softmax (a
-// multiply-add, an exponential that counts as two, halves of a conversion and of
-// a sum), so the matrix cores go on without a pause.
+// 32x32x16 product takes 32 cycles of the matrix cores; for heads of 128 there are
+// two elements' worth of softmax beside it (two multiply-adds, two exponentials at 8
+// cycles, a conversion and a sum of two), for heads of 64 four.  What bounds it:
+// products of random data alone run at 1709 TFLOP/s (the card's power takes the
+// clock to 1.7 GHz), with that much softmax beside them and nothing else at 1267;
+// one prompt of 12001 tokens, 32 heads of 128, takes 1098 us, 1076 TFLOP/s, with the
+// clock at 1.55 GHz and the matrix cores busy for 57% of it.  16x16x32 products need
+// twice the issue slots and ran at 1116 beside the same softmax.  Heads of 64 (16 and
+// 32 of 1000 to 8192 tokens) reach 650 to 720 TFLOP/s, bound by vector instructions.
+//
+// A workgroup's start and end (which rows, operands' first trip, output) take 17000
+// cycles, of which the other workgroup of its CU can use most: 16 prompts of 65 to
+// 2000 tokens run at 740 TFLOP/s.  128 rows per workgroup and two workgroups per CU:
+// eight waves of one (986 TFLOP/s then, against 1120) wait for each other, one wave of 64 rows per
+// SIMD (972) issues an instruction every five cycles at most.
 template <int DT, int DP, int NB, int NW>
 __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pipe_kernel(PrefillParams p) {
   using Sh = PrefillShape<DT, DP, NB, NW>;

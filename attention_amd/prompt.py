@@ -57,9 +57,9 @@ def kv_append_q8(key, value, k_cache, v_cache, k_scales, v_scales, block_table, 
     value: a page that the call begins takes the one of its new rows; one that it
     goes on with keeps the old one, or takes a larger one, and the rows before are
     rounded to it.  An Inf or NaN (or a scale past 2^100) makes the scale NaN, and
-    with it every value of that page and head.  Sequences with a negative position write nothing, nor do
-    tokens past the table or in pages outside the pool.  Pages that are written to
-    must be their sequence's own.
+    with it every value of that page and head.  Sequences with a negative position
+    write nothing, nor do tokens past the table or in pages outside the pool.  Pages
+    that are written to must be their sequence's own.
     """
     _require_extension()
     torch.ops.qd_serving.kv_append_q8(key, value, k_cache, v_cache, k_scales, v_scales, block_table, positions,
@@ -80,9 +80,10 @@ def kv_gather_q8(key, value, k_cache, v_cache, k_scales, v_scales, block_table, 
 
 def gqa_decode_q8(q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens, *, scale=None):
     """:func:`gqa_decode` over an 8-bit cache: q ``[B, Hq, D]`` (float16 or
-    bfloat16), scales of any magnitude from 2^-100 to 2^100, or 0.  Returns ``[B, Hq, D]``; a sequence of
-    length 0 gives zeros.  How the work is cut follows from the width of
-    ``block_table``, since lengths are not read on the host.
+    bfloat16), scales of any magnitude from 2^-100 to 2^100, or 0.  Returns ``[B, Hq,
+    D]``; a sequence of length 0 gives zeros.  Lengths are not read on the host: the
+    width of ``block_table`` decides whether contexts may be split (with a second
+    kernel that merges them), so trim it to the longest.
     """
     _require_extension()
     if scale is None:

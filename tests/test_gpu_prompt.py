@@ -619,6 +619,17 @@ def test_decode(gpu, i, flags):
     check_decode(gpu, decode_case(dtype, kind, lens, Hq, Hkv, D, P, seed=i, power=i % 2 == 0), flags, f"decode {i}")
 
 
+@pytest.mark.parametrize("i", range(len(DECODE)))
+def test_decode_split(gpu, i):
+    """The same in tables wide enough for contexts to be split."""
+    dtype, kind, lens, Hq, Hkv, D, P = DECODE[i]
+    say(f"decode split {i} {dtype} {kind} {lens[:4]} {Hq} {Hkv} {D} {P}")
+    case = decode_case(dtype, kind, lens, Hq, Hkv, D, P, seed=i, power=i % 2 == 1, spare=-(-3000 // P))
+    if D % 16 == 0 and P % 16 == 0 and len(lens) <= 1024:
+        assert cabi.gqa_decode_q8_info(len(lens), Hq, Hkv, D, P, case[5].shape[1], cabi.DTYPE[dtype])[0] == 2
+    check_decode(gpu, case, None, f"decode split {i}")
+
+
 def test_decode_wide_table(gpu):
     """Short contexts in a table of many pages: the ranges are cut by its width."""
     say("wide table")
