@@ -442,6 +442,9 @@ int q8_fail(char* msg, size_t cap, const char* text) {
   return QD_ERR_INVALID_VALUE;
 }
 
+// Workgroups of 256 threads, which are counted in 32 bits.
+constexpr int64_t kMaxGrid = (1 << 24) - 1;
+
 bool float_dtype(int dt) { return dt == QD_DTYPE_F32 || dt == QD_DTYPE_F16 || dt == QD_DTYPE_BF16; }
 bool cache_dtype_ok(int dt) { return dt == QD_DTYPE_E4M3 || dt == QD_DTYPE_I8; }
 uintptr_t bits_of(const void* p) { return reinterpret_cast<uintptr_t>(p); }
@@ -587,7 +590,7 @@ int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_c
     return q8_fail(nullptr, 0, "k_scales and v_scales must not overlap");
   p.parts = cu ? tokens / block_size + 2 * static_cast<int64_t>(batch) : batch;
   // Rows and items are counted in 32 bits, past their ends.
-  if (tokens > INT32_MAX - 255 || 2 * p.parts * kv_heads > INT32_MAX - 3)
+  if (tokens > INT32_MAX - 255 || 2 * p.parts * kv_heads > 4 * kMaxGrid)
     return q8_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   const bool vec = (bits_of(key) | bits_of(value) | static_cast<uintptr_t>(head_dim * es) |
@@ -637,7 +640,10 @@ int qd_kv_gather_q8(void* key, void* value, const void* k_cache, const void* v_c
                        cache_dtype);
   if (bad != QD_OK) return bad;
   if (batch == 0 || tokens == 0) return QD_OK;
+  if (tokens > 1 && std::min(k_stride, v_stride) < static_cast<int64_t>(kv_heads) * head_dim)
+    return q8_fail(nullptr, 0, "rows of key and value must not overlap");
   p.parts = tokens / kGatherRows + batch;
+  if (p.parts > kMaxGrid) return q8_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
   p.by_page = packed_divide_by(static_cast<uint32_t>(block_size));
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   const bool out16 = (bits_of(key) | bits_of(value) | static_cast<uintptr_t>(k_stride * es) |

@@ -283,6 +283,8 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
     flags |= QD_FLAG_FORCE_GENERIC;
   const PrefillPlan pl =
       prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, window, sinks, flags);
+  // Threads of a launch are counted in 32 bits.
+  if (pl.grid >= (1 << 24)) return prefill_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return prefill_fail(nullptr, 0, "workspace too small or not 16-byte aligned");
   PrefillParams p;

@@ -596,6 +596,9 @@ size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tok
  * does not reach that query's row.  q [q_tokens, q_heads, head_dim], key and
  * value [k_tokens, kv_heads, head_dim], their tokens q_stride, k_stride and
  * v_stride elements apart; out is contiguous.
+ * Calls of more than 2^24 workgroups are refused: 2^24 rows (queries x q-heads)
+ * of the VALU kernel, which takes unaligned tensors and rows of no whole 16
+ * bytes, or 2^31 of the other.
  * flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
 int qd_gqa_prefill(const void* q, const void* key, const void* value, const int32_t* cu, const int32_t* cu_k,
                    void* out, void* workspace, size_t workspace_bytes, int batch, int64_t q_tokens, int64_t k_tokens,
@@ -636,7 +639,8 @@ int qd_kv_gather_q8_validate(const qd_tensor_desc* key, const qd_tensor_desc* va
 
 /* Row cu[b] + i of key and value becomes token i of sequence b's cache, for
  * every i < context_lens[b] inside the sequence's rows and its table; other
- * rows are left as they were.  Page ids are clamped to the pool. */
+ * rows are left as they were.  Page ids are clamped to the pool.  Rows of key,
+ * and of value, must not overlap. */
 int qd_kv_gather_q8(void* key, void* value, const void* k_cache, const void* v_cache, const float* k_scales,
                     const float* v_scales, const int32_t* block_table, const int32_t* context_lens,
                     const int32_t* cu, int batch, int64_t tokens, int kv_heads, int head_dim, int block_size,

@@ -819,3 +819,53 @@ def test_streams_and_graphs(gpu):
         eager = step()
         for x, y in zip(replayed, eager):
             assert torch.equal(bits(x), bits(y)), i
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_split_prompts_on_streams_and_in_graphs(gpu, dtype):
+    """Two calls at once whose keys are split, and captured ones that share nothing but the graphs' memory."""
+    say(f"split prompts, streams and graphs {dtype}")
+    a, b = ([x.to(gpu) for x in prefill_case(dtype, nq, nk, 8, 2, 64, seed=s)] for nq, nk, s in (([9, 2], [2000, 1500], 1), ([3], [2500], 2)))
+    run = lambda c: attention_amd.gqa_prefill(*c[:4], cu_seqlens_k=c[4])  # noqa: E731
+    want = [run(a), run(b)]
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s, c in zip(side, (a, b)):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(run(c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    graphs, out = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g, c in zip(graphs, (a, b)):
+        with torch.cuda.graph(g):
+            out.append(run(c))
+    for i in range(3):
+        a[0].mul_(-1)
+        b[2].mul_(0.5)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        replayed = [x.clone() for x in out]
+        assert all(torch.equal(x, y) for x, y in zip(replayed, (run(a), run(b)))), i
+
+
+def test_decode_short_tables_in_a_graph(gpu):
+    """The launch without a merge, captured; lengths change between replays."""
+    say("short tables in a graph")
+    case = [x.to(gpu) for x in decode_case(HF, "int8", [90, 0, 33], 8, 2, 128, 16, seed=4)]
+    assert cabi.gqa_decode_q8_info(3, 8, 2, 128, 16, case[5].shape[1], cabi.DTYPE[HF])[0] == 1
+    graph = torch.cuda.CUDAGraph()
+    attention_amd.gqa_decode_q8(*case)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = attention_amd.gqa_decode_q8(*case)
+    for lens in ([90, 0, 33], [1, 96, 0], [0, 0, 0], [50, 51, 52]):
+        case[6].copy_(torch.tensor(lens, dtype=torch.int32))
+        case[5].clamp_(min=0)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        assert torch.equal(replayed, attention_amd.gqa_decode_q8(*case)), lens
+        assert not replayed[[i for i, n in enumerate(lens) if n == 0]].any()

@@ -245,6 +245,28 @@ def test_append_refuses_overlap_and_missing_rows():
         assert cabi.lib().qd_kv_append_q8(*a.values()) == 0 and cabi.lib().qd_kv_gather_q8(*a.values()) == 0
 
 
+def test_gather_refuses_rows_that_overlap():
+    for over in (dict(k_stride=0), dict(v_stride=127), dict(k_stride=64)):
+        a = rows_args()
+        a.update(over)
+        assert cabi.lib().qd_kv_gather_q8(*a.values()) == 1
+        assert cabi.error_string(1) == "rows of key and value must not overlap"
+
+
+def test_launches_beyond_the_grid_are_refused():
+    text = "tensor sizes exceed int32 CUDA launch limits"
+    a = prefill_args()
+    a.update(Tq=1 << 22, Tk=1 << 22, cu_k=None, flags=cabi.QD_FLAG_FORCE_GENERIC)   # 2^25 rows
+    assert cabi.lib().qd_gqa_prefill(*a.values()) == 1 and cabi.error_string(1) == text
+    a = prefill_args()
+    a.update(B=1 << 23, Tq=1 << 23, Tk=1 << 23, cu_k=None)
+    assert cabi.lib().qd_gqa_prefill(*a.values()) == 1 and cabi.error_string(1) == text
+    a = rows_args()
+    a.update(T=1 << 30, P=16)
+    assert cabi.lib().qd_kv_append_q8(*a.values()) == 1 and cabi.error_string(1) == text
+    assert cabi.lib().qd_kv_gather_q8(*a.values()) == 1 and cabi.error_string(1) == text
+
+
 def decode_descs():
     return dict(q=desc([4, 8, 64], F16), kc=desc([9, 16, 2, 64], I8), vc=desc([9, 16, 2, 64], I8), ks=desc([9, 2], F32),
                 vs=desc([9, 2], F32), table=desc([4, 3], I32), lens=desc([4], I32))
