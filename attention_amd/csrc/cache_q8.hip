@@ -176,20 +176,22 @@ __device__ __forceinline__ Packed packed_at(const CacheParams& p, int per, int s
 
 // A wave writes a run (the new tokens of one page) of one head's keys or values:
 // largest value, scale, elements, with the rows in registers in between where
-// they fit (kHold pieces per lane, 1024 in all: 64 tokens of 128 16-bit
-// elements); longer runs are read again, from L2.  What it moves is 2 T rows in
-// and half as many bytes out: HBM bounds it for prompts, the round trips
-// position -> page -> scale for single tokens (TOKENS: a row per sequence, read
+// they fit (HOLD pieces of 16 bytes per lane: 16 are 64 tokens of 128 16-bit
+// elements, 32 twice that); longer runs are read again, from L2.  What it moves is 2
+// T rows in and half as many bytes out: HBM bounds it for prompts, the round trips
+// position -> page -> scale for single tokens (HOLD 0: a row per sequence, read
 // beside the position).  24 prompts of up to 6000 tokens, 8 heads of 128, bf16 to
-// e4m3: 93 us, 5.0 TB/s (a copy reaches 4.8); with the pieces' addresses kept from
-// reading to writing it was 138 (160 registers, three waves per SIMD instead of
-// four).  512 single tokens: 4.9 us, of 3 that an empty trip takes.
+// e4m3, pages of 64: 93 us, 5.0 TB/s (a copy reaches 4.8); with the pieces' addresses
+// kept from reading to writing it was 138 (160 registers, three waves per SIMD
+// instead of four).  Up to 4000 tokens, pages of 128: 72 us, 101 with the runs read
+// twice.  512 single tokens: 4.2 us, of 3 that an empty trip takes.
 // grid ceil(2 parts Hkv / 4), block 256; a workgroup's waves have neighbouring
 // heads, whose rows are neighbours in memory.
-template <int DT, int KIND, int VEC, bool TOKENS>
-__global__ __launch_bounds__(256, 4) void append_q8_kernel(CacheParams p) {
+template <int DT, int KIND, int VEC, int HOLD>
+__global__ __launch_bounds__(256, HOLD == 32 ? 2 : 4) void append_q8_kernel(CacheParams p) {
   using S = typename Elem<DT>::S;
-  constexpr int kHold = !TOKENS ? 16 : VEC == 1 ? 4 : 1;
+  constexpr bool TOKENS = HOLD == 0;
+  constexpr int kHold = !TOKENS ? HOLD : VEC == 1 ? 4 : 1;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= 2 * p.parts * p.Hkv) return;
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(256, 4) void append_q8_kernel(CacheParams p) {
       next(w);
     }
   };
-  constexpr int kSome = 4;  // pieces in flight of a longer run
+  constexpr int kSome = 8;  // pieces in flight of a longer run
   Walk all = begin();
   if (held_all) {
     weigh(held, all);
@@ -607,14 +609,18 @@ int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_c
   by_types(dtype, cache_dtype, [&](auto dt, auto kind) {
     constexpr int DT = decltype(dt)::value, KIND = decltype(kind)::value, VEC = DT == QD_DTYPE_F32 ? 4 : 8;
     const dim3 grid(static_cast<uint32_t>((2 * p.parts * kv_heads + 3) / 4));
-    if (vec && cu)
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, false>), grid, dim3(256), 0, st, p);
+    // A page's pieces that 32 per lane hold and 16 do not.
+    const int64_t pieces = static_cast<int64_t>(block_size) * per_row;
+    if (vec && cu && pieces > 64 * 16 && pieces <= 64 * 32)
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, 32>), grid, dim3(256), 0, st, p);
+    else if (vec && cu)
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, 16>), grid, dim3(256), 0, st, p);
     else if (vec)
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, true>), grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, VEC, 0>), grid, dim3(256), 0, st, p);
     else if (cu)
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, false>), grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, 16>), grid, dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, true>), grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((append_q8_kernel<DT, KIND, 1, 0>), grid, dim3(256), 0, st, p);
   });
   return launched("kv_append_q8");
 }

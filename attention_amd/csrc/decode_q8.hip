@@ -209,6 +209,10 @@ constexpr float kQ8Shift = 7.f, kQ8Lazy = 8.f;
 // of up to 2000 with one kv-head 15.8 for 12.2.
 constexpr int kQ8ItemCost = 2;
 constexpr int kQ8MinCost = 2;
+// Ranges per item from which a workgroup merges each row: one sequence of 30000
+// tokens 37.6 -> 23.9 us, of 1500 11.1 -> 10.1, 16 of 2000 (16 ranges each) 22.2 ->
+// 21.4, 20 of 2000 (12 each) 24.0 for 24.1.
+constexpr int kQ8WideMerge = 12;
 // Sequences whose prefix of costs fits the kernel's LDS.
 constexpr int kQ8MaxBalanced = 1024;
 
@@ -651,14 +655,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
 
 // Log-sum-exp merge of the items that a balanced launch split, and the rows of
 // sequences without tokens: a wave per row, LANES lanes stride its columns four at
-// a time, the others its partials.
-// grid (items, ceil(hw per / 4)), block 256.
-template <int DT, int DP>
+// a time, the others its partials; or, where items have many, a workgroup.
+// grid (items, ceil(hw per / 4) or hw per), block 256.
+template <int DT, int DP, int WAVES>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
-  constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, TEAMS = 64 / LANES, STEP = 4 * LANES;
+  constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, TEAMS = 64 / LANES * WAVES, STEP = 4 * LANES;
+  __shared__ f32x2 stats[4];
+  __shared__ f32x4 joined[4][LANES];
   const int item = static_cast<int>(blockIdx.x), b = packed_divide(blockIdx.x, p.by_groups), hg = item - b * p.groups;
   const int lane = static_cast<int>(threadIdx.x) & 63;
-  const int row = 4 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x >> 6);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = WAVES == 4 ? static_cast<int>(blockIdx.y) : 4 * static_cast<int>(blockIdx.y) + wv;
   if (row >= p.hw * p.per) return;
   const int wh = row / p.per, n = row - wh * p.per;
   const int v = hg * p.hw + wh, h = v / p.chunks, g = (v - h * p.chunks) * p.per + n;
@@ -668,7 +675,7 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
   const bool empty = q8_len(p, b) == 0;
   const int first = empty ? 0 : first_of, count = empty ? 0 : last_of - first_of + 1;
   if (count == 1) return;
-  const int team = lane / LANES, l = lane % LANES;
+  const int team = lane / LANES + (WAVES == 4 ? 64 / LANES * wv : 0), l = lane % LANES;
   const int64_t slot_floats = static_cast<int64_t>(p.hw) * 16 * (p.D + 4);
   auto part = [&](int s) {
     return p.part + (2 * static_cast<int64_t>(first + s) + (s == 0 ? 1 : 0)) * slot_floats + (wh * 16 + n) * (p.D + 4);
@@ -716,6 +723,24 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
       sum = f * sum + of * os;
       a = f * a + of * oa;
       mx = most;
+    }
+    if constexpr (WAVES == 4) {
+      if (lane < LANES) joined[wv][lane] = a;
+      if (lane == 0) stats[wv] = f32x2{mx, sum};
+      __syncthreads();
+      float most = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) most = fmaxf(most, stats[w][0]);
+      const float ref = most == -INFINITY ? 0.f : most;
+      sum = 0.f;
+      a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = fast_exp2(stats[w][0] - ref);
+        sum += f * stats[w][1];
+        a += f * joined[w][l];
+      }
+      __syncthreads();
     }
     if (team == 0 && d < p.D) {
       const bool has = sum > 0.f || sum != sum;
@@ -835,10 +860,12 @@ hipError_t launch_mfma(const Q8Params& p, int grid, hipStream_t st) {
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(grid)), dim3(256), lds, st, p);
-  if (p.W > 0)
-    hipLaunchKernelGGL((q8_merge_kernel<DT, DP>),
-                       dim3(static_cast<uint32_t>(p.B * p.groups), static_cast<uint32_t>((p.hw * p.per + 3) / 4)), dim3(256),
-                       0, st, p);
+  if (p.W == 0) return hipGetLastError();
+  const uint32_t items = static_cast<uint32_t>(p.B * p.groups), rows = static_cast<uint32_t>(p.hw * p.per);
+  if (p.W >= kQ8WideMerge * p.B * p.groups)
+    hipLaunchKernelGGL((q8_merge_kernel<DT, DP, 4>), dim3(items, rows), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((q8_merge_kernel<DT, DP, 1>), dim3(items, (rows + 3) / 4), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

@@ -412,6 +412,8 @@ APPEND = [
     (BF, "int8", [9, 0, 2], [4, 5, 6], 2, 80, 1),
     (BF, "e4m3", [10, 0], [700, 300], 1, 256, 256),  # runs longer than the registers hold
     (FP, "int8", [100, 0], [300, 500], 1, 256, 512),
+    (BF, "e4m3", [5, 0, 127], [300, 128, 2], 2, 128, 128),  # twice the pieces per lane
+    (FP, "int8", [3, 64], [100, 1], 2, 128, 64), (HF, "int8", [0, 70], [64, 200], 1, 256, 64),
 ]
 
 
