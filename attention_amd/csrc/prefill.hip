@@ -154,7 +154,8 @@ PrefillPlan prefill_plan(int batch, int64_t q_tokens, int64_t k_tokens, int q_he
   pl.grid = q_tokens * q_heads;
   const int group = q_heads / kv_heads;
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
-  if (head_dim * es % 16 != 0 || (flags & QD_FLAG_FORCE_GENERIC)) return pl;
+  if (head_dim * es % 16 != 0 || static_cast<int64_t>(q_heads) * head_dim > (1 << 21) || (flags & QD_FLAG_FORCE_GENERIC))
+    return pl;
   const auto grid_of = [&](int rows) { return (q_tokens * group / rows + batch + 1) * kv_heads; };
   pl.dp = es == 4 ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256)
                   : (head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : head_dim <= 192 ? 192 : 256);
@@ -279,7 +280,7 @@ int qd_gqa_prefill(const void* q, const void* key, const void* value, const int3
         reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(q_stride * es) |
         static_cast<uintptr_t>(k_stride * es) | static_cast<uintptr_t>(v_stride * es)) &
        15u) != 0 ||
-      std::max({q_stride, k_stride, v_stride}) > (int64_t{1} << 22))
+      std::max({q_stride, k_stride, v_stride}) > (int64_t{1} << 21))
     flags |= QD_FLAG_FORCE_GENERIC;
   const PrefillPlan pl =
       prefill_plan(batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, dtype, window, sinks, flags);

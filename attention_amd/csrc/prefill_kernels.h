@@ -159,6 +159,20 @@ __device__ __forceinline__ PrefillRow prefill_row(const PrefillParams& p, const 
   r.g = y - r.query * p.G;
   return r;
 }
+// Bytes of a row from query q0's first head on, where queries lie `pitch` and heads
+// `head` bytes apart: query pitch + (y - query G) head, in products of 24 bits
+// (heads and strides within 2^21 elements).
+struct PrefillRowAt {
+  const PrefillParams& p;
+  int rest, rest_pitch, head;
+  __device__ __forceinline__ PrefillRowAt(const PrefillParams& p, const PrefillItem& x, int pitch, int head)
+      : p(p), rest(x.rest), rest_pitch(pitch - p.G * head), head(head) {}
+  __device__ __forceinline__ uint32_t operator()(int row) const {
+    const int y = rest + row;
+    const int query = p.G > 4096 ? static_cast<int>(y >= p.G) : static_cast<int>((static_cast<float>(y) + 0.5f) * p.inv_g);
+    return static_cast<uint32_t>(__mul24(query, rest_pitch) + __mul24(y, head));
+  }
+};
 // Position of a row of the workgroup, or of its last one.
 __device__ __forceinline__ int prefill_place(const PrefillParams& p, const PrefillItem& x, int row) {
   return max(x.at0 + prefill_row(p, x, min(row, x.rows - 1)).query, -1);
@@ -423,8 +437,8 @@ __device__ __forceinline__ void prefill_store_rows(const PrefillParams& p, const
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const float sum = prefill_sum_halves(l[nb]);
-    const bool has = sum > 0.f || sum != sum;
-    const float scale = has ? 1.f / sum : 0.f;
+    // Without weights the output is 0 already (what was not finite there was left out).
+    const float scale = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     char* row = place + (32 * nb + n32) * Sh::kRow;
     const int swizzle = 16 * prefill_swizzle(Sh::kSlots, n32);
 #pragma unroll
@@ -433,22 +447,23 @@ __device__ __forceinline__ void prefill_store_rows(const PrefillParams& p, const
       for (int e = 0; e < 16; e += 4) {
         f32x4 y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = has ? acc[c][nb][e + j] * scale : 0.f;
+        for (int j = 0; j < 4; ++j) y[j] = acc[c][nb][e + j] * scale;
         // Column 32 c + 2 e + 4 half.
         *reinterpret_cast<u32x2*>(row + ((64 * c + 4 * e) ^ swizzle) + 8 * half) =
             u32x2{MfmaOps<DT>::pack2(y[0], y[1]), MfmaOps<DT>::pack2(y[2], y[3])};
       }
   }
   const int row_bytes = 2 * p.D;
+  char* base = const_cast<char*>(prefill_scalar(static_cast<const char*>(p.out) +
+                                                (static_cast<int64_t>(x.q0) * p.Hq + static_cast<int64_t>(x.h) * p.G) * row_bytes));
+  const PrefillRowAt at(p, x, p.Hq * row_bytes, row_bytes);
 #pragma unroll
   for (int i = 0; i < NB * Sh::kSlots / 2; ++i) {
     const int r = (64 * i + lane) / Sh::kSlots;
     const int slot = lane & (Sh::kSlots - 1), col = 16 * (slot ^ prefill_swizzle(Sh::kSlots, r));
     const u32x4 y = *reinterpret_cast<const u32x4*>(place + r * Sh::kRow + 16 * slot);
     if (wave_row + r >= x.rows || col >= row_bytes) continue;
-    const PrefillRow row = prefill_row(p, x, wave_row + r);
-    const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
-    *reinterpret_cast<u32x4*>(static_cast<char*>(p.out) + at * row_bytes + col) = y;
+    *reinterpret_cast<u32x4*>(base + (at(wave_row + r) + col)) = y;
   }
 }
 
@@ -549,7 +564,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
 //
 // A workgroup's start and end (which rows, operands' first trip, output) take 17000
 // cycles, of which the other workgroup of its CU can use most: 16 prompts of 65 to
-// 2000 tokens run at 740 TFLOP/s.  128 rows per workgroup and two workgroups per CU:
+// 2000 tokens run at 750 TFLOP/s.  128 rows per workgroup and two workgroups per CU:
 // eight waves of one (986 TFLOP/s then, against 1120) wait for each other, one wave of 64 rows per
 // SIMD (972) issues an instruction every five cycles at most.
 template <int DT, int DP, int NB, int NW>
@@ -595,7 +610,11 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
       for (int c = 0; c < kCols; ++c) acc[c][nb] = f32x16{};
     }
   };
-  clear();
+  // Wide heads' accumulators lie in both register files and are cleared ahead of the
+  // loop (4 x 2048 tokens, 16 heads of 256: 192 us, 219 in it); others in it, where
+  // they are not copied (64 prompts of 200 tokens, heads of 128: 82 us for 84).
+  constexpr bool kClearAhead = DP > 128;
+  if (kClearAhead || x.tiles == 0) clear();
   if (x.tiles == 0) {  // the same for all waves
     if (p.splits > 1)
       prefill_store<DT, DP, NB>(p, x, wave_row, acc, m, l);
@@ -608,15 +627,14 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   {
     const char* base = prefill_scalar(static_cast<const char*>(p.q) +
                                       (x.q0 * p.q_stride + static_cast<int64_t>(x.h) * p.G * p.D) * Sh::kES);
-    const uint32_t q_bytes = static_cast<uint32_t>(p.q_stride * Sh::kES);
+    const PrefillRowAt at(p, x, static_cast<int>(p.q_stride) * Sh::kES, load.row_bytes);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + Sh::rows_at(wv));
 #pragma unroll
     for (int i = 0; i < NB * Sh::kSlots / 2; ++i) {
       const int r = (64 * i + lane) / Sh::kSlots;
       const uint32_t col = 16 * ((lane & (Sh::kSlots - 1)) ^ prefill_swizzle(Sh::kSlots, r));
-      const PrefillRow row = prefill_row(p, x, min(wave_row + r, x.rows - 1));
       if (static_cast<int>(col) < load.row_bytes)
-        tile_load_lds<false>(base, row.query * q_bytes + row.g * load.row_bytes + col, to + 1024 * i);
+        tile_load_lds<false>(base, at(min(wave_row + r, x.rows - 1)) + col, to + 1024 * i);
     }
   }
   load(0, prefill_first<64>(x, 0), k_buf(0));
@@ -806,6 +824,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
   // them at the end.
 #pragma unroll 1
   for (bool careful = false;; careful = true) {
+    if constexpr (!kClearAhead) clear();
     f32x16 s0[NB], s1[NB];
     Weights w0, w1;
     // The first K has arrived, and every wave has its queries.
@@ -895,7 +914,6 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) acc[i % kCols][nb] = PrefillMma<DT>::mma(a, w1.w[i / kCols][nb], acc[i % kCols][nb]);
     }
-    if (x.tiles & 1) next_buffers();  // as at the start: K's first, V's second
     if (!careful) {
       float test[4] = {0.f, 0.f, 0.f, 0.f};  // NaN if anything is not finite
 #pragma unroll
@@ -910,11 +928,13 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
       if (all != all) *word = 1;
       tile_barrier();
       if (__builtin_amdgcn_readfirstlane(*word) == 0) break;
-      clear();
+      if constexpr (kClearAhead) clear();
+      if (x.tiles & 1) next_buffers();  // as at the start: K's first, V's second
       load(0, prefill_first<64>(x, 0), k_buf(0));
       load(1, prefill_first<64>(x, 0), v_buf(0));
       continue;
     }
+    if (x.tiles & 1) next_buffers();
     // A product of what is visible with the flags of values that are not finite.
 #pragma unroll 1
     for (int t = 0; t < x.tiles; ++t) {

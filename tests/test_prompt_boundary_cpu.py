@@ -120,6 +120,8 @@ def test_prefill_plans_fit_the_launch():
     generic = cabi.QD_FLAG_FORCE_GENERIC
     assert cabi.gqa_prefill_info(1, 10, 10, 8, 2, 64, BF16, generic)[:2] == (0, 80)
     assert cabi.gqa_prefill_info(1, 10, 10, 7, 2, 64)[0] == -1
+    assert cabi.gqa_prefill_info(1, 10, 10, 1 << 13, 8, 256, BF16)[0] == 1
+    assert cabi.gqa_prefill_info(1, 10, 10, 1 << 14, 8, 256, BF16)[0] == 0  # a token's heads: 2^21 elements at most
     for B, Tq, Hq, Hkv, D in ((1, 1, 1, 1, 64), (16, 20000, 32, 8, 128), (1000, 7, 71, 1, 64), (3, 50, 4, 4, 256),
                               ((1 << 24) - 1, 1, 1, 1, 64), (1, (1 << 31) // 32 - 1, 32, 1, 128)):
         for dtype in (F32, F16, BF16):
