@@ -557,16 +557,16 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
 // cycles, a conversion and a sum of two), for heads of 64 four.  What bounds it:
 // products of random data alone run at 1709 TFLOP/s (the card's power takes the
 // clock to 1.7 GHz), with that much softmax beside them and nothing else at 1267;
-// one prompt of 12001 tokens, 32 heads of 128, takes 1098 us, 1076 TFLOP/s, with the
-// clock at 1.55 GHz and the matrix cores busy for 57% of it.  16x16x32 products need
+// one prompt of 12001 tokens, 32 heads of 128, takes 1065 to 1115 us, 1060 to 1110
+// TFLOP/s, with the clock at 1.6 GHz and the matrix cores busy for 57% of it.  16x16x32 products need
 // twice the issue slots and ran at 1116 beside the same softmax.  Heads of 64 (16 and
 // 32 of 1000 to 8192 tokens) reach 650 to 720 TFLOP/s, bound by vector instructions.
 //
 // A workgroup's start and end (which rows, operands' first trip, output) take 17000
 // cycles, of which the other workgroup of its CU can use most: 16 prompts of 65 to
 // 2000 tokens run at 750 TFLOP/s.  128 rows per workgroup and two workgroups per CU:
-// eight waves of one (986 TFLOP/s then, against 1120) wait for each other, one wave of 64 rows per
-// SIMD (972) issues an instruction every five cycles at most.
+// eight waves of one (986 TFLOP/s then, against 1120) wait for each other, one wave
+// of 64 rows per SIMD (972) issues an instruction every five cycles at most.
 template <int DT, int DP, int NB, int NW>
 __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pipe_kernel(PrefillParams p) {
   using Sh = PrefillShape<DT, DP, NB, NW>;
