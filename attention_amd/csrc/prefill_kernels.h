@@ -500,8 +500,9 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
       a *= old;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        // A part without weight has no say, whatever it holds.
-        if (s0 + i >= p.splits || ml[i][0] == -INFINITY) continue;
+        // A part without weight has no say, whatever it holds.  One whose scores are
+        // all NaN has a NaN for its sum, which goes on to the row.
+        if (s0 + i >= p.splits || (ml[i][0] == -INFINITY && ml[i][1] == 0.f)) continue;
         const float f = fast_exp2(ml[i][0] - ref);
         sum += f * ml[i][1];
         a += f * x[i];

@@ -1,0 +1,62 @@
+"""GPU tests of prompt attention and of 8-bit caches where scores, scales, values and
+sizes are far from ordinary.  Every case prints its name first."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from attention_amd import cabi
+from oracle.prompt_oracle import oracle_prefill
+from tests.test_gpu_prompt import BF, FP, HF, f64, prefill, prefill_case, prefill_tolerance, say
+
+pytestmark = pytest.mark.gpu
+
+
+def split_bytes(case, window=0, sinks=0):
+    q, k, _, cu, _ = case
+    return cabi.lib().qd_gqa_prefill_workspace_bytes(cu.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
+                                                     cabi.DTYPE[q.dtype], window, sinks, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("flags", [None, cabi.QD_FLAG_FORCE_GENERIC])
+def test_prefill_split_nan_scores(gpu, dtype, flags):
+    """A NaN query, and NaN keys that are all that a row sees of a part, give NaN rows, and no others."""
+    say(f"split NaN scores {dtype} flags {flags}")
+    case = prefill_case(dtype, [6], [3000], 4, 2, 128, seed=31)
+    assert split_bytes(case) > 0
+    q, k, v, cu, cu_k = case
+    want, spread, size = oracle_prefill(f64(q), f64(k), f64(v), cu.tolist(), cu_k.tolist(), 0, 0, 128 ** -0.5)
+    tol = prefill_tolerance(case, want, spread, size)
+    q[2, 1, 77] = float("nan")
+    for keys in (None, slice(0, 1000), slice(1500, 2990), slice(2995, 2996)):
+        kk = k.clone()
+        hit = np.zeros((q.shape[0], 4), dtype=bool)
+        hit[2, 1] = True
+        if keys is not None:
+            kk[keys, 1, 5] = float("nan")
+            hit[max(0, keys.start - 2994):6, 2:] = True  # query i sees the keys up to 2994 + i
+        out = f64(prefill(gpu, (q, kk, v, cu, cu_k), flags=flags))
+        assert np.isnan(out[hit]).all(), keys
+        assert (np.abs(out - want)[~hit] <= tol[~hit]).all(), keys
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_prefill_split_one_nan_key(gpu, dtype):
+    """One NaN key.  For one row it is the only key that it sees of its part: parts begin at token 1344, and the
+    first ends with token 1471 (fp32: 1407), which is the first that query 98 (34) sees."""
+    case = prefill_case(dtype, [128], [3000], 2, 2, 64, seed=32)
+    assert split_bytes(case, 1500) > 0
+    q, k, v, cu, cu_k = case
+    want, spread, size = oracle_prefill(f64(q), f64(k), f64(v), cu.tolist(), cu_k.tolist(), 1500, 0, 0.125)
+    tol = prefill_tolerance(case, want, spread, size)
+    for token in (1407, 1471):
+        say(f"split, one NaN key {dtype} {token}")
+        kk = k.clone()
+        kk[token, 1, 3] = float("nan")
+        out = f64(prefill(gpu, (q, kk, v, cu, cu_k), window=1500))
+        hit = np.zeros((q.shape[0], 2), dtype=bool)
+        hit[:token - 1373 + 1, 1] = True  # query i sees the keys from 1373 + i on
+        assert np.isnan(out[hit]).all(), token
+        assert (np.abs(out - want)[~hit] <= tol[~hit]).all(), token
