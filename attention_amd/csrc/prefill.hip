@@ -40,8 +40,9 @@ __global__ __launch_bounds__(256) void prefill_generic_kernel(PrefillParams p) {
   const S* q = static_cast<const S*>(p.q) + t * p.q_stride + static_cast<int64_t>(hq) * p.D;
   for (int d = tid; d < p.D; d += 256) qs[d] = E::to_f(q[d]);
   const int b = packed_find(p.cu, p.B, p.Tq, 1, 1, 0, t);
-  const int q0 = packed_start(p.cu, b, p.Tq), q1 = packed_start(p.cu, b + 1, p.Tq);
-  const int k0 = packed_start(p.cu_k, b, p.Tk), k1 = packed_start(p.cu_k, b + 1, p.Tk);
+  const int next = min(b + 1, p.B);  // no sequences: cu has one entry, and no row sees anything
+  const int q0 = packed_start(p.cu, b, p.Tq), q1 = packed_start(p.cu, next, p.Tq);
+  const int k0 = packed_start(p.cu_k, b, p.Tk), k1 = packed_start(p.cu_k, next, p.Tk);
   // Keys [0, sinks) and [lo, at] are seen; none by rows outside the sequences.
   const int at = t < q1 ? max(max(k1 - k0, 0) - (q1 - q0) + (t - q0), -1) : -1;
   const int lo = p.window > 0 ? max(at - p.window + 1, 0) : 0;

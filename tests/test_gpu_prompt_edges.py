@@ -60,3 +60,17 @@ def test_prefill_split_one_nan_key(gpu, dtype):
         hit[:token - 1373 + 1, 1] = True  # query i sees the keys from 1373 + i on
         assert np.isnan(out[hit]).all(), token
         assert (np.abs(out - want)[~hit] <= tol[~hit]).all(), token
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("flags", [0, cabi.QD_FLAG_FORCE_GENERIC])
+@pytest.mark.parametrize("D", [64, 33])
+def test_prefill_no_sequences(gpu, dtype, flags, D):
+    """Only rows behind the last sequence, whatever lies behind the one entry of cu_seqlens."""
+    say(f"no sequences {dtype} flags {flags} {D}")
+    q, k = torch.ones(5, 4, D, device=gpu, dtype=dtype), torch.ones(5, 2, D, device=gpu, dtype=dtype)
+    cu, cu_k = (torch.tensor([0, 5, 5], dtype=torch.int32, device=gpu)[:1] for _ in range(2))
+    for ends in (None, cu_k):
+        out = torch.full_like(q, float("nan"))
+        assert cabi.gqa_prefill(q, k, k, cu, ends, out, scale=0.1, flags=flags) == 0
+        assert not out.any()
