@@ -591,8 +591,10 @@ int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_c
   if (!apart(k_scales, v_scales, 4 * static_cast<uint64_t>(kv_heads)))
     return q8_fail(nullptr, 0, "k_scales and v_scales must not overlap");
   p.parts = cu ? tokens / block_size + 2 * static_cast<int64_t>(batch) : batch;
-  // Rows and items are counted in 32 bits, past their ends.
-  if (tokens > INT32_MAX - 255 || 2 * p.parts * kv_heads > 4 * kMaxGrid)
+  // Rows and items are counted in 32 bits, past their ends: a lane's pieces of a run
+  // are up to 64 rows apart, and go on eight at a time.
+  if (tokens > INT32_MAX - 255 || std::min<int64_t>(tokens, block_size) > INT32_MAX - 1023 ||
+      2 * p.parts * kv_heads > 4 * kMaxGrid)
     return q8_fail(nullptr, 0, "tensor sizes exceed int32 CUDA launch limits");
   const int es = dtype == QD_DTYPE_F32 ? 4 : 2;
   const bool vec = (bits_of(key) | bits_of(value) | static_cast<uintptr_t>(head_dim * es) |

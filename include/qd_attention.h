@@ -625,7 +625,8 @@ int qd_kv_append_q8_validate(const qd_tensor_desc* key, const qd_tensor_desc* va
  * Other rows keep their elements.  Sequences with a negative position write
  * nothing, nor do tokens past the table or in pages outside the pool.  Pages
  * that are written to must be their sequence's own.  Caches, scales and inputs
- * must not overlap (the caches and the scales are checked). */
+ * must not overlap (the caches and the scales are checked).  Calls that could
+ * write 2^31 - 1023 tokens or more to one page are refused. */
 int qd_kv_append_q8(const void* key, const void* value, void* k_cache, void* v_cache, float* k_scales,
                     float* v_scales, const int32_t* block_table, const int32_t* positions, const int32_t* cu,
                     int batch, int64_t tokens, int kv_heads, int head_dim, int block_size, int max_pages,
