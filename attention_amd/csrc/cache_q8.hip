@@ -288,8 +288,8 @@ __global__ __launch_bounds__(256, HOLD == 32 ? 2 : 4) void append_q8_kernel(Cach
     }
   }
   const float fresh = power_scale<KIND>(q8_dpp_max(most.f32_bits()));
-  // A NaN on either side stays.
-  const float scale = slot0 == 0 || !(old >= fresh) ? (old != old ? old : fresh) : old;
+  // A NaN on either side stays; a caller's own scale may be negative.
+  const float scale = slot0 == 0 || !(fabsf(old) >= fresh) ? (old != old ? old : fresh) : old;
   if (slot0 > 0 && !(scale == old)) {
     // The page's earlier rows, on the new scale (a power of two, so the factor
     // is exact).

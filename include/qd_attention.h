@@ -618,7 +618,8 @@ int qd_kv_append_q8_validate(const qd_tensor_desc* key, const qd_tensor_desc* va
  * |x| of the new rows and s = 2^e the smallest power of two with a <= s * 448
  * (e4m3) or a <= s * 127 (int8), at least 2^-100.  If the call begins the page
  * (its first new row is the page's first), its scale becomes s; else the larger
- * of s and the old one, and if that is s, the rows before are rounded to it.
+ * in magnitude of s and the old one, and if that is s, the rows before are rounded
+ * to it.
  * Elements are x / scale rounded to nearest, ties to even.  With an Inf or NaN
  * among the new rows, or if s would pass 2^100, the scale becomes NaN, and the
  * elements are unspecified.

@@ -85,7 +85,7 @@ def oracle_append(key, value, k_cache, v_cache, k_scales, v_scales, table, posit
                             scale = power_scale(np.max(np.abs(new[:, h])), kind)
                         if at % P:
                             old = scales[phys, h]
-                            scale = np.nan if np.isnan(old) or np.isnan(scale) else max(old, scale)
+                            scale = np.nan if np.isnan(old) or np.isnan(scale) else old if abs(old) >= scale else scale
                             if scale != old:
                                 cache[phys, :at % P, h] = round_to(cache[phys, :at % P, h] * (old / scale), kind)
                         with np.errstate(invalid="ignore"):

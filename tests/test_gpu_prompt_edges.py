@@ -8,7 +8,7 @@ import torch
 
 from attention_amd import cabi
 from oracle.prompt_oracle import oracle_prefill
-from tests.test_gpu_prompt import BF, FP, HF, f64, prefill, prefill_case, prefill_tolerance, say
+from tests.test_gpu_prompt import BF, FP, HF, cache_case, check_append, f64, prefill, prefill_case, prefill_tolerance, say, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,15 @@ def test_prefill_no_sequences(gpu, dtype, flags, D):
         out = torch.full_like(q, float("nan"))
         assert cabi.gqa_prefill(q, k, k, cu, ends, out, scale=0.1, flags=flags) == 0
         assert not out.any()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_append_goes_on_with_scales_below_zero(gpu, kind):
+    """A page's scale may be negative: it stays while its magnitude holds the new rows, and is replaced else."""
+    say(f"scales below zero {kind}")
+    kc, vc, ks, vs, table, gen = cache_case(kind, [9, 20, 3, 40], [5, 5, 1, 30], 2, 64, 16, power=False)
+    key = torch.randn(41, 2, 64, generator=gen).to(BF)
+    ks, vs = -32 * ks, -vs
+    at, cu = torch.tensor([9, 20, 3, 40], dtype=torch.int32), starts([5, 5, 1, 30])
+    d = check_append(gpu, key * 100, key * 0.001, kc, vc, ks, vs, table, at, cu, kind, "small and large scales below zero")
+    assert (d[3] < 0).any() and (d[2] < 0).any() and (d[2] > 0).any()
