@@ -111,6 +111,9 @@ struct PrefillMma {
 // see one: sums over a tile of up to 64 tokens keep the three apart.
 constexpr float kPrefillPlusInf = 1.f, kPrefillMinusInf = 256.f, kPrefillNan = 32768.f;
 
+// Scaled scores (of base 2) from which a row's weights come of differences.
+constexpr float kPrefillFar = 0x1p20f;
+
 template <int DT>
 __device__ __forceinline__ float prefill_flag(typename Elem<DT>::S x) {
   const float f = Elem<DT>::to_f(x);
@@ -384,7 +387,8 @@ __device__ __forceinline__ float prefill_add_bad(float y, float seen) {
 }
 
 // out rows of a lane, or their partials: acc of column block c, element e is
-// column 32 c + 8 (e / 4) + 4 half + e % 4 of row wave_row + 32 nb + lane % 32.
+// column 32 c + 8 (e / 4) + 4 half + e % 4 of row wave_row + 32 nb + lane % 32, m a
+// score that the row's weights count from.
 template <int DT, int DP, int NB>
 __device__ __forceinline__ void prefill_store(const PrefillParams& p, const PrefillItem& x, int wave_row,
                                               const f32x16 (&acc)[DP / 32][NB], const float (&m)[NB], const float (&l)[NB]) {
@@ -400,7 +404,7 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
     const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
     if (p.splits > 1) {
       float* to = p.part + (x.split * (static_cast<int64_t>(p.Tq) * p.Hq) + at) * (p.D + 4);
-      if (half == 0) *reinterpret_cast<f32x2*>(to) = has ? f32x2{m[nb], sum} : f32x2{-INFINITY, 0.f};
+      if (half == 0) *reinterpret_cast<f32x2*>(to) = has ? f32x2{m[nb] * p.sl2, sum} : f32x2{-INFINITY, 0.f};
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
@@ -543,7 +547,10 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
 //            was one of its scores.  m moves only when a lane's weights of a
 //            step sum to more than 2^kLazy (which every weight beyond that
 //            does): the maximum is not computed otherwise, and lanes exchange
-//            nothing.
+//            nothing.  A weight is 2^(s c + r), r = -m c rounded once, and where |m c|
+//            passes 2^20 that rounding would show (past 2^27 it takes weights out of
+//            fp16's range): such rows find m in every step, and subtract before they
+//            multiply.
 //   output   O^T += V^T P^T: the score layout is already the B operand (the
 //            products sum over tokens in the order that the lanes hold them in),
 //            V^T comes from transposing LDS reads.
@@ -697,7 +704,12 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
-    return fmaxf(m, prefill_max_halves(mx) * p.sl2);
+    return fmaxf(m, prefill_max_halves(mx));
+  };
+  // What to add to scaled scores that count from m; Inf: m has to be found anew.
+  auto reference = [&](float m) {
+    const float x = m * p.sl2;
+    return fabsf(x) < kPrefillFar ? kShift - x : INFINITY;
   };
 
   u32x4 ka[kRing], va[kRing];  // operands read ahead of their products
@@ -781,9 +793,14 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
       for (int nb = 0; nb < NB; ++nb) {
         asm volatile("" : "+v"(cur[nb]));  // nothing of this is computed ahead of the branch
         const float mn = largest(cur[nb], m[nb]);
-        const float alpha = mn == m[nb] ? 1.f : fast_exp2(m[nb] - mn);
+        const float alpha = mn == m[nb] ? 1.f : fast_exp2((m[nb] - mn) * p.sl2);
         m[nb] = mn;
-        ref[nb] = mn == -INFINITY ? kShift : kShift - mn;
+        ref[nb] = reference(mn);
+        const bool far = ref[nb] == INFINITY;
+        const float from = far && mn != -INFINITY ? mn : 0.f;
+        if (far) ref[nb] = kShift;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) cur[nb][e] -= from;
         l[nb] *= alpha;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) acc[c][nb] *= alpha;
@@ -797,8 +814,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-        if (m[nb] == -INFINITY) ref[nb] = INFINITY;
+      for (int nb = 0; nb < NB; ++nb) ref[nb] = reference(m[nb]);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) l[nb] += sum[nb];
@@ -855,7 +871,7 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       m[nb] = largest(s0[nb], -INFINITY);
-      if (m[nb] != -INFINITY) ref[nb] = kShift - m[nb];
+      ref[nb] = reference(m[nb]);
     }
     tile_barrier();  // the zeros are there
 #pragma unroll
@@ -1066,16 +1082,24 @@ __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p
     for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][e]);
-    // The reference maximum moves when a score exceeds it by 2^kLazy.
-    if (__ballot(mx * p.sl2 > m[0] + kLazy)) {
-      const float mn = fmaxf(m[0], prefill_max_halves(mx) * p.sl2);
-      const float alpha = mn == m[0] ? 1.f : fast_exp2(m[0] - mn);
+    // The reference maximum moves when a weight would exceed 2^kLazy.
+    if (__ballot((mx - m[0]) * p.sl2 > kLazy)) {
+      const float mn = fmaxf(m[0], prefill_max_halves(mx));
+      const float alpha = mn == m[0] ? 1.f : fast_exp2((m[0] - mn) * p.sl2);
       m[0] = mn;
       l[0] *= alpha;
 #pragma unroll
       for (int c = 0; c < Sh::kCols; ++c) acc[c][0] *= alpha;
     }
-    const float ref = m[0] == -INFINITY ? 0.f : -m[0];
+    // As above, large scores are subtracted before they are multiplied.
+    const float from = m[0] != -INFINITY && fabsf(m[0] * p.sl2) >= kPrefillFar ? m[0] : 0.f;
+    if (__ballot(from != 0.f)) {
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[tb][e] -= from;
+    }
+    const float ref = from != 0.f || m[0] == -INFINITY ? 0.f : -m[0] * p.sl2;
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb)
 #pragma unroll

@@ -8,7 +8,8 @@ import torch
 
 from attention_amd import cabi
 from oracle.prompt_oracle import oracle_prefill
-from tests.test_gpu_prompt import BF, FP, HF, cache_case, check_append, f64, prefill, prefill_case, prefill_tolerance, say, starts
+from tests.test_gpu_prompt import (BF, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, f64, prefill, prefill_case,
+                                   prefill_tolerance, say, starts)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,74 @@ def test_append_goes_on_with_scales_below_zero(gpu, kind):
     at, cu = torch.tensor([9, 20, 3, 40], dtype=torch.int32), starts([5, 5, 1, 30])
     d = check_append(gpu, key * 100, key * 0.001, kc, vc, ks, vs, table, at, cu, kind, "small and large scales below zero")
     assert (d[3] < 0).any() and (d[2] < 0).any() and (d[2] > 0).any()
+
+
+LEVELS = {
+    "same": lambda j, n: 0 * j + 5, "negative": lambda j, n: 0 * j - 7, "rising": lambda j, n: -60 + j * 120 // n,
+    "falling": lambda j, n: 60 - j * 120 // n, "mixed": lambda j, n: (j * 37) % 101 - 50,
+}
+
+
+def far_case(dtype, nq, nk, Hq, Hkv, D, level):
+    """Scores that are exact in float32: 8 times a small whole number that each key has."""
+    q, k, v, cu, cu_k = prefill_case(dtype, nq, nk, Hq, Hkv, D, seed=41)
+    q[:], k[:] = 0, 0
+    q[:, :, 0] = 8
+    levels = LEVELS[level](torch.arange(k.shape[0]), k.shape[0])
+    k[:, :, 0] = levels[:, None].to(dtype)
+    return (q, k, v, cu, cu_k), levels.numpy()
+
+
+def far_want(case, levels):
+    """Only the largest scores that a query sees have a weight, all the same: the mean of their values."""
+    q, k, v, cu, cu_k = case
+    cu_k = cu if cu_k is None else cu_k
+    want, spread = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(len(cu) - 1):
+        q0, q1, k0, k1 = int(cu[b]), int(cu[b + 1]), int(cu_k[b]), int(cu_k[b + 1])
+        for i in range(q1 - q0):
+            seen = levels[k0:k1 - (q1 - q0) + i + 1]
+            top = f64(v)[k0 + np.flatnonzero(seen == seen.max())]
+            want[q0 + i] = np.repeat(top.mean(0), q.shape[1] // k.shape[1], 0)
+            spread[q0 + i] = np.repeat(np.abs(top).mean(0), q.shape[1] // k.shape[1], 0)
+    return want, spread
+
+
+FAR = [([300], None, 2, 1, 64), ([200, 3], None, 4, 2, 128), ([6], [3000], 4, 2, 128), ([70], None, 2, 1, 96), ([100], None, 2, 2, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("i", range(len(FAR)))
+@pytest.mark.parametrize("level", LEVELS)
+def test_prefill_far_scores(gpu, dtype, i, level):
+    """Scores of 2^16 to 2^109.  They are exact and at least 2^16 apart: weights are 0 or all the same.  Their sum of
+    n terms is off by 2 n u, their exponentials by 8 u, and both halves of the quotient are rounded as always; the
+    grid of fp16 weights is 2^-32 of the largest."""
+    case, levels = far_case(dtype, *FAR[i], level)
+    want, spread = far_want(case, levels)
+    n = case[1].shape[0]
+    tol = HALF[dtype] * np.abs(want) + (WEIGHT[dtype] + 2 * n * U + 8 * U) * spread + TINY[dtype]
+    if dtype == HF:
+        tol = tol + n * 2.0 ** -32 * case[2].abs().max().item()
+    for e in (13, 17, 18, 22, 25, 28, 33, 60, 100):
+        say(f"far scores {dtype} {FAR[i]} {level} 2^{e}")
+        for flags in (None, cabi.QD_FLAG_FORCE_GENERIC):
+            out = f64(prefill(gpu, case, flags=flags, scale=2.0 ** e))
+            assert (np.abs(out - want) <= tol).all(), (e, flags)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prefill_far_scores_of_64_rows(gpu, dtype):
+    """The same, where a wave has 64 rows: rising scores, whose last key alone has a weight."""
+    case = prefill_case(dtype, [1000] * 4, None, 66, 2, 64, seed=42, spare=0)
+    q, k, v, cu, _ = case
+    assert cabi.gqa_prefill_info(4, 4000, 4000, 66, 2, 64, cabi.DTYPE[dtype])[2] == 256
+    q[:], k[:] = 0, 0
+    q[:, :, 0] = 8
+    k[:, :, 0] = torch.arange(1, 1001).repeat(4)[:, None] // 8
+    k[:, :, 1] = torch.arange(1, 1001).repeat(4)[:, None] % 8
+    q[:, :, 1] = 1  # scores 1, 2, .. of a sequence's keys
+    for e in (10, 17, 25, 33, 60, 90):
+        say(f"far scores, 64 rows {dtype} 2^{e}")
+        out = prefill(gpu, case, scale=2.0 ** e).cpu()
+        assert torch.equal(out, v.repeat_interleave(33, 1)), e
