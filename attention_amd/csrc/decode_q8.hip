@@ -181,7 +181,10 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(Q8Params p) {
 //   softmax  per lane; a token's weight is p = 2^(s - m) and goes into the values'
 //            product as p s_v, whose running reference m is that of s + log2 |s_v|:
 //            whatever the pages' scales, the largest p s_v of a row is near 2^kShift
-//            and fp16 holds the rest as far below it as fp16 goes.
+//            and fp16 holds the rest as far below it as fp16 goes.  p itself is up to
+//            2^115 where scales are 2^-100 (a page of zeros): its sum is kept times
+//            2^-12, so that 2^24 such terms fit, and one of scales of 2^100 (p down to
+//            2^-93) loses nothing.
 //   output   O^T += V^T (p s_v)^T, 16x16x32 in fp16: a lane reads E = DP / 16
 //            neighbouring elements of 8 tokens' V rows and exchanges bytes
 //            between token pairs in registers.
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(Q8Params p) {
 // Up to four waves of a workgroup take neighbouring virtual heads at the same
 // tokens (whole rows of memory), or, with fewer heads, neighbouring 32 tokens.
 
-constexpr float kQ8Shift = 7.f, kQ8Lazy = 8.f;
+constexpr float kQ8Shift = 7.f, kQ8Lazy = 8.f, kQ8Sum = 0x1p-12f;
 // Balanced launches: what an item's start costs, in tiles, and the least cost of a
 // workgroup's range.  Starts of 1 or 4 tiles: 256 sequences of 50 to 200 tokens 28.0
 // us for 26.7; ranges of 4: one sequence of 1500 tokens 12.2 for 11.5, 16 sequences
@@ -445,7 +448,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
       for (int tb = 0; tb < 2; ++tb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[tb][e] = fast_exp2(s[tb][e] + ref);
-        l += (s[tb][0] + s[tb][1]) + (s[tb][2] + s[tb][3]);
+        l = fmaf((s[tb][0] + s[tb][1]) + (s[tb][2] + s[tb][3]), kQ8Sum, l);
         w[2 * tb] = Ops::pack2(s[tb][0] * vs[tb], s[tb][1] * vs[tb]);
         w[2 * tb + 1] = Ops::pack2(s[tb][2] * vs[tb], s[tb][3] * vs[tb]);
       }
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     if (!real) return;
     const bool has = sum > 0.f || sum != sum;
     if (whole) {
-      const float inv = has ? 1.f / sum : 0.f;
+      const float inv = has ? kQ8Sum / sum : 0.f;
       char* to = static_cast<char*>(p.out) + q_row * p.D * 2;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -744,7 +747,7 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
     }
     if (team == 0 && d < p.D) {
       const bool has = sum > 0.f || sum != sum;
-      const float inv = has ? 1.f / sum : 0.f;
+      const float inv = has ? kQ8Sum / sum : 0.f;
       if (!has) a = f32x4{0.f, 0.f, 0.f, 0.f};
       *reinterpret_cast<u32x2*>(out + 2 * d) =
           u32x2{MfmaOps<DT>::pack2(a[0] * inv, a[1] * inv), MfmaOps<DT>::pack2(a[2] * inv, a[3] * inv)};

@@ -8,8 +8,8 @@ import torch
 
 from attention_amd import cabi
 from oracle.prompt_oracle import oracle_prefill
-from tests.test_gpu_prompt import (BF, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, f64, prefill, prefill_case,
-                                   prefill_tolerance, say, starts)
+from tests.test_gpu_prompt import (BF, CACHE, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, decode, f64,
+                                   prefill, prefill_case, prefill_tolerance, say, starts)
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,33 @@ def test_prefill_far_scores_of_64_rows(gpu, dtype):
         say(f"far scores, 64 rows {dtype} 2^{e}")
         out = prefill(gpu, case, scale=2.0 ** e).cpu()
         assert torch.equal(out, v.repeat_interleave(33, 1)), e
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("last", [True, False])
+def test_decode_long_stretch_of_zero_values(gpu, kind, last):
+    """65552 tokens, of which only 16 have values, with the others' scales as kv_append_q8 writes them (2^-100).
+    All scores are the same but for the first 32, which are lower."""
+    say(f"zero values {kind} {last}")
+    B, P, pages = 512, 16, 4097
+    kc, vc = torch.zeros(4, P, 4, 64), torch.zeros(4, P, 4, 64)
+    kc[1:, :, :, 0] = 8
+    vc[2] = torch.randint(-15, 16, (P, 4, 64), generator=torch.Generator().manual_seed(3)).float()
+    ks, vs = torch.full((4, 4), 0.125), torch.full((4, 4), 2.0 ** -100)
+    vs[2] = 0.25
+    row = [0, 0] + [1] * (pages - 2)
+    row[-1 if last else 2000] = 2
+    table = torch.tensor([row] * B, dtype=torch.int32)
+    q = torch.zeros(B, 4, 64, dtype=BF)
+    q[:, :, 0] = 5.25  # scores 5.25, or 0: 7.57 binary places apart
+    out = decode(gpu, (q, kc.to(CACHE[kind]), vc.to(CACHE[kind]), ks, vs, table, torch.full((B,), P * pages, dtype=torch.int32)),
+                 scale=1.0)
+    v = f64(vc[2]) * 0.25
+    total = 32 * np.exp(-5.25) + P * (pages - 2)
+    want = (v.sum(0) / total)[None]
+    # Weights are rounded once, to fp16 with the scale of their page, on a grid of 2^-32 of the largest such product;
+    # n terms are off by 2 n u, exponentials by 8 u, the output by half a step.  The largest weight times scale is
+    # 0.25 / total, the values at most 15 steps of it.
+    tol = (HALF[BF] * np.abs(want) + (2.0 ** -11 + 2 * P * pages * U + 8 * U) * (np.abs(v).sum(0) / total)[None]
+           + P * pages * 2.0 ** -32 * 0.25 * 15 / total)
+    assert (np.abs(f64(out) - want) <= tol).all()
