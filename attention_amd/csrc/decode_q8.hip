@@ -179,7 +179,9 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(Q8Params p) {
 //            operands of two products as they lie (the order of the head's
 //            elements is the queries' too)
 //   softmax  per lane; a token's weight is p = 2^(s - m) and goes into the values'
-//            product as p s_v, whose running reference m is that of s + log2 |s_v|:
+//            product as p s_v, whose running reference m is that of s + log2 |s_v|
+//            (in two parts, a score and the rest, so that neither is lost beside
+//            scores past 2^24):
 //            whatever the pages' scales, the largest p s_v of a row is near 2^kShift
 //            and fp16 holds the rest as far below it as fp16 goes.  p itself is up to
 //            2^115 where scales are 2^-100 (a page of zeros): its sum is kept times
@@ -270,12 +272,41 @@ __device__ __forceinline__ void q8_pairs(uint32_t a, uint32_t b, uint32_t (&out)
   }
 }
 
+// a b, rounded by itself: the same score is the same number whatever follows.
+__device__ __forceinline__ float q8_rounded(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// What a row's weights count from: a score, and what to add to it.  -Inf: nothing yet.
+struct Q8Ref {
+  float score = -INFINITY, rest = -INFINITY;
+  __device__ __forceinline__ Q8Ref() {}
+  // Statistics of a part: score, sum of weights, rest.
+  __device__ __forceinline__ explicit Q8Ref(f32x4 x) : score(x[0]), rest(x[2]) {}
+  __device__ __forceinline__ f32x4 with(float sum) const { return f32x4{score, sum, rest, 0.f}; }
+  __device__ __forceinline__ float from() const { return score == -INFINITY ? 0.f : score; }
+  // The same with the score of n, which is not smaller.
+  __device__ __forceinline__ float rest_from(const Q8Ref& n) const { return (score - n.from()) + rest; }
+  // 2^(this - n).
+  __device__ __forceinline__ float weight(const Q8Ref& n) const {
+    return fast_exp2(rest_from(n) - (n.rest == -INFINITY ? 0.f : n.rest));
+  }
+  // The larger of both.
+  __device__ __forceinline__ Q8Ref joined(const Q8Ref& o) const {
+    Q8Ref n;
+    n.score = fmaxf(score, o.score);
+    n.rest = fmaxf(rest_from(n), o.rest_from(n));
+    return n;
+  }
+};
+
 template <int DP>
 struct Q8Shape {
   static constexpr int E = DP / 16;       // V elements of a lane per token
   static constexpr int kPieces = DP / 64; // 16-byte pieces of a K row per lane
   static constexpr int kFrags = DP / 32;  // operands of the queries
-  static constexpr int kLds = 4 * E * 1024 + 4 * 16 * 8;  // parts of waves that share heads, {m, l} of their rows
+  static constexpr int kLds = 4 * E * 1024 + 4 * 16 * 16;  // parts of waves that share heads, their rows' statistics
 };
 
 template <int DT, int KIND, int DP>
@@ -400,12 +431,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
     f32x4 acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    Q8Ref m;
+    float l = 0.f;
 
     auto compute = [&](Raw& x, int i, int tile) {
       const int first = (tile * tw_count + tw) * 32;
       f32x4 s[2];
-      float mx = -INFINITY, vs[2], ksc[2];
+      float high[2], lv[2], vs[2], ksc[2];
       const bool cut = first + 32 > len;
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
@@ -419,9 +451,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
           }
         vs[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_lane), 2 * i + tb));
         ksc[tb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), 2 * i + tb)) * (p.sl2 * q_inv);
-        const float lv = __builtin_amdgcn_logf(fmaxf(fabsf(vs[tb]), 0x1p-100f));
+        lv[tb] = __builtin_amdgcn_logf(fmaxf(fabsf(vs[tb]), 0x1p-100f));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[tb][e] *= ksc[tb];
+        for (int e = 0; e < 4; ++e) s[tb][e] = q8_rounded(s[tb][e], ksc[tb]);
         if (cut) {
           // Behind the last token: no weight, and no value (a NaN x 0).
           const int left = len - first - 16 * tb - 4 * g4;
@@ -432,22 +464,25 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
             for (int w = 0; w < E / 4; ++w) x.v[tb][e][w] = e < left ? x.v[tb][e][w] : 0u;
           }
         }
-        mx = fmaxf(mx, fmaxf(fmaxf(s[tb][0], s[tb][1]), fmaxf(s[tb][2], s[tb][3])) + lv);
+        high[tb] = fmaxf(fmaxf(s[tb][0], s[tb][1]), fmaxf(s[tb][2], s[tb][3]));
       }
-      if (__ballot(mx > m + kQ8Lazy)) {
-        const float mn = fmaxf(m, q8_max_groups(mx));
-        const float alpha = mn == m ? 1.f : fast_exp2(m - mn);
-        m = mn;
+      auto rest = [&](float from) { return fmaxf((high[0] - from) + lv[0], (high[1] - from) + lv[1]); };
+      if (__ballot(rest(m.from()) > m.rest + kQ8Lazy)) {
+        Q8Ref n;
+        n.score = fmaxf(m.score, q8_max_groups(fmaxf(high[0], high[1])));
+        n.rest = fmaxf(m.rest_from(n), q8_max_groups(rest(n.from())));
+        const float alpha = m.weight(n);
+        m = n;
         l *= alpha;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= alpha;
       }
-      const float ref = m == -INFINITY ? kQ8Shift : kQ8Shift - m;
+      const float from = m.from(), ref = m.rest == -INFINITY ? kQ8Shift : kQ8Shift - m.rest;
       u32x4 w;
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[tb][e] = fast_exp2(s[tb][e] + ref);
+        for (int e = 0; e < 4; ++e) s[tb][e] = fast_exp2((s[tb][e] - from) + ref);
         l = fmaf((s[tb][0] + s[tb][1]) + (s[tb][2] + s[tb][3]), kQ8Sum, l);
         w[2 * tb] = Ops::pack2(s[tb][0] * vs[tb], s[tb][1] * vs[tb]);
         w[2 * tb + 1] = Ops::pack2(s[tb][2] * vs[tb], s[tb][3] * vs[tb]);
@@ -493,23 +528,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
       // Waves of the same heads: each leaves its part in LDS, the first of them
       // takes them up.
       __syncthreads();
-      f32x2* stats = reinterpret_cast<f32x2*>(smem + 4 * E * 1024);
+      f32x4* stats = reinterpret_cast<f32x4*>(smem + 4 * E * 1024);
       f32x4* parts = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
       for (int e = 0; e < E; ++e) parts[(wv * E + e) * 64 + lane] = acc[e];
-      if (g4 == 0) stats[wv * 16 + r16] = f32x2{m, sum};
+      if (g4 == 0) stats[wv * 16 + r16] = m.with(sum);
       __syncthreads();
       if (tw == 0) {
-        float most = -INFINITY;
-        for (int w = 0; w < tw_count; ++w) most = fmaxf(most, stats[(w * p.hw + wh) * 16 + r16][0]);
-        const float ref = most == -INFINITY ? 0.f : most;
+        Q8Ref most;
+        for (int w = 0; w < tw_count; ++w) most = most.joined(Q8Ref(stats[(w * p.hw + wh) * 16 + r16]));
         sum = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int w = 0; w < tw_count; ++w) {
-          const f32x2 ml = stats[(w * p.hw + wh) * 16 + r16];
-          const float f = fast_exp2(ml[0] - ref);
-          sum += f * ml[1];
+          const f32x4 x = stats[(w * p.hw + wh) * 16 + r16];
+          const float f = Q8Ref(x).weight(most);
+          sum += f * x[1];
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += f * parts[((w * p.hw + wh) * E + e) * 64 + lane];
         }
@@ -537,7 +571,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
       }
     } else {
       float* part = p.part + (slot * p.hw * 16 + wh * 16 + r16) * (p.D + 4);
-      if (g4 == 0) *reinterpret_cast<f32x2*>(part) = has ? f32x2{m, sum} : f32x2{-INFINITY, 0.f};
+      if (g4 == 0) *reinterpret_cast<f32x4*>(part) = has ? m.with(sum) : Q8Ref().with(0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = E * (4 * g4 + i);
@@ -663,7 +697,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void q8_mfma_kernel(Q8Param
 template <int DT, int DP, int WAVES>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
   constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, TEAMS = 64 / LANES * WAVES, STEP = 4 * LANES;
-  __shared__ f32x2 stats[4];
+  __shared__ f32x4 stats[4];
   __shared__ f32x4 joined[4][LANES];
   const int item = static_cast<int>(blockIdx.x), b = packed_divide(blockIdx.x, p.by_groups), hg = item - b * p.groups;
   const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -686,60 +720,71 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8Params p) {
   char* out = static_cast<char*>(p.out) + (static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G + g) * p.D * 2;
   for (int d0 = 0; d0 < p.D; d0 += STEP) {
     const int d = d0 + 4 * l;
-    float mx = -INFINITY, sum = 0.f;
+    Q8Ref m;
+    float sum = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     // Eight partials at a time, statistics and values in flight together.
     constexpr int kAhead = 8;
     for (int s0 = kAhead * team; s0 < count; s0 += kAhead * TEAMS) {
       f32x2 ml[kAhead];
+      float rest[kAhead];
       f32x4 x[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const float* src = part(min(s0 + i, count - 1));
         ml[i] = *reinterpret_cast<const f32x2*>(src);
+        rest[i] = src[2];
         x[i] = d < p.D ? *reinterpret_cast<const f32x4*>(src + 4 + d) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      float most = mx;
+      Q8Ref most = m;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) most = fmaxf(most, ml[i][0]);
-      const float ref = most == -INFINITY ? 0.f : most;
-      const float old = fast_exp2(mx - ref);
+      for (int i = 0; i < kAhead; ++i) most.score = fmaxf(most.score, ml[i][0]);
+      const float from = most.from(), mine = (m.score - from) + m.rest;
+      most.rest = mine;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        rest[i] += ml[i][0] - from;
+        most.rest = fmaxf(most.rest, rest[i]);
+      }
+      const float ref = most.rest == -INFINITY ? 0.f : most.rest, old = fast_exp2(mine - ref);
       sum *= old;
       a *= old;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (s0 + i >= count) continue;
-        const float f = fast_exp2(ml[i][0] - ref);
+        const float f = fast_exp2(rest[i] - ref);
         sum += f * ml[i][1];
         a += f * x[i];
       }
-      mx = most;
+      m = most;
     }
 #pragma unroll
     for (int off = LANES; off < 64; off <<= 1) {
-      const float om = __shfl_xor(mx, off), os = __shfl_xor(sum, off);
+      Q8Ref o;
+      o.score = __shfl_xor(m.score, off);
+      o.rest = __shfl_xor(m.rest, off);
+      const float os = __shfl_xor(sum, off);
       f32x4 oa;
 #pragma unroll
       for (int i = 0; i < 4; ++i) oa[i] = __shfl_xor(a[i], off);
-      const float most = fmaxf(mx, om), ref = most == -INFINITY ? 0.f : most;
-      const float f = fast_exp2(mx - ref), of = fast_exp2(om - ref);
+      const Q8Ref most = m.joined(o);
+      const float f = m.weight(most), of = o.weight(most);
       sum = f * sum + of * os;
       a = f * a + of * oa;
-      mx = most;
+      m = most;
     }
     if constexpr (WAVES == 4) {
       if (lane < LANES) joined[wv][lane] = a;
-      if (lane == 0) stats[wv] = f32x2{mx, sum};
+      if (lane == 0) stats[wv] = m.with(sum);
       __syncthreads();
-      float most = -INFINITY;
+      Q8Ref most;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) most = fmaxf(most, stats[w][0]);
-      const float ref = most == -INFINITY ? 0.f : most;
+      for (int w = 0; w < 4; ++w) most = most.joined(Q8Ref(stats[w]));
       sum = 0.f;
       a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float f = fast_exp2(stats[w][0] - ref);
+        const float f = Q8Ref(stats[w]).weight(most);
         sum += f * stats[w][1];
         a += f * joined[w][l];
       }

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from attention_amd import cabi
-from oracle.prompt_oracle import oracle_prefill
-from tests.test_gpu_prompt import (BF, CACHE, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, decode, f64,
+from oracle.prompt_oracle import TOP, cached_rows, oracle_prefill
+from tests.test_gpu_prompt import (BF, CACHE, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, decode, decode_case, f64,
                                    prefill, prefill_case, prefill_tolerance, say, starts)
 
 pytestmark = pytest.mark.gpu
@@ -158,6 +158,45 @@ def test_prefill_far_scores_of_64_rows(gpu, dtype):
         say(f"far scores, 64 rows {dtype} 2^{e}")
         out = prefill(gpu, case, scale=2.0 ** e).cpu()
         assert torch.equal(out, v.repeat_interleave(33, 1)), e
+
+
+FAR_DECODE = [
+    # lens, Hq, Hkv, D, P, spare pages
+    ([300, 1, 77], 8, 2, 64, 16, 0), ([300, 129], 8, 4, 128, 16, 200), ([2000], 4, 1, 128, 64, 0), ([100, 500], 6, 3, 256, 16, 0),
+    ([700], 40, 8, 128, 32, 100),
+]
+
+
+@pytest.mark.parametrize("dtype, values", [(HF, 1.0), (BF, 1.0), (BF, 2.0 ** 40), (BF, 2.0 ** -40)])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("i", range(len(FAR_DECODE)))
+@pytest.mark.parametrize("flags", [0, cabi.QD_FLAG_FORCE_GENERIC])
+def test_decode_far_scores(gpu, dtype, values, kind, i, flags):
+    """Scores of 2^16 to 2^100, exact and at least 2^16 apart: only the largest have a weight, all the same.
+    Tolerance: weights once to fp16 with the scale of their page, on a grid of 2^-32 of the largest such
+    product; n terms by 2 n u, exponentials by 8 u, the output's rounding."""
+    lens, Hq, Hkv, D, P, spare = FAR_DECODE[i]
+    q, kc, vc, ks, vs, table, n = decode_case(dtype, kind, lens, Hq, Hkv, D, P, seed=51 + i, spare=spare)
+    q[:] = 0
+    q[:, :, 0] = 8
+    ks[:], vs = 0.5, vs * values
+    for level in LEVELS:
+        levels = LEVELS[level](torch.arange(max(lens)), max(lens)) // 5  # -12 to 12: both types hold them
+        k = torch.zeros(kc.shape)
+        want, tol = np.zeros(q.shape), np.zeros(q.shape)
+        for b, len_ in enumerate(lens):
+            for t in range(len_):
+                k[table[b, t // P], t % P, :, 0] = levels[t].float()
+            v, scales = cached_rows(f64(vc), f64(vs), table[b].numpy(), len_)
+            top = np.flatnonzero(levels[:len_] == levels[:len_].max())
+            mean, spread = v[top].mean(0), np.abs(v[top]).mean(0)
+            err = (HALF[dtype] * np.abs(mean) + (2.0 ** -11 + 2 * len_ * U + 8 * U) * spread
+                   + len_ * 2.0 ** -32 * TOP[kind] * scales[top].max(0)[:, None] / len(top) + TINY[dtype])
+            want[b], tol[b] = np.repeat(mean, Hq // Hkv, 0), np.repeat(err, Hq // Hkv, 0)
+        for e in (14, 20, 24, 26, 28, 33, 60, 94):
+            say(f"far decode {dtype} {values} {kind} {FAR_DECODE[i]} {level} 2^{e} flags {flags}")
+            out = f64(decode(gpu, (q, k.to(CACHE[kind]), vc, ks, vs, table, n), flags, 2.0 ** e))
+            assert (np.abs(out - want) <= tol).all(), (level, e)
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
