@@ -13,6 +13,7 @@ here hipcc compiles the HIP source directly so nothing is hipified.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -85,19 +86,26 @@ def hip_link_cmd() -> list[str]:
             "-o", HIP_LIB + ".tmp", f"-Wl,-rpath,{ROCM}/lib"]
 
 
+def _sources_of(path: str) -> set[str]:
+    """A source and every file of the tree that it includes, directly or not."""
+    found, todo = set(), [path]
+    while todo:
+        path = todo.pop()
+        if path in found:
+            continue
+        found.add(path)
+        with open(path) as f:
+            names = re.findall(r'^\s*#\s*include\s*"([^"]+)"', f.read(), re.M)
+        todo += [p for p in (os.path.join(d, n) for n in names for d in (os.path.dirname(path), INCLUDE)) if os.path.exists(p)]
+    return found
+
+
+def _older(obj: str, source: str) -> bool:
+    return not os.path.exists(obj) or any(os.path.getmtime(d) > os.path.getmtime(obj) for d in _sources_of(source))
+
+
 def _stale(name: str) -> bool:
-    obj = os.path.join(OBJ_DIR, f"{name}.o")
-    if not os.path.exists(obj):
-        return True
-    deps = [os.path.join(CSRC, f"{name}.hip"), os.path.join(CSRC, "qd_device.h"),
-            os.path.join(INCLUDE, "qd_attention.h")]
-    if name.startswith("tree_"):
-        deps += [os.path.join(CSRC, h) for h in ("tree_kernels.h", "tile_device.h")]
-    if name.startswith("prefill"):
-        deps += [os.path.join(CSRC, h) for h in ("prefill_kernels.h", "packed.h", "tile_device.h")]
-    if name == "cache_q8":
-        deps.append(os.path.join(CSRC, "packed.h"))
-    return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
+    return _older(os.path.join(OBJ_DIR, f"{name}.o"), os.path.join(CSRC, f"{name}.hip"))
 
 
 def _torch_flags() -> tuple[list[str], str]:
@@ -117,12 +125,7 @@ def torch_object_cmd(name: str) -> list[str]:
 
 
 def _torch_stale(name: str) -> bool:
-    obj = os.path.join(OBJ_DIR, f"{name}.o")
-    if not os.path.exists(obj):
-        return True
-    deps = [os.path.join(CSRC, f"{name}.cpp"), os.path.join(CSRC, "torch_desc.h"),
-            os.path.join(INCLUDE, "qd_attention.h")]
-    return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
+    return _older(os.path.join(OBJ_DIR, f"{name}.o"), os.path.join(CSRC, f"{name}.cpp"))
 
 
 def torch_link_cmd() -> list[str]:
