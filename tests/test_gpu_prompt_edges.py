@@ -2,14 +2,17 @@
 sizes are far from ordinary.  Every case prints its name first."""
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from attention_amd import cabi
 from oracle.prompt_oracle import TOP, cached_rows, oracle_prefill
-from tests.test_gpu_prompt import (BF, CACHE, FP, HALF, HF, TINY, U, WEIGHT, cache_case, check_append, decode, decode_case, f64,
-                                   prefill, prefill_case, prefill_tolerance, say, starts)
+from tests.test_gpu_prompt import (BF, CACHE, DECODE, FP, HALF, HF, SPLIT, TINY, U, WEIGHT, cache_case, check_append,
+                                   check_gather, decode, decode_case, f64, prefill, prefill_case, prefill_tolerance, say,
+                                   starts)
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +230,124 @@ def test_decode_long_stretch_of_zero_values(gpu, kind, last):
     tol = (HALF[BF] * np.abs(want) + (2.0 ** -11 + 2 * P * pages * U + 8 * U) * (np.abs(v).sum(0) / total)[None]
            + P * pages * 2.0 ** -32 * 0.25 * 15 / total)
     assert (np.abs(f64(out) - want) <= tol).all()
+
+
+# ---- What a workspace holds before a call, lookups of many sequences ---------------
+
+
+@pytest.mark.parametrize("i", range(len(SPLIT)))
+def test_prefill_split_reads_what_it_wrote(gpu, i):
+    """Whatever the workspace holds before the call."""
+    dtype, nq, nk, Hq, Hkv, D, window, sinks = SPLIT[i]
+    say(f"split workspace {i} {SPLIT[i]}")
+    case = prefill_case(dtype, nq, nk, Hq, Hkv, D, seed=50 + i)
+    d = [x if x is None else x.to(gpu) for x in case]
+    bytes_ = split_bytes(case, window, sinks)
+    assert bytes_ > 0
+    outs = []
+    for fill in (0x00, 0xFF, 0x7F):  # zeros, NaN, the largest numbers
+        ws = torch.full((bytes_ + 256,), fill, dtype=torch.uint8, device=gpu)
+        out = torch.full_like(d[0], float("nan"))
+        assert cabi.gqa_prefill(*d, out, scale=1 / math.sqrt(D), window=window, sinks=sinks, workspace=ws[:bytes_]) == 0
+        outs.append(out)
+        assert (ws[bytes_:] == fill).all()
+    assert torch.isfinite(outs[0]).all() and all(torch.equal(x, outs[0]) for x in outs)
+
+
+@pytest.mark.parametrize("i", range(len(DECODE)))
+def test_decode_split_reads_what_it_wrote(gpu, i):
+    dtype, kind, lens, Hq, Hkv, D, P = DECODE[i]
+    say(f"decode workspace {i} {dtype} {kind} {lens[:4]} {Hq} {Hkv} {D} {P}")
+    case = [x.to(gpu) for x in decode_case(dtype, kind, lens, Hq, Hkv, D, P, seed=i, spare=-(-3000 // P))]
+    bytes_ = cabi.lib().qd_gqa_decode_q8_workspace_bytes(len(lens), Hq, Hkv, D, P, case[5].shape[1], cabi.DTYPE[dtype], 0)
+    outs = []
+    for fill in (0x00, 0xFF, 0x7F):
+        ws = torch.full((bytes_ + 256,), fill, dtype=torch.uint8, device=gpu)
+        out = torch.full_like(case[0], float("nan"))
+        assert cabi.gqa_decode_q8(*case, out, scale=1 / math.sqrt(D), workspace=ws[:bytes_]) == 0
+        outs.append(out)
+        assert (ws[bytes_:] == fill).all()
+    assert torch.isfinite(outs[0]).all() and all(torch.equal(x, outs[0]) for x in outs)
+
+
+@pytest.mark.parametrize("B", [62, 63, 64, 65, 200, 4100])
+@pytest.mark.parametrize("P", [1, 7, 16])
+def test_append_many_sequences(gpu, B, P):
+    """Runs are found by one round trip up to 63 sequences and by searches from 64 on; empty sequences, and runs
+    begun anywhere in a page."""
+    say(f"append {B} sequences, pages of {P}")
+    gen = torch.Generator().manual_seed(B)
+    counts = torch.randint(0, 40, (B,), generator=gen).tolist()
+    for b in (0, B // 2, B - 1):
+        counts[b] = 0
+    at = torch.randint(0, 30, (B,), generator=gen).tolist()
+    kc, vc, ks, vs, table, gen = cache_case("int8" if P == 7 else "e4m3", at, counts, 1, 16, P, seed=B)
+    rows = torch.randn(sum(counts) + 2, 2, 16, generator=gen).to(BF)
+    check_append(gpu, rows[:, :1], rows[:, 1:], kc, vc, ks, vs, table, torch.tensor(at, dtype=torch.int32), starts(counts),
+                 "int8" if P == 7 else "e4m3", f"{B} sequences")
+
+
+@pytest.mark.parametrize("B", [62, 63, 64, 65, 1000])
+def test_gather_many_sequences(gpu, B):
+    say(f"gather {B} sequences")
+    gen = torch.Generator().manual_seed(B)
+    counts = torch.randint(0, 70, (B,), generator=gen)
+    lens = torch.minimum(counts, torch.randint(0, 70, (B,), generator=gen))
+    counts[0], lens[0], lens[B - 1] = 0, 0, 0
+    case = cache_case("e4m3", lens.tolist(), [0] * B, 1, 16, 16, seed=B)
+    check_gather(gpu, case, lens.int(), starts(counts.tolist()), BF, f"{B} sequences")
+
+
+# ---- Values that are not finite, where a wave has 64 rows and where heads are padded ----
+
+
+def bad_values(case, places, bad):
+    q, k, v, cu, cu_k = case
+    v = v.clone()
+    for token, col in places:
+        v[token, :, col] = bad
+    return q, k, v, cu, cu_k
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype, D", [(HF, 80), (BF, 96), (BF, 72), (HF, 192), (BF, 160), (FP, 80), (FP, 200)])
+def test_prefill_hidden_values_of_padded_heads(gpu, bad, dtype, D):
+    """A value that is not finite reaches the rows that see it, and no other; the last column of a head too."""
+    say(f"hidden, padded heads {bad} {dtype} {D}")
+    for window, sinks in ((0, 0), (20, 3)):
+        case = prefill_case(dtype, [130, 70], None, 2, 1, D, seed=61)
+        q, k, v, cu, _ = case
+        want, spread, size = oracle_prefill(f64(q), f64(k), f64(v), cu.tolist(), None, window, sinks, 1 / math.sqrt(D))
+        tol = prefill_tolerance(case, want, spread, size)
+        places = ((60, 0), (129, D - 1), (2, D // 2), (131, D - 1))
+        out = f64(prefill(gpu, bad_values(case, places, bad), window, sinks))
+        hit = np.zeros_like(want, dtype=bool)
+        for t in range(200):
+            b = 0 if t < 130 else 130
+            for token, col in places:
+                hit[t, :, col] |= b <= token <= t and (not window or token > t - window or token - b < sinks)
+        assert not np.isfinite(out[hit]).any() and (np.abs(out - want)[~hit] <= tol[~hit]).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), -float("inf")])
+@pytest.mark.parametrize("dtype, window, sinks", [(BF, 0, 0), (HF, 100, 5)])
+def test_prefill_hidden_values_of_64_rows(gpu, bad, dtype, window, sinks):
+    """The same where a wave has 64 rows, against the call without such values: rows that see none are as there."""
+    say(f"hidden, 64 rows {bad} {dtype} {window}")
+    counts = [3000, 1, 0, 1095]
+    case = prefill_case(dtype, counts, None, 64, 8, 64, seed=62, spare=1)
+    assert cabi.gqa_prefill_info(4, 4097, 4097, 64, 8, 64, cabi.DTYPE[dtype])[2] == 256
+    places = ((3, 0), (700, 63), (2999, 5), (3000, 6), (3500, 7))
+    want = prefill(gpu, case, window, sinks)
+    got = prefill(gpu, bad_values(case, places, bad), window, sinks)
+    t = torch.arange(4097)
+    begin = torch.where(t < 3000, 0, torch.where(t < 3001, 3000, torch.where(t < 4096, 3001, 4096)))
+    hit = torch.zeros(4097, 64, 64, dtype=torch.bool)
+    for token, col in places:
+        sees = (begin <= token) & (token <= t)
+        if window:
+            sees &= (token > t - window) | (token - begin < sinks)
+        hit[sees, :, col] = True
+    hit = hit.to(gpu)
+    assert not got[hit].isfinite().any()
+    assert torch.equal(got[~hit], want[~hit])
