@@ -53,7 +53,6 @@ struct CacheParams {
 template <int DT, int VEC>
 struct Piece {
   using S = typename Elem<DT>::S;
-  static constexpr int kWords = VEC * static_cast<int>(sizeof(S)) / 4;
   typedef S Vec __attribute__((ext_vector_type(VEC)));
   Vec x;
   __device__ __forceinline__ void load(const S* p) { x = *reinterpret_cast<const Vec*>(p); }
@@ -181,8 +180,8 @@ __device__ __forceinline__ Packed packed_at(const CacheParams& p, int per, int s
 // T rows in and half as many bytes out: HBM bounds it for prompts, the round trips
 // position -> page -> scale for single tokens (HOLD 0: a row per sequence, read
 // beside the position).  24 prompts of up to 6000 tokens, 8 heads of 128, bf16 to
-// e4m3, pages of 64: 93 us, 5.0 TB/s (a copy reaches 4.8); with the pieces' addresses
-// kept from reading to writing it was 138 (160 registers, three waves per SIMD
+// e4m3, pages of 64: 93 us, 5.0 TB/s (streaming two bytes in for one out reaches 6.2
+// over 4 GB); with the pieces' addresses kept from reading to writing it was 138 (160 registers, three waves per SIMD
 // instead of four).  Up to 4000 tokens, pages of 128: 72 us, 101 with the runs read
 // twice.  512 single tokens: 4.2 us, of 3 that an empty trip takes.
 // grid ceil(2 parts Hkv / 4), block 256; a workgroup's waves have neighbouring
@@ -357,7 +356,7 @@ constexpr int kGatherRows = 32;
 // elements per lane at a time; a lane keeps its column, and so its head.  Bound by
 // HBM: one byte in and an element out.  Lanes write 16 neighbouring bytes each (16
 // elements per lane, written in two halves: 111 us instead of 104 for 16 contexts
-// of 1000 to 9000 tokens, 8 heads of 128), past the caches (104 -> 100 us, 5.3 TB/s):
+// of 1000 to 9000 tokens, 8 heads of 128), past the caches (104 -> 100 us, 5.3 TB/s; streaming one byte in for two out reaches 5.9):
 // what reads the rows next mostly runs behind another L2.
 // grid (tokens / kGatherRows + B, 2), block 256.
 template <int DT, int KIND, int VEC>

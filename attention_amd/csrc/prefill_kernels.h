@@ -388,11 +388,11 @@ __device__ __forceinline__ float prefill_add_bad(float y, float seen) {
 
 // out rows of a lane, or their partials: acc of column block c, element e is
 // column 32 c + 8 (e / 4) + 4 half + e % 4 of row wave_row + 32 nb + lane % 32, m a
-// score that the row's weights count from.
+// score that the row's weights count from.  16-bit rows: partials only, whole ones go
+// through prefill_store_rows.
 template <int DT, int DP, int NB>
 __device__ __forceinline__ void prefill_store(const PrefillParams& p, const PrefillItem& x, int wave_row,
                                               const f32x16 (&acc)[DP / 32][NB], const float (&m)[NB], const float (&l)[NB]) {
-  constexpr int ES = DT == QD_DTYPE_F32 ? 4 : 2;
   const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -402,7 +402,7 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
     if (rr >= x.rows) continue;
     const PrefillRow row = prefill_row(p, x, rr);
     const int64_t at = static_cast<int64_t>(x.q0 + row.query) * p.Hq + static_cast<int64_t>(x.h) * p.G + row.g;
-    if (p.splits > 1) {
+    if (DT != QD_DTYPE_F32 || p.splits > 1) {
       float* to = p.part + (x.split * (static_cast<int64_t>(p.Tq) * p.Hq) + at) * (p.D + 4);
       if (half == 0) *reinterpret_cast<f32x2*>(to) = has ? f32x2{m[nb] * p.sl2, sum} : f32x2{-INFINITY, 0.f};
 #pragma unroll
@@ -417,7 +417,7 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
       continue;
     }
     const float scale = has ? 1.f / sum : 0.f;
-    char* to = static_cast<char*>(p.out) + at * p.D * ES;
+    float* to = static_cast<float*>(p.out) + at * p.D;
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
@@ -427,7 +427,7 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
         f32x4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = has ? acc[c][nb][e + j] * scale : 0.f;
-        *reinterpret_cast<f32x4*>(to + d * ES) = y;
+        *reinterpret_cast<f32x4*>(to + d) = y;
       }
   }
 }
@@ -565,8 +565,10 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams p) {
 // cycles, a conversion and a sum of two), for heads of 64 four.  What bounds it:
 // products of random data alone run at 1709 TFLOP/s (the card's power takes the
 // clock to 1.7 GHz), with that much softmax beside them and nothing else at 1267;
-// one prompt of 12001 tokens, 32 heads of 128, takes 1065 to 1115 us, 1060 to 1110
-// TFLOP/s, with the clock at 1.6 GHz and the matrix cores busy for 57% of it.  16x16x32 products need
+// one prompt of 12001 tokens, 32 heads of 128, takes 1060 to 1125 us, 1050 to 1110
+// TFLOP/s: 2.0 million cycles, of which the matrix cores are busy for 57%, at a clock
+// that the card moves with its load (1.82 GHz in dispatches of 1100 us; 1.43 and 1376 us
+// at times under counters).  16x16x32 products need
 // twice the issue slots and ran at 1116 beside the same softmax.  Heads of 64 (16 and
 // 32 of 1000 to 8192 tokens) reach 650 to 720 TFLOP/s, bound by vector instructions.
 //
@@ -992,7 +994,10 @@ __global__ __launch_bounds__(64 * NW, (NB * DP <= 128 ? 2 : 1)) void prefill_pip
 }
 
 // fp32: the same products on the fp32 matrix cores, tile by tile, without the
-// overlap: they take eight times as long as the 16-bit ones, and hide the rest.
+// overlap: they take eight times as long as the 16-bit ones.  Scores, softmax and values
+// follow each other, and a barrier each tile, with one workgroup per CU: 2 prompts of
+// 2048 tokens, 16 heads of 128, take 378 us, 91 TFLOP/s of the 137 that a large product
+// reaches.
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void prefill_f32_kernel(PrefillParams p) {
   using Sh = PrefillShape<QD_DTYPE_F32, DP, 1, NW>;
