@@ -37,6 +37,8 @@ def gqa_prefill(q, key, value, cu_seqlens, *, cu_seqlens_k=None, window=None, si
     query sees the keys up to its own position, or with ``window`` the last
     ``window`` of them and the first ``sinks`` of the sequence.  Returns ``[Tq, Hq,
     D]``; queries that see nothing, and rows behind the last sequence, give zeros.
+    Sums are float32; float16 and bfloat16 round each softmax weight to the type
+    once, where :func:`gqa_decode` keeps it in more bits.
     """
     _require_extension()
     if scale is None:
@@ -55,11 +57,11 @@ def kv_append_q8(key, value, k_cache, v_cache, k_scales, v_scales, block_table, 
 
     A page's scale of a head is the smallest power of two that holds its largest
     value: a page that the call begins takes the one of its new rows; one that it
-    goes on with keeps the old one, or takes a larger one, and the rows before are
-    rounded to it.  An Inf or NaN (or a scale past 2^100) makes the scale NaN, and
-    with it every value of that page and head.  Sequences with a negative position
-    write nothing, nor do tokens past the table or in pages outside the pool.  Pages
-    that are written to must be their sequence's own.
+    goes on with keeps the old one, or takes a larger one (in magnitude), and the rows
+    before are rounded to it.  An Inf or NaN (or a scale past 2^100) makes the scale
+    NaN, and with it every value of that page and head.  Sequences with a negative
+    position write nothing, nor do tokens past the table or in pages outside the pool.
+    Pages that are written to must be their sequence's own.
     """
     _require_extension()
     torch.ops.qd_serving.kv_append_q8(key, value, k_cache, v_cache, k_scales, v_scales, block_table, positions,
@@ -83,7 +85,9 @@ def gqa_decode_q8(q, k_cache, v_cache, k_scales, v_scales, block_table, context_
     bfloat16), scales of any magnitude from 2^-100 to 2^100, or 0.  Returns ``[B, Hq,
     D]``; a sequence of length 0 gives zeros.  Lengths are not read on the host: the
     width of ``block_table`` decides whether contexts may be split (with a second
-    kernel that merges them), so trim it to the longest.
+    kernel that merges them), so trim it to the longest.  Sums are float32; weights
+    times their values' scale are rounded to float16 once, and there is no ``window``
+    as in :func:`gqa_decode_window`.
     """
     _require_extension()
     if scale is None:

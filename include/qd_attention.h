@@ -596,9 +596,11 @@ size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tok
  * does not reach that query's row.  q [q_tokens, q_heads, head_dim], key and
  * value [k_tokens, kv_heads, head_dim], their tokens q_stride, k_stride and
  * v_stride elements apart; out is contiguous.
- * Calls of more than 2^24 workgroups are refused: 2^24 rows (queries x q-heads)
- * of the VALU kernel, which takes unaligned tensors and rows of no whole 16
- * bytes, or 2^31 of the other.
+ * Products and sums are float32; 16-bit types round each softmax weight to the
+ * type once, and divide by the sum of the rounded ones.
+ * Calls of 2^24 workgroups or more are refused: 2^24 rows (queries x q-heads) of
+ * the VALU kernel, which takes unaligned tensors and rows of no whole 16 bytes, or
+ * about 2^31 of the other.
  * flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
 int qd_gqa_prefill(const void* q, const void* key, const void* value, const int32_t* cu, const int32_t* cu_k,
                    void* out, void* workspace, size_t workspace_bytes, int batch, int64_t q_tokens, int64_t k_tokens,
@@ -673,7 +675,9 @@ int qd_gqa_decode_q8_info(int batch, int q_heads, int kv_heads, int head_dim, in
  * each sequence; q and out are 16-bit.  Lengths are clamped to [0, max_pages *
  * block_size] (0: a zero row), page ids to the pool.  Scales may be any float32
  * of a magnitude in [2^-100, 2^100], or 0; a NaN one (qd_kv_append_q8) makes the
- * rows that see its page NaN.  flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
+ * rows that see its page NaN.  Sums are float32; the matrix-core kernel rounds a
+ * softmax weight times s_v to fp16 once, and holds bf16 queries exactly but for what
+ * lies below 2^-38 of a head's largest element.  flags: QD_FLAG_FORCE_GENERIC selects the VALU kernel. */
 int qd_gqa_decode_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scales,
                      const float* v_scales, const int32_t* block_table, const int32_t* context_lens, void* out,
                      void* workspace, size_t workspace_bytes, int batch, int q_heads, int kv_heads, int head_dim,
