@@ -436,13 +436,20 @@ __device__ __forceinline__ void prefill_store(const PrefillParams& p, const Pref
 // they lie in registers, a store reaches 16 bytes of 32 rows).
 template <typename Sh, int DT, int DP, int NB>
 __device__ __forceinline__ void prefill_store_rows(const PrefillParams& p, const PrefillItem& x, int wave_row, char* place,
-                                                   const f32x16 (&acc)[DP / 32][NB], const float (&l)[NB]) {
+                                                   f32x16 (&acc)[DP / 32][NB], const float (&l)[NB]) {
   const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5, n32 = lane & 31;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const float sum = prefill_sum_halves(l[nb]);
-    // Without weights the output is 0 already (what was not finite there was left out).
-    const float scale = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const bool has = sum > 0.f || sum != sum;
+    const float scale = has ? 1.f / sum : 0.f;
+    // Without weights the output is 0, whatever values scores of -inf belong to.
+    if (__ballot(!has)) {
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[c][nb][e] = has ? acc[c][nb][e] : 0.f;
+    }
     char* row = place + (32 * nb + n32) * Sh::kRow;
     const int swizzle = 16 * prefill_swizzle(Sh::kSlots, n32);
 #pragma unroll

@@ -591,7 +591,8 @@ size_t qd_gqa_prefill_workspace_bytes(int batch, int64_t q_tokens, int64_t k_tok
 /* out = softmax(q . k * scale) . v over the keys that a query sees.  Query i of
  * the nq of a sequence with nk keys lies at position p = nk - nq + i and sees
  * key j iff j <= p and (window == 0 or j > p - window or j < sinks); one that
- * sees nothing gets a zero row, and so do rows behind the last sequence.
+ * sees nothing, or nothing but scores of -inf, gets a zero row, and so do rows
+ * behind the last sequence.
  * Whatever a key or value holds that a query does not see (NaN included)
  * does not reach that query's row.  q [q_tokens, q_heads, head_dim], key and
  * value [k_tokens, kv_heads, head_dim], their tokens q_stride, k_stride and

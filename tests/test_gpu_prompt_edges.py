@@ -351,3 +351,24 @@ def test_prefill_hidden_values_of_64_rows(gpu, bad, dtype, window, sinks):
     hit = hit.to(gpu)
     assert not got[hit].isfinite().any()
     assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("D", [8, 64, 128, 256])
+@pytest.mark.parametrize("flags", [0, cabi.QD_FLAG_FORCE_GENERIC])
+def test_prefill_rows_of_scores_without_weight(gpu, dtype, D, flags):
+    """A query all of whose scores are -inf gets zeros, whatever the values hold; others are as ever."""
+    say(f"scores of -inf {dtype} {D} flags {flags}")
+    case = prefill_case(dtype, [70, 3], None, 2, 1, D, seed=71)
+    q, k, v, cu, _ = case
+    q[:, :, 3] = 1
+    want, spread, size = oracle_prefill(f64(q[70:73]), f64(k[70:73]), f64(v[70:73]), [0, 3], None, 0, 0, 1 / math.sqrt(D))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        kk, vv = k.clone(), v.clone()
+        kk[:70, 0, 3] = -float("inf")
+        vv[:66, 0, 5] = bad
+        vv[69, 0, 1] = bad
+        out = prefill(gpu, (q, kk, vv, cu, None), flags=flags)
+        assert not out[:70].any()
+        tol = prefill_tolerance((q, k, v, cu, None), want, spread, size)
+        assert (np.abs(f64(out[70:73]) - want) <= tol).all()
