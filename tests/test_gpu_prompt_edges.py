@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import attention_amd
 from attention_amd import cabi
 from oracle.prompt_oracle import TOP, cached_rows, oracle_prefill
 from tests.test_gpu_prompt import (BF, CACHE, DECODE, FP, HALF, HF, SPLIT, TINY, U, WEIGHT, cache_case, check_append,
@@ -372,3 +373,24 @@ def test_prefill_rows_of_scores_without_weight(gpu, dtype, D, flags):
         assert not out[:70].any()
         tol = prefill_tolerance((q, k, v, cu, None), want, spread, size)
         assert (np.abs(f64(out[70:73]) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prefill_past_2_32_bytes(gpu, dtype):
+    """Queries, keys, values and output of one projection of 5.6 GB: sequences at both ends against the oracle."""
+    say(f"past 2^32 bytes {dtype}")
+    Hq, Hkv, D, T = 32, 4, 128, 550_000
+    counts = [37] + [499] * 1102 + [0, 55, 3]
+    cu = starts(counts)
+    assert 0 < T - int(cu[-1]) < 500
+    qkv = torch.empty(T, Hq + 2 * Hkv, D, dtype=dtype, device=gpu)
+    qkv[:] = torch.randn(997, Hq + 2 * Hkv, D, device=gpu, generator=torch.Generator(device=gpu).manual_seed(1)).to(dtype).repeat(552, 1, 1)[:T]
+    q, k, v = qkv.split([Hq, Hkv, Hkv], dim=1)
+    out = attention_amd.gqa_prefill(q, k, v, cu.to(gpu))
+    assert out.numel() * 2 > 2 ** 32 and qkv.numel() * 2 > 2 ** 32
+    assert not out[int(cu[-1]):].any()
+    for b in (0, len(counts) - 2, len(counts) - 1):
+        part = tuple(x[cu[b]:cu[b + 1]].cpu() for x in (q, k, v)) + (torch.tensor([0, counts[b]], dtype=torch.int32), None)
+        want, spread, size = oracle_prefill(*(f64(x) for x in part[:3]), [0, counts[b]], None, 0, 0, D ** -0.5)
+        tol = prefill_tolerance(part, want, spread, size)
+        assert (np.abs(f64(out[cu[b]:cu[b + 1]]) - want) <= tol).all(), b
