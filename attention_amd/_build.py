@@ -94,7 +94,7 @@ def _sources_of(path: str) -> set[str]:
         if path in found:
             continue
         found.add(path)
-        with open(path) as f:
+        with open(path, encoding="utf-8") as f:
             names = re.findall(r'^\s*#\s*include\s*"([^"]+)"', f.read(), re.M)
         todo += [p for p in (os.path.join(d, n) for n in names for d in (os.path.dirname(path), INCLUDE)) if os.path.exists(p)]
     return found
